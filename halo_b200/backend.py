@@ -3,9 +3,11 @@
 The names follow include/halo/backend/backend.h of the reference: a `CudaBackend` hands out
 `Buffer`s and a `Stream`, operands are `TensorRef`s (buffer, byte offset, byte length, row stride),
 `gemv(GemvArgs)` / `lm_head(LmHeadArgs)` / `get_rows(GetRowsArgs)` validate on the host and enqueue,
-and failures raise `HaloError` carrying the reference's error class.  Everything else the interface
-lists (norms, attention, ...) is not part of this backend and raises Unsupported; nothing ever falls
-back to the CPU.  The C++ adapter in halo_b200/adapter implements the same mapping for C++ callers;
+and failures raise `HaloError` carrying the reference's error class.  `partial_rope(RopeArgs)`,
+`kv_write(KvWriteArgs)` and `attention(AttentionArgs)` are the attention layer's operators over a paged
+8-bit cache (include/halo_cuda_attention.h), with argument structs of this library's own.  Everything else
+the interface lists (norms, the Gated-DeltaNet operators, ...) is not part of this backend and raises
+Unsupported; nothing ever falls back to the CPU.  The C++ adapter in halo_b200/adapter implements the same mapping for C++ callers;
 this module exists so that tests and the benchmark can drive the library from Python.
 """
 from __future__ import annotations
@@ -133,6 +135,95 @@ class GetRowsArgs:
     n_ids: int = 0
 
 
+ACTIVATION_BYTES = {capi.T_F32: 4, capi.T_F16: 2, capi.T_BF16: 2}
+
+
+def rope_freqs(rot_dim: int, base: float, scaling: str = "none", factor: float = 1.0, original_context: float = 0.0, fast: float = 32.0,
+               slow: float = 1.0, magnitude: float = 0.0, pair_factors: list[float] | None = None) -> capi.RopeFreqs:
+    """The rotary frequencies of a model, made once (halo_cuda_rope_freqs); `scaling` is a key of capi.ROPE_SCALINGS."""
+    if scaling not in capi.ROPE_SCALINGS:
+        raise HaloError(capi.E_UNSUPPORTED, f"PARTIAL_ROPE: no scaling {scaling!r}")
+    if pair_factors is not None and len(pair_factors) != rot_dim // 2:
+        raise HaloError(capi.E_KERNEL, f"PARTIAL_ROPE: {len(pair_factors)} pair factors for {rot_dim // 2} pairs")
+    s = capi.RopeScaling(kind=capi.ROPE_SCALINGS[scaling], factor=factor, original_context=original_context, fast=fast, slow=slow, magnitude=magnitude)
+    if pair_factors is not None:
+        s.pair_factors = (C.c_double * len(pair_factors))(*pair_factors)
+    freqs = capi.RopeFreqs()
+    _check(capi.load().halo_cuda_rope_freqs(rot_dim, base, C.byref(s), C.byref(freqs)))
+    return freqs
+
+
+@dataclass
+class HeadsRef:
+    """Rows of heads: `ref` (its row_stride is the token stride, 0 = dense) and the bytes from one head to the next (0 = dense)."""
+    ref: TensorRef = field(default_factory=TensorRef)
+    head_stride: int = 0
+
+
+@dataclass
+class RopeArgs:
+    """PARTIAL_ROPE (halo_cuda_rope): an empty q_out / k_out turns q / k in place."""
+    freqs: capi.RopeFreqs | None = None
+    positions: TensorRef = field(default_factory=TensorRef)
+    q: HeadsRef = field(default_factory=HeadsRef)
+    k: HeadsRef = field(default_factory=HeadsRef)
+    q_out: HeadsRef = field(default_factory=HeadsRef)
+    k_out: HeadsRef = field(default_factory=HeadsRef)
+    n_tokens: int = 0
+    n_q: int = 0
+    n_kv: int = 0
+    head_dim: int = 0
+    interleaved: bool = False
+    type: int = capi.T_F32
+
+
+@dataclass
+class KvCache:
+    """A paged 8-bit cache (HaloCudaKvCache): the pools' row_stride is the bytes from page to page, the scales' likewise, the table's from
+    sequence to sequence; 0 = dense."""
+    k: TensorRef = field(default_factory=TensorRef)
+    v: TensorRef = field(default_factory=TensorRef)
+    k_scale: TensorRef = field(default_factory=TensorRef)
+    v_scale: TensorRef = field(default_factory=TensorRef)
+    table: TensorRef = field(default_factory=TensorRef)
+    n_pages: int = 0
+    n_kv: int = 0
+    head_dim: int = 0
+    page_tokens: int = 0
+    max_pages: int = 0
+    n_seq: int = 0
+
+
+@dataclass
+class KvWriteArgs:
+    """KV_WRITE (halo_cuda_kv_write); `start` may be empty: max_tokens rows of every sequence."""
+    cache: KvCache = field(default_factory=KvCache)
+    k: HeadsRef = field(default_factory=HeadsRef)
+    v: HeadsRef = field(default_factory=HeadsRef)
+    start: TensorRef = field(default_factory=TensorRef)
+    length: TensorRef = field(default_factory=TensorRef)
+    n_tokens: int = 0
+    max_tokens: int = 0
+    type: int = capi.T_F32
+
+
+@dataclass
+class AttentionArgs:
+    """ATTENTION (halo_cuda_attention); `start` may be empty: max_tokens rows of every sequence."""
+    cache: KvCache = field(default_factory=KvCache)
+    q: HeadsRef = field(default_factory=HeadsRef)
+    out: HeadsRef = field(default_factory=HeadsRef)
+    start: TensorRef = field(default_factory=TensorRef)
+    length: TensorRef = field(default_factory=TensorRef)
+    n_tokens: int = 0
+    max_tokens: int = 0
+    n_q: int = 0
+    scale: float = 1.0
+    causal: bool = True
+    window: int = 0
+    type: int = capi.T_F32
+
+
 class Stream:
     """Ordered work queue (Stream, backend.h:494-506)."""
 
@@ -166,7 +257,7 @@ class Stream:
 
 
 class CudaBackend:
-    """The `cuda` backend: MATMUL, LM_HEAD, GET_ROWS, COPY, upload / download."""
+    """The `cuda` backend: MATMUL, LM_HEAD, GET_ROWS, PARTIAL_ROPE, KV_WRITE, ATTENTION, COPY, upload / download."""
 
     def __init__(self, device: int = 0):
         self.lib = capi.load()
@@ -363,6 +454,61 @@ class CudaBackend:
         g.status = status.ptr if status is not None else None
         _check(self.lib.halo_cuda_get_rows(self.ctx, C.byref(g), s.handle))
 
+    # ---- the attention layer ---------------------------------------------------------------------------
+    def _heads(self, h: HeadsRef, name: str, op: str, n_tokens: int, n_heads: int, head_dim: int, kind: int, write: bool = False) -> capi.Heads:
+        if kind not in ACTIVATION_BYTES:
+            raise HaloError(capi.E_UNSUPPORTED, f"{op}: no activations of type id {kind}")
+        head = head_dim * ACTIVATION_BYTES[kind]
+        row = self._extent(n_heads, head, h.head_stride)
+        need = self._extent(n_tokens, row, h.ref.row_stride or n_heads * (h.head_stride or head)) if row else 0
+        return capi.Heads(self._resolve(h.ref, need, name, op, write) or None, h.ref.row_stride, h.head_stride)
+
+    def _cache(self, c: KvCache, op: str, write: bool) -> capi.KvCache:
+        page = c.n_kv * c.page_tokens * c.head_dim
+        out = capi.KvCache(type=capi.KV_E4M3, n_pages=c.n_pages, n_kv=c.n_kv, head_dim=c.head_dim, page_tokens=c.page_tokens, max_pages=c.max_pages,
+                           n_seq=c.n_seq, page_stride=c.k.row_stride, scale_stride=c.k_scale.row_stride, table_stride=c.table.row_stride)
+        if c.k.row_stride != c.v.row_stride or c.k_scale.row_stride != c.v_scale.row_stride:
+            raise HaloError(capi.E_KERNEL, f"{op}: the two pools have one stride")
+        for name, row in (("k", page), ("v", page), ("k_scale", c.n_kv), ("v_scale", c.n_kv)):
+            ref = getattr(c, name)
+            setattr(out, name, self._resolve(ref, self._extent(c.n_pages, row, ref.row_stride), name, op, write) or None)
+        out.table = self._resolve(c.table, self._extent(c.n_seq, c.max_pages * 4, c.table.row_stride), "table", op) or None
+        return out
+
+    def _rows(self, a, op: str) -> capi.KvRows:
+        return capi.KvRows(self._resolve(a.start, (a.cache.n_seq + 1) * 4, "start", op) or None,
+                           self._resolve(a.length, a.cache.n_seq * 4, "length", op) or None, a.n_tokens, a.max_tokens)
+
+    def partial_rope(self, s: Stream, a: RopeArgs) -> None:
+        op = "PARTIAL_ROPE"
+        g = capi.Rope(type=a.type, interleaved=a.interleaved, n_tokens=a.n_tokens, n_q=a.n_q, n_kv=a.n_kv, head_dim=a.head_dim)
+        if a.freqs is None:
+            raise HaloError(capi.E_API, f"{op}: no frequencies")
+        g.freqs = C.pointer(a.freqs)
+        g.positions = self._resolve(a.positions, a.n_tokens * 4, "positions", op) or None
+        for name, n in (("q", a.n_q), ("k", a.n_kv)):
+            x, y = getattr(a, name), getattr(a, name + "_out")
+            in_place = y.ref.empty()
+            setattr(g, name, self._heads(x, name, op, a.n_tokens, n, a.head_dim, a.type, write=in_place))
+            setattr(g, name + "_out", getattr(g, name) if in_place else self._heads(y, name + "_out", op, a.n_tokens, n, a.head_dim, a.type, write=True))
+        _check(self.lib.halo_cuda_rope(self.ctx, C.byref(g), s.handle))
+
+    def kv_write(self, s: Stream, a: KvWriteArgs, status: Buffer | None = None) -> None:
+        op, c = "KV_WRITE", a.cache
+        g = capi.KvWrite(type=a.type, cache=self._cache(c, op, True), rows=self._rows(a, op))
+        g.k = self._heads(a.k, "k", op, a.n_tokens, c.n_kv, c.head_dim, a.type)
+        g.v = self._heads(a.v, "v", op, a.n_tokens, c.n_kv, c.head_dim, a.type)
+        g.status = status.ptr if status is not None else None
+        _check(self.lib.halo_cuda_kv_write(self.ctx, C.byref(g), s.handle))
+
+    def attention(self, s: Stream, a: AttentionArgs, status: Buffer | None = None) -> None:
+        op, c = "ATTENTION", a.cache
+        g = capi.Attention(type=a.type, n_q=a.n_q, cache=self._cache(c, op, False), rows=self._rows(a, op), causal=a.causal, window=a.window, scale=a.scale)
+        g.q = self._heads(a.q, "q", op, a.n_tokens, a.n_q, c.head_dim, a.type)
+        g.out = self._heads(a.out, "out", op, a.n_tokens, a.n_q, c.head_dim, a.type, write=True)
+        g.status = status.ptr if status is not None else None
+        _check(self.lib.halo_cuda_attention(self.ctx, C.byref(g), s.handle))
+
     def repacked_row_bytes(self, wtype: int, cols: int) -> int:
         rb = C.c_uint64()
         _check(self.lib.halo_cuda_repacked_row_bytes(wtype, cols, C.byref(rb)))
@@ -396,7 +542,7 @@ class CudaBackend:
         raise HaloError(capi.E_UNSUPPORTED, "this op is not part of the cuda matmul backend")
 
     rms_norm = add_rms_norm = gdn_gates = conv1d_silu = gated_delta_rule = gated_rms_norm = _unsupported
-    partial_rope = kv_write = attention = swiglu = mul_sigmoid = add = argmax = top_k = _unsupported
+    swiglu = mul_sigmoid = add = argmax = top_k = _unsupported
 
 
 def decode_argmax(words: np.ndarray) -> list[tuple[int, float]]:

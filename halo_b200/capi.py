@@ -1,4 +1,4 @@
-"""ctypes binding of libhalo_cuda.so (the C ABI declared in include/halo_cuda.h and include/halo_cuda_gguf.h).
+"""ctypes binding of libhalo_cuda.so (the C ABI declared in include/halo_cuda.h, halo_cuda_attention.h and halo_cuda_gguf.h).
 
 The library is the product; this module only loads it and mirrors its structs.  There is no CPU
 fallback: if the library is missing, or no sm_100 device is present, the calls fail loudly.
@@ -25,6 +25,10 @@ GEMM_TCGEN05_F16_R, GEMM_TCGEN05_BF16_R = 10, 11
 REPACKED_VARIANTS = (GEMV_MMA_R, GEMV_MMA_I8X2_R, GEMM_TCGEN05_F16_R, GEMM_TCGEN05_BF16_R)  # W is in the layout of halo_cuda_repack_rows
 FLAG_ALLOW_GEMM = 1
 FLAG_NO_SCRATCH = 0x80000000
+T_F32, T_F16, T_BF16 = 0, 1, 30  # activation types of the attention layer's operators
+ROPE_SCALINGS = {"none": 0, "linear": 1, "base": 2, "ramp": 3, "bands": 4, "factors": 5}
+KV_E4M3 = 1
+KV_SCALE_MIN, KV_SCALE_MAX = 87, 207
 
 
 class DeviceInfo(C.Structure):
@@ -72,6 +76,45 @@ class GetRows(C.Structure):
     _fields_ = [("type", C.c_uint32), ("variant_id", C.c_uint32), ("table", C.c_void_p), ("table_stride", C.c_uint64),
                 ("ids", C.c_void_p), ("out", C.c_void_p), ("out_stride", C.c_uint64), ("n_rows", C.c_uint32), ("cols", C.c_uint32),
                 ("n_ids", C.c_uint32), ("status", C.c_void_p)]
+
+
+class Heads(C.Structure):
+    _fields_ = [("p", C.c_void_p), ("token_stride", C.c_uint64), ("head_stride", C.c_uint64)]
+
+
+class RopeScaling(C.Structure):
+    _fields_ = [("kind", C.c_uint32), ("reserved", C.c_uint32), ("factor", C.c_double), ("original_context", C.c_double), ("fast", C.c_double),
+                ("slow", C.c_double), ("magnitude", C.c_double), ("pair_factors", C.POINTER(C.c_double))]
+
+
+class RopeFreqs(C.Structure):
+    _fields_ = [("n_pairs", C.c_uint32), ("magnitude", C.c_float), ("turns", C.c_uint64 * 128)]
+
+
+class Rope(C.Structure):
+    _fields_ = [("type", C.c_uint32), ("interleaved", C.c_uint32), ("freqs", C.POINTER(RopeFreqs)), ("positions", C.c_void_p), ("q", Heads),
+                ("k", Heads), ("q_out", Heads), ("k_out", Heads), ("n_tokens", C.c_uint32), ("n_q", C.c_uint32), ("n_kv", C.c_uint32),
+                ("head_dim", C.c_uint32)]
+
+
+class KvCache(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p), ("table", C.c_void_p),
+                ("page_stride", C.c_uint64), ("scale_stride", C.c_uint64), ("table_stride", C.c_uint64), ("type", C.c_uint32), ("n_pages", C.c_uint32),
+                ("n_kv", C.c_uint32), ("head_dim", C.c_uint32), ("page_tokens", C.c_uint32), ("max_pages", C.c_uint32), ("n_seq", C.c_uint32),
+                ("reserved", C.c_uint32)]
+
+
+class KvRows(C.Structure):
+    _fields_ = [("start", C.c_void_p), ("length", C.c_void_p), ("n_tokens", C.c_uint32), ("max_tokens", C.c_uint32)]
+
+
+class KvWrite(C.Structure):
+    _fields_ = [("type", C.c_uint32), ("reserved", C.c_uint32), ("cache", KvCache), ("rows", KvRows), ("k", Heads), ("v", Heads), ("status", C.c_void_p)]
+
+
+class Attention(C.Structure):
+    _fields_ = [("type", C.c_uint32), ("n_q", C.c_uint32), ("cache", KvCache), ("rows", KvRows), ("q", Heads), ("out", Heads), ("causal", C.c_uint32),
+                ("window", C.c_uint32), ("scale", C.c_float), ("reserved", C.c_uint32), ("status", C.c_void_p)]
 
 
 class GgufInfo(C.Structure):
@@ -141,6 +184,10 @@ SYMBOLS = {
     "halo_cuda_ipc_open": (C.c_int, [_P, C.c_char_p, C.POINTER(_P)]),
     "halo_cuda_ipc_close": (C.c_int, [_P, _P]),
     "halo_cuda_gemv_reduce": (C.c_int, [_P, C.POINTER(Gemv), C.POINTER(PeerReduce), _P]),
+    "halo_cuda_rope_freqs": (C.c_int, [C.c_uint32, C.c_double, C.POINTER(RopeScaling), C.POINTER(RopeFreqs)]),
+    "halo_cuda_rope": (C.c_int, [_P, C.POINTER(Rope), _P]),
+    "halo_cuda_kv_write": (C.c_int, [_P, C.POINTER(KvWrite), _P]),
+    "halo_cuda_attention": (C.c_int, [_P, C.POINTER(Attention), _P]),
     "halo_gguf_open": (C.c_int, [C.c_char_p, C.POINTER(_P)]),
     "halo_gguf_parse": (C.c_int, [_P, C.c_uint64, C.POINTER(_P)]),
     "halo_gguf_close": (C.c_int, [_P]),
