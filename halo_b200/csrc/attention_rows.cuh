@@ -1,0 +1,649 @@
+// ATTENTION for few rows to a sequence (decoded tokens, drafts), and for fp32 operands of any number of rows: warp-level fp16 tensor-core products
+// over the cache's codes, converted in registers.
+//
+//   x_t = q . k_t * (s_K(t) * scale * log2 e) + log2 s_V(t),   m = max x_t,   p_t = 2^(x_t - m + 14)
+//   o = sum p_t code(v_t),   l = sum p_t / s_V(t),   out = o / l
+//
+// The scale of a value's page rides in its token's exponent, so that o needs no rescaling between pages and p_t, at most 2^14, is an fp16 number with
+// 11 bits down to 2^-28 of the largest.  e4m3 codes are exact in fp16.  A row of q is multiplied by the power of two that puts its largest magnitude
+// into [2^14, 2^15) and rounded to fp16: exact for fp16 and bf16 operands (but for elements below 2^-29 of the row's largest);
+// fp32 operands are taken as two fp16 terms, and so are their p_t.  Accumulators, maxima and sums are fp32.
+//
+// A CTA has RG groups of TS warps.  A group has 16 packed rows (attention_work.cuh); its warps share the keys of a tile, each with a running maximum,
+// sum and accumulators of its own that are joined at the end of a segment, so no warp waits for another inside the walk.  A producer warp
+// brings the tiles' codes by TMA, a box for each page, into a ring, and with them the scales of every 16 tokens (a page is at least 16).
+//
+// What bounds it: HBM.  A byte of the cache costs a warp half a conversion, and a sixteenth of a 16 x 8 x 16 product for 16 rows.
+#pragma once
+#include <cuda.h>
+
+#include "attention_work.cuh"
+
+namespace halo_cuda {
+namespace attn {
+
+constexpr uint32_t kRowsTile = 64;             // keys of a tile
+constexpr uint32_t kGroups = kRowsTile / 16;   // of 16 tokens, each inside one page
+
+struct GroupScale {
+    float k, log_v, inv_v;  // s_K * scale * log2 e; log2 s_V, -inf for tokens of no page; 1 / s_V
+    float pad;
+};
+
+/// CPS: CTAs that share an SM.
+template <int D, int TS, int RG, int CPS, int TERMS>
+struct RowsShape {
+    static constexpr int kWarps = TS * RG, kThreads = (kWarps + 1) * 32, kRows = 16 * RG;
+    static constexpr uint32_t kHalfTile = kRowsTile * D;  // K or V of a tile
+    static constexpr uint32_t kStage = 2 * kHalfTile;
+    static constexpr uint32_t kQ = RG * (D / 16) * TERMS * 512;
+    static constexpr uint32_t kJoin = TS > 1 ? RG * 16 * D * 4 : 0;
+    static constexpr uint32_t kFixed = 1024 + kQ + kJoin;  // alignment, q, the warps' joined rows
+    // an SM's 228 KiB, less 1 KiB a CTA for the system and 3 KiB for what is declared in the kernel
+    static constexpr uint32_t kStagesRoom = (228 / CPS * 1024 - 4096 - kFixed) / kStage;
+    static constexpr int kStages = kStagesRoom > 6 ? 6 : kStagesRoom;
+    static constexpr uint32_t kSmem = kFixed + kStages * kStage;
+    static_assert(kStages >= 2);
+};
+
+__device__ __forceinline__ uint32_t swizzled(uint32_t row, uint32_t chunk, int dim) {  // of a tile's half: 128-byte rows, or 64-byte rows of 64 elements
+    return dim == 64 ? row * 64 + ((chunk ^ (row >> 1 & 3)) << 4) : row * 128 + ((chunk ^ (row & 7)) << 4);
+}
+__device__ __forceinline__ uint4 lds128(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+    return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t at) {
+    uint2 v;
+    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at));
+    return v;
+}
+/// Two codes -> two fp16.
+__device__ __forceinline__ uint32_t widen(uint16_t codes) {
+    uint32_t h;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(codes));
+    return h;
+}
+__device__ __forceinline__ uint32_t widen_lo(uint32_t w) { return widen(static_cast<uint16_t>(w & 0xFFFFu)); }
+__device__ __forceinline__ uint32_t widen_hi(uint32_t w) { return widen(static_cast<uint16_t>(w >> 16)); }
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t half2_bits(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+/// What two-term rounding leaves behind the first term.
+__device__ __forceinline__ uint32_t half2_rest(float a, float b, uint32_t first) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&first));
+    return half2_bits(a - f.x, b - f.y);
+}
+/// Zeroes the NaN codes of four; true if there were any.
+__device__ __forceinline__ bool drop_nan(uint32_t& w) {
+    const uint32_t hit = ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;  // bit 7 of a byte that is 0x7F or 0xFF
+    if (hit == 0) return false;
+    w &= ~((hit >> 7) * 255u);
+    return true;
+}
+
+/// Writes NaN over the results of rows that see a token whose value is NaN there: the walk left those codes out in tiles that some rows do not see
+/// whole, where a product with weight zero would have spread them.  `at(row, d)` is the result's address.
+template <class At>
+__device__ void spread_nan(const AttentionCall& c, const Work& w, const Unit& u, const Segment& g, uint32_t threads, At&& at) {
+    const uint32_t rows = u.rows(w), r0 = u.row0(w), dim = c.cache.head_dim;
+    for (int32_t t = g.lo * static_cast<int32_t>(w.tile); t < min(g.hi * static_cast<int32_t>(w.tile), u.s.length); ++t) {
+        const int32_t page = page_of(c.cache, u.seq, t >> c.cache.page_shift);
+        if (static_cast<uint32_t>(page) >= c.cache.n_pages) continue;
+        const uint8_t* v = c.cache.v + page * c.cache.page_stride + (uint64_t{u.head} * c.cache.page_tokens + (t & (c.cache.page_tokens - 1))) * dim;
+        for (uint32_t d = threadIdx.x; d < dim; d += threads) {
+            if ((v[d] & 127) != 127) continue;
+            for (uint32_t r = 0; r < rows; ++r) {
+                const uint32_t j = (r0 + r) / c.group;
+                if (t >= first_key(u.s, w.window, j) && t < end_key(u.s, c.causal, j)) at(r, d);
+            }
+        }
+    }
+}
+
+/// Joins the shares of a unit in CTA order and stores its rows.  All `threads` of the caller take part.
+template <class T, int D>
+__device__ void join_partials(const AttentionCall& c, const Work& w, const Unit& u, const Segment& g, uint64_t total, uint32_t threads) {
+    const uint32_t n = gridDim.x, c0 = owner(g.unit_begin, total, n), c1 = owner(g.unit_end - 1, total, n);
+    const uint32_t shares = total >= n ? c1 - c0 + 1 : static_cast<uint32_t>(g.unit_end - g.unit_begin);
+    const uint32_t rows = u.rows(w), r0 = u.row0(w);
+    auto slot = [&](uint32_t i) { return partial_slot(w, D, total >= n ? c0 + i : owner(g.unit_begin + i, total, n), i == 0); };
+    for (uint32_t i = threadIdx.x; i < rows * (D / 4); i += threads) {
+        const uint32_t r = i / (D / 4), d = i % (D / 4) * 4;
+        float m = -INFINITY;
+        for (uint32_t k = 0; k < shares; ++k) m = fmaxf(m, __ldcg(slot(k) + w.rows * D + 2 * r));
+        float4 o = make_float4(0, 0, 0, 0);
+        float l = 0;
+        for (uint32_t k = 0; k < shares; ++k) {
+            const float* s = slot(k);
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(s + w.rows * D + 2 * r));
+            const float4 x = __ldcg(reinterpret_cast<const float4*>(s + r * D + d));
+            const float f = ml.x == -INFINITY ? 1.0f : exp2_approx(ml.x - m);  // without a maximum sum and row are zero, or NaN
+            l += f * ml.y;
+            // a share of weight zero adds nothing, but a NaN among its rows is one of a token that the row sees
+            o.x += f * x.x, o.y += f * x.y, o.z += f * x.z, o.w += f * x.w;
+        }
+        const float inv = l != 0 ? 1.0f / l : 0.0f;
+        const uint32_t j = (r0 + r) / c.group, h = u.head * c.group + (r0 + r) % c.group;
+        T* out = reinterpret_cast<T*>(c.out.p + uint64_t{u.s.row0 + j} * c.out.token_stride + uint64_t{h} * c.out.head_stride) + d;
+        out[0] = from_f32<T>(o.x * inv), out[1] = from_f32<T>(o.y * inv), out[2] = from_f32<T>(o.z * inv), out[3] = from_f32<T>(o.w * inv);
+    }
+}
+
+template <class T, int D, int TS, int RG, int CPS>
+__global__ void __launch_bounds__(RowsShape<D, TS, RG, CPS, sizeof(T) == 4 ? 2 : 1>::kThreads, CPS)
+    rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const __grid_constant__ AttentionCall c,
+                const __grid_constant__ Work w) {
+    constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;
+    using S = RowsShape<D, TS, RG, CPS, TERMS>;
+    constexpr int kParts = D > 128 ? D / 128 : 1, kPartDim = D / kParts;  // 128-byte columns of a tile
+    constexpr int kChunk = kPartDim / 8;                                  // dims of a lane group in a part: 16, or 8
+    constexpr int NT = kRowsTile / TS / 8;                                // blocks of 8 tokens of a warp
+    constexpr bool kKeepQ = TERMS == 1 && D <= 128;                       // a row group's q in registers
+    extern __shared__ uint8_t raw_smem[];
+    __shared__ PlanSmem plan;
+    __shared__ uint64_t bars[2 * S::kStages];
+    __shared__ GroupScale scales[S::kStages][kGroups];
+    __shared__ uint32_t partly[S::kStages];  // a page of the stage's tile is missing
+    __shared__ float2 row_ml[RG][TS][16];
+    __shared__ float q_unscale[S::kRows];
+    __shared__ uint32_t nan_seen, is_last;
+
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;");
+    const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    const uint32_t smem = (smem_u32(raw_smem) + 1023u) & ~1023u;
+    const uint32_t ring = smem, q_at = smem + S::kStages * S::kStage;
+    float* join = reinterpret_cast<float*>(raw_smem + (smem - smem_u32(raw_smem)) + S::kStages * S::kStage + S::kQ);
+    const uint32_t full = smem_u32(bars), empty = full + 8 * S::kStages;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < S::kStages; ++i) {
+            mbar_init(full + 8 * i, 1);
+            mbar_init(empty + 8 * i, S::kWarps);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        nan_seen = 0;
+    }
+    Range range;
+    if (!find_range(c, w, plan, &range)) return;  // (its barriers order the initialisation above)
+    __syncthreads();
+    Unit u = range.unit;
+    uint64_t unit_begin = range.unit_begin;
+    uint32_t stage = 0, parity = 0;
+    bool alive = true;  // no wait has run out
+    auto advance = [&] {
+        if (++stage == S::kStages) stage = 0, parity ^= 1;
+    };
+
+    if (warp == S::kWarps) {
+        // ---- producer --------------------------------------------------------------------------------------------------------------
+        const uint32_t page_rows = min(c.cache.page_tokens, kRowsTile), boxes = kRowsTile / page_rows;
+        const float scale = c.scale * 1.4426950408889634f;
+        uint32_t issued = 0;
+        for (uint64_t pos = range.begin; pos < range.end;) {
+            const Segment g = segment(range, u, unit_begin);
+            const int32_t first = first_key(u.s, w.window, u.row0(w) / c.group), end = end_key(u.s, c.causal, (u.row0(w) + u.rows(w) - 1) / c.group);
+            // a lane knows the page and the scales of one group of 16 tokens: eight tiles at a time, the next eight on their way
+            int32_t page_next = -1;
+            uint32_t kb_next = 0, vb_next = 0;
+            auto fetch = [&](int32_t tile) {
+                const int32_t t = tile * static_cast<int32_t>(kRowsTile) + static_cast<int32_t>(lane) * 16;
+                page_next = -1;
+                if (t < end && t + 16 > first && tile + static_cast<int32_t>(lane / kGroups) < g.hi) {
+                    const int32_t p = page_of(c.cache, u.seq, t >> c.cache.page_shift);
+                    if (static_cast<uint32_t>(p) < c.cache.n_pages) {
+                        page_next = p;
+                        const uint64_t at = p * c.cache.scale_stride + u.head;
+                        kb_next = __ldg(c.cache.k_scale + at);
+                        vb_next = __ldg(c.cache.v_scale + at);
+                    } else {
+                        page_next = -2;  // a visible token's page is not there
+                    }
+                }
+            };
+            fetch(g.lo);
+            for (int32_t base = g.lo; base < g.hi; base += 32 / kGroups) {
+                const int32_t page = page_next;
+                const float k = exp2_int(scale_byte(kb_next) - 127) * scale;
+                const int32_t v = scale_byte(vb_next) - 127;
+                if (base + 32 / static_cast<int32_t>(kGroups) < g.hi) fetch(base + 32 / kGroups);
+                if (page == -2 && c.status != nullptr) atomicOr(c.status, 8u);  // kStatusBadIndex
+                for (int32_t tile = base; tile < min(base + static_cast<int32_t>(32 / kGroups), g.hi); ++tile) {
+                    if (alive) alive = __all_sync(0xFFFFFFFFu, mbar_wait(empty + 8 * stage, parity ^ 1));
+                    if (!alive) break;
+                    const uint32_t in_tile = (tile - base) * kGroups;
+                    if (lane >= in_tile && lane < in_tile + kGroups) {
+                        GroupScale& s = scales[stage][lane - in_tile];
+                        s.k = page >= 0 ? k : 0.0f;
+                        s.log_v = page >= 0 ? static_cast<float>(v) : -INFINITY;
+                        s.inv_v = page >= 0 ? exp2_int(-v) : 0.0f;
+                    }
+                    const uint32_t here = __ballot_sync(0xFFFFFFFFu, page >= 0) >> in_tile & ((1u << kGroups) - 1);
+                    if (lane == 0) partly[stage] = here != (1u << kGroups) - 1;
+                    const uint32_t step = page_rows / 16;  // groups of a box
+                    uint32_t present = 0;
+                    for (uint32_t b = 0; b < boxes; ++b) present += here >> (b * step) & ((1u << step) - 1) ? 1 : 0;
+                    __syncwarp();
+                    if (elect_one()) mbar_expect(full + 8 * stage, present * page_rows * D * 2);
+                    for (uint32_t b = 0; b < boxes; ++b) {
+                        const uint32_t of = here >> (b * step) & ((1u << step) - 1);
+                        if (of == 0) continue;
+                        const int32_t p = __shfl_sync(0xFFFFFFFFu, page, in_tile + b * step + __ffs(of) - 1);
+                        const int32_t t = tile * static_cast<int32_t>(kRowsTile) + static_cast<int32_t>(b * page_rows);
+                        const int32_t y = static_cast<int32_t>(u.head * c.cache.page_tokens) + (t & static_cast<int32_t>(c.cache.page_tokens - 1));
+                        if (elect_one()) {
+                            const uint32_t dst = ring + stage * S::kStage + b * page_rows * kPartDim;
+#pragma unroll
+                            for (int part = 0; part < kParts; ++part) {
+                                tma_3d(dst + part * kRowsTile * kPartDim, &k_map, part * 128, y, p, full + 8 * stage);
+                                tma_3d(dst + S::kHalfTile + part * kRowsTile * kPartDim, &v_map, part * 128, y, p, full + 8 * stage);
+                            }
+                        }
+                    }
+                    ++issued;
+                    advance();
+                }
+                if (!alive) break;
+            }
+            pos = g.to_end ? g.unit_end : range.end;
+            unit_begin = g.unit_end;
+            if (!alive || pos >= range.end || !next_unit(c, w, u)) break;
+        }
+        if (!alive) {
+            if (lane == 0) atomicOr(w.error_word, 1u);
+            // nothing may land in this CTA's shared memory once it is gone
+            for (uint32_t i = 0; i < min(issued, static_cast<uint32_t>(S::kStages)); ++i) {
+                stage = stage == 0 ? S::kStages - 1 : stage - 1;
+                if (stage == S::kStages - 1) parity ^= 1;
+                mbar_wait(full + 8 * stage, parity);
+            }
+        }
+        __syncthreads();
+        return;
+    }
+
+    // ---- consumers -------------------------------------------------------------------------------------------------------------------
+    constexpr uint32_t kConsumers = S::kWarps * 32;
+    const uint32_t rg = warp / TS, ts = warp % TS, g8 = lane / 4, t4 = lane % 4;
+    const uint32_t my_q = q_at + rg * (D / 16) * TERMS * 512 + lane * 16;
+    auto tau = [](uint32_t n) { return n ^ ((n & 1) << 2); };  // token of column n of a block of 8: spreads a quarter warp's reads over the banks
+    for (uint64_t pos = range.begin; pos < range.end;) {
+        const Segment g = segment(range, u, unit_begin);
+        const uint32_t rows = u.rows(w), r0 = u.row0(w);
+        // q: a warp takes a row at a time, scales it and stores its fp16 terms in the order of the products' operands
+        bar_sync(1, kConsumers);  // the q of the segment before is no longer read
+        for (uint32_t r = warp; r < S::kRows; r += S::kWarps) {
+            constexpr int E = D / 32;
+            float x[E];
+            float top = 0;
+            if (r < rows) {
+                const uint32_t j = (r0 + r) / c.group, h = u.head * c.group + (r0 + r) % c.group;
+                const T* q = reinterpret_cast<const T*>(c.q.p + uint64_t{u.s.row0 + j} * c.q.token_stride + uint64_t{h} * c.q.head_stride) + lane * E;
+                if (c.q.vec) {
+                    constexpr int kBytes = E * sizeof(T) < 16 ? E * sizeof(T) : 16, kPer = kBytes / sizeof(T);
+#pragma unroll
+                    for (int e = 0; e < E; e += kPer) {
+                        T v[kPer];
+                        if constexpr (kBytes == 16) *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(q + e);
+                        else if constexpr (kBytes == 8) *reinterpret_cast<uint2*>(v) = *reinterpret_cast<const uint2*>(q + e);
+                        else *reinterpret_cast<uint32_t*>(v) = *reinterpret_cast<const uint32_t*>(q + e);
+#pragma unroll
+                        for (int i = 0; i < kPer; ++i) x[e + i] = to_f32(v[i]);
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < E; ++e) x[e] = to_f32(q[e]);
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < E; ++e) x[e] = 0;
+            }
+#pragma unroll
+            for (int e = 0; e < E; ++e) top = fmaxf(top, fabsf(x[e]) < INFINITY ? fabsf(x[e]) : 0.0f);
+#pragma unroll
+            for (int d = 16; d != 0; d /= 2) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+            const int32_t exponent = max(static_cast<int32_t>(__float_as_uint(top) >> 23) - 127, -100);
+            const float by = exp2_int(14 - exponent);
+            if (lane == 0) q_unscale[r] = exp2_int(exponent - 14);
+#pragma unroll
+            for (int e = 0; e < E; e += 2) {
+                // dim 64 a + 16 t + 4 s + 2 p + {0, 1}: k step 4 a + s, lane t of a quad, register 2 p (+ 1 for the rows 8 and up)
+                const uint32_t d = lane * E + e, step = d / 64 * 4 + d % 16 / 4, t = d % 64 / 16, p = d % 4 / 2;
+                const uint32_t at = q_at + (r / 16) * (D / 16) * TERMS * 512 + step * TERMS * 512 + (r % 8 * 4 + t) * 16 + (2 * p + r / 8 % 2) * 4;
+                const float a = x[e] * by, b = x[e + 1] * by;
+                const uint32_t hi = half2_bits(a, b);
+                asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(hi) : "memory");
+                if constexpr (TERMS == 2) asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + 512), "r"(half2_rest(a, b, hi)) : "memory");
+            }
+        }
+        bar_sync(1, kConsumers);
+        uint4 q_reg[kKeepQ ? D / 16 : 1];
+        if constexpr (kKeepQ) {
+#pragma unroll
+            for (int s = 0; s < D / 16; ++s) q_reg[s] = lds128(my_q + s * 512);
+        }
+        // this lane's rows of the accumulators: g8 and g8 + 8 of the group
+        int32_t lo[2], hi[2];
+        float qs[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t r = rg * 16 + g8 + 8 * i, j = (r0 + min(r, rows - 1)) / c.group;
+            lo[i] = first_key(u.s, w.window, j);
+            hi[i] = end_key(u.s, c.causal, j);
+            qs[i] = q_unscale[r];
+        }
+        // tiles that every row sees whole, and what any row sees
+        const int32_t all_lo = first_key(u.s, w.window, (r0 + rows - 1) / c.group), all_hi = end_key(u.s, c.causal, r0 / c.group);
+        const int32_t any_lo = first_key(u.s, w.window, r0 / c.group), any_hi = end_key(u.s, c.causal, (r0 + rows - 1) / c.group);
+
+        float o[kParts][kChunk][4];
+#pragma unroll
+        for (int a = 0; a < kParts; ++a)
+#pragma unroll
+            for (int b = 0; b < kChunk; ++b) o[a][b][0] = o[a][b][1] = o[a][b][2] = o[a][b][3] = 0;
+        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0, 0};
+
+        for (int32_t tile = g.lo; tile < g.hi; ++tile) {
+            if (alive) alive = __all_sync(0xFFFFFFFFu, mbar_wait(full + 8 * stage, parity));
+            const uint32_t k_at = ring + stage * S::kStage, v_at = k_at + S::kHalfTile;
+            const uint32_t tok = ts * (NT * 8);  // this warp's first token of the tile
+            const int32_t t0 = tile * static_cast<int32_t>(kRowsTile);
+            float x[NT][4];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) x[n][0] = x[n][1] = x[n][2] = x[n][3] = 0;
+#pragma unroll
+            for (int a = 0; a < D / 64; ++a) {
+                uint4 kw[NT];
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+                    kw[n] = lds128(k_at + (D > 64 ? a / 2 * kRowsTile * 128 : 0) + swizzled(tok + 8 * n + tau(g8), (D > 64 ? a % 2 * 4 : 0) + t4, D));
+#pragma unroll
+                for (int s = 0; s < 4; ++s) {
+                    uint4 q[TERMS];
+                    if constexpr (kKeepQ) q[0] = q_reg[a * 4 + s];
+                    else {
+#pragma unroll
+                        for (int term = 0; term < TERMS; ++term) q[term] = lds128(my_q + ((a * 4 + s) * TERMS + term) * 512);
+                    }
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        const uint32_t word = s == 0 ? kw[n].x : s == 1 ? kw[n].y : s == 2 ? kw[n].z : kw[n].w;
+                        const uint32_t b0 = widen_lo(word), b1 = widen_hi(word);
+#pragma unroll
+                        for (int term = 0; term < TERMS; ++term) mma16816(x[n], q[term].x, q[term].y, q[term].z, q[term].w, b0, b1);
+                    }
+                }
+            }
+            const bool masked = t0 < all_lo || t0 + static_cast<int32_t>(kRowsTile) > all_hi || partly[stage] != 0;
+            float top[2] = {-INFINITY, -INFINITY}, inv[NT];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const GroupScale s = scales[stage][(tok + 8 * n) / 16];
+                inv[n] = s.inv_v;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float by = s.k * qs[i];
+                    x[n][2 * i] = fmaf(x[n][2 * i], by, s.log_v);
+                    x[n][2 * i + 1] = fmaf(x[n][2 * i + 1], by, s.log_v);
+                }
+                if (masked) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int32_t t = t0 + static_cast<int32_t>(tok + 8 * n + tau(2 * t4 + e % 2));
+                        if (t < lo[e / 2] || t >= hi[e / 2] || s.log_v == -INFINITY) x[n][e] = -INFINITY;
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 2; ++i) top[i] = fmaxf(top[i], fmaxf(x[n][2 * i], x[n][2 * i + 1]));
+            }
+            bool grows = false;
+            float fade[2], base[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                top[i] = fmaxf(top[i], __shfl_xor_sync(0xFFFFFFFFu, top[i], 1));
+                top[i] = fmaxf(top[i], __shfl_xor_sync(0xFFFFFFFFu, top[i], 2));
+                const float next = fmaxf(m[i], top[i]);
+                grows |= next > m[i];
+                fade[i] = m[i] == -INFINITY ? 1.0f : exp2_approx(m[i] - next);  // without a maximum sum and row are zero, or NaN
+                m[i] = next;
+                base[i] = next == -INFINITY ? 0.0f : next - 14.0f;
+            }
+            if (__any_sync(0xFFFFFFFFu, grows)) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    l[i] *= fade[i];
+#pragma unroll
+                    for (int a = 0; a < kParts; ++a)
+#pragma unroll
+                        for (int b = 0; b < kChunk; ++b) o[a][b][2 * i] *= fade[i], o[a][b][2 * i + 1] *= fade[i];
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[n][e] = exp2_approx(x[n][e] - base[e / 2]);
+                l[0] = fmaf(x[n][0] + x[n][1], inv[n], l[0]);
+                l[1] = fmaf(x[n][2] + x[n][3], inv[n], l[1]);
+            }
+            bool nan = false;
+#pragma unroll
+            for (int s = 0; s < NT / 2; ++s) {
+                uint32_t p[TERMS][4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float a = x[2 * s + i / 2][i % 2 * 2], b = x[2 * s + i / 2][i % 2 * 2 + 1];
+                    p[0][i] = half2_bits(a, b);
+                    if constexpr (TERMS == 2) p[1][i] = half2_rest(a, b, p[0][i]);
+                }
+                uint32_t row[4];  // the tokens of b0's and b1's halves
+#pragma unroll
+                for (int i = 0; i < 4; ++i) row[i] = tok + 16 * s + 8 * (i / 2) + tau(2 * t4 + i % 2);
+#pragma unroll
+                for (int a = 0; a < kParts; ++a) {
+                    uint32_t vw[4][kChunk / 4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if constexpr (D > 64) {
+                            const uint4 v = lds128(v_at + a * kRowsTile * 128 + swizzled(row[i], g8, D));
+                            vw[i][0] = v.x, vw[i][1] = v.y, vw[i][2] = v.z, vw[i][3] = v.w;
+                        } else {
+                            const uint2 v = lds64(v_at + swizzled(row[i], g8 / 2, D) + g8 % 2 * 8);
+                            vw[i][0] = v.x, vw[i][1] = v.y;
+                        }
+                    }
+                    if (masked) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int32_t t = t0 + static_cast<int32_t>(row[i]);
+                            const bool held = t >= any_lo && t < any_hi && scales[stage][row[i] / 16].log_v != -INFINITY;
+#pragma unroll
+                            for (int b = 0; b < kChunk / 4; ++b) {
+                                if (!held) vw[i][b] = 0;
+                                nan |= drop_nan(vw[i][b]);
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int b = 0; b < kChunk / 4; ++b) {
+                        const uint32_t l0 = __byte_perm(vw[0][b], vw[1][b], 0x5140), h0 = __byte_perm(vw[0][b], vw[1][b], 0x7362);
+                        const uint32_t l1 = __byte_perm(vw[2][b], vw[3][b], 0x5140), h1 = __byte_perm(vw[2][b], vw[3][b], 0x7362);
+                        const uint32_t b0[4] = {widen_lo(l0), widen_hi(l0), widen_lo(h0), widen_hi(h0)};
+                        const uint32_t b1[4] = {widen_lo(l1), widen_hi(l1), widen_lo(h1), widen_hi(h1)};
+#pragma unroll
+                        for (int d = 0; d < 4; ++d)
+#pragma unroll
+                            for (int term = 0; term < TERMS; ++term) mma16816(o[a][4 * b + d], p[term][0], p[term][1], p[term][2], p[term][3], b0[d], b1[d]);
+                    }
+                }
+            }
+            if (nan) nan_seen = 1;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(empty + 8 * stage);
+            advance();
+        }
+
+        // ---- the segment's rows: joined over the group's warps, then stored or left in scratch ---------------------------------------------------
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            l[i] += __shfl_xor_sync(0xFFFFFFFFu, l[i], 1);
+            l[i] += __shfl_xor_sync(0xFFFFFFFFu, l[i], 2);
+        }
+        float* slot = g.whole() ? nullptr : partial_slot(w, D, blockIdx.x, g.from_start);
+        auto out_at = [&](uint32_t r) {
+            const uint32_t j = (r0 + r) / c.group, h = u.head * c.group + (r0 + r) % c.group;
+            return reinterpret_cast<T*>(c.out.p + uint64_t{u.s.row0 + j} * c.out.token_stride + uint64_t{h} * c.out.head_stride);
+        };
+        if constexpr (TS > 1) {
+            if (t4 == 0) row_ml[rg][ts][g8] = make_float2(m[0], l[0]), row_ml[rg][ts][g8 + 8] = make_float2(m[1], l[1]);
+            bar_sync(1, kConsumers);
+            float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0, 0}, f[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                for (int k = 0; k < TS; ++k) top[i] = fmaxf(top[i], row_ml[rg][k][g8 + 8 * i].x);
+#pragma unroll
+                for (int k = 0; k < TS; ++k) {
+                    const float2 ml = row_ml[rg][k][g8 + 8 * i];
+                    sum[i] += ml.x == -INFINITY ? ml.y : exp2_approx(ml.x - top[i]) * ml.y;
+                }
+                f[i] = m[i] == -INFINITY ? 1.0f : exp2_approx(m[i] - top[i]);
+            }
+            float* mine = join + rg * 16 * D;
+            for (int k = 0; k < TS; ++k) {
+                if (ts == static_cast<uint32_t>(k)) {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int a = 0; a < kParts; ++a)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                                for (int b = 0; b < kChunk; ++b) {
+                                    // a part's dim (2 t4 + e) * kChunk + b, kept at a place that spreads the lanes over the banks
+                                    float* at = mine + (g8 + 8 * i) * D + a * kPartDim + b * 8 + ((2 * t4 + e + g8) & 7);
+                                    const float v = o[a][b][2 * i + e] * f[i];
+                                    *at = k == 0 ? v : *at + v;
+                                }
+                }
+                bar_sync(1, kConsumers);
+            }
+            if (ts == 0 && t4 == 0) row_ml[rg][0][g8] = make_float2(top[0], sum[0]), row_ml[rg][0][g8 + 8] = make_float2(top[1], sum[1]);
+            bar_sync(1, kConsumers);
+            for (uint32_t i = threadIdx.x; i < rows * D; i += kConsumers) {
+                const uint32_t r = i / D, d = i % D, a = d / kPartDim, n = d % kPartDim / kChunk, b = d % kChunk;
+                const float v = join[r * D + a * kPartDim + b * 8 + ((n + r) & 7)];
+                const float sum_r = row_ml[r / 16][0][r % 16].y;
+                if (slot == nullptr) out_at(r)[d] = from_f32<T>(sum_r != 0 ? v / sum_r : 0.0f);
+                else slot[r * D + d] = v;
+            }
+            if (slot != nullptr)
+                for (uint32_t r = threadIdx.x; r < rows; r += kConsumers) *reinterpret_cast<float2*>(slot + w.rows * D + 2 * r) = row_ml[r / 16][0][r % 16];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const uint32_t r = rg * 16 + g8 + 8 * i;
+                if (r >= rows) continue;
+                const float inv = l[i] != 0 ? 1.0f / l[i] : 0.0f;
+#pragma unroll
+                for (int a = 0; a < kParts; ++a)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+#pragma unroll
+                        for (int b = 0; b < kChunk; b += 4) {
+                            const uint32_t d = a * kPartDim + (2 * t4 + e) * kChunk + b;
+                            if (slot != nullptr) {
+                                *reinterpret_cast<float4*>(slot + r * D + d) =
+                                    make_float4(o[a][b][2 * i + e], o[a][b + 1][2 * i + e], o[a][b + 2][2 * i + e], o[a][b + 3][2 * i + e]);
+                            } else {
+                                T* out = out_at(r) + d;
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) out[k] = from_f32<T>(o[a][b + k][2 * i + e] * inv);
+                            }
+                        }
+                if (slot != nullptr && t4 == 0) *reinterpret_cast<float2*>(slot + w.rows * D + 2 * r) = make_float2(m[i], l[i]);
+            }
+        }
+        bar_sync(1, kConsumers);
+        if (nan_seen != 0) {
+            spread_nan(c, w, u, g, kConsumers, [&](uint32_t r, uint32_t d) {
+                if (slot == nullptr) out_at(r)[d] = from_f32<T>(NAN);
+                else slot[r * D + d] = NAN;
+            });
+            bar_sync(1, kConsumers);
+            if (threadIdx.x == 0) nan_seen = 0;
+        }
+        if (slot != nullptr) {
+            const uint32_t n = gridDim.x, c0 = owner(g.unit_begin, range.total, n), c1 = owner(g.unit_end - 1, range.total, n);
+            const uint32_t shares = range.total >= n ? c1 - c0 + 1 : u.span.tiles();
+            __threadfence();
+            bar_sync(1, kConsumers);
+            if (threadIdx.x == 0) {
+                const bool last = atomicAdd(w.counters + c0, 1u) == shares - 1;
+                if (last) w.counters[c0] = 0;
+                is_last = last;
+            }
+            bar_sync(1, kConsumers);
+            if (is_last != 0) {
+                __threadfence();
+                join_partials<T, D>(c, w, u, g, range.total, kConsumers);
+            }
+        }
+        pos = g.to_end ? g.unit_end : range.end;
+        unit_begin = g.unit_end;
+        if (pos >= range.end || !next_unit(c, w, u)) break;
+    }
+    if (!alive && lane == 0) atomicOr(w.error_word, 1u);
+    __syncthreads();
+}
+
+/// The cache's pool as {dim, rows of all heads of a page, pages}, a box of one page's rows of one head.
+int pool_map(const Cache& c, const uint8_t* pool, uint32_t box_rows, CUtensorMap* out);
+
+template <class T, int D, int TS, int RG, int CPS>
+int launch_rows_kernel(HaloCudaCtx* ctx, const AttentionCall& c, Work w, cudaStream_t s) {
+    using S = RowsShape<D, TS, RG, CPS, sizeof(T) == 4 ? 2 : 1>;
+    w.rows = S::kRows;
+    w.tile = kRowsTile;
+    w.row_tiles = (c.rows.max_tokens * c.group + S::kRows - 1) / S::kRows;
+    w.lanes = 1;
+    while (w.lanes < 32 && w.lanes < w.row_tiles) w.lanes *= 2;
+    CUtensorMap k_map, v_map;
+    const uint32_t box = std::min(c.cache.page_tokens, kRowsTile);
+    if (int rc = pool_map(c.cache, c.cache.k, box, &k_map)) return rc;
+    if (int rc = pool_map(c.cache, c.cache.v, box, &v_map)) return rc;
+    const uint32_t ctas = CPS * static_cast<uint32_t>(ctx->prop.multiProcessorCount);
+    void* p = nullptr;
+    if (int rc = workspace(ctx, 5, ctas * sizeof(uint32_t), s, &p, true)) return rc;
+    w.counters = static_cast<uint32_t*>(p);
+    if (int rc = workspace(ctx, 6, partial_bytes(S::kRows, D, ctas), s, &p)) return rc;
+    w.partials = static_cast<float*>(p);
+    w.error_word = ctx->error_word_dev;
+    auto kernel = rows_kernel<T, D, TS, RG, CPS>;
+    if (int rc = allow_dynamic_smem(ctx, reinterpret_cast<const void*>(kernel), S::kSmem)) return rc;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(ctas);
+    cfg.blockDim = dim3(S::kThreads);
+    cfg.dynamicSmemBytes = S::kSmem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    HC_CUDA(cudaLaunchKernelEx(&cfg, kernel, k_map, v_map, c, w));
+    return 0;
+}
+
+/// One of the kernels above by operand type; instantiated for each head size in a file of its own.
+template <int D>
+int launch_rows(HaloCudaCtx* ctx, const AttentionCall& c, const Work& w, cudaStream_t s);
+
+}  // namespace attn
+}  // namespace halo_cuda

@@ -1,0 +1,19 @@
+// Which of the row kernels a launch takes.  Internal.
+#pragma once
+#include "attention_rows.cuh"
+
+namespace halo_cuda {
+namespace attn {
+
+template <int D>
+int launch_rows(HaloCudaCtx* ctx, const AttentionCall& c, const Work& w, cudaStream_t s) {
+    return with_type(c.type, [&](auto t) {
+        using T = decltype(t);
+        if (w.max_rows <= 16) return launch_rows_kernel<T, D, 4, 1, 2>(ctx, c, w, s);
+        if (w.max_rows <= 32) return launch_rows_kernel<T, D, 4, 2, 1>(ctx, c, w, s);
+        return launch_rows_kernel<T, D, 2, 4, 1>(ctx, c, w, s);
+    });
+}
+
+}  // namespace attn
+}  // namespace halo_cuda

@@ -15,9 +15,10 @@ struct ScratchBlock {
 
 /// Slot 0 serves the matmul kernels (staged x), slot 1 the LM head (its logits and argmax partials live across a matmul), slot 2 the row-block
 /// counters of the balanced kernels (zeroed when allocated, left zeroed by every kernel), slot 3 their partial sums, slot 4 the partial sums of
-/// the prefill GEMM's K splits (its own, so that a prompt that cannot have them leaves what a decode step needs).
+/// the prefill GEMM's K splits (its own, so that a prompt that cannot have them leaves what a decode step needs), slots 5 and 6 the attention's
+/// counters (zeroed when allocated, left zeroed by every kernel) and its shares of units that several CTAs walk.
 struct Scratch {
-    static constexpr int kSlots = 5;
+    static constexpr int kSlots = 7;
     ScratchBlock block[kSlots];
     std::vector<ScratchBlock> kept;  // outgrown blocks whose address a graph holds: they live as long as the stream's scratch
 
