@@ -37,7 +37,8 @@ struct RowsShape {
     static constexpr uint32_t kHalfTile = kRowsTile * D;  // K or V of a tile
     static constexpr uint32_t kStage = 2 * kHalfTile;
     static constexpr uint32_t kQ = RG * (D / 16) * TERMS * 512;
-    static constexpr uint32_t kJoin = TS > 1 ? RG * 16 * D * 4 : 0;
+    static constexpr uint32_t kJoinRow = D + D / 8 + (D == 256 ? 16 : 0);  // floats of a row of the warps' joined rows
+    static constexpr uint32_t kJoin = RG * 16 * kJoinRow * 4;
     static constexpr uint32_t kFixed = 1024 + kQ + kJoin;  // alignment, q, the warps' joined rows
     // an SM's 228 KiB, less 1 KiB a CTA for the system and 3 KiB for what is declared in the kernel
     static constexpr uint32_t kStagesRoom = (228 / CPS * 1024 - 4096 - kFixed) / kStage;
@@ -108,34 +109,71 @@ __device__ void spread_nan(const AttentionCall& c, const Work& w, const Unit& u,
     }
 }
 
-/// Joins the shares of a unit in CTA order and stores its rows.  All `threads` of the caller take part.
+/// Joins the shares of a unit in CTA order and stores its rows.  All `warps` of the caller take part, each with a row's 128 dims (or 64) at a time.
 template <class T, int D>
-__device__ void join_partials(const AttentionCall& c, const Work& w, const Unit& u, const Segment& g, uint64_t total, uint32_t threads) {
-    const uint32_t n = gridDim.x, c0 = owner(g.unit_begin, total, n), c1 = owner(g.unit_end - 1, total, n);
-    const uint32_t shares = total >= n ? c1 - c0 + 1 : static_cast<uint32_t>(g.unit_end - g.unit_begin);
-    const uint32_t rows = u.rows(w), r0 = u.row0(w);
-    auto slot = [&](uint32_t i) { return partial_slot(w, D, total >= n ? c0 + i : owner(g.unit_begin + i, total, n), i == 0); };
-    for (uint32_t i = threadIdx.x; i < rows * (D / 4); i += threads) {
-        const uint32_t r = i / (D / 4), d = i % (D / 4) * 4;
-        float m = -INFINITY;
-        for (uint32_t k = 0; k < shares; ++k) m = fmaxf(m, __ldcg(slot(k) + w.rows * D + 2 * r));
-        float4 o = make_float4(0, 0, 0, 0);
-        float l = 0;
-        for (uint32_t k = 0; k < shares; ++k) {
-            const float* s = slot(k);
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(s + w.rows * D + 2 * r));
-            const float4 x = __ldcg(reinterpret_cast<const float4*>(s + r * D + d));
-            const float f = ml.x == -INFINITY ? 1.0f : exp2_approx(ml.x - m);  // without a maximum sum and row are zero, or NaN
-            l += f * ml.y;
-            // a share of weight zero adds nothing, but a NaN among its rows is one of a token that the row sees
-            o.x += f * x.x, o.y += f * x.y, o.z += f * x.z, o.w += f * x.w;
+__device__ __forceinline__ void join_partials(const AttentionCall& c, const Work& w, uint32_t seq_row0, uint32_t head, uint32_t r0, uint32_t rows, uint32_t c0, uint32_t shares,
+                                              uint32_t warps) {
+    constexpr uint32_t kPerLane = D < 128 ? 2 : 4, kParts = D / (32 * kPerLane), kAhead = 8;  // shares whose loads are under way together
+    using Word = std::conditional_t<kPerLane == 4, float4, float2>;
+    const uint32_t lane = threadIdx.x % 32;
+#pragma unroll 1
+    for (uint32_t i = threadIdx.x / 32; i < rows * kParts; i += warps) {
+        const uint32_t r = i / kParts, d = (i % kParts * 32 + lane) * kPerLane;
+        float m = -INFINITY, l = 0, o[kPerLane] = {};
+#pragma unroll 1
+        for (uint32_t k0 = 0; k0 < shares; k0 += kAhead) {
+            // every lane holds one share's maximum and sum; behind the last share the last one again, with weight zero
+            const uint32_t mine = min(k0 + lane % kAhead, shares - 1);
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(partial_slot(w, D, c0 + mine, mine == 0) + w.rows * D + 2 * r));
+            Word x[kAhead];
+#pragma unroll
+            for (uint32_t k = 0; k < kAhead; ++k) {
+                const uint32_t at = min(k0 + k, shares - 1);
+                x[k] = __ldcg(reinterpret_cast<const Word*>(partial_slot(w, D, c0 + at, at == 0) + r * D + d));
+            }
+            float top = fmaxf(m, ml.x);
+#pragma unroll
+            for (uint32_t s = kAhead / 2; s != 0; s /= 2) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, s));
+            // without a maximum sum and row are zero, or NaN; a share of weight zero adds nothing, but a NaN in it is one of a token that the row sees
+            const float fade = m == -INFINITY ? 1.0f : exp2_approx(m - top);
+            const float f = k0 + lane % kAhead >= shares ? 0.0f : ml.x == -INFINITY ? 1.0f : exp2_approx(ml.x - top);
+            m = top;
+            l *= fade;
+#pragma unroll
+            for (uint32_t e = 0; e < kPerLane; ++e) o[e] *= fade;
+#pragma unroll
+            for (uint32_t k = 0; k < kAhead; ++k) {
+                const float fk = __shfl_sync(0xFFFFFFFFu, f, k);
+                l += fk * __shfl_sync(0xFFFFFFFFu, ml.y, k);
+                o[0] += fk * x[k].x, o[1] += fk * x[k].y;
+                if constexpr (kPerLane == 4) o[2] += fk * x[k].z, o[3] += fk * x[k].w;
+            }
         }
         const float inv = l != 0 ? 1.0f / l : 0.0f;
-        const uint32_t j = (r0 + r) / c.group, h = u.head * c.group + (r0 + r) % c.group;
-        T* out = reinterpret_cast<T*>(c.out.p + uint64_t{u.s.row0 + j} * c.out.token_stride + uint64_t{h} * c.out.head_stride) + d;
-        out[0] = from_f32<T>(o.x * inv), out[1] = from_f32<T>(o.y * inv), out[2] = from_f32<T>(o.z * inv), out[3] = from_f32<T>(o.w * inv);
+        const uint32_t j = (r0 + r) / c.group, h = head * c.group + (r0 + r) % c.group;
+        T* out = reinterpret_cast<T*>(c.out.p + uint64_t{seq_row0 + j} * c.out.token_stride + uint64_t{h} * c.out.head_stride) + d;
+#pragma unroll
+        for (uint32_t e = 0; e < kPerLane; ++e) out[e] = from_f32<T>(o[e] * inv);
     }
 }
+
+/// Where a CTA's consumers are: in shared memory, so that the walk over the tiles has the registers.
+struct Walk {
+    Range range;
+    Unit u;
+    Segment g;
+    uint32_t rows, r0;  // of the unit
+    uint32_t more;
+    __device__ void enter(const Work& w, uint64_t unit_begin) {
+        g = segment(range, u, unit_begin);
+        rows = u.rows(w), r0 = u.row0(w);
+        more = 1;
+    }
+    __device__ void advance(const AttentionCall& c, const Work& w) {
+        more = g.unit_end < range.end && next_unit(c, w, u);
+        if (more) enter(w, g.unit_end);
+    }
+};
 
 template <class T, int D, int TS, int RG, int CPS>
 __global__ void __launch_bounds__(RowsShape<D, TS, RG, CPS, sizeof(T) == 4 ? 2 : 1>::kThreads, CPS)
@@ -146,7 +184,7 @@ __global__ void __launch_bounds__(RowsShape<D, TS, RG, CPS, sizeof(T) == 4 ? 2 :
     constexpr int kParts = D > 128 ? D / 128 : 1, kPartDim = D / kParts;  // 128-byte columns of a tile
     constexpr int kChunk = kPartDim / 8;                                  // dims of a lane group in a part: 16, or 8
     constexpr int NT = kRowsTile / TS / 8;                                // blocks of 8 tokens of a warp
-    constexpr bool kKeepQ = TERMS == 1 && D <= 128;                       // a row group's q in registers
+    constexpr bool kKeepQ = TERMS == 1 && D <= 64;                        // a row group's q in registers
     extern __shared__ uint8_t raw_smem[];
     __shared__ PlanSmem plan;
     __shared__ uint64_t bars[2 * S::kStages];
@@ -155,6 +193,7 @@ __global__ void __launch_bounds__(RowsShape<D, TS, RG, CPS, sizeof(T) == 4 ? 2 :
     __shared__ float2 row_ml[RG][TS][16];
     __shared__ float q_unscale[S::kRows];
     __shared__ uint32_t nan_seen, is_last;
+    __shared__ Walk walk;
 
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
@@ -171,11 +210,16 @@ __global__ void __launch_bounds__(RowsShape<D, TS, RG, CPS, sizeof(T) == 4 ? 2 :
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         nan_seen = 0;
     }
-    Range range;
-    if (!find_range(c, w, plan, &range)) return;  // (its barriers order the initialisation above)
+    {
+        Range range;
+        if (!find_range(c, w, plan, &range)) return;  // (its barriers order the initialisation above)
+        if (threadIdx.x == 0) {
+            walk.range = range;
+            walk.u = range.unit;
+            walk.enter(w, range.unit_begin);
+        }
+    }
     __syncthreads();
-    Unit u = range.unit;
-    uint64_t unit_begin = range.unit_begin;
     uint32_t stage = 0, parity = 0;
     bool alive = true;  // no wait has run out
     auto advance = [&] {
@@ -187,6 +231,10 @@ __global__ void __launch_bounds__(RowsShape<D, TS, RG, CPS, sizeof(T) == 4 ? 2 :
         const uint32_t page_rows = min(c.cache.page_tokens, kRowsTile), boxes = kRowsTile / page_rows;
         const float scale = c.scale * 1.4426950408889634f;
         uint32_t issued = 0;
+        const Range range = walk.range;
+        Unit u = range.unit;
+        uint64_t unit_begin = range.unit_begin;
+        __syncthreads();  // the consumers move `walk` on from here
         for (uint64_t pos = range.begin; pos < range.end;) {
             const Segment g = segment(range, u, unit_begin);
             const int32_t first = first_key(u.s, w.window, u.row0(w) / c.group), end = end_key(u.s, c.causal, (u.row0(w) + u.rows(w) - 1) / c.group);
@@ -274,53 +322,57 @@ __global__ void __launch_bounds__(RowsShape<D, TS, RG, CPS, sizeof(T) == 4 ? 2 :
     const uint32_t rg = warp / TS, ts = warp % TS, g8 = lane / 4, t4 = lane % 4;
     const uint32_t my_q = q_at + rg * (D / 16) * TERMS * 512 + lane * 16;
     auto tau = [](uint32_t n) { return n ^ ((n & 1) << 2); };  // token of column n of a block of 8: spreads a quarter warp's reads over the banks
-    for (uint64_t pos = range.begin; pos < range.end;) {
-        const Segment g = segment(range, u, unit_begin);
-        const uint32_t rows = u.rows(w), r0 = u.row0(w);
+    __syncthreads();
+    do {
         // q: a warp takes a row at a time, scales it and stores its fp16 terms in the order of the products' operands
-        bar_sync(1, kConsumers);  // the q of the segment before is no longer read
-        for (uint32_t r = warp; r < S::kRows; r += S::kWarps) {
-            constexpr int E = D / 32;
-            float x[E];
-            float top = 0;
-            if (r < rows) {
+        const Unit& u = walk.u;
+        const uint32_t rows = walk.rows, r0 = walk.r0;
+        constexpr int E = D / 32, kBatch = 4;  // rows of a warp whose loads are under way together
+        static_assert(S::kRows % (S::kWarps * kBatch) == 0);
+        for (uint32_t first = warp; first < rows; first += S::kWarps * kBatch) {
+            T raw[kBatch][E];
+#pragma unroll
+            for (int n = 0; n < kBatch; ++n) {
+                const uint32_t r = min(first + n * S::kWarps, rows - 1);
                 const uint32_t j = (r0 + r) / c.group, h = u.head * c.group + (r0 + r) % c.group;
                 const T* q = reinterpret_cast<const T*>(c.q.p + uint64_t{u.s.row0 + j} * c.q.token_stride + uint64_t{h} * c.q.head_stride) + lane * E;
                 if (c.q.vec) {
                     constexpr int kBytes = E * sizeof(T) < 16 ? E * sizeof(T) : 16, kPer = kBytes / sizeof(T);
+                    using Word = std::conditional_t<kBytes == 16, uint4, std::conditional_t<kBytes == 8, uint2, uint32_t>>;
 #pragma unroll
                     for (int e = 0; e < E; e += kPer) {
-                        T v[kPer];
-                        if constexpr (kBytes == 16) *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(q + e);
-                        else if constexpr (kBytes == 8) *reinterpret_cast<uint2*>(v) = *reinterpret_cast<const uint2*>(q + e);
-                        else *reinterpret_cast<uint32_t*>(v) = *reinterpret_cast<const uint32_t*>(q + e);
-#pragma unroll
-                        for (int i = 0; i < kPer; ++i) x[e + i] = to_f32(v[i]);
+                        const Word v = __ldg(reinterpret_cast<const Word*>(q + e));
+                        __builtin_memcpy(&raw[n][e], &v, kBytes);
                     }
                 } else {
 #pragma unroll
-                    for (int e = 0; e < E; ++e) x[e] = to_f32(q[e]);
+                    for (int e = 0; e < E; ++e) raw[n][e] = q[e];
                 }
-            } else {
-#pragma unroll
-                for (int e = 0; e < E; ++e) x[e] = 0;
             }
 #pragma unroll
-            for (int e = 0; e < E; ++e) top = fmaxf(top, fabsf(x[e]) < INFINITY ? fabsf(x[e]) : 0.0f);
+            for (int n = 0; n < kBatch; ++n) {
+                const uint32_t r = first + n * S::kWarps;
+                float x[E], top = 0;
 #pragma unroll
-            for (int d = 16; d != 0; d /= 2) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
-            const int32_t exponent = max(static_cast<int32_t>(__float_as_uint(top) >> 23) - 127, -100);
-            const float by = exp2_int(14 - exponent);
-            if (lane == 0) q_unscale[r] = exp2_int(exponent - 14);
+                for (int e = 0; e < E; ++e) {
+                    x[e] = r < rows ? to_f32(raw[n][e]) : 0.0f;
+                    top = fmaxf(top, fabsf(x[e]) < INFINITY ? fabsf(x[e]) : 0.0f);
+                }
 #pragma unroll
-            for (int e = 0; e < E; e += 2) {
-                // dim 64 a + 16 t + 4 s + 2 p + {0, 1}: k step 4 a + s, lane t of a quad, register 2 p (+ 1 for the rows 8 and up)
-                const uint32_t d = lane * E + e, step = d / 64 * 4 + d % 16 / 4, t = d % 64 / 16, p = d % 4 / 2;
-                const uint32_t at = q_at + (r / 16) * (D / 16) * TERMS * 512 + step * TERMS * 512 + (r % 8 * 4 + t) * 16 + (2 * p + r / 8 % 2) * 4;
-                const float a = x[e] * by, b = x[e + 1] * by;
-                const uint32_t hi = half2_bits(a, b);
-                asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(hi) : "memory");
-                if constexpr (TERMS == 2) asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + 512), "r"(half2_rest(a, b, hi)) : "memory");
+                for (int d = 16; d != 0; d /= 2) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+                const int32_t exponent = max(static_cast<int32_t>(__float_as_uint(top) >> 23) - 127, -100);
+                const float by = exp2_int(14 - exponent);
+                if (lane == 0) q_unscale[r] = exp2_int(exponent - 14);
+#pragma unroll
+                for (int e = 0; e < E; e += 2) {
+                    // dim 64 a + 16 t + 4 s + 2 p + {0, 1}: k step 4 a + s, lane t of a quad, register 2 p (+ 1 for the rows 8 and up)
+                    const uint32_t d = lane * E + e, step = d / 64 * 4 + d % 16 / 4, t = d % 64 / 16, p = d % 4 / 2;
+                    const uint32_t at = q_at + (r / 16) * (D / 16) * TERMS * 512 + step * TERMS * 512 + (r % 8 * 4 + t) * 16 + (2 * p + r / 8 % 2) * 4;
+                    const float a = x[e] * by, b = x[e + 1] * by;
+                    const uint32_t hi = half2_bits(a, b);
+                    asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(hi) : "memory");
+                    if constexpr (TERMS == 2) asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + 512), "r"(half2_rest(a, b, hi)) : "memory");
+                }
             }
         }
         bar_sync(1, kConsumers);
@@ -350,12 +402,9 @@ __global__ void __launch_bounds__(RowsShape<D, TS, RG, CPS, sizeof(T) == 4 ? 2 :
             for (int b = 0; b < kChunk; ++b) o[a][b][0] = o[a][b][1] = o[a][b][2] = o[a][b][3] = 0;
         float m[2] = {-INFINITY, -INFINITY}, l[2] = {0, 0};
 
-        for (int32_t tile = g.lo; tile < g.hi; ++tile) {
-            if (alive) alive = __all_sync(0xFFFFFFFFu, mbar_wait(full + 8 * stage, parity));
-            const uint32_t k_at = ring + stage * S::kStage, v_at = k_at + S::kHalfTile;
-            const uint32_t tok = ts * (NT * 8);  // this warp's first token of the tile
-            const int32_t t0 = tile * static_cast<int32_t>(kRowsTile);
-            float x[NT][4];
+        const uint32_t tok = ts * (NT * 8);  // this warp's first token of a tile
+        auto scores = [&](uint32_t st, float (&x)[NT][4]) {  // q . k of a stage's tile
+            const uint32_t k_at = ring + st * S::kStage;
 #pragma unroll
             for (int n = 0; n < NT; ++n) x[n][0] = x[n][1] = x[n][2] = x[n][3] = 0;
 #pragma unroll
@@ -381,7 +430,10 @@ __global__ void __launch_bounds__(RowsShape<D, TS, RG, CPS, sizeof(T) == 4 ? 2 :
                     }
                 }
             }
-            const bool masked = t0 < all_lo || t0 + static_cast<int32_t>(kRowsTile) > all_hi || partly[stage] != 0;
+        };
+        // the weights of a tile's scores, and what they add to the sums and rows.  MASKED: some row does not see some token of the tile.
+        auto weigh = [&](const bool MASKED, int32_t t0, float (&x)[NT][4]) __attribute__((always_inline)) {
+            const uint32_t v_at = ring + stage * S::kStage + S::kHalfTile;
             float top[2] = {-INFINITY, -INFINITY}, inv[NT];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
@@ -393,7 +445,7 @@ __global__ void __launch_bounds__(RowsShape<D, TS, RG, CPS, sizeof(T) == 4 ? 2 :
                     x[n][2 * i] = fmaf(x[n][2 * i], by, s.log_v);
                     x[n][2 * i + 1] = fmaf(x[n][2 * i + 1], by, s.log_v);
                 }
-                if (masked) {
+                if (MASKED) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const int32_t t = t0 + static_cast<int32_t>(tok + 8 * n + tau(2 * t4 + e % 2));
@@ -458,7 +510,7 @@ __global__ void __launch_bounds__(RowsShape<D, TS, RG, CPS, sizeof(T) == 4 ? 2 :
                             vw[i][0] = v.x, vw[i][1] = v.y;
                         }
                     }
-                    if (masked) {
+                    if (MASKED) {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const int32_t t = t0 + static_cast<int32_t>(row[i]);
@@ -484,6 +536,31 @@ __global__ void __launch_bounds__(RowsShape<D, TS, RG, CPS, sizeof(T) == 4 ? 2 :
                 }
             }
             if (nan) nan_seen = 1;
+        };
+        // The next tile's scores are issued in front of this tile's weights: two independent chains for a warp that has few neighbours.  Behind the last
+        // tile they are those of whatever the next stage holds, and unused.
+        if (alive) alive = __all_sync(0xFFFFFFFFu, mbar_wait(full + 8 * stage, parity));
+        float x[NT][4];
+        scores(stage, x);
+        const int32_t last = walk.g.hi;
+        for (int32_t tile = walk.g.lo; tile < last; ++tile) {
+            const bool wraps = stage + 1 == S::kStages;
+            const uint32_t next = wraps ? 0 : stage + 1;
+            if (alive && tile + 1 < last) alive = __all_sync(0xFFFFFFFFu, mbar_wait(full + 8 * next, parity ^ (wraps ? 1 : 0)));
+            const int32_t t0 = tile * static_cast<int32_t>(kRowsTile);
+            const bool masked = t0 < all_lo || t0 + static_cast<int32_t>(kRowsTile) > all_hi || partly[stage] != 0;
+            float ahead[NT][4];
+            if (masked) {
+                scores(next, ahead);
+                weigh(true, t0, x);
+            } else {
+                scores(next, ahead);
+                weigh(false, t0, x);
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[n][e] = ahead[n][e];
             __syncwarp();
             if (lane == 0) mbar_arrive(empty + 8 * stage);
             advance();
@@ -495,84 +572,68 @@ __global__ void __launch_bounds__(RowsShape<D, TS, RG, CPS, sizeof(T) == 4 ? 2 :
             l[i] += __shfl_xor_sync(0xFFFFFFFFu, l[i], 1);
             l[i] += __shfl_xor_sync(0xFFFFFFFFu, l[i], 2);
         }
+        const Segment& g = walk.g;
         float* slot = g.whole() ? nullptr : partial_slot(w, D, blockIdx.x, g.from_start);
         auto out_at = [&](uint32_t r) {
-            const uint32_t j = (r0 + r) / c.group, h = u.head * c.group + (r0 + r) % c.group;
-            return reinterpret_cast<T*>(c.out.p + uint64_t{u.s.row0 + j} * c.out.token_stride + uint64_t{h} * c.out.head_stride);
+            const uint32_t p = walk.r0 + r, j = p / c.group, h = walk.u.head * c.group + p % c.group;
+            return reinterpret_cast<T*>(c.out.p + uint64_t{walk.u.s.row0 + j} * c.out.token_stride + uint64_t{h} * c.out.head_stride);
         };
-        if constexpr (TS > 1) {
-            if (t4 == 0) row_ml[rg][ts][g8] = make_float2(m[0], l[0]), row_ml[rg][ts][g8 + 8] = make_float2(m[1], l[1]);
-            bar_sync(1, kConsumers);
-            float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0, 0}, f[2];
+        if (t4 == 0) row_ml[rg][ts][g8] = make_float2(m[0], l[0]), row_ml[rg][ts][g8 + 8] = make_float2(m[1], l[1]);
+        bar_sync(1, kConsumers);
+        float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0, 0}, f[2];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < 2; ++i) {
 #pragma unroll
-                for (int k = 0; k < TS; ++k) top[i] = fmaxf(top[i], row_ml[rg][k][g8 + 8 * i].x);
+            for (int k = 0; k < TS; ++k) top[i] = fmaxf(top[i], row_ml[rg][k][g8 + 8 * i].x);
 #pragma unroll
-                for (int k = 0; k < TS; ++k) {
-                    const float2 ml = row_ml[rg][k][g8 + 8 * i];
-                    sum[i] += ml.x == -INFINITY ? ml.y : exp2_approx(ml.x - top[i]) * ml.y;
-                }
-                f[i] = m[i] == -INFINITY ? 1.0f : exp2_approx(m[i] - top[i]);
-            }
-            float* mine = join + rg * 16 * D;
             for (int k = 0; k < TS; ++k) {
-                if (ts == static_cast<uint32_t>(k)) {
-#pragma unroll
-                    for (int i = 0; i < 2; ++i)
-#pragma unroll
-                        for (int a = 0; a < kParts; ++a)
-#pragma unroll
-                            for (int e = 0; e < 2; ++e)
-#pragma unroll
-                                for (int b = 0; b < kChunk; ++b) {
-                                    // a part's dim (2 t4 + e) * kChunk + b, kept at a place that spreads the lanes over the banks
-                                    float* at = mine + (g8 + 8 * i) * D + a * kPartDim + b * 8 + ((2 * t4 + e + g8) & 7);
-                                    const float v = o[a][b][2 * i + e] * f[i];
-                                    *at = k == 0 ? v : *at + v;
-                                }
-                }
-                bar_sync(1, kConsumers);
+                const float2 ml = row_ml[rg][k][g8 + 8 * i];
+                sum[i] += ml.x == -INFINITY ? ml.y : exp2_approx(ml.x - top[i]) * ml.y;
             }
-            if (ts == 0 && t4 == 0) row_ml[rg][0][g8] = make_float2(top[0], sum[0]), row_ml[rg][0][g8 + 8] = make_float2(top[1], sum[1]);
+            f[i] = m[i] == -INFINITY ? 1.0f : exp2_approx(m[i] - top[i]);
+        }
+        // Dim d of a row lies at d + d / 32 * 4: the lanes of a 16-byte store spread over the banks.
+        float* mine = join + (rg * 16 + g8) * S::kJoinRow + t4 * (2 * kChunk) + t4 * (2 * kChunk) / 32 * 4;
+#pragma unroll 1
+        for (int k = 0; k < TS; ++k) {
+            if (ts == static_cast<uint32_t>(k)) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int a = 0; a < kParts; ++a)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+#pragma unroll
+                            for (int b = 0; b < kChunk; b += 4) {
+                                float4* to = reinterpret_cast<float4*>(mine + 8 * i * S::kJoinRow + a * (kPartDim / 32 * 36) + e * kChunk + b);
+                                float4 v = make_float4(o[a][b][2 * i + e] * f[i], o[a][b + 1][2 * i + e] * f[i], o[a][b + 2][2 * i + e] * f[i], o[a][b + 3][2 * i + e] * f[i]);
+                                if (k != 0) {
+                                    const float4 x = *to;
+                                    v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+                                }
+                                *to = v;
+                            }
+            }
             bar_sync(1, kConsumers);
-            for (uint32_t i = threadIdx.x; i < rows * D; i += kConsumers) {
-                const uint32_t r = i / D, d = i % D, a = d / kPartDim, n = d % kPartDim / kChunk, b = d % kChunk;
-                const float v = join[r * D + a * kPartDim + b * 8 + ((n + r) & 7)];
-                const float sum_r = row_ml[r / 16][0][r % 16].y;
-                if (slot == nullptr) out_at(r)[d] = from_f32<T>(sum_r != 0 ? v / sum_r : 0.0f);
+        }
+        if (ts == 0 && t4 == 0) row_ml[rg][0][g8] = make_float2(top[0], sum[0]), row_ml[rg][0][g8 + 8] = make_float2(top[1], sum[1]);
+        bar_sync(1, kConsumers);
+        for (uint32_t r = warp; r < walk.rows; r += S::kWarps) {
+            const float2 ml = row_ml[r / 16][0][r % 16];
+            const float inv = ml.y != 0 ? 1.0f / ml.y : 0.0f;
+            T* out = out_at(r);
+#pragma unroll
+            for (int e = 0; e < D / 32; ++e) {
+                const uint32_t d = e * 32 + lane;
+                const float v = join[r * S::kJoinRow + e * 36 + lane];
+                if (slot == nullptr) out[d] = from_f32<T>(v * inv);
                 else slot[r * D + d] = v;
             }
-            if (slot != nullptr)
-                for (uint32_t r = threadIdx.x; r < rows; r += kConsumers) *reinterpret_cast<float2*>(slot + w.rows * D + 2 * r) = row_ml[r / 16][0][r % 16];
-        } else {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const uint32_t r = rg * 16 + g8 + 8 * i;
-                if (r >= rows) continue;
-                const float inv = l[i] != 0 ? 1.0f / l[i] : 0.0f;
-#pragma unroll
-                for (int a = 0; a < kParts; ++a)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e)
-#pragma unroll
-                        for (int b = 0; b < kChunk; b += 4) {
-                            const uint32_t d = a * kPartDim + (2 * t4 + e) * kChunk + b;
-                            if (slot != nullptr) {
-                                *reinterpret_cast<float4*>(slot + r * D + d) =
-                                    make_float4(o[a][b][2 * i + e], o[a][b + 1][2 * i + e], o[a][b + 2][2 * i + e], o[a][b + 3][2 * i + e]);
-                            } else {
-                                T* out = out_at(r) + d;
-#pragma unroll
-                                for (int k = 0; k < 4; ++k) out[k] = from_f32<T>(o[a][b + k][2 * i + e] * inv);
-                            }
-                        }
-                if (slot != nullptr && t4 == 0) *reinterpret_cast<float2*>(slot + w.rows * D + 2 * r) = make_float2(m[i], l[i]);
-            }
+            if (slot != nullptr && lane == 0) *reinterpret_cast<float2*>(slot + w.rows * D + 2 * r) = ml;
         }
         bar_sync(1, kConsumers);
         if (nan_seen != 0) {
-            spread_nan(c, w, u, g, kConsumers, [&](uint32_t r, uint32_t d) {
+            spread_nan(c, w, walk.u, walk.g, kConsumers, [&](uint32_t r, uint32_t d) {
                 if (slot == nullptr) out_at(r)[d] = from_f32<T>(NAN);
                 else slot[r * D + d] = NAN;
             });
@@ -580,8 +641,8 @@ __global__ void __launch_bounds__(RowsShape<D, TS, RG, CPS, sizeof(T) == 4 ? 2 :
             if (threadIdx.x == 0) nan_seen = 0;
         }
         if (slot != nullptr) {
-            const uint32_t n = gridDim.x, c0 = owner(g.unit_begin, range.total, n), c1 = owner(g.unit_end - 1, range.total, n);
-            const uint32_t shares = range.total >= n ? c1 - c0 + 1 : u.span.tiles();
+            const Range& range = walk.range;
+            const uint32_t c0 = owner(g.unit_begin, range.total, range.ctas), shares = owner(g.unit_end - 1, range.total, range.ctas) - c0 + 1;
             __threadfence();
             bar_sync(1, kConsumers);
             if (threadIdx.x == 0) {
@@ -592,13 +653,13 @@ __global__ void __launch_bounds__(RowsShape<D, TS, RG, CPS, sizeof(T) == 4 ? 2 :
             bar_sync(1, kConsumers);
             if (is_last != 0) {
                 __threadfence();
-                join_partials<T, D>(c, w, u, g, range.total, kConsumers);
+                join_partials<T, D>(c, w, walk.u.s.row0, walk.u.head, walk.r0, walk.rows, c0, shares, S::kWarps);
             }
         }
-        pos = g.to_end ? g.unit_end : range.end;
-        unit_begin = g.unit_end;
-        if (pos >= range.end || !next_unit(c, w, u)) break;
-    }
+        bar_sync(1, kConsumers);  // nobody reads q, the joined rows or `walk` any more
+        if (threadIdx.x == 0) walk.advance(c, w);
+        bar_sync(1, kConsumers);
+    } while (walk.more != 0);
     if (!alive && lane == 0) atomicOr(w.error_word, 1u);
     __syncthreads();
 }

@@ -81,14 +81,17 @@ __device__ __forceinline__ bool next_unit(const AttentionCall& c, const Work& w,
     return false;
 }
 
-/// The CTA that has position x of `total` (range b is [total * b / n, total * (b + 1) / n)).
+/// The CTA that has position x of `total` (range b of n is [total * b / n, total * (b + 1) / n)).
 __device__ __forceinline__ uint32_t owner(uint64_t x, uint64_t total, uint32_t n) { return static_cast<uint32_t>(((x + 1) * n - 1) / total); }
 
 struct Range {
     uint64_t begin, end, total;  // this CTA's tiles
+    uint32_t ctas;               // that have a range
     uint64_t unit_begin;         // position of the first unit's first tile
     Unit unit;                   // of tile `begin`
 };
+
+constexpr uint32_t kLeastTiles = 2;  // of a CTA, where a call has few
 
 struct PlanSmem {
     uint64_t warp_sum[32];
@@ -138,9 +141,12 @@ __device__ inline bool find_range(const AttentionCall& c, const Work& w, PlanSme
     }
     out->total = total;
     if (total == 0) return false;
-    out->begin = total * blockIdx.x / gridDim.x;
-    out->end = total * (blockIdx.x + 1) / gridDim.x;
-    if (out->begin == out->end) return false;
+    // A share of a unit costs its CTA, and the one that joins the shares, about what kLeastTiles tiles do.
+    const uint32_t ctas = static_cast<uint32_t>(min(uint64_t{gridDim.x}, max(total / kLeastTiles, uint64_t{1})));
+    if (blockIdx.x >= ctas) return false;
+    out->ctas = ctas;
+    out->begin = total * blockIdx.x / ctas;
+    out->end = total * (blockIdx.x + 1) / ctas;
     uint64_t before = 0;
     for (uint32_t base = 0; base < n_seq; base += per_pass) {
         uint64_t all = total;
