@@ -22,19 +22,18 @@
 namespace halo_cuda {
 namespace attn {
 
-constexpr uint32_t kRowsTile = 64;             // keys of a tile
-constexpr uint32_t kGroups = kRowsTile / 16;   // of 16 tokens, each inside one page
-
 struct GroupScale {
     float k, log_v, inv_v;  // s_K * scale * log2 e; log2 s_V, -inf for tokens of no page; 1 / s_V
     float pad;
 };
 
-/// CPS: CTAs that share an SM.
-template <int D, int TS, int RG, int CPS, int TERMS>
+/// TILE: keys of a tile.  CPS: CTAs that share an SM.
+template <int D, int TS, int RG, int TILE, int CPS, int TERMS>
 struct RowsShape {
+    static constexpr uint32_t kTile = TILE, kGroups = TILE / 16;  // groups of 16 tokens, each inside one page
+    static_assert(TILE % 64 == 0 && TILE % (16 * TS) == 0 && kGroups <= 32);
     static constexpr int kWarps = TS * RG, kThreads = (kWarps + 1) * 32, kRows = 16 * RG;
-    static constexpr uint32_t kHalfTile = kRowsTile * D;  // K or V of a tile
+    static constexpr uint32_t kHalfTile = kTile * D;  // K or V of a tile
     static constexpr uint32_t kStage = 2 * kHalfTile;
     static constexpr uint32_t kQ = RG * (D / 16) * TERMS * 512;
     static constexpr uint32_t kJoinRow = D + D / 8 + (D == 256 ? 16 : 0);  // floats of a row of the warps' joined rows
@@ -175,15 +174,16 @@ struct Walk {
     }
 };
 
-template <class T, int D, int TS, int RG, int CPS>
-__global__ void __launch_bounds__(RowsShape<D, TS, RG, CPS, sizeof(T) == 4 ? 2 : 1>::kThreads, CPS)
+template <class T, int D, int TS, int RG, int TILE, int CPS>
+__global__ void __launch_bounds__(RowsShape<D, TS, RG, TILE, CPS, sizeof(T) == 4 ? 2 : 1>::kThreads, CPS)
     rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const __grid_constant__ AttentionCall c,
                 const __grid_constant__ Work w) {
     constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;
-    using S = RowsShape<D, TS, RG, CPS, TERMS>;
+    using S = RowsShape<D, TS, RG, TILE, CPS, TERMS>;
     constexpr int kParts = D > 128 ? D / 128 : 1, kPartDim = D / kParts;  // 128-byte columns of a tile
     constexpr int kChunk = kPartDim / 8;                                  // dims of a lane group in a part: 16, or 8
-    constexpr int NT = kRowsTile / TS / 8;                                // blocks of 8 tokens of a warp
+    constexpr uint32_t kTile = S::kTile, kGroups = S::kGroups;
+    constexpr int NT = TILE / TS / 8;                                        // blocks of 8 tokens of a warp
     constexpr bool kKeepQ = TERMS == 1 && D <= 64;                        // a row group's q in registers
     extern __shared__ uint8_t raw_smem[];
     __shared__ PlanSmem plan;
@@ -228,7 +228,7 @@ __global__ void __launch_bounds__(RowsShape<D, TS, RG, CPS, sizeof(T) == 4 ? 2 :
 
     if (warp == S::kWarps) {
         // ---- producer --------------------------------------------------------------------------------------------------------------
-        const uint32_t page_rows = min(c.cache.page_tokens, kRowsTile), boxes = kRowsTile / page_rows;
+        const uint32_t page_rows = min(c.cache.page_tokens, 64u);
         const float scale = c.scale * 1.4426950408889634f;
         uint32_t issued = 0;
         const Range range = walk.range;
@@ -238,63 +238,62 @@ __global__ void __launch_bounds__(RowsShape<D, TS, RG, CPS, sizeof(T) == 4 ? 2 :
         for (uint64_t pos = range.begin; pos < range.end;) {
             const Segment g = segment(range, u, unit_begin);
             const int32_t first = first_key(u.s, w.window, u.row0(w) / c.group), end = end_key(u.s, c.causal, (u.row0(w) + u.rows(w) - 1) / c.group);
-            // a lane knows the page and the scales of one group of 16 tokens: eight tiles at a time, the next eight on their way
+            // a lane knows the page and the scale bytes of one group of 16 tokens, for as many tiles as 32 lanes cover; the next lot is on its way
+            constexpr int32_t kLot = 32 / kGroups;
             int32_t page_next = -1;
-            uint32_t kb_next = 0, vb_next = 0;
+            uint32_t k_next = 0, v_next = 0;
             auto fetch = [&](int32_t tile) {
-                const int32_t t = tile * static_cast<int32_t>(kRowsTile) + static_cast<int32_t>(lane) * 16;
+                const int32_t t = tile * static_cast<int32_t>(kTile) + static_cast<int32_t>(lane) * 16;
                 page_next = -1;
-                if (t < end && t + 16 > first && tile + static_cast<int32_t>(lane / kGroups) < g.hi) {
+                if (lane < kLot * kGroups && t < end && t + 16 > first && tile + static_cast<int32_t>(lane / kGroups) < g.hi) {
                     const int32_t p = page_of(c.cache, u.seq, t >> c.cache.page_shift);
                     if (static_cast<uint32_t>(p) < c.cache.n_pages) {
                         page_next = p;
                         const uint64_t at = p * c.cache.scale_stride + u.head;
-                        kb_next = __ldg(c.cache.k_scale + at);
-                        vb_next = __ldg(c.cache.v_scale + at);
+                        k_next = __ldg(c.cache.k_scale + at);
+                        v_next = __ldg(c.cache.v_scale + at);
                     } else {
                         page_next = -2;  // a visible token's page is not there
                     }
                 }
             };
             fetch(g.lo);
-            for (int32_t base = g.lo; base < g.hi; base += 32 / kGroups) {
+            for (int32_t base = g.lo; base < g.hi; base += kLot) {
                 const int32_t page = page_next;
-                const float k = exp2_int(scale_byte(kb_next) - 127) * scale;
-                const int32_t v = scale_byte(vb_next) - 127;
-                if (base + 32 / static_cast<int32_t>(kGroups) < g.hi) fetch(base + 32 / kGroups);
+                const uint32_t k_byte = k_next, v_byte = v_next;
+                if (base + kLot < g.hi) fetch(base + kLot);
                 if (page == -2 && c.status != nullptr) atomicOr(c.status, 8u);  // kStatusBadIndex
-                for (int32_t tile = base; tile < min(base + static_cast<int32_t>(32 / kGroups), g.hi); ++tile) {
+                const uint32_t present = __ballot_sync(0xFFFFFFFFu, page >= 0);
+                for (int32_t tile = base; tile < min(base + kLot, g.hi); ++tile) {
                     if (alive) alive = __all_sync(0xFFFFFFFFu, mbar_wait(empty + 8 * stage, parity ^ 1));
                     if (!alive) break;
-                    const uint32_t in_tile = (tile - base) * kGroups;
+                    const uint32_t in_tile = (tile - base) * kGroups, here = present >> in_tile & static_cast<uint32_t>((uint64_t{1} << kGroups) - 1);
+                    const uint32_t step = page_rows / 16;  // groups of a box
+                    // a box is issued by the lane that knows its page: the first of its groups that is there
+                    const uint32_t box = (lane - in_tile) / step, of = lane >= in_tile && lane < in_tile + kGroups ? here >> (box * step) & ((1u << step) - 1) : 0;
+                    const bool issues = of != 0 && lane == in_tile + box * step + __ffs(of) - 1;
+                    const uint32_t bytes = __popc(__ballot_sync(0xFFFFFFFFu, issues)) * page_rows * D * 2;
+                    if (issues) {
+                        const int32_t t = tile * static_cast<int32_t>(kTile) + static_cast<int32_t>(box * page_rows);
+                        const int32_t y = static_cast<int32_t>(u.head * c.cache.page_tokens) + (t & static_cast<int32_t>(c.cache.page_tokens - 1));
+                        const uint32_t dst = ring + stage * S::kStage + box * page_rows * kPartDim;
+#pragma unroll
+                        for (int part = 0; part < kParts; ++part) {
+                            tma_3d(dst + part * kTile * kPartDim, &k_map, part * 128, y, page, full + 8 * stage);
+                            tma_3d(dst + S::kHalfTile + part * kTile * kPartDim, &v_map, part * 128, y, page, full + 8 * stage);
+                        }
+                    }
+                    // The scales, whose bytes arrive while the copies run; the arrival that completes the barrier's phase comes behind them.
                     if (lane >= in_tile && lane < in_tile + kGroups) {
                         GroupScale& s = scales[stage][lane - in_tile];
-                        s.k = page >= 0 ? k : 0.0f;
+                        const int32_t v = scale_byte(v_byte) - 127;
+                        s.k = page >= 0 ? exp2_int(scale_byte(k_byte) - 127) * scale : 0.0f;
                         s.log_v = page >= 0 ? static_cast<float>(v) : -INFINITY;
                         s.inv_v = page >= 0 ? exp2_int(-v) : 0.0f;
                     }
-                    const uint32_t here = __ballot_sync(0xFFFFFFFFu, page >= 0) >> in_tile & ((1u << kGroups) - 1);
-                    if (lane == 0) partly[stage] = here != (1u << kGroups) - 1;
-                    const uint32_t step = page_rows / 16;  // groups of a box
-                    uint32_t present = 0;
-                    for (uint32_t b = 0; b < boxes; ++b) present += here >> (b * step) & ((1u << step) - 1) ? 1 : 0;
+                    if (lane == 0) partly[stage] = here != static_cast<uint32_t>((uint64_t{1} << kGroups) - 1);
                     __syncwarp();
-                    if (elect_one()) mbar_expect(full + 8 * stage, present * page_rows * D * 2);
-                    for (uint32_t b = 0; b < boxes; ++b) {
-                        const uint32_t of = here >> (b * step) & ((1u << step) - 1);
-                        if (of == 0) continue;
-                        const int32_t p = __shfl_sync(0xFFFFFFFFu, page, in_tile + b * step + __ffs(of) - 1);
-                        const int32_t t = tile * static_cast<int32_t>(kRowsTile) + static_cast<int32_t>(b * page_rows);
-                        const int32_t y = static_cast<int32_t>(u.head * c.cache.page_tokens) + (t & static_cast<int32_t>(c.cache.page_tokens - 1));
-                        if (elect_one()) {
-                            const uint32_t dst = ring + stage * S::kStage + b * page_rows * kPartDim;
-#pragma unroll
-                            for (int part = 0; part < kParts; ++part) {
-                                tma_3d(dst + part * kRowsTile * kPartDim, &k_map, part * 128, y, p, full + 8 * stage);
-                                tma_3d(dst + S::kHalfTile + part * kRowsTile * kPartDim, &v_map, part * 128, y, p, full + 8 * stage);
-                            }
-                        }
-                    }
+                    if (elect_one()) mbar_expect(full + 8 * stage, bytes);
                     ++issued;
                     advance();
                 }
@@ -327,8 +326,7 @@ __global__ void __launch_bounds__(RowsShape<D, TS, RG, CPS, sizeof(T) == 4 ? 2 :
         // q: a warp takes a row at a time, scales it and stores its fp16 terms in the order of the products' operands
         const Unit& u = walk.u;
         const uint32_t rows = walk.rows, r0 = walk.r0;
-        constexpr int E = D / 32, kBatch = 4;  // rows of a warp whose loads are under way together
-        static_assert(S::kRows % (S::kWarps * kBatch) == 0);
+        constexpr int E = D / 32, kEach = (S::kRows + S::kWarps - 1) / S::kWarps, kBatch = kEach < 4 ? kEach : 4;  // rows of a warp whose loads are under way together
         for (uint32_t first = warp; first < rows; first += S::kWarps * kBatch) {
             T raw[kBatch][E];
 #pragma unroll
@@ -352,6 +350,7 @@ __global__ void __launch_bounds__(RowsShape<D, TS, RG, CPS, sizeof(T) == 4 ? 2 :
 #pragma unroll
             for (int n = 0; n < kBatch; ++n) {
                 const uint32_t r = first + n * S::kWarps;
+                if (r >= S::kRows) break;
                 float x[E], top = 0;
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
@@ -412,7 +411,7 @@ __global__ void __launch_bounds__(RowsShape<D, TS, RG, CPS, sizeof(T) == 4 ? 2 :
                 uint4 kw[NT];
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
-                    kw[n] = lds128(k_at + (D > 64 ? a / 2 * kRowsTile * 128 : 0) + swizzled(tok + 8 * n + tau(g8), (D > 64 ? a % 2 * 4 : 0) + t4, D));
+                    kw[n] = lds128(k_at + (D > 64 ? a / 2 * kTile * 128 : 0) + swizzled(tok + 8 * n + tau(g8), (D > 64 ? a % 2 * 4 : 0) + t4, D));
 #pragma unroll
                 for (int s = 0; s < 4; ++s) {
                     uint4 q[TERMS];
@@ -503,7 +502,7 @@ __global__ void __launch_bounds__(RowsShape<D, TS, RG, CPS, sizeof(T) == 4 ? 2 :
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         if constexpr (D > 64) {
-                            const uint4 v = lds128(v_at + a * kRowsTile * 128 + swizzled(row[i], g8, D));
+                            const uint4 v = lds128(v_at + a * kTile * 128 + swizzled(row[i], g8, D));
                             vw[i][0] = v.x, vw[i][1] = v.y, vw[i][2] = v.z, vw[i][3] = v.w;
                         } else {
                             const uint2 v = lds64(v_at + swizzled(row[i], g8 / 2, D) + g8 % 2 * 8);
@@ -547,8 +546,8 @@ __global__ void __launch_bounds__(RowsShape<D, TS, RG, CPS, sizeof(T) == 4 ? 2 :
             const bool wraps = stage + 1 == S::kStages;
             const uint32_t next = wraps ? 0 : stage + 1;
             if (alive && tile + 1 < last) alive = __all_sync(0xFFFFFFFFu, mbar_wait(full + 8 * next, parity ^ (wraps ? 1 : 0)));
-            const int32_t t0 = tile * static_cast<int32_t>(kRowsTile);
-            const bool masked = t0 < all_lo || t0 + static_cast<int32_t>(kRowsTile) > all_hi || partly[stage] != 0;
+            const int32_t t0 = tile * static_cast<int32_t>(kTile);
+            const bool masked = t0 < all_lo || t0 + static_cast<int32_t>(kTile) > all_hi || partly[stage] != 0;
             float ahead[NT][4];
             if (masked) {
                 scores(next, ahead);
@@ -667,16 +666,17 @@ __global__ void __launch_bounds__(RowsShape<D, TS, RG, CPS, sizeof(T) == 4 ? 2 :
 /// The cache's pool as {dim, rows of all heads of a page, pages}, a box of one page's rows of one head.
 int pool_map(const Cache& c, const uint8_t* pool, uint32_t box_rows, CUtensorMap* out);
 
-template <class T, int D, int TS, int RG, int CPS>
+template <class T, int D, int TS, int RG, int TILE, int CPS>
 int launch_rows_kernel(HaloCudaCtx* ctx, const AttentionCall& c, Work w, cudaStream_t s) {
-    using S = RowsShape<D, TS, RG, CPS, sizeof(T) == 4 ? 2 : 1>;
+    using S = RowsShape<D, TS, RG, TILE, CPS, sizeof(T) == 4 ? 2 : 1>;
     w.rows = S::kRows;
-    w.tile = kRowsTile;
+    w.tile = S::kTile;
+    w.least = 1;
     w.row_tiles = (c.rows.max_tokens * c.group + S::kRows - 1) / S::kRows;
     w.lanes = 1;
     while (w.lanes < 32 && w.lanes < w.row_tiles) w.lanes *= 2;
     CUtensorMap k_map, v_map;
-    const uint32_t box = std::min(c.cache.page_tokens, kRowsTile);
+    const uint32_t box = std::min(c.cache.page_tokens, 64u);
     if (int rc = pool_map(c.cache, c.cache.k, box, &k_map)) return rc;
     if (int rc = pool_map(c.cache, c.cache.v, box, &v_map)) return rc;
     const uint32_t ctas = CPS * static_cast<uint32_t>(ctx->prop.multiProcessorCount);
@@ -686,7 +686,7 @@ int launch_rows_kernel(HaloCudaCtx* ctx, const AttentionCall& c, Work w, cudaStr
     if (int rc = workspace(ctx, 6, partial_bytes(S::kRows, D, ctas), s, &p)) return rc;
     w.partials = static_cast<float*>(p);
     w.error_word = ctx->error_word_dev;
-    auto kernel = rows_kernel<T, D, TS, RG, CPS>;
+    auto kernel = rows_kernel<T, D, TS, RG, TILE, CPS>;
     if (int rc = allow_dynamic_smem(ctx, reinterpret_cast<const void*>(kernel), S::kSmem)) return rc;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(ctas);

@@ -9,9 +9,9 @@ template <int D>
 int launch_rows(HaloCudaCtx* ctx, const AttentionCall& c, const Work& w, cudaStream_t s) {
     return with_type(c.type, [&](auto t) {
         using T = decltype(t);
-        if (w.max_rows <= 16) return launch_rows_kernel<T, D, 4, 1, 2>(ctx, c, w, s);
-        if (w.max_rows <= 32) return launch_rows_kernel<T, D, 4, 2, 1>(ctx, c, w, s);
-        return launch_rows_kernel<T, D, 2, 4, 1>(ctx, c, w, s);
+        if (w.max_rows <= 16) return launch_rows_kernel<T, D, 4, 1, 64, D == 256 ? 2 : 3>(ctx, c, w, s);
+        if (w.max_rows <= 32) return launch_rows_kernel<T, D, 4, 2, 64, 1>(ctx, c, w, s);
+        return launch_rows_kernel<T, D, 2, 4, 64, 1>(ctx, c, w, s);
     });
 }
 

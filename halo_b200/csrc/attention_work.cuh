@@ -16,6 +16,7 @@ namespace attn {
 
 struct Work {  // what every kernel of a call is told besides the call
     uint32_t rows, tile;          // packed rows of a unit, keys of a tile
+    uint32_t least;               // tiles of a CTA, where a call has few
     uint32_t row_tiles;           // of the longest sequence at most
     uint32_t lanes;               // of a warp that look at one sequence when the tiles are counted: a power of two
     int32_t window;               // 0: none
@@ -81,8 +82,12 @@ __device__ __forceinline__ bool next_unit(const AttentionCall& c, const Work& w,
     return false;
 }
 
+/// Quotients of 64-bit numbers that are small as a rule: a 64-bit division is a hundred dependent instructions.
+__device__ __forceinline__ uint64_t quotient(uint64_t a, uint64_t b) {
+    return a >> 32 == 0 && b >> 32 == 0 ? static_cast<uint32_t>(a) / static_cast<uint32_t>(b) : a / b;
+}
 /// The CTA that has position x of `total` (range b of n is [total * b / n, total * (b + 1) / n)).
-__device__ __forceinline__ uint32_t owner(uint64_t x, uint64_t total, uint32_t n) { return static_cast<uint32_t>(((x + 1) * n - 1) / total); }
+__device__ __forceinline__ uint32_t owner(uint64_t x, uint64_t total, uint32_t n) { return static_cast<uint32_t>(quotient((x + 1) * n - 1, total)); }
 
 struct Range {
     uint64_t begin, end, total;  // this CTA's tiles
@@ -90,8 +95,6 @@ struct Range {
     uint64_t unit_begin;         // position of the first unit's first tile
     Unit unit;                   // of tile `begin`
 };
-
-constexpr uint32_t kLeastTiles = 2;  // of a CTA, where a call has few
 
 struct PlanSmem {
     uint64_t warp_sum[32];
@@ -141,12 +144,12 @@ __device__ inline bool find_range(const AttentionCall& c, const Work& w, PlanSme
     }
     out->total = total;
     if (total == 0) return false;
-    // A share of a unit costs its CTA, and the one that joins the shares, about what kLeastTiles tiles do.
-    const uint32_t ctas = static_cast<uint32_t>(min(uint64_t{gridDim.x}, max(total / kLeastTiles, uint64_t{1})));
+    // where a call has few tiles, a share of a unit has at least `least`: it costs its CTA, and the one that joins the shares, as much as a few
+    const uint32_t ctas = static_cast<uint32_t>(min(uint64_t{gridDim.x}, max(total / w.least, uint64_t{1})));
     if (blockIdx.x >= ctas) return false;
     out->ctas = ctas;
-    out->begin = total * blockIdx.x / ctas;
-    out->end = total * (blockIdx.x + 1) / ctas;
+    out->begin = quotient(total * blockIdx.x, ctas);
+    out->end = quotient(total * (blockIdx.x + 1), ctas);
     uint64_t before = 0;
     for (uint32_t base = 0; base < n_seq; base += per_pass) {
         uint64_t all = total;
@@ -190,8 +193,8 @@ __device__ inline bool find_range(const AttentionCall& c, const Work& w, PlanSme
     }
     set_row_tile(c, w, u, row_tile);
     at -= front;
-    u.head = static_cast<uint32_t>(at / u.span.tiles());
-    out->unit_begin = out->begin - at % u.span.tiles();
+    u.head = static_cast<uint32_t>(quotient(at, u.span.tiles()));
+    out->unit_begin = out->begin - (at - uint64_t{u.head} * u.span.tiles());
     return true;
 }
 
