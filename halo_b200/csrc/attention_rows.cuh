@@ -92,13 +92,13 @@ __device__ __forceinline__ bool drop_nan(uint32_t& w) {
 /// Writes NaN over the results of rows that see a token whose value is NaN there: the walk left those codes out in tiles that some rows do not see
 /// whole, where a product with weight zero would have spread them.  `at(row, d)` is the result's address.
 template <class At>
-__device__ void spread_nan(const AttentionCall& c, const Work& w, const Unit& u, const Segment& g, uint32_t threads, At&& at) {
+__device__ void spread_nan(const AttentionCall& c, const Work& w, const Unit& u, const Segment& g, uint32_t thread0, uint32_t threads, At&& at) {
     const uint32_t rows = u.rows(w), r0 = u.row0(w), dim = c.cache.head_dim;
     for (int32_t t = g.lo * static_cast<int32_t>(w.tile); t < min(g.hi * static_cast<int32_t>(w.tile), u.s.length); ++t) {
         const int32_t page = page_of(c.cache, u.seq, t >> c.cache.page_shift);
         if (static_cast<uint32_t>(page) >= c.cache.n_pages) continue;
         const uint8_t* v = c.cache.v + page * c.cache.page_stride + (uint64_t{u.head} * c.cache.page_tokens + (t & (c.cache.page_tokens - 1))) * dim;
-        for (uint32_t d = threadIdx.x; d < dim; d += threads) {
+        for (uint32_t d = threadIdx.x - thread0; d < dim; d += threads) {
             if ((v[d] & 127) != 127) continue;
             for (uint32_t r = 0; r < rows; ++r) {
                 const uint32_t j = (r0 + r) / c.group;
@@ -108,15 +108,15 @@ __device__ void spread_nan(const AttentionCall& c, const Work& w, const Unit& u,
     }
 }
 
-/// Joins the shares of a unit in CTA order and stores its rows.  All `warps` of the caller take part, each with a row's 128 dims (or 64) at a time.
+/// Joins the shares of a unit in CTA order and stores its rows.  All `warps` of the caller, from warp0 on, take part, each with a row's 128 dims (or 64) at a time.
 template <class T, int D>
 __device__ __forceinline__ void join_partials(const AttentionCall& c, const Work& w, uint32_t seq_row0, uint32_t head, uint32_t r0, uint32_t rows, uint32_t c0, uint32_t shares,
-                                              uint32_t warps) {
+                                              uint32_t warp0, uint32_t warps) {
     constexpr uint32_t kPerLane = D < 128 ? 2 : 4, kParts = D / (32 * kPerLane), kAhead = 8;  // shares whose loads are under way together
     using Word = std::conditional_t<kPerLane == 4, float4, float2>;
     const uint32_t lane = threadIdx.x % 32;
 #pragma unroll 1
-    for (uint32_t i = threadIdx.x / 32; i < rows * kParts; i += warps) {
+    for (uint32_t i = threadIdx.x / 32 - warp0; i < rows * kParts; i += warps) {
         const uint32_t r = i / kParts, d = (i % kParts * 32 + lane) * kPerLane;
         float m = -INFINITY, l = 0, o[kPerLane] = {};
 #pragma unroll 1
@@ -632,7 +632,7 @@ __global__ void __launch_bounds__(RowsShape<D, TS, RG, TILE, CPS, sizeof(T) == 4
         }
         bar_sync(1, kConsumers);
         if (nan_seen != 0) {
-            spread_nan(c, w, walk.u, walk.g, kConsumers, [&](uint32_t r, uint32_t d) {
+            spread_nan(c, w, walk.u, walk.g, 0, kConsumers, [&](uint32_t r, uint32_t d) {
                 if (slot == nullptr) out_at(r)[d] = from_f32<T>(NAN);
                 else slot[r * D + d] = NAN;
             });
@@ -652,7 +652,7 @@ __global__ void __launch_bounds__(RowsShape<D, TS, RG, TILE, CPS, sizeof(T) == 4
             bar_sync(1, kConsumers);
             if (is_last != 0) {
                 __threadfence();
-                join_partials<T, D>(c, w, walk.u.s.row0, walk.u.head, walk.r0, walk.rows, c0, shares, S::kWarps);
+                join_partials<T, D>(c, w, walk.u.s.row0, walk.u.head, walk.r0, walk.rows, c0, shares, 0, S::kWarps);
             }
         }
         bar_sync(1, kConsumers);  // nobody reads q, the joined rows or `walk` any more

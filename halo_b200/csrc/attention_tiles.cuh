@@ -1,0 +1,616 @@
+// ATTENTION for 16-bit operands and many rows to a sequence (prompts, chunks of prompts): tcgen05 products with fp16 operands, the cache's codes
+// converted to fp16 once for 256 packed rows (128 for heads of 256 elements).
+//
+//   x_t = q . k_t * (s_K(t) * scale * log2 e) + log2 s_V(t),   p_t = 2^(x_t - r + 6),   o = sum p_t code(v_t),   l = sum p_t / s_V(t),   out = o / l
+//
+// as in attention_rows.cuh; r is a reference that follows the running maximum lazily: the accumulators are rescaled only when a row's maximum
+// passes r by 8, so p_t is at most 2^14 and keeps 11 bits down to 2^-20 of the reference.
+//
+// Packed rows are the M side (a TMEM lane each), keys the N side of S = Q K^T, dims the N side of O = P V.  A CTA (one an SM) holds NS tiles of
+// 128 rows: two, each with scores, weights and accumulators of its own (128 + D columns), or one with two score buffers where D is 256.  A step
+// is (tile of 128 keys, row tile) and takes score buffer step % 2: while the softmax of one step runs, the tensor cores run the other's products.  The
+// weights overwrite the scores in TMEM as fp16 and are the A operand of P V from there.
+// Warps:
+//   0       tcgen05.mma issue;  1: TMEM allocation
+//   4-7     conversion: codes by 16-byte loads straight from their pages to registers, three slots ahead, to fp16 in a ring of eight
+//           16 KiB slots (a K slot: 128 keys x 64 dims; a V slot: 8192 / D keys x all dims, the N operand with dims contiguous);
+//           rows that no row of the CTA sees, missing pages and NaN codes of values become zeros (spread_nan puts the latter back)
+//   8-15    softmax, a thread to a row (8-11 where NS is 1); also q -> fp16 in shared memory, the epilogue, and the joining of shares
+// Work is dealt as in attention_work.cuh, so a causal prompt's long and short rows and a short chunk behind a long context fill the device alike.
+//
+// What bounds it: the tensor pipe and, for D = 128, the exponentials (256 x 128 of them per 2048 clocks of products at 16 a clock); shared memory
+// carries 128 bytes a clock, of which the products' operands take about 96.
+#pragma once
+#include "attention_rows.cuh"
+
+namespace halo_cuda {
+namespace attn {
+
+template <int D>
+struct TilesShape {
+    static constexpr int kStreams = D == 256 ? 1 : 2, kTile = 128, kRows = 128 * kStreams, kSlots = 8;
+    static constexpr uint32_t kSlot = 16384, kQ = kRows * D * 2;
+    static constexpr int kParts = D / 64;               // slots of a tile of K, and of V
+    static constexpr int kVTokens = 128 * 64 / D;       // keys of a V slot
+    static constexpr uint32_t kSmem = 1024 + kQ + kSlots * kSlot;
+    static constexpr int kSoftWarps = 4 * kStreams, kThreads = 256 + 32 * kSoftWarps;
+    static constexpr uint32_t kO = 256;                 // first accumulator column; scores are columns 0 .. 255
+    static constexpr int kLag = kStreams == 1 ? 1 : 0;  // V of a tile is fetched behind K of the next one
+};
+
+__device__ __forceinline__ uint64_t desc_k(uint32_t addr) {  // K-major, 128-byte rows and swizzle: atoms of 8 rows, 1024 bytes apart
+    return static_cast<uint64_t>((addr & 0x3FFFFu) >> 4) | (uint64_t{1} << 16) | (uint64_t{64} << 32) | (uint64_t{1} << 46) | (uint64_t{2} << 61);
+}
+__device__ __forceinline__ uint64_t desc_mn(uint32_t addr, uint32_t block) {  // N-major: atoms of 64 elements x 8 keys, 1024 bytes apart along the keys, `block` along N
+    return static_cast<uint64_t>((addr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(block >> 4) << 16) | (uint64_t{64} << 32) | (uint64_t{1} << 46) | (uint64_t{2} << 61);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add)
+                 : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(add)
+                 : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void tmem_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tmem_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+#define HALO_R8(v, i) "=r"(v[i]), "=r"(v[i + 1]), "=r"(v[i + 2]), "=r"(v[i + 3]), "=r"(v[i + 4]), "=r"(v[i + 5]), "=r"(v[i + 6]), "=r"(v[i + 7])
+#define HALO_W8(v, i) "r"(v[i]), "r"(v[i + 1]), "r"(v[i + 2]), "r"(v[i + 3]), "r"(v[i + 4]), "r"(v[i + 5]), "r"(v[i + 6]), "r"(v[i + 7])
+/// 32 columns of this warp's lanes.
+__device__ __forceinline__ void tmem_ld32(uint32_t at, uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : HALO_R8(v, 0), HALO_R8(v, 8), HALO_R8(v, 16), HALO_R8(v, 24)
+        : "r"(at)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t at, const uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::HALO_W8(v, 0),
+        HALO_W8(v, 8), HALO_W8(v, 16), HALO_W8(v, 24), "r"(at)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t (&v)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::HALO_W8(v, 0), HALO_W8(v, 8), "r"(at)
+                 : "memory");
+}
+#undef HALO_R8
+#undef HALO_W8
+__device__ __forceinline__ void sts128(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+/// Index of a tile's first K or V slot among its segment's slots (n tiles).
+template <int D>
+__device__ __forceinline__ uint32_t k_slot(uint32_t t) {
+    using S = TilesShape<D>;
+    return S::kLag == 0 ? 2 * t * S::kParts : (t == 0 ? 0 : 2 * t - 1) * S::kParts;
+}
+template <int D>
+__device__ __forceinline__ uint32_t v_slot(uint32_t t, uint32_t n) {
+    using S = TilesShape<D>;
+    return S::kLag == 0 ? (2 * t + 1) * S::kParts : (t + 1 < n ? 2 * t + 2 : 2 * n - 1) * S::kParts;
+}
+
+template <class T, int D>
+__global__ void __launch_bounds__(TilesShape<D>::kThreads, 1) tiles_kernel(const __grid_constant__ AttentionCall c, const __grid_constant__ Work w) {
+    using S = TilesShape<D>;
+    constexpr int kStreams = S::kStreams, kParts = S::kParts, kSlots = S::kSlots, kScaleTiles = 8;
+    extern __shared__ uint8_t raw_smem[];
+    __shared__ PlanSmem plan;
+    __shared__ uint64_t bars[2 * kSlots + 3 * 2 + 2];
+    __shared__ GroupScale scales[kScaleTiles][8];  // a tile's stay until the slots' ring has gone round behind it: at most six tiles ahead are written
+    __shared__ uint32_t partly[kScaleTiles];
+    __shared__ float q_unscale[S::kRows];
+    __shared__ uint32_t nan_seen, is_last, tmem_word;
+    __shared__ Walk walk;
+
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;");
+    const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    const uint32_t q_at = (smem_u32(raw_smem) + 1023u) & ~1023u, ring = q_at + S::kQ;
+    const uint32_t full = smem_u32(bars), empty = full + 8 * kSlots, s_full = empty + 8 * kSlots, p_ready = s_full + 16, pv_done = p_ready + 16, q_ready = pv_done + 16;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kSlots; ++i) {
+            mbar_init(full + 8 * i, 4);
+            mbar_init(empty + 8 * i, 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(s_full + 8 * i, 1);
+            mbar_init(p_ready + 8 * i, 4);
+            mbar_init(pv_done + 8 * i, 1);
+            mbar_init(q_ready + 8 * i, 4);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        nan_seen = 0;
+    }
+    {
+        Range range;
+        if (!find_range(c, w, plan, &range)) return;
+        if (threadIdx.x == 0) {
+            walk.range = range;
+            walk.u = range.unit;
+            walk.enter(w, range.unit_begin);
+        }
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_word)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tmem_before();
+    __syncthreads();
+    tmem_after();
+    const uint32_t tmem = tmem_word;
+    bool alive = true;  // no wait has run out; behind one nothing is waited for and the results are void (the context is lost)
+    auto wait = [&](uint32_t bar, uint32_t parity) {
+        if (alive) alive = __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity));
+    };
+    const Range range = walk.range;
+    __syncthreads();  // `walk` belongs to the softmax warps from here
+
+    if (warp == 0) {
+        // ---- products --------------------------------------------------------------------------------------------------------------------
+        constexpr uint32_t kScores = (1u << 4) | (128u / 8 << 17) | (128u / 16 << 24), kRowsOut = (1u << 4) | (1u << 16) | (static_cast<uint32_t>(D) / 8 << 17) | (128u / 16 << 24);
+        Unit u = range.unit;
+        uint64_t unit_begin = range.unit_begin;
+        uint32_t base = 0, segments = 0;
+        uint32_t uses[2] = {0, 0};  // of the score buffers, whose weights have been waited for
+        for (;;) {
+            const Segment g = segment(range, u, unit_begin);
+            const uint32_t n = static_cast<uint32_t>(g.hi - g.lo), steps = n * kStreams;
+            auto scores = [&](uint32_t i) {
+                const uint32_t t = i / kStreams, s = i % kStreams;
+                if (t == 0) wait(q_ready + 8 * s, segments & 1);
+                const uint32_t first = base + k_slot<D>(t);
+#pragma unroll
+                for (int part = 0; part < kParts; ++part) {
+                    const uint32_t slot = (first + part) % kSlots;
+                    if (s == 0) wait(full + 8 * slot, (first + part) / kSlots & 1);
+                    tmem_after();
+                    if (alive && elect_one()) {
+                        const uint64_t a = desc_k(q_at + (s * kParts + part) * 16384), b = desc_k(ring + slot * S::kSlot);
+#pragma unroll
+                        for (uint32_t k = 0; k < 4; ++k) mma_ss(tmem + i % 2 * 128, a + k * 2, b + k * 2, kScores, part + k != 0);
+                        if (s == kStreams - 1) mma_commit(empty + 8 * slot);
+                        if (part == kParts - 1) mma_commit(s_full + 8 * (i % 2));
+                    }
+                    __syncwarp();
+                }
+            };
+            auto rows = [&](uint32_t i) {
+                const uint32_t t = i / kStreams, s = i % kStreams, b = i % 2, use = b == 0 ? uses[0]++ : uses[1]++;
+                wait(p_ready + 8 * b, use & 1);
+                const uint32_t first = base + v_slot<D>(t, n);
+#pragma unroll
+                for (int part = 0; part < kParts; ++part) {
+                    const uint32_t slot = (first + part) % kSlots;
+                    if (s == 0) wait(full + 8 * slot, (first + part) / kSlots & 1);
+                    tmem_after();
+                    if (alive && elect_one()) {
+                        constexpr uint32_t kSteps = S::kVTokens / 16;
+                        const uint64_t v = desc_mn(ring + slot * S::kSlot, S::kVTokens * 128);
+#pragma unroll
+                        for (uint32_t k = 0; k < kSteps; ++k)
+                            mma_ts(tmem + S::kO + s * D, tmem + b * 128 + (part * kSteps + k) * 8, v + k * 128, kRowsOut, t + part + k != 0);
+                        if (s == kStreams - 1) mma_commit(empty + 8 * slot);
+                        if (part == kParts - 1) mma_commit(pv_done + 8 * b);
+                    }
+                    __syncwarp();
+                }
+            };
+            scores(0);
+            if (steps > 1) scores(1);
+            for (uint32_t i = 0; i < steps; ++i) {
+                rows(i);
+                if (i + 2 < steps) scores(i + 2);
+            }
+            base += 2 * n * kParts;
+            ++segments;
+            unit_begin = g.unit_end;
+            if (unit_begin >= range.end || !next_unit(c, w, u)) break;
+        }
+    } else if (warp >= 4 && warp < 8) {
+        // ---- conversion ------------------------------------------------------------------------------------------------------------------
+        const uint32_t thread = threadIdx.x - 128, cw = warp - 4;
+        uint4 raw[3][4];
+        uint32_t f = 0, kinds = 0;  // slots asked for; bit i of kinds: slot f - 1 - i is one of V
+        // this thread's 16-byte pieces of a slot: of K rows thread / 4 + 32 i, piece thread % 4; of V the two rows and four pieces of every eight lanes
+        // lie in eight different banks' groups
+        constexpr uint32_t kVRows = 32 / kParts;  // of V that the threads cover at a time
+        const uint32_t v_row = thread / 8 / kParts * 2 + thread / 4 % 2, v_piece = thread % 4 + thread / 8 % kParts * 4;
+        auto convert = [&](const uint4 (&x)[4], uint32_t at, bool is_v) {  // slot number `at`
+            const uint32_t slot = ring + at % kSlots * S::kSlot;
+            wait(empty + 8 * (at % kSlots), (at / kSlots & 1) ^ 1);
+            bool nan = false;
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) {
+                const uint32_t row = is_v ? v_row + kVRows * i : thread / 4 + 32 * i;
+                const uint32_t row_at = slot + (is_v ? thread / 8 % kParts * (S::kVTokens * 128) : 0) + row * 128, piece = 2 * (thread % 4);
+                uint32_t word[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+                if (is_v) {
+#pragma unroll
+                    for (uint32_t j = 0; j < 4; ++j) nan |= drop_nan(word[j]);
+                }
+#pragma unroll
+                for (uint32_t h = 0; h < 2; ++h)
+                    sts128(row_at + (((piece + h) ^ (row & 7)) << 4), widen_lo(word[2 * h]), widen_hi(word[2 * h]), widen_lo(word[2 * h + 1]), widen_hi(word[2 * h + 1]));
+            }
+            if (nan) nan_seen = 1;
+            proxy_fence();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(full + 8 * (at % kSlots));
+        };
+        Unit u = range.unit;
+        uint64_t unit_begin = range.unit_begin;
+        const float scale = c.scale * 1.4426950408889634f;
+        uint32_t tiles = 0;  // of this CTA so far
+        for (;;) {
+            const Segment g = segment(range, u, unit_begin);
+            const int32_t n = g.hi - g.lo;
+            const uint32_t r0 = u.row0(w), r1 = r0 + u.rows(w) - 1;
+            const int32_t any_lo = first_key(u.s, w.window, r0 / c.group), any_hi = end_key(u.s, c.causal, r1 / c.group);
+            // lane i < 8 of every warp knows page and scale bytes of the i-th 16 keys of a tile: of the tile at hand, the one behind and the next
+            int32_t page = -1, page_behind = -1, page_next = -1;
+            uint32_t k_next = 0, v_next = 0;
+            auto fetch = [&](int32_t tile) {
+                const int32_t t = tile * 128 + static_cast<int32_t>(lane) * 16;
+                page_next = -1;
+                if (lane < 8 && tile < g.hi && t < any_hi && t + 16 > any_lo) {
+                    const int32_t p = page_of(c.cache, u.seq, t >> c.cache.page_shift);
+                    page_next = static_cast<uint32_t>(p) < c.cache.n_pages ? p : -2;  // -2: a visible key's page is not there
+                    if (page_next >= 0) {
+                        const uint64_t at = p * c.cache.scale_stride + u.head;
+                        k_next = __ldg(c.cache.k_scale + at);
+                        v_next = __ldg(c.cache.v_scale + at);
+                    }
+                }
+            };
+            fetch(g.lo);
+            for (int32_t phase = 0; phase < n + S::kLag; ++phase) {
+                page_behind = page;
+                page = page_next;
+                if (phase < n) {
+                    if (cw == 0) {
+                        GroupScale& s = scales[tiles % kScaleTiles][lane % 8];
+                        const int32_t v = scale_byte(v_next) - 127;
+                        if (lane < 8) {
+                            s.k = page >= 0 ? exp2_int(scale_byte(k_next) - 127) * scale : 0.0f;
+                            s.log_v = page >= 0 ? static_cast<float>(v) : -INFINITY;
+                            s.inv_v = page >= 0 ? exp2_int(-v) : 0.0f;
+                            if (page == -2 && c.status != nullptr) atomicOr(c.status, 8u);  // kStatusBadIndex
+                        }
+                        const uint32_t here = __ballot_sync(0xFFFFFFFFu, page >= 0) & 255u;
+                        if (lane == 0) partly[tiles % kScaleTiles] = here != 255u;
+                    }
+                    ++tiles;
+                }
+                if (phase + 1 < n) fetch(g.lo + phase + 1);
+                const uint32_t slots = (phase < n ? kParts : 0) + (phase >= S::kLag ? kParts : 0);
+                for (uint32_t j = 0; j < slots; ++j) {
+                    const bool is_v = phase >= n || j >= kParts;
+                    const uint32_t part = j % kParts;
+                    const int32_t t0 = (g.lo + phase - (is_v ? S::kLag : 0)) * 128;
+                    const int32_t pages = is_v && S::kLag != 0 ? page_behind : page;
+                    const uint8_t* pool = is_v ? c.cache.v : c.cache.k;
+                    auto load = [&](uint4 (&x)[4]) {
+#pragma unroll
+                        for (uint32_t i = 0; i < 4; ++i) {
+                            const uint32_t row = is_v ? part * S::kVTokens + v_row + kVRows * i : thread / 4 + 32 * i;
+                            const int32_t p = __shfl_sync(0xFFFFFFFFu, pages, row / 16), t = t0 + static_cast<int32_t>(row);
+                            x[i] = make_uint4(0, 0, 0, 0);
+                            if (p >= 0 && t >= any_lo && t < any_hi) {
+                                const uint64_t at = p * c.cache.page_stride + (uint64_t{u.head} << c.cache.page_shift | (t & (c.cache.page_tokens - 1))) * D;
+                                x[i] = __ldg(reinterpret_cast<const uint4*>(pool + at + (is_v ? v_piece * 16 : part * 64 + thread % 4 * 16)));
+                            }
+                        }
+                    };
+                    // slot f is asked for, slot f - 2 converted; the buffers' numbers have to be known at compile time
+                    if (f % 3 == 0) {
+                        load(raw[0]);
+                        if (f >= 2) convert(raw[1], f - 2, kinds >> 1 & 1);
+                    } else if (f % 3 == 1) {
+                        load(raw[1]);
+                        if (f >= 2) convert(raw[2], f - 2, kinds >> 1 & 1);
+                    } else {
+                        load(raw[2]);
+                        convert(raw[0], f - 2, kinds >> 1 & 1);
+                    }
+                    kinds = kinds << 1 | (is_v ? 1u : 0u);
+                    ++f;
+                }
+            }
+            unit_begin = g.unit_end;
+            if (unit_begin >= range.end || !next_unit(c, w, u)) break;
+        }
+        for (uint32_t i = 2; i != 0; --i) {  // at least one tile's two slots were asked for
+            const uint32_t at = f - i;
+            if (at % 3 == 0) convert(raw[0], at, kinds >> (i - 1) & 1);
+            else if (at % 3 == 1) convert(raw[1], at, kinds >> (i - 1) & 1);
+            else convert(raw[2], at, kinds >> (i - 1) & 1);
+        }
+    } else if (warp >= 8) {
+        // ---- softmax ---------------------------------------------------------------------------------------------------------------------
+        constexpr uint32_t kSoft = S::kSoftWarps * 32;
+        const uint32_t stream = (warp - 8) / 4, quarter = warp % 4, r = stream * 128 + quarter * 32 + lane;  // this thread's row of the unit
+        const uint32_t lanes = quarter * 32 << 16, o_at = tmem + lanes + S::kO + stream * D;
+        uint32_t uses[2] = {0, 0}, tiles = 0;
+        const bool leader = threadIdx.x == 256;
+        do {
+            // q: eight lanes to a row
+            {
+                constexpr int E = D / 8, kVecs = E * 2 / 16, kBatch = 16 / kVecs < 4 ? 16 / kVecs : 4;
+                const uint32_t l8 = lane % 8, rows = walk.rows, r0 = walk.r0;
+                for (int it = 0; it < 8; it += kBatch) {
+                    uint4 v[kBatch][kVecs];
+#pragma unroll
+                    for (int b = 0; b < kBatch; ++b) {
+                        const uint32_t row = stream * 128 + quarter * 32 + (it + b) * 4 + lane / 8, p = r0 + min(row, rows - 1);
+                        const uint32_t j = p / c.group, h = walk.u.head * c.group + p % c.group;
+                        const uint8_t* q = c.q.p + uint64_t{walk.u.s.row0 + j} * c.q.token_stride + uint64_t{h} * c.q.head_stride + l8 * (E * 2);
+#pragma unroll
+                        for (int k = 0; k < kVecs; ++k) {
+                            if (c.q.vec) v[b][k] = __ldg(reinterpret_cast<const uint4*>(q) + k);
+                            else {
+                                uint32_t x[4];
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    const uint16_t* at = reinterpret_cast<const uint16_t*>(q) + 8 * k + 2 * e;
+                                    x[e] = at[0] | static_cast<uint32_t>(at[1]) << 16;
+                                }
+                                v[b][k] = make_uint4(x[0], x[1], x[2], x[3]);
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int b = 0; b < kBatch; ++b) {
+                        const uint32_t in_tile = quarter * 32 + (it + b) * 4 + lane / 8, row = stream * 128 + in_tile;
+                        float x[E], top = 0;
+#pragma unroll
+                        for (int k = 0; k < kVecs; ++k) {
+                            T e8[8];
+                            __builtin_memcpy(e8, &v[b][k], 16);
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) {
+                                x[8 * k + e] = row < rows ? to_f32(e8[e]) : 0.0f;
+                                top = fmaxf(top, fabsf(x[8 * k + e]) < INFINITY ? fabsf(x[8 * k + e]) : 0.0f);
+                            }
+                        }
+#pragma unroll
+                        for (int d = 4; d != 0; d /= 2) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+                        const int32_t exponent = max(static_cast<int32_t>(__float_as_uint(top) >> 23) - 127, -100);
+                        const float by = exp2_int(14 - exponent);
+                        if (l8 == 0) q_unscale[row] = exp2_int(exponent - 14);
+#pragma unroll
+                        for (int k = 0; k < kVecs; ++k) {
+                            const uint32_t d = l8 * E + 8 * k;  // 64-element blocks of [128 rows][128 bytes]
+                            sts128(q_at + (stream * kParts + d / 64) * 16384 + in_tile * 128 + ((d % 64 / 8 ^ (in_tile & 7)) << 4), half2_bits(x[8 * k] * by, x[8 * k + 1] * by),
+                                   half2_bits(x[8 * k + 2] * by, x[8 * k + 3] * by), half2_bits(x[8 * k + 4] * by, x[8 * k + 5] * by), half2_bits(x[8 * k + 6] * by, x[8 * k + 7] * by));
+                        }
+                    }
+                }
+                proxy_fence();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(q_ready + 8 * stream);
+            }
+            const float qs = q_unscale[r];
+            const uint32_t p = walk.r0 + min(r, walk.rows - 1), j = p / c.group;
+            const int32_t lo = first_key(walk.u.s, w.window, j), hi = end_key(walk.u.s, c.causal, j);
+            // keys that every row of this row tile sees (a tile without rows sees none of them: nothing of it is kept)
+            const uint32_t first_row = walk.r0 + min(stream * 128, walk.rows - 1), last_row = walk.r0 + min(stream * 128 + 127, walk.rows - 1);
+            const int32_t all_lo = first_key(walk.u.s, w.window, last_row / c.group), all_hi = end_key(walk.u.s, c.causal, first_row / c.group);
+            const int32_t last_tile = walk.g.hi;
+            float ref = -INFINITY, l = 0;
+            uint32_t prev_bar = 0, prev_parity = 0;
+            uint32_t b = kStreams == 2 ? stream : 0;
+            for (int32_t tile = walk.g.lo; tile < last_tile; ++tile) {
+                const uint32_t use = b == 0 ? uses[0]++ : uses[1]++, s_at = tmem + lanes + b * 128;
+                wait(s_full + 8 * b, use & 1);
+                tmem_after();
+                const GroupScale* sc = scales[tiles % kScaleTiles];
+                const int32_t t0 = tile * 128;
+                const bool masked = t0 < all_lo || t0 + 128 > all_hi || partly[tiles % kScaleTiles] != 0;
+                uint32_t x[2][32];
+                float top = -INFINITY;
+                tmem_ld32(s_at, x[0]);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    tmem_wait_ld();
+                    if (q < 3) tmem_ld32(s_at + 32 * (q + 1), x[(q + 1) % 2]);
+                    uint32_t(&v)[32] = x[q % 2];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const GroupScale s = sc[2 * q + i];
+                        const float by = s.k * qs;
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            float y = fmaf(__uint_as_float(v[16 * i + e]), by, s.log_v);
+                            if (masked) {
+                                const int32_t t = t0 + 32 * q + 16 * i + e;
+                                if (t < lo || t >= hi || s.log_v == -INFINITY) y = -INFINITY;
+                            }
+                            top = fmaxf(top, y);
+                        }
+                    }
+                }
+                const float next = fmaxf(ref, top);
+                const bool first = ref == -INFINITY, grows = !first && next > ref + 8.0f;
+                if (__any_sync(0xFFFFFFFFu, grows)) {
+                    // the products into the accumulators so far have to be done; a row without a reference has accumulators of zero, or NaN
+                    const float fade = grows ? exp2_approx(ref - next) : 1.0f;
+                    wait(prev_bar, prev_parity);
+                    tmem_after();
+#pragma unroll 1
+                    for (int d = 0; d < D; d += 32) {
+                        uint32_t o[32];
+                        tmem_ld32(o_at + d, o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * fade);
+                        tmem_st32(o_at + d, o);
+                    }
+                    tmem_wait_st();
+                    l *= fade;
+                }
+                if (first || grows) ref = next;
+                const float base = ref == -INFINITY ? 0.0f : ref - 6.0f;
+                tmem_ld32(s_at, x[0]);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    tmem_wait_ld();
+                    if (q < 3) tmem_ld32(s_at + 32 * (q + 1), x[(q + 1) % 2]);
+                    uint32_t(&v)[32] = x[q % 2];
+                    uint32_t weights[16];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const GroupScale s = sc[2 * q + i];
+                        const float by = s.k * qs, add = s.log_v - base;
+                        float sum = 0;
+#pragma unroll
+                        for (int e = 0; e < 16; e += 2) {
+                            float y[2];
+#pragma unroll
+                            for (int k = 0; k < 2; ++k) {
+                                y[k] = fmaf(__uint_as_float(v[16 * i + e + k]), by, add);
+                                if (masked) {
+                                    const int32_t t = t0 + 32 * q + 16 * i + e + k;
+                                    if (t < lo || t >= hi || s.log_v == -INFINITY) y[k] = -INFINITY;
+                                }
+                                y[k] = exp2_approx(y[k]);
+                            }
+                            sum += y[0] + y[1];
+                            weights[8 * i + e / 2] = half2_bits(y[0], y[1]);
+                        }
+                        l = fmaf(sum, s.inv_v, l);
+                    }
+                    tmem_st16(s_at + 16 * q, weights);  // columns whose scores have been read
+                }
+                tmem_wait_st();
+                tmem_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_ready + 8 * b);
+                prev_bar = pv_done + 8 * b, prev_parity = use & 1;
+                if (kStreams == 1) b ^= 1;
+                ++tiles;
+            }
+            wait(prev_bar, prev_parity);
+            tmem_after();
+            // ---- the segment's rows ------------------------------------------------------------------------------------------------------
+            const bool keep = r < walk.rows;
+            float* slot = walk.g.whole() ? nullptr : partial_slot(w, D, blockIdx.x, walk.g.from_start) + r * D;
+            auto out_at = [&](uint32_t row) {
+                const uint32_t p = walk.r0 + row, j = p / c.group, h = walk.u.head * c.group + p % c.group;
+                return reinterpret_cast<T*>(c.out.p + uint64_t{walk.u.s.row0 + j} * c.out.token_stride + uint64_t{h} * c.out.head_stride);
+            };
+            T* out = out_at(min(r, walk.rows - 1));
+            const float inv = l != 0 ? 1.0f / l : 0.0f;
+#pragma unroll 1
+            for (int d = 0; d < D; d += 32) {
+                uint32_t o[32];
+                tmem_ld32(o_at + d, o);
+                tmem_wait_ld();
+                if (!keep) continue;
+                if (slot != nullptr) {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4) *reinterpret_cast<uint4*>(slot + d + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                } else {
+                    T y[32];
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) y[e] = from_f32<T>(__uint_as_float(o[e]) * inv);
+                    if (c.out.vec) {
+#pragma unroll
+                        for (int e = 0; e < 32; e += 8) {
+                            uint4 v;
+                            __builtin_memcpy(&v, &y[e], 16);
+                            *reinterpret_cast<uint4*>(out + d + e) = v;
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) out[d + e] = y[e];
+                    }
+                }
+            }
+            if (keep && slot != nullptr) {
+                float* ml = partial_slot(w, D, blockIdx.x, walk.g.from_start) + w.rows * D + 2 * r;
+                *reinterpret_cast<float2*>(ml) = make_float2(ref, l);
+            }
+            tmem_before();
+            bar_sync(1, kSoft);
+            if (nan_seen != 0) {  // stays set: the conversion is ahead, and what it saw may belong to a segment to come
+                spread_nan(c, w, walk.u, walk.g, 256, kSoft, [&](uint32_t row, uint32_t d) {
+                    if (walk.g.whole()) out_at(row)[d] = from_f32<T>(NAN);
+                    else partial_slot(w, D, blockIdx.x, walk.g.from_start)[row * D + d] = NAN;
+                });
+                bar_sync(1, kSoft);
+            }
+            if (!walk.g.whole()) {
+                const uint32_t c0 = owner(walk.g.unit_begin, range.total, range.ctas), shares = owner(walk.g.unit_end - 1, range.total, range.ctas) - c0 + 1;
+                __threadfence();
+                bar_sync(1, kSoft);
+                if (leader) {
+                    const bool last = atomicAdd(w.counters + c0, 1u) == shares - 1;
+                    if (last) w.counters[c0] = 0;
+                    is_last = last;
+                }
+                bar_sync(1, kSoft);
+                if (is_last != 0) {
+                    __threadfence();
+                    join_partials<T, D>(c, w, walk.u.s.row0, walk.u.head, walk.r0, walk.rows, c0, shares, 8, S::kSoftWarps);
+                }
+            }
+            bar_sync(1, kSoft);  // nobody reads `walk` any more
+            if (leader) walk.advance(c, w);
+            bar_sync(1, kSoft);
+        } while (walk.more != 0);
+    }
+    if (!alive && lane == 0) atomicOr(w.error_word, 1u);
+    tmem_before();
+    __syncthreads();
+    if (warp == 1) {
+        tmem_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
+}
+
+template <class T, int D>
+int launch_tiles_kernel(HaloCudaCtx* ctx, const AttentionCall& c, Work w, cudaStream_t s) {
+    using S = TilesShape<D>;
+    w.rows = S::kRows;
+    w.tile = S::kTile;
+    w.least = 1;
+    w.row_tiles = (c.rows.max_tokens * c.group + S::kRows - 1) / S::kRows;
+    w.lanes = 1;
+    while (w.lanes < 32 && w.lanes < w.row_tiles) w.lanes *= 2;
+    const uint32_t ctas = static_cast<uint32_t>(ctx->prop.multiProcessorCount);
+    void* p = nullptr;
+    if (int rc = workspace(ctx, 5, ctas * sizeof(uint32_t), s, &p, true)) return rc;
+    w.counters = static_cast<uint32_t*>(p);
+    if (int rc = workspace(ctx, 6, partial_bytes(S::kRows, D, ctas), s, &p)) return rc;
+    w.partials = static_cast<float*>(p);
+    w.error_word = ctx->error_word_dev;
+    auto kernel = tiles_kernel<T, D>;
+    if (int rc = allow_dynamic_smem(ctx, reinterpret_cast<const void*>(kernel), S::kSmem)) return rc;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(ctas);
+    cfg.blockDim = dim3(S::kThreads);
+    cfg.dynamicSmemBytes = S::kSmem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    HC_CUDA(cudaLaunchKernelEx(&cfg, kernel, c, w));
+    return 0;
+}
+
+}  // namespace attn
+}  // namespace halo_cuda
