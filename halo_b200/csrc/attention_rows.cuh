@@ -81,9 +81,11 @@ __device__ __forceinline__ uint32_t half2_rest(float a, float b, uint32_t first)
     const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&first));
     return half2_bits(a - f.x, b - f.y);
 }
+/// Bit 7 of every byte of four that is a NaN code, 0x7F or 0xFF.
+__device__ __forceinline__ uint32_t nan_bits(uint32_t w) { return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u; }
 /// Zeroes the NaN codes of four; true if there were any.
 __device__ __forceinline__ bool drop_nan(uint32_t& w) {
-    const uint32_t hit = ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;  // bit 7 of a byte that is 0x7F or 0xFF
+    const uint32_t hit = nan_bits(w);
     if (hit == 0) return false;
     w &= ~((hit >> 7) * 255u);
     return true;
@@ -156,24 +158,6 @@ __device__ __forceinline__ void join_partials(const AttentionCall& c, const Work
     }
 }
 
-/// Where a CTA's consumers are: in shared memory, so that the walk over the tiles has the registers.
-struct Walk {
-    Range range;
-    Unit u;
-    Segment g;
-    uint32_t rows, r0;  // of the unit
-    uint32_t more;
-    __device__ void enter(const Work& w, uint64_t unit_begin) {
-        g = segment(range, u, unit_begin);
-        rows = u.rows(w), r0 = u.row0(w);
-        more = 1;
-    }
-    __device__ void advance(const AttentionCall& c, const Work& w) {
-        more = g.unit_end < range.end && next_unit(c, w, u);
-        if (more) enter(w, g.unit_end);
-    }
-};
-
 template <class T, int D, int TS, int RG, int TILE, int CPS>
 __global__ void __launch_bounds__(RowsShape<D, TS, RG, TILE, CPS, sizeof(T) == 4 ? 2 : 1>::kThreads, CPS)
     rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const __grid_constant__ AttentionCall c,
@@ -216,7 +200,7 @@ __global__ void __launch_bounds__(RowsShape<D, TS, RG, TILE, CPS, sizeof(T) == 4
         if (threadIdx.x == 0) {
             walk.range = range;
             walk.u = range.unit;
-            walk.enter(w, range.unit_begin);
+            walk.enter(c, w, range.unit_begin);
         }
     }
     __syncthreads();
@@ -325,15 +309,14 @@ __global__ void __launch_bounds__(RowsShape<D, TS, RG, TILE, CPS, sizeof(T) == 4
     do {
         // q: a warp takes a row at a time, scales it and stores its fp16 terms in the order of the products' operands
         const Unit& u = walk.u;
-        const uint32_t rows = walk.rows, r0 = walk.r0;
+        const uint32_t rows = walk.rows;
         constexpr int E = D / 32, kEach = (S::kRows + S::kWarps - 1) / S::kWarps, kBatch = kEach < 4 ? kEach : 4;  // rows of a warp whose loads are under way together
         for (uint32_t first = warp; first < rows; first += S::kWarps * kBatch) {
             T raw[kBatch][E];
 #pragma unroll
             for (int n = 0; n < kBatch; ++n) {
                 const uint32_t r = min(first + n * S::kWarps, rows - 1);
-                const uint32_t j = (r0 + r) / c.group, h = u.head * c.group + (r0 + r) % c.group;
-                const T* q = reinterpret_cast<const T*>(c.q.p + uint64_t{u.s.row0 + j} * c.q.token_stride + uint64_t{h} * c.q.head_stride) + lane * E;
+                const T* q = reinterpret_cast<const T*>(walk.at(c, w, c.q, r)) + lane * E;
                 if (c.q.vec) {
                     constexpr int kBytes = E * sizeof(T) < 16 ? E * sizeof(T) : 16, kPer = kBytes / sizeof(T);
                     using Word = std::conditional_t<kBytes == 16, uint4, std::conditional_t<kBytes == 8, uint2, uint32_t>>;
@@ -385,14 +368,15 @@ __global__ void __launch_bounds__(RowsShape<D, TS, RG, TILE, CPS, sizeof(T) == 4
         float qs[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const uint32_t r = rg * 16 + g8 + 8 * i, j = (r0 + min(r, rows - 1)) / c.group;
+            const uint32_t r = rg * 16 + g8 + 8 * i, j = walk.token(w, min(r, rows - 1));
             lo[i] = first_key(u.s, w.window, j);
             hi[i] = end_key(u.s, c.causal, j);
             qs[i] = q_unscale[r];
         }
         // tiles that every row sees whole, and what any row sees
-        const int32_t all_lo = first_key(u.s, w.window, (r0 + rows - 1) / c.group), all_hi = end_key(u.s, c.causal, r0 / c.group);
-        const int32_t any_lo = first_key(u.s, w.window, r0 / c.group), any_hi = end_key(u.s, c.causal, (r0 + rows - 1) / c.group);
+        const uint32_t first_token = walk.token0, last_token = walk.token(w, rows - 1);
+        const int32_t all_lo = first_key(u.s, w.window, last_token), all_hi = end_key(u.s, c.causal, first_token);
+        const int32_t any_lo = first_key(u.s, w.window, first_token), any_hi = end_key(u.s, c.causal, last_token);
 
         float o[kParts][kChunk][4];
 #pragma unroll
@@ -574,8 +558,7 @@ __global__ void __launch_bounds__(RowsShape<D, TS, RG, TILE, CPS, sizeof(T) == 4
         const Segment& g = walk.g;
         float* slot = g.whole() ? nullptr : partial_slot(w, D, blockIdx.x, g.from_start);
         auto out_at = [&](uint32_t r) {
-            const uint32_t p = walk.r0 + r, j = p / c.group, h = walk.u.head * c.group + p % c.group;
-            return reinterpret_cast<T*>(c.out.p + uint64_t{walk.u.s.row0 + j} * c.out.token_stride + uint64_t{h} * c.out.head_stride);
+            return reinterpret_cast<T*>(walk.at(c, w, c.out, r));
         };
         if (t4 == 0) row_ml[rg][ts][g8] = make_float2(m[0], l[0]), row_ml[rg][ts][g8 + 8] = make_float2(m[1], l[1]);
         bar_sync(1, kConsumers);
@@ -672,6 +655,8 @@ int launch_rows_kernel(HaloCudaCtx* ctx, const AttentionCall& c, Work w, cudaStr
     w.rows = S::kRows;
     w.tile = S::kTile;
     w.least = 1;
+    w.group = c.group;
+    w.group_inverse = static_cast<uint32_t>((0xFFFFFFFFull + c.group) / c.group);
     w.row_tiles = (c.rows.max_tokens * c.group + S::kRows - 1) / S::kRows;
     w.lanes = 1;
     while (w.lanes < 32 && w.lanes < w.row_tiles) w.lanes *= 2;

@@ -85,6 +85,22 @@ __device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t (&v)[16]) 
 }
 #undef HALO_R8
 #undef HALO_W8
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+    return d;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
 __device__ __forceinline__ void sts128(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
@@ -109,10 +125,9 @@ __global__ void __launch_bounds__(TilesShape<D>::kThreads, 1) tiles_kernel(const
     __shared__ PlanSmem plan;
     __shared__ uint64_t bars[2 * kSlots + 3 * 2 + 2];
     __shared__ GroupScale scales[kScaleTiles][8];  // a tile's stay until the slots' ring has gone round behind it: at most six tiles ahead are written
-    __shared__ uint32_t partly[kScaleTiles];
     __shared__ float q_unscale[S::kRows];
     __shared__ uint32_t nan_seen, is_last, tmem_word;
-    __shared__ Walk walk;
+    __shared__ Walk walks[2];  // the segment at hand and the next one, in turn
 
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
@@ -137,9 +152,9 @@ __global__ void __launch_bounds__(TilesShape<D>::kThreads, 1) tiles_kernel(const
         Range range;
         if (!find_range(c, w, plan, &range)) return;
         if (threadIdx.x == 0) {
-            walk.range = range;
-            walk.u = range.unit;
-            walk.enter(w, range.unit_begin);
+            walks[0].range = range;
+            walks[0].u = range.unit;
+            walks[0].enter(c, w, range.unit_begin);
         }
     }
     if (warp == 1) {
@@ -154,8 +169,8 @@ __global__ void __launch_bounds__(TilesShape<D>::kThreads, 1) tiles_kernel(const
     auto wait = [&](uint32_t bar, uint32_t parity) {
         if (alive) alive = __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity));
     };
-    const Range range = walk.range;
-    __syncthreads();  // `walk` belongs to the softmax warps from here
+    const Range range = walks[0].range;
+    __syncthreads();  // `walks` belong to the softmax warps from here
 
     if (warp == 0) {
         // ---- products --------------------------------------------------------------------------------------------------------------------
@@ -236,9 +251,10 @@ __global__ void __launch_bounds__(TilesShape<D>::kThreads, 1) tiles_kernel(const
                 const uint32_t row = is_v ? v_row + kVRows * i : thread / 4 + 32 * i;
                 const uint32_t row_at = slot + (is_v ? thread / 8 % kParts * (S::kVTokens * 128) : 0) + row * 128, piece = 2 * (thread % 4);
                 uint32_t word[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-                if (is_v) {
+                if (is_v && (nan_bits(word[0]) | nan_bits(word[1]) | nan_bits(word[2]) | nan_bits(word[3])) != 0) {
+                    nan = true;
 #pragma unroll
-                    for (uint32_t j = 0; j < 4; ++j) nan |= drop_nan(word[j]);
+                    for (uint32_t j = 0; j < 4; ++j) drop_nan(word[j]);
                 }
 #pragma unroll
                 for (uint32_t h = 0; h < 2; ++h)
@@ -251,7 +267,7 @@ __global__ void __launch_bounds__(TilesShape<D>::kThreads, 1) tiles_kernel(const
         };
         Unit u = range.unit;
         uint64_t unit_begin = range.unit_begin;
-        const float scale = c.scale * 1.4426950408889634f;
+        const float scale = fabsf(c.scale) * 1.4426950408889634f;  // its sign is q's
         uint32_t tiles = 0;  // of this CTA so far
         for (;;) {
             const Segment g = segment(range, u, unit_begin);
@@ -288,8 +304,6 @@ __global__ void __launch_bounds__(TilesShape<D>::kThreads, 1) tiles_kernel(const
                             s.inv_v = page >= 0 ? exp2_int(-v) : 0.0f;
                             if (page == -2 && c.status != nullptr) atomicOr(c.status, 8u);  // kStatusBadIndex
                         }
-                        const uint32_t here = __ballot_sync(0xFFFFFFFFu, page >= 0) & 255u;
-                        if (lane == 0) partly[tiles % kScaleTiles] = here != 255u;
                     }
                     ++tiles;
                 }
@@ -300,17 +314,17 @@ __global__ void __launch_bounds__(TilesShape<D>::kThreads, 1) tiles_kernel(const
                     const uint32_t part = j % kParts;
                     const int32_t t0 = (g.lo + phase - (is_v ? S::kLag : 0)) * 128;
                     const int32_t pages = is_v && S::kLag != 0 ? page_behind : page;
-                    const uint8_t* pool = is_v ? c.cache.v : c.cache.k;
+                    const uint8_t* pool = (is_v ? c.cache.v : c.cache.k) + (uint64_t{u.head} << c.cache.page_shift) * D + (is_v ? v_piece * 16 : part * 64 + thread % 4 * 16);
+                    const uint32_t row0 = is_v ? part * S::kVTokens + v_row : thread / 4, every = is_v ? kVRows : 32;
+                    const bool inside = t0 >= any_lo && t0 + 128 <= any_hi;
                     auto load = [&](uint4 (&x)[4]) {
 #pragma unroll
                         for (uint32_t i = 0; i < 4; ++i) {
-                            const uint32_t row = is_v ? part * S::kVTokens + v_row + kVRows * i : thread / 4 + 32 * i;
+                            const uint32_t row = row0 + every * i;  // (a tile begins with a page)
                             const int32_t p = __shfl_sync(0xFFFFFFFFu, pages, row / 16), t = t0 + static_cast<int32_t>(row);
                             x[i] = make_uint4(0, 0, 0, 0);
-                            if (p >= 0 && t >= any_lo && t < any_hi) {
-                                const uint64_t at = p * c.cache.page_stride + (uint64_t{u.head} << c.cache.page_shift | (t & (c.cache.page_tokens - 1))) * D;
-                                x[i] = __ldg(reinterpret_cast<const uint4*>(pool + at + (is_v ? v_piece * 16 : part * 64 + thread % 4 * 16)));
-                            }
+                            if (p >= 0 && (inside || (t >= any_lo && t < any_hi)))
+                                x[i] = __ldg(reinterpret_cast<const uint4*>(pool + static_cast<uint32_t>(p) * c.cache.page_stride + (row & (c.cache.page_tokens - 1)) * D));
                         }
                     };
                     // slot f is asked for, slot f - 2 converted; the buffers' numbers have to be known at compile time
@@ -344,69 +358,74 @@ __global__ void __launch_bounds__(TilesShape<D>::kThreads, 1) tiles_kernel(const
         const uint32_t lanes = quarter * 32 << 16, o_at = tmem + lanes + S::kO + stream * D;
         uint32_t uses[2] = {0, 0}, tiles = 0;
         const bool leader = threadIdx.x == 256;
-        do {
-            // q: eight lanes to a row
-            {
-                constexpr int E = D / 8, kVecs = E * 2 / 16, kBatch = 16 / kVecs < 4 ? 16 / kVecs : 4;
-                const uint32_t l8 = lane % 8, rows = walk.rows, r0 = walk.r0;
-                for (int it = 0; it < 8; it += kBatch) {
-                    uint4 v[kBatch][kVecs];
+        // q: eight lanes to a row
+        auto load_q = [&](const Walk& walk) {
+            constexpr int E = D / 8, kVecs = E * 2 / 16, kBatch = 16 / kVecs < 4 ? 16 / kVecs : 4;
+            const uint32_t l8 = lane % 8, rows = walk.rows;
+            for (int it = 0; it < 8; it += kBatch) {
+                uint4 v[kBatch][kVecs];
 #pragma unroll
-                    for (int b = 0; b < kBatch; ++b) {
-                        const uint32_t row = stream * 128 + quarter * 32 + (it + b) * 4 + lane / 8, p = r0 + min(row, rows - 1);
-                        const uint32_t j = p / c.group, h = walk.u.head * c.group + p % c.group;
-                        const uint8_t* q = c.q.p + uint64_t{walk.u.s.row0 + j} * c.q.token_stride + uint64_t{h} * c.q.head_stride + l8 * (E * 2);
+                for (int b = 0; b < kBatch; ++b) {
+                    const uint32_t row = stream * 128 + quarter * 32 + (it + b) * 4 + lane / 8;
+                    const uint8_t* q = walk.at(c, w, c.q, min(row, rows - 1)) + l8 * (E * 2);
 #pragma unroll
-                        for (int k = 0; k < kVecs; ++k) {
-                            if (c.q.vec) v[b][k] = __ldg(reinterpret_cast<const uint4*>(q) + k);
-                            else {
-                                uint32_t x[4];
+                    for (int k = 0; k < kVecs; ++k) {
+                        if (c.q.vec) v[b][k] = __ldg(reinterpret_cast<const uint4*>(q) + k);
+                        else {
+                            uint32_t x[4];
 #pragma unroll
-                                for (int e = 0; e < 4; ++e) {
-                                    const uint16_t* at = reinterpret_cast<const uint16_t*>(q) + 8 * k + 2 * e;
-                                    x[e] = at[0] | static_cast<uint32_t>(at[1]) << 16;
-                                }
-                                v[b][k] = make_uint4(x[0], x[1], x[2], x[3]);
+                            for (int e = 0; e < 4; ++e) {
+                                const uint16_t* at = reinterpret_cast<const uint16_t*>(q) + 8 * k + 2 * e;
+                                x[e] = at[0] | static_cast<uint32_t>(at[1]) << 16;
                             }
-                        }
-                    }
-#pragma unroll
-                    for (int b = 0; b < kBatch; ++b) {
-                        const uint32_t in_tile = quarter * 32 + (it + b) * 4 + lane / 8, row = stream * 128 + in_tile;
-                        float x[E], top = 0;
-#pragma unroll
-                        for (int k = 0; k < kVecs; ++k) {
-                            T e8[8];
-                            __builtin_memcpy(e8, &v[b][k], 16);
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) {
-                                x[8 * k + e] = row < rows ? to_f32(e8[e]) : 0.0f;
-                                top = fmaxf(top, fabsf(x[8 * k + e]) < INFINITY ? fabsf(x[8 * k + e]) : 0.0f);
-                            }
-                        }
-#pragma unroll
-                        for (int d = 4; d != 0; d /= 2) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
-                        const int32_t exponent = max(static_cast<int32_t>(__float_as_uint(top) >> 23) - 127, -100);
-                        const float by = exp2_int(14 - exponent);
-                        if (l8 == 0) q_unscale[row] = exp2_int(exponent - 14);
-#pragma unroll
-                        for (int k = 0; k < kVecs; ++k) {
-                            const uint32_t d = l8 * E + 8 * k;  // 64-element blocks of [128 rows][128 bytes]
-                            sts128(q_at + (stream * kParts + d / 64) * 16384 + in_tile * 128 + ((d % 64 / 8 ^ (in_tile & 7)) << 4), half2_bits(x[8 * k] * by, x[8 * k + 1] * by),
-                                   half2_bits(x[8 * k + 2] * by, x[8 * k + 3] * by), half2_bits(x[8 * k + 4] * by, x[8 * k + 5] * by), half2_bits(x[8 * k + 6] * by, x[8 * k + 7] * by));
+                            v[b][k] = make_uint4(x[0], x[1], x[2], x[3]);
                         }
                     }
                 }
-                proxy_fence();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(q_ready + 8 * stream);
+#pragma unroll
+                for (int b = 0; b < kBatch; ++b) {
+                    const uint32_t in_tile = quarter * 32 + (it + b) * 4 + lane / 8, row = stream * 128 + in_tile;
+                    float x[E], top = 0;
+#pragma unroll
+                    for (int k = 0; k < kVecs; ++k) {
+                        T e8[8];
+                        __builtin_memcpy(e8, &v[b][k], 16);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            x[8 * k + e] = row < rows ? to_f32(e8[e]) : 0.0f;
+                            top = fmaxf(top, fabsf(x[8 * k + e]) < INFINITY ? fabsf(x[8 * k + e]) : 0.0f);
+                        }
+                    }
+#pragma unroll
+                    for (int d = 4; d != 0; d /= 2) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+                    const int32_t exponent = max(static_cast<int32_t>(__float_as_uint(top) >> 23) - 127, -100);
+                    const float by = c.scale < 0 ? -exp2_int(14 - exponent) : exp2_int(14 - exponent);
+                    if (l8 == 0) q_unscale[row] = exp2_int(exponent - 14);
+#pragma unroll
+                    for (int k = 0; k < kVecs; ++k) {
+                        const uint32_t d = l8 * E + 8 * k;  // 64-element blocks of [128 rows][128 bytes]
+                        sts128(q_at + (stream * kParts + d / 64) * 16384 + in_tile * 128 + ((d % 64 / 8 ^ (in_tile & 7)) << 4), half2_bits(x[8 * k] * by, x[8 * k + 1] * by),
+                               half2_bits(x[8 * k + 2] * by, x[8 * k + 3] * by), half2_bits(x[8 * k + 4] * by, x[8 * k + 5] * by), half2_bits(x[8 * k + 6] * by, x[8 * k + 7] * by));
+                    }
+                }
+            }
+            proxy_fence();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_ready + 8 * stream);
+        };
+        load_q(walks[0]);
+        for (uint32_t turn = 0;; turn ^= 1) {
+            const Walk& walk = walks[turn];
+            if (leader) {
+                walks[turn ^ 1] = walk;
+                walks[turn ^ 1].advance(c, w);
             }
             const float qs = q_unscale[r];
-            const uint32_t p = walk.r0 + min(r, walk.rows - 1), j = p / c.group;
+            const uint32_t j = walk.token(w, min(r, walk.rows - 1));
             const int32_t lo = first_key(walk.u.s, w.window, j), hi = end_key(walk.u.s, c.causal, j);
-            // keys that every row of this row tile sees (a tile without rows sees none of them: nothing of it is kept)
-            const uint32_t first_row = walk.r0 + min(stream * 128, walk.rows - 1), last_row = walk.r0 + min(stream * 128 + 127, walk.rows - 1);
-            const int32_t all_lo = first_key(walk.u.s, w.window, last_row / c.group), all_hi = end_key(walk.u.s, c.causal, first_row / c.group);
+            // keys that every row of this row tile sees (a tile without rows: of its last row's; nothing of it is kept)
+            const int32_t all_lo = first_key(walk.u.s, w.window, walk.token(w, min(stream * 128 + 127, walk.rows - 1)));
+            const int32_t all_hi = end_key(walk.u.s, c.causal, walk.token(w, min(stream * 128, walk.rows - 1)));
             const int32_t last_tile = walk.g.hi;
             float ref = -INFINITY, l = 0;
             uint32_t prev_bar = 0, prev_parity = 0;
@@ -417,30 +436,37 @@ __global__ void __launch_bounds__(TilesShape<D>::kThreads, 1) tiles_kernel(const
                 tmem_after();
                 const GroupScale* sc = scales[tiles % kScaleTiles];
                 const int32_t t0 = tile * 128;
-                const bool masked = t0 < all_lo || t0 + 128 > all_hi || partly[tiles % kScaleTiles] != 0;
+                const bool masked = t0 < all_lo || t0 + 128 > all_hi;
+                const uint32_t from = static_cast<uint32_t>(t0 - lo), seen = static_cast<uint32_t>(max(hi - lo, 0));  // key e of the tile: from + e < seen
                 uint32_t x[2][32];
                 float top = -INFINITY;
-                tmem_ld32(s_at, x[0]);
+                // Missing keys are zeros with log_v = -inf; the factor of a group's scores is not negative: the largest score is the largest exponent.
+                auto largest = [&](const bool MASKED) __attribute__((always_inline)) {
+                    tmem_ld32(s_at, x[0]);
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    tmem_wait_ld();
-                    if (q < 3) tmem_ld32(s_at + 32 * (q + 1), x[(q + 1) % 2]);
-                    uint32_t(&v)[32] = x[q % 2];
+                    for (int q = 0; q < 4; ++q) {
+                        tmem_wait_ld();
+                        if (q < 3) tmem_ld32(s_at + 32 * (q + 1), x[(q + 1) % 2]);
+                        uint32_t(&v)[32] = x[q % 2];
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const GroupScale s = sc[2 * q + i];
-                        const float by = s.k * qs;
+                        for (int i = 0; i < 2; ++i) {
+                            const GroupScale s = sc[2 * q + i];
+                            float y[16];
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) {
-                            float y = fmaf(__uint_as_float(v[16 * i + e]), by, s.log_v);
-                            if (masked) {
-                                const int32_t t = t0 + 32 * q + 16 * i + e;
-                                if (t < lo || t >= hi || s.log_v == -INFINITY) y = -INFINITY;
+                            for (int e = 0; e < 16; ++e) {
+                                y[e] = __uint_as_float(v[16 * i + e]);
+                                if (MASKED) y[e] = from + static_cast<uint32_t>(32 * q + 16 * i + e) < seen ? y[e] : -INFINITY;
                             }
-                            top = fmaxf(top, y);
+                            float m = fmaxf(y[0], y[1]);
+#pragma unroll
+                            for (int e = 2; e < 16; e += 2) m = fmaxf(fmaxf(m, y[e]), y[e + 1]);
+                            const float z = fmaf(m, s.k * qs, s.log_v);
+                            top = fmaxf(top, MASKED && m == -INFINITY ? m : z);
                         }
                     }
-                }
+                };
+                if (masked) largest(true);
+                else largest(false);
                 const float next = fmaxf(ref, top);
                 const bool first = ref == -INFINITY, grows = !first && next > ref + 8.0f;
                 if (__any_sync(0xFFFFFFFFu, grows)) {
@@ -462,37 +488,41 @@ __global__ void __launch_bounds__(TilesShape<D>::kThreads, 1) tiles_kernel(const
                 }
                 if (first || grows) ref = next;
                 const float base = ref == -INFINITY ? 0.0f : ref - 6.0f;
-                tmem_ld32(s_at, x[0]);
+                auto weigh = [&](const bool MASKED) __attribute__((always_inline)) {
+                    tmem_ld32(s_at, x[0]);
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    tmem_wait_ld();
-                    if (q < 3) tmem_ld32(s_at + 32 * (q + 1), x[(q + 1) % 2]);
-                    uint32_t(&v)[32] = x[q % 2];
-                    uint32_t weights[16];
+                    for (int q = 0; q < 4; ++q) {
+                        tmem_wait_ld();
+                        if (q < 3) tmem_ld32(s_at + 32 * (q + 1), x[(q + 1) % 2]);
+                        uint32_t(&v)[32] = x[q % 2];
+                        uint32_t weights[16];
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const GroupScale s = sc[2 * q + i];
-                        const float by = s.k * qs, add = s.log_v - base;
-                        float sum = 0;
+                        for (int i = 0; i < 2; ++i) {
+                            const GroupScale s = sc[2 * q + i];
+                            const float by = s.k * qs, add = s.log_v - base;
+                            const uint64_t by2 = pair(by, by), add2 = pair(add, add);
+                            uint64_t sum = 0;
 #pragma unroll
-                        for (int e = 0; e < 16; e += 2) {
-                            float y[2];
-#pragma unroll
-                            for (int k = 0; k < 2; ++k) {
-                                y[k] = fmaf(__uint_as_float(v[16 * i + e + k]), by, add);
-                                if (masked) {
-                                    const int32_t t = t0 + 32 * q + 16 * i + e + k;
-                                    if (t < lo || t >= hi || s.log_v == -INFINITY) y[k] = -INFINITY;
+                            for (int e = 0; e < 16; e += 2) {
+                                float y0, y1;
+                                unpair(fma_pair(pair(__uint_as_float(v[16 * i + e]), __uint_as_float(v[16 * i + e + 1])), by2, add2), y0, y1);
+                                if (MASKED) {
+                                    y0 = from + static_cast<uint32_t>(32 * q + 16 * i + e) < seen ? y0 : -INFINITY;
+                                    y1 = from + static_cast<uint32_t>(32 * q + 16 * i + e + 1) < seen ? y1 : -INFINITY;
                                 }
-                                y[k] = exp2_approx(y[k]);
+                                y0 = exp2_approx(y0), y1 = exp2_approx(y1);
+                                sum = add_pair(sum, pair(y0, y1));
+                                weights[8 * i + e / 2] = half2_bits(y0, y1);
                             }
-                            sum += y[0] + y[1];
-                            weights[8 * i + e / 2] = half2_bits(y[0], y[1]);
+                            float s0, s1;
+                            unpair(sum, s0, s1);
+                            l = fmaf(s0 + s1, s.inv_v, l);
                         }
-                        l = fmaf(sum, s.inv_v, l);
+                        tmem_st16(s_at + 16 * q, weights);  // columns whose scores have been read
                     }
-                    tmem_st16(s_at + 16 * q, weights);  // columns whose scores have been read
-                }
+                };
+                if (masked) weigh(true);
+                else weigh(false);
                 tmem_wait_st();
                 tmem_before();
                 __syncwarp();
@@ -501,14 +531,16 @@ __global__ void __launch_bounds__(TilesShape<D>::kThreads, 1) tiles_kernel(const
                 if (kStreams == 1) b ^= 1;
                 ++tiles;
             }
+            bar_sync(1, kSoft);  // the next segment is known
+            // q is free with this segment's last scores; the next one's goes in front of the rows, so that its products begin
+            if (walks[turn ^ 1].more != 0) load_q(walks[turn ^ 1]);
             wait(prev_bar, prev_parity);
             tmem_after();
             // ---- the segment's rows ------------------------------------------------------------------------------------------------------
             const bool keep = r < walk.rows;
             float* slot = walk.g.whole() ? nullptr : partial_slot(w, D, blockIdx.x, walk.g.from_start) + r * D;
             auto out_at = [&](uint32_t row) {
-                const uint32_t p = walk.r0 + row, j = p / c.group, h = walk.u.head * c.group + p % c.group;
-                return reinterpret_cast<T*>(c.out.p + uint64_t{walk.u.s.row0 + j} * c.out.token_stride + uint64_t{h} * c.out.head_stride);
+                return reinterpret_cast<T*>(walk.at(c, w, c.out, row));
             };
             T* out = out_at(min(r, walk.rows - 1));
             const float inv = l != 0 ? 1.0f / l : 0.0f;
@@ -566,10 +598,10 @@ __global__ void __launch_bounds__(TilesShape<D>::kThreads, 1) tiles_kernel(const
                     join_partials<T, D>(c, w, walk.u.s.row0, walk.u.head, walk.r0, walk.rows, c0, shares, 8, S::kSoftWarps);
                 }
             }
+            const bool more = walks[turn ^ 1].more != 0;
             bar_sync(1, kSoft);  // nobody reads `walk` any more
-            if (leader) walk.advance(c, w);
-            bar_sync(1, kSoft);
-        } while (walk.more != 0);
+            if (!more) break;
+        }
     }
     if (!alive && lane == 0) atomicOr(w.error_word, 1u);
     tmem_before();
@@ -586,6 +618,8 @@ int launch_tiles_kernel(HaloCudaCtx* ctx, const AttentionCall& c, Work w, cudaSt
     w.rows = S::kRows;
     w.tile = S::kTile;
     w.least = 1;
+    w.group = c.group;
+    w.group_inverse = static_cast<uint32_t>((0xFFFFFFFFull + c.group) / c.group);
     w.row_tiles = (c.rows.max_tokens * c.group + S::kRows - 1) / S::kRows;
     w.lanes = 1;
     while (w.lanes < 32 && w.lanes < w.row_tiles) w.lanes *= 2;

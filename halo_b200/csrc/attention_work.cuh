@@ -17,6 +17,7 @@ namespace attn {
 struct Work {  // what every kernel of a call is told besides the call
     uint32_t rows, tile;          // packed rows of a unit, keys of a tile
     uint32_t least;               // tiles of a CTA, where a call has few
+    uint32_t group, group_inverse;  // query heads of a kv head; ceil(2^32 / group)
     uint32_t row_tiles;           // of the longest sequence at most
     uint32_t lanes;               // of a warp that look at one sequence when the tiles are counted: a power of two
     int32_t window;               // 0: none
@@ -215,6 +216,33 @@ __device__ __forceinline__ Segment segment(const Range& r, const Unit& u, uint64
     g.hi = g.to_end ? u.span.hi : u.span.lo + static_cast<int32_t>(r.end - unit_begin);
     return g;
 }
+
+/// Where a CTA's consumers are: in shared memory, so that the walk over the tiles has the registers.
+struct Walk {
+    Range range;
+    Unit u;
+    Segment g;
+    uint32_t rows, r0;        // of the unit
+    uint32_t token0, behind;  // row 0's token, and which of the token's heads it is
+    uint32_t more;
+    __device__ void enter(const AttentionCall& c, const Work& w, uint64_t unit_begin) {
+        g = segment(range, u, unit_begin);
+        rows = u.rows(w), r0 = u.row0(w);
+        token0 = r0 / c.group, behind = r0 - token0 * c.group;
+        more = 1;
+    }
+    __device__ void advance(const AttentionCall& c, const Work& w) {
+        more = g.unit_end < range.end && next_unit(c, w, u);
+        if (more) enter(c, w, g.unit_end);
+    }
+    /// The token of row r < 256 of the unit (group_inverse = ceil(2^32 / group): exact while (group + 256) * group < 2^32).
+    __device__ __forceinline__ uint32_t token(const Work& w, uint32_t r) const { return token0 + (w.group == 1 ? r : __umulhi(behind + r, w.group_inverse)); }
+    /// Where row r's head begins.
+    __device__ __forceinline__ uint8_t* at(const AttentionCall& c, const Work& w, const Heads& x, uint32_t r) const {
+        const uint32_t t = token(w, r), h = r0 + r - t * w.group + u.head * w.group;
+        return x.p + uint64_t{u.s.row0 + t} * x.token_stride + uint64_t{h} * x.head_stride;
+    }
+};
 
 /// Where a CTA's share of a unit that it has not alone lies: [row][dim] weighted rows, then (maximum, sum) of every row.
 __device__ __forceinline__ float* partial_slot(const Work& w, uint32_t dim, uint32_t cta, bool from_start) {
