@@ -110,51 +110,74 @@ __device__ void spread_nan(const AttentionCall& c, const Work& w, const Unit& u,
     }
 }
 
-/// Joins the shares of a unit in CTA order and stores its rows.  All `warps` of the caller, from warp0 on, take part, each with a row's 128 dims (or 64) at a time.
+/// Joins the shares of a unit in CTA order and stores its rows.  All `warps` of the caller, from warp0 on, take part; `row_ml` has room for every row's
+/// (maximum, 1 / sum).
 template <class T, int D>
-__device__ __forceinline__ void join_partials(const AttentionCall& c, const Work& w, uint32_t seq_row0, uint32_t head, uint32_t r0, uint32_t rows, uint32_t c0, uint32_t shares,
-                                              uint32_t warp0, uint32_t warps) {
-    constexpr uint32_t kPerLane = D < 128 ? 2 : 4, kParts = D / (32 * kPerLane), kAhead = 8;  // shares whose loads are under way together
-    using Word = std::conditional_t<kPerLane == 4, float4, float2>;
-    const uint32_t lane = threadIdx.x % 32;
+__device__ __forceinline__ void join_partials(const AttentionCall& c, const Work& w, const Walk& walk, uint32_t c0, uint32_t shares, uint32_t warp0, uint32_t warps, float2* row_ml) {
+    constexpr uint32_t kAhead = 4;  // shares whose loads are under way together
+    const uint32_t thread = threadIdx.x - warp0 * 32, threads = warps * 32, rows = walk.rows;
+    auto slot = [&](uint32_t k) { return partial_slot(w, D, c0 + min(k, shares - 1), k == 0); };
 #pragma unroll 1
-    for (uint32_t i = threadIdx.x / 32 - warp0; i < rows * kParts; i += warps) {
-        const uint32_t r = i / kParts, d = (i % kParts * 32 + lane) * kPerLane;
-        float m = -INFINITY, l = 0, o[kPerLane] = {};
+    for (uint32_t r = thread; r < rows; r += threads) {
+        float m = -INFINITY, l = 0;
+#pragma unroll 1
+        for (uint32_t k0 = 0; k0 < shares; k0 += 2 * kAhead) {
+            float2 ml[2 * kAhead];
+#pragma unroll
+            for (uint32_t k = 0; k < 2 * kAhead; ++k) ml[k] = __ldcg(reinterpret_cast<const float2*>(slot(k0 + k) + w.rows * D + 2 * r));
+            float top = m;
+#pragma unroll
+            for (uint32_t k = 0; k < 2 * kAhead; ++k) top = fmaxf(top, ml[k].x);
+            l *= m == -INFINITY ? 1.0f : exp2_approx(m - top);  // without a maximum sum and row are zero, or NaN
+            m = top;
+#pragma unroll
+            for (uint32_t k = 0; k < 2 * kAhead; ++k)
+                if (k0 + k < shares) l += ml[k].x == -INFINITY ? ml[k].y : exp2_approx(ml[k].x - top) * ml[k].y;
+        }
+        row_ml[r] = make_float2(m, l != 0 ? 1.0f / l : 0.0f);
+    }
+    bar_sync(1, threads);
+#pragma unroll 1
+    for (uint32_t i = thread; i < rows * (D / 4); i += 2 * threads) {
+        float4 o[2];
+        float m[2];
+        uint32_t row[2], dim[2];
+#pragma unroll
+        for (uint32_t h = 0; h < 2; ++h) {
+            const uint32_t at = min(i + h * threads, rows * (D / 4) - 1);
+            row[h] = at / (D / 4), dim[h] = at % (D / 4) * 4;
+            m[h] = row_ml[row[h]].x;
+            o[h] = make_float4(0, 0, 0, 0);
+        }
 #pragma unroll 1
         for (uint32_t k0 = 0; k0 < shares; k0 += kAhead) {
-            // every lane holds one share's maximum and sum; behind the last share the last one again, with weight zero
-            const uint32_t mine = min(k0 + lane % kAhead, shares - 1);
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(partial_slot(w, D, c0 + mine, mine == 0) + w.rows * D + 2 * r));
-            Word x[kAhead];
+            float f[2][kAhead];
+            float4 x[2][kAhead];
 #pragma unroll
             for (uint32_t k = 0; k < kAhead; ++k) {
-                const uint32_t at = min(k0 + k, shares - 1);
-                x[k] = __ldcg(reinterpret_cast<const Word*>(partial_slot(w, D, c0 + at, at == 0) + r * D + d));
+                const float* s = slot(k0 + k);
+#pragma unroll
+                for (uint32_t h = 0; h < 2; ++h) {
+                    f[h][k] = __ldcg(s + w.rows * D + 2 * row[h]);
+                    x[h][k] = __ldcg(reinterpret_cast<const float4*>(s + row[h] * D + dim[h]));
+                }
             }
-            float top = fmaxf(m, ml.x);
 #pragma unroll
-            for (uint32_t s = kAhead / 2; s != 0; s /= 2) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, s));
-            // without a maximum sum and row are zero, or NaN; a share of weight zero adds nothing, but a NaN in it is one of a token that the row sees
-            const float fade = m == -INFINITY ? 1.0f : exp2_approx(m - top);
-            const float f = k0 + lane % kAhead >= shares ? 0.0f : ml.x == -INFINITY ? 1.0f : exp2_approx(ml.x - top);
-            m = top;
-            l *= fade;
+            for (uint32_t k = 0; k < kAhead; ++k)
 #pragma unroll
-            for (uint32_t e = 0; e < kPerLane; ++e) o[e] *= fade;
-#pragma unroll
-            for (uint32_t k = 0; k < kAhead; ++k) {
-                const float fk = __shfl_sync(0xFFFFFFFFu, f, k);
-                l += fk * __shfl_sync(0xFFFFFFFFu, ml.y, k);
-                o[0] += fk * x[k].x, o[1] += fk * x[k].y;
-                if constexpr (kPerLane == 4) o[2] += fk * x[k].z, o[3] += fk * x[k].w;
-            }
+                for (uint32_t h = 0; h < 2; ++h) {
+                    // a share of weight zero adds nothing, but a NaN in it is one of a token that the row sees; behind the last share: the last again
+                    const float by = k0 + k >= shares ? 0.0f : f[h][k] == -INFINITY ? 1.0f : exp2_approx(f[h][k] - m[h]);
+                    o[h].x += by * x[h][k].x, o[h].y += by * x[h][k].y, o[h].z += by * x[h][k].z, o[h].w += by * x[h][k].w;
+                }
         }
-        const float inv = l != 0 ? 1.0f / l : 0.0f;
-        const uint32_t j = (r0 + r) / c.group, h = head * c.group + (r0 + r) % c.group;
-        T* out = reinterpret_cast<T*>(c.out.p + uint64_t{seq_row0 + j} * c.out.token_stride + uint64_t{h} * c.out.head_stride) + d;
 #pragma unroll
-        for (uint32_t e = 0; e < kPerLane; ++e) out[e] = from_f32<T>(o[e] * inv);
+        for (uint32_t h = 0; h < 2; ++h) {
+            if (i + h * threads >= rows * (D / 4)) break;
+            const float inv = row_ml[row[h]].y;
+            T* out = reinterpret_cast<T*>(walk.at(c, w, c.out, row[h])) + dim[h];
+            out[0] = from_f32<T>(o[h].x * inv), out[1] = from_f32<T>(o[h].y * inv), out[2] = from_f32<T>(o[h].z * inv), out[3] = from_f32<T>(o[h].w * inv);
+        }
     }
 }
 
@@ -178,6 +201,7 @@ __global__ void __launch_bounds__(RowsShape<D, TS, RG, TILE, CPS, sizeof(T) == 4
     __shared__ float q_unscale[S::kRows];
     __shared__ uint32_t nan_seen, is_last;
     __shared__ Walk walk;
+    __shared__ float2 joined_ml[S::kRows];
 
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
@@ -635,7 +659,7 @@ __global__ void __launch_bounds__(RowsShape<D, TS, RG, TILE, CPS, sizeof(T) == 4
             bar_sync(1, kConsumers);
             if (is_last != 0) {
                 __threadfence();
-                join_partials<T, D>(c, w, walk.u.s.row0, walk.u.head, walk.r0, walk.rows, c0, shares, 0, S::kWarps);
+                join_partials<T, D>(c, w, walk, c0, shares, 0, S::kWarps, joined_ml);
             }
         }
         bar_sync(1, kConsumers);  // nobody reads q, the joined rows or `walk` any more

@@ -12,10 +12,10 @@
 // weights overwrite the scores in TMEM as fp16 and are the A operand of P V from there.
 // Warps:
 //   0       tcgen05.mma issue;  1: TMEM allocation
-//   4-7     conversion: codes by 16-byte loads straight from their pages to registers, three slots ahead, to fp16 in a ring of eight
-//           16 KiB slots (a K slot: 128 keys x 64 dims; a V slot: 8192 / D keys x all dims, the N operand with dims contiguous);
-//           rows that no row of the CTA sees, missing pages and NaN codes of values become zeros (spread_nan puts the latter back)
-//   8-15    softmax, a thread to a row (8-11 where NS is 1); also q -> fp16 in shared memory, the epilogue, and the joining of shares
+//   4-7     conversion (4-11 where D is 256): each warp makes one part of K or V of every tile in a ring of eight 16 KiB slots (a K slot: 128 keys x
+//           64 dims; a V slot: 8192 / D keys x all dims, the N operand with dims contiguous); keys that no row of the CTA sees, missing pages and,
+//           in tiles that some row does not see whole, NaN codes of values become zeros (spread_nan puts the latter back)
+//   last 8  softmax, a thread to a row (the last 4 where NS is 1); also q -> fp16 in shared memory, the epilogue, and the joining of shares
 // Work is dealt as in attention_work.cuh, so a causal prompt's long and short rows and a short chunk behind a long context fill the device alike.
 //
 // What bounds it: the tensor pipe and, for D = 128, the exponentials (256 x 128 of them per 2048 clocks of products at 16 a clock); shared memory
@@ -33,9 +33,15 @@ struct TilesShape {
     static constexpr int kParts = D / 64;               // slots of a tile of K, and of V
     static constexpr int kVTokens = 128 * 64 / D;       // keys of a V slot
     static constexpr uint32_t kSmem = 1024 + kQ + kSlots * kSlot;
-    static constexpr int kSoftWarps = 4 * kStreams, kThreads = 256 + 32 * kSoftWarps;
+    static constexpr int kConvWarps = D == 256 ? 8 : 4, kSoftWarp = 4 + kConvWarps, kSoftWarps = 4 * kStreams, kThreads = 512;
+    static_assert((kSoftWarp + kSoftWarps) * 32 == kThreads);
+    // Slot number i of a CTA (the parts of K of its first tile, those of V, those of K of the second, ...) has place i % kSlots.  A place's user waits for
+    // its last use by the parity of that use, so all of a place's uses are to be one warp's: 2 * kParts * kEvery of convert_slots divides kSlots.
+    static_assert(kSlots % kConvWarps == 0);
+    // 128 registers a thread at launch; the warpgroups hand each other what they leave: (56 + conversion's and softmax's groups) = 4 * 128
+    static constexpr int kIdleRegs = 56, kConvRegs = 104, kSoftRegs = kStreams == 2 ? 176 : 248;
+    static_assert(kIdleRegs + kConvRegs * (kConvWarps / 4) + kSoftRegs * kStreams <= 512);
     static constexpr uint32_t kO = 256;                 // first accumulator column; scores are columns 0 .. 255
-    static constexpr int kLag = kStreams == 1 ? 1 : 0;  // V of a tile is fetched behind K of the next one
 };
 
 __device__ __forceinline__ uint64_t desc_k(uint32_t addr) {  // K-major, 128-byte rows and swizzle: atoms of 8 rows, 1024 bytes apart
@@ -105,16 +111,154 @@ __device__ __forceinline__ void sts128(uint32_t at, uint32_t a, uint32_t b, uint
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
-/// Index of a tile's first K or V slot among its segment's slots (n tiles).
-template <int D>
-__device__ __forceinline__ uint32_t k_slot(uint32_t t) {
+/// The slots of one part of K or V, of every `every`-th tile from `turn` on, over a CTA's whole range, by one warp: 16-byte pieces straight from the
+/// pages, half a slot ahead of the half that is converted.  The warp of K's part 0 publishes the tile's scales with its slot.
+template <int D, bool IS_V>
+__device__ __forceinline__ void convert_slots(const AttentionCall& c, const Work& w, const Range& range, uint32_t part, uint32_t turn, uint32_t every, uint32_t ring, uint32_t full,
+                                              uint32_t empty, GroupScale (*scales)[8], uint32_t* nan_seen, bool& alive) {
     using S = TilesShape<D>;
-    return S::kLag == 0 ? 2 * t * S::kParts : (t == 0 ? 0 : 2 * t - 1) * S::kParts;
-}
-template <int D>
-__device__ __forceinline__ uint32_t v_slot(uint32_t t, uint32_t n) {
-    using S = TilesShape<D>;
-    return S::kLag == 0 ? (2 * t + 1) * S::kParts : (t + 1 < n ? 2 * t + 2 : 2 * n - 1) * S::kParts;
+    constexpr uint32_t kBlocks = IS_V ? S::kParts : 1;                   // 64-dim blocks of a slot's rows
+    constexpr uint32_t kRows = IS_V ? S::kVTokens : 128, kStep = 8 / kBlocks;  // rows of a slot; of one access of the warp
+    constexpr int kHalf = 8;                                             // accesses of half a slot
+    constexpr uint32_t kGroups = kRows / 16, kPerGroup = 16 / kStep;     // groups of 16 rows; accesses of one
+    const uint32_t lane = threadIdx.x % 32;
+    // a quarter warp has four pieces of two rows: its eight 16-byte stores lie in different banks
+    const uint32_t lane_row = lane / 8 / kBlocks * 2 + lane / 4 % 2, block = lane / 8 % kBlocks;
+    const uint32_t from = lane_row * D + (IS_V ? block * 64 : part * 64) + lane % 4 * 16;             // of a group's first row
+    const uint32_t to = block * (kRows * 128) + lane_row * 128 + ((lane % 4 * 2 ^ (lane_row & 7)) << 4);  // second half: the same ^ 16
+    const float scale = fabsf(c.scale) * 1.4426950408889634f;  // its sign is q's
+    auto wait = [&](uint32_t bar, uint32_t parity) {
+        if (alive) alive = __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity));
+    };
+    // where the loads are: a tile of a segment; lane i < 8 knows page and scale bytes of its i-th 16 keys, and those of the next tile to come
+    Unit u = range.unit;
+    Segment g = segment(range, u, range.unit_begin);
+    int32_t tile = g.lo, any_lo, any_hi, all_lo, all_hi, page = -1, page_next = -1;
+    uint32_t k_byte = 0, v_byte = 0, k_next = 0, v_next = 0, count = 0;  // count: tiles of the CTA before this one
+    auto limits = [&] {
+        const uint32_t first = u.row0(w) / c.group, last = (u.row0(w) + u.rows(w) - 1) / c.group;
+        any_lo = first_key(u.s, w.window, first), any_hi = end_key(u.s, c.causal, last);
+        all_lo = first_key(u.s, w.window, last), all_hi = end_key(u.s, c.causal, first);
+    };
+    auto fetch = [&](int32_t of) {
+        const int32_t t = of * 128 + static_cast<int32_t>(lane) * 16;
+        page_next = -1;
+        if (lane < 8 && of < g.hi && t < any_hi && t + 16 > any_lo) {
+            const int32_t p = page_of(c.cache, u.seq, t >> c.cache.page_shift);
+            page_next = static_cast<uint32_t>(p) < c.cache.n_pages ? p : -2;  // -2: a visible key's page is not there
+            if (!IS_V && part == 0 && page_next >= 0) {
+                const uint64_t at = p * c.cache.scale_stride + u.head;
+                k_next = __ldg(c.cache.k_scale + at);
+                v_next = __ldg(c.cache.v_scale + at);
+            }
+        }
+    };
+    auto take = [&] { page = page_next, k_byte = k_next, v_byte = v_next; };
+    /// On to this warp's next tile; false at the end of the range.
+    auto advance = [&]() -> bool {
+        const int32_t by = static_cast<int32_t>(every);
+        if (tile + by < g.hi) {
+            tile += by, count += every;
+            take();
+            fetch(tile + by);
+            return true;
+        }
+        // tiles that the segments in between leave behind count towards `every`
+        uint32_t ahead = every;
+        for (;;) {
+            const uint32_t left = static_cast<uint32_t>(g.hi - tile);
+            if (ahead < left) break;
+            ahead -= left, count += left;
+            if (g.unit_end >= range.end) return false;
+            const uint64_t begin = g.unit_end;
+            if (!next_unit(c, w, u)) return false;
+            g = segment(range, u, begin);
+            tile = g.lo;
+        }
+        tile += static_cast<int32_t>(ahead), count += ahead;
+        limits();
+        fetch(tile);
+        take();
+        fetch(tile + by);
+        return true;
+    };
+    auto load = [&](uint32_t half, uint4 (&x)[kHalf]) {
+        const int32_t t0 = tile * 128 + (IS_V ? static_cast<int32_t>(part * kRows) : 0);
+        const bool inside = t0 >= any_lo && t0 + static_cast<int32_t>(kRows) <= any_hi;
+        const uint8_t* pool = (IS_V ? c.cache.v : c.cache.k) + (uint64_t{u.head} << c.cache.page_shift) * D + from;
+        constexpr uint32_t kLoadGroups = kGroups / 2;  // of a half
+#pragma unroll
+        for (uint32_t i = 0; i < kLoadGroups; ++i) {
+            const uint32_t group = half * kLoadGroups + i, row = group * 16, in_tile = (IS_V ? part * kGroups : 0) + group;
+            const int32_t p = __shfl_sync(0xFFFFFFFFu, page, in_tile);
+            const uint8_t* src = pool + static_cast<uint32_t>(max(p, 0)) * c.cache.page_stride + ((IS_V ? part * kRows : 0) + row & (c.cache.page_tokens - 1)) * D;
+#pragma unroll
+            for (uint32_t k = 0; k < kPerGroup; ++k) {
+                uint4& v = x[i * kPerGroup + k];
+                const int32_t t = t0 + static_cast<int32_t>(row + k * kStep + lane_row);
+                v = make_uint4(0, 0, 0, 0);
+                if (p >= 0 && (inside || (t >= any_lo && t < any_hi))) v = __ldg(reinterpret_cast<const uint4*>(src + k * kStep * D));
+            }
+        }
+    };
+    auto store = [&](uint32_t half, uint4 (&x)[kHalf], uint32_t slot, bool check) {
+        if (check) {  // some row does not see some key: a NaN among the values would spread through a weight of zero
+            bool nan = false;
+#pragma unroll
+            for (int i = 0; i < kHalf; ++i) nan |= drop_nan(x[i].x) | drop_nan(x[i].y) | drop_nan(x[i].z) | drop_nan(x[i].w);
+            if (nan) *nan_seen = 1;
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < kHalf; ++i) {
+            const uint32_t row = (half * kHalf + i) * kStep, at = (slot + to + row * 128) ^ ((row & 7) << 4);
+            sts128(at, widen_lo(x[i].x), widen_hi(x[i].x), widen_lo(x[i].y), widen_hi(x[i].y));
+            sts128(at ^ 16, widen_lo(x[i].z), widen_hi(x[i].z), widen_lo(x[i].w), widen_hi(x[i].w));
+        }
+    };
+    limits();
+    fetch(tile);
+    take();
+    fetch(tile + static_cast<int32_t>(every));
+    if (turn != 0) {
+        // the first tile of this warp is the CTA's tile number `turn`
+        uint32_t skip = turn;
+        while (skip >= static_cast<uint32_t>(g.hi - tile)) {
+            const uint32_t left = static_cast<uint32_t>(g.hi - tile);
+            skip -= left, count += left;
+            const uint64_t begin = g.unit_end;
+            if (begin >= range.end || !next_unit(c, w, u)) return;
+            g = segment(range, u, begin);
+            tile = g.lo;
+        }
+        tile += static_cast<int32_t>(skip), count += skip;
+        limits();
+        fetch(tile);
+        take();
+        fetch(tile + static_cast<int32_t>(every));
+    }
+    uint4 a[kHalf], b[kHalf];
+    load(0, a);
+    for (bool more = true; more;) {
+        load(1, b);
+        const uint32_t number = (2 * count + (IS_V ? 1 : 0)) * S::kParts + part, at = number % S::kSlots, slot = ring + at * S::kSlot;
+        const bool check = IS_V && (tile * 128 < all_lo || tile * 128 + 128 > all_hi);
+        wait(empty + 8 * at, (number / S::kSlots & 1) ^ 1);
+        if (!IS_V && part == 0 && lane < 8) {
+            GroupScale& s = scales[count % 8][lane];
+            const int32_t v = scale_byte(v_byte) - 127;
+            s.k = page >= 0 ? exp2_int(scale_byte(k_byte) - 127) * scale : 0.0f;
+            s.log_v = page >= 0 ? static_cast<float>(v) : -INFINITY;
+            s.inv_v = page >= 0 ? exp2_int(-v) : 0.0f;
+            if (page == -2 && c.status != nullptr) atomicOr(c.status, 8u);  // kStatusBadIndex
+        }
+        store(0, a, slot, check);
+        more = advance();
+        if (more) load(0, a);
+        store(1, b, slot, check);
+        proxy_fence();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(full + 8 * at);
+    }
 }
 
 template <class T, int D>
@@ -126,6 +270,7 @@ __global__ void __launch_bounds__(TilesShape<D>::kThreads, 1) tiles_kernel(const
     __shared__ uint64_t bars[2 * kSlots + 3 * 2 + 2];
     __shared__ GroupScale scales[kScaleTiles][8];  // a tile's stay until the slots' ring has gone round behind it: at most six tiles ahead are written
     __shared__ float q_unscale[S::kRows];
+    __shared__ float2 joined_ml[S::kRows];
     __shared__ uint32_t nan_seen, is_last, tmem_word;
     __shared__ Walk walks[2];  // the segment at hand and the next one, in turn
 
@@ -136,7 +281,7 @@ __global__ void __launch_bounds__(TilesShape<D>::kThreads, 1) tiles_kernel(const
     const uint32_t full = smem_u32(bars), empty = full + 8 * kSlots, s_full = empty + 8 * kSlots, p_ready = s_full + 16, pv_done = p_ready + 16, q_ready = pv_done + 16;
     if (threadIdx.x == 0) {
         for (int i = 0; i < kSlots; ++i) {
-            mbar_init(full + 8 * i, 4);
+            mbar_init(full + 8 * i, 1);
             mbar_init(empty + 8 * i, 1);
         }
         for (int i = 0; i < 2; ++i) {
@@ -172,6 +317,7 @@ __global__ void __launch_bounds__(TilesShape<D>::kThreads, 1) tiles_kernel(const
     const Range range = walks[0].range;
     __syncthreads();  // `walks` belong to the softmax warps from here
 
+    if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::kIdleRegs));
     if (warp == 0) {
         // ---- products --------------------------------------------------------------------------------------------------------------------
         constexpr uint32_t kScores = (1u << 4) | (128u / 8 << 17) | (128u / 16 << 24), kRowsOut = (1u << 4) | (1u << 16) | (static_cast<uint32_t>(D) / 8 << 17) | (128u / 16 << 24);
@@ -185,7 +331,7 @@ __global__ void __launch_bounds__(TilesShape<D>::kThreads, 1) tiles_kernel(const
             auto scores = [&](uint32_t i) {
                 const uint32_t t = i / kStreams, s = i % kStreams;
                 if (t == 0) wait(q_ready + 8 * s, segments & 1);
-                const uint32_t first = base + k_slot<D>(t);
+                const uint32_t first = base + 2 * t * kParts;
 #pragma unroll
                 for (int part = 0; part < kParts; ++part) {
                     const uint32_t slot = (first + part) % kSlots;
@@ -204,7 +350,7 @@ __global__ void __launch_bounds__(TilesShape<D>::kThreads, 1) tiles_kernel(const
             auto rows = [&](uint32_t i) {
                 const uint32_t t = i / kStreams, s = i % kStreams, b = i % 2, use = b == 0 ? uses[0]++ : uses[1]++;
                 wait(p_ready + 8 * b, use & 1);
-                const uint32_t first = base + v_slot<D>(t, n);
+                const uint32_t first = base + (2 * t + 1) * kParts;
 #pragma unroll
                 for (int part = 0; part < kParts; ++part) {
                     const uint32_t slot = (first + part) % kSlots;
@@ -233,131 +379,23 @@ __global__ void __launch_bounds__(TilesShape<D>::kThreads, 1) tiles_kernel(const
             unit_begin = g.unit_end;
             if (unit_begin >= range.end || !next_unit(c, w, u)) break;
         }
-    } else if (warp >= 4 && warp < 8) {
+    } else if (warp >= 4 && warp < S::kSoftWarp) {
         // ---- conversion ------------------------------------------------------------------------------------------------------------------
-        const uint32_t thread = threadIdx.x - 128, cw = warp - 4;
-        uint4 raw[3][4];
-        uint32_t f = 0, kinds = 0;  // slots asked for; bit i of kinds: slot f - 1 - i is one of V
-        // this thread's 16-byte pieces of a slot: of K rows thread / 4 + 32 i, piece thread % 4; of V the two rows and four pieces of every eight lanes
-        // lie in eight different banks' groups
-        constexpr uint32_t kVRows = 32 / kParts;  // of V that the threads cover at a time
-        const uint32_t v_row = thread / 8 / kParts * 2 + thread / 4 % 2, v_piece = thread % 4 + thread / 8 % kParts * 4;
-        auto convert = [&](const uint4 (&x)[4], uint32_t at, bool is_v) {  // slot number `at`
-            const uint32_t slot = ring + at % kSlots * S::kSlot;
-            wait(empty + 8 * (at % kSlots), (at / kSlots & 1) ^ 1);
-            bool nan = false;
-#pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) {
-                const uint32_t row = is_v ? v_row + kVRows * i : thread / 4 + 32 * i;
-                const uint32_t row_at = slot + (is_v ? thread / 8 % kParts * (S::kVTokens * 128) : 0) + row * 128, piece = 2 * (thread % 4);
-                uint32_t word[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-                if (is_v && (nan_bits(word[0]) | nan_bits(word[1]) | nan_bits(word[2]) | nan_bits(word[3])) != 0) {
-                    nan = true;
-#pragma unroll
-                    for (uint32_t j = 0; j < 4; ++j) drop_nan(word[j]);
-                }
-#pragma unroll
-                for (uint32_t h = 0; h < 2; ++h)
-                    sts128(row_at + (((piece + h) ^ (row & 7)) << 4), widen_lo(word[2 * h]), widen_hi(word[2 * h]), widen_lo(word[2 * h + 1]), widen_hi(word[2 * h + 1]));
-            }
-            if (nan) nan_seen = 1;
-            proxy_fence();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(full + 8 * (at % kSlots));
-        };
-        Unit u = range.unit;
-        uint64_t unit_begin = range.unit_begin;
-        const float scale = fabsf(c.scale) * 1.4426950408889634f;  // its sign is q's
-        uint32_t tiles = 0;  // of this CTA so far
-        for (;;) {
-            const Segment g = segment(range, u, unit_begin);
-            const int32_t n = g.hi - g.lo;
-            const uint32_t r0 = u.row0(w), r1 = r0 + u.rows(w) - 1;
-            const int32_t any_lo = first_key(u.s, w.window, r0 / c.group), any_hi = end_key(u.s, c.causal, r1 / c.group);
-            // lane i < 8 of every warp knows page and scale bytes of the i-th 16 keys of a tile: of the tile at hand, the one behind and the next
-            int32_t page = -1, page_behind = -1, page_next = -1;
-            uint32_t k_next = 0, v_next = 0;
-            auto fetch = [&](int32_t tile) {
-                const int32_t t = tile * 128 + static_cast<int32_t>(lane) * 16;
-                page_next = -1;
-                if (lane < 8 && tile < g.hi && t < any_hi && t + 16 > any_lo) {
-                    const int32_t p = page_of(c.cache, u.seq, t >> c.cache.page_shift);
-                    page_next = static_cast<uint32_t>(p) < c.cache.n_pages ? p : -2;  // -2: a visible key's page is not there
-                    if (page_next >= 0) {
-                        const uint64_t at = p * c.cache.scale_stride + u.head;
-                        k_next = __ldg(c.cache.k_scale + at);
-                        v_next = __ldg(c.cache.v_scale + at);
-                    }
-                }
-            };
-            fetch(g.lo);
-            for (int32_t phase = 0; phase < n + S::kLag; ++phase) {
-                page_behind = page;
-                page = page_next;
-                if (phase < n) {
-                    if (cw == 0) {
-                        GroupScale& s = scales[tiles % kScaleTiles][lane % 8];
-                        const int32_t v = scale_byte(v_next) - 127;
-                        if (lane < 8) {
-                            s.k = page >= 0 ? exp2_int(scale_byte(k_next) - 127) * scale : 0.0f;
-                            s.log_v = page >= 0 ? static_cast<float>(v) : -INFINITY;
-                            s.inv_v = page >= 0 ? exp2_int(-v) : 0.0f;
-                            if (page == -2 && c.status != nullptr) atomicOr(c.status, 8u);  // kStatusBadIndex
-                        }
-                    }
-                    ++tiles;
-                }
-                if (phase + 1 < n) fetch(g.lo + phase + 1);
-                const uint32_t slots = (phase < n ? kParts : 0) + (phase >= S::kLag ? kParts : 0);
-                for (uint32_t j = 0; j < slots; ++j) {
-                    const bool is_v = phase >= n || j >= kParts;
-                    const uint32_t part = j % kParts;
-                    const int32_t t0 = (g.lo + phase - (is_v ? S::kLag : 0)) * 128;
-                    const int32_t pages = is_v && S::kLag != 0 ? page_behind : page;
-                    const uint8_t* pool = (is_v ? c.cache.v : c.cache.k) + (uint64_t{u.head} << c.cache.page_shift) * D + (is_v ? v_piece * 16 : part * 64 + thread % 4 * 16);
-                    const uint32_t row0 = is_v ? part * S::kVTokens + v_row : thread / 4, every = is_v ? kVRows : 32;
-                    const bool inside = t0 >= any_lo && t0 + 128 <= any_hi;
-                    auto load = [&](uint4 (&x)[4]) {
-#pragma unroll
-                        for (uint32_t i = 0; i < 4; ++i) {
-                            const uint32_t row = row0 + every * i;  // (a tile begins with a page)
-                            const int32_t p = __shfl_sync(0xFFFFFFFFu, pages, row / 16), t = t0 + static_cast<int32_t>(row);
-                            x[i] = make_uint4(0, 0, 0, 0);
-                            if (p >= 0 && (inside || (t >= any_lo && t < any_hi)))
-                                x[i] = __ldg(reinterpret_cast<const uint4*>(pool + static_cast<uint32_t>(p) * c.cache.page_stride + (row & (c.cache.page_tokens - 1)) * D));
-                        }
-                    };
-                    // slot f is asked for, slot f - 2 converted; the buffers' numbers have to be known at compile time
-                    if (f % 3 == 0) {
-                        load(raw[0]);
-                        if (f >= 2) convert(raw[1], f - 2, kinds >> 1 & 1);
-                    } else if (f % 3 == 1) {
-                        load(raw[1]);
-                        if (f >= 2) convert(raw[2], f - 2, kinds >> 1 & 1);
-                    } else {
-                        load(raw[2]);
-                        convert(raw[0], f - 2, kinds >> 1 & 1);
-                    }
-                    kinds = kinds << 1 | (is_v ? 1u : 0u);
-                    ++f;
-                }
-            }
-            unit_begin = g.unit_end;
-            if (unit_begin >= range.end || !next_unit(c, w, u)) break;
-        }
-        for (uint32_t i = 2; i != 0; --i) {  // at least one tile's two slots were asked for
-            const uint32_t at = f - i;
-            if (at % 3 == 0) convert(raw[0], at, kinds >> (i - 1) & 1);
-            else if (at % 3 == 1) convert(raw[1], at, kinds >> (i - 1) & 1);
-            else convert(raw[2], at, kinds >> (i - 1) & 1);
-        }
-    } else if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::kConvRegs));
+        // A warp makes one slot of every tile: its part of K, or of V (of every other tile where a tile has two slots).
+        constexpr uint32_t kEvery = S::kConvWarps / (2 * kParts);
+        const uint32_t role = (warp - 4) % (2 * kParts), turn = (warp - 4) / (2 * kParts), part = role % kParts;
+        const bool is_v = role >= kParts;
+        if (is_v) convert_slots<D, true>(c, w, range, part, turn, kEvery, ring, full, empty, scales, &nan_seen, alive);
+        else convert_slots<D, false>(c, w, range, part, turn, kEvery, ring, full, empty, scales, &nan_seen, alive);
+    } else if (warp >= S::kSoftWarp) {
         // ---- softmax ---------------------------------------------------------------------------------------------------------------------
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::kSoftRegs));
         constexpr uint32_t kSoft = S::kSoftWarps * 32;
-        const uint32_t stream = (warp - 8) / 4, quarter = warp % 4, r = stream * 128 + quarter * 32 + lane;  // this thread's row of the unit
+        const uint32_t stream = (warp - S::kSoftWarp) / 4, quarter = warp % 4, r = stream * 128 + quarter * 32 + lane;  // this thread's row of the unit
         const uint32_t lanes = quarter * 32 << 16, o_at = tmem + lanes + S::kO + stream * D;
         uint32_t uses[2] = {0, 0}, tiles = 0;
-        const bool leader = threadIdx.x == 256;
+        const bool leader = threadIdx.x == S::kSoftWarp * 32;
         // q: eight lanes to a row
         auto load_q = [&](const Walk& walk) {
             constexpr int E = D / 8, kVecs = E * 2 / 16, kBatch = 16 / kVecs < 4 ? 16 / kVecs : 4;
@@ -438,35 +476,28 @@ __global__ void __launch_bounds__(TilesShape<D>::kThreads, 1) tiles_kernel(const
                 const int32_t t0 = tile * 128;
                 const bool masked = t0 < all_lo || t0 + 128 > all_hi;
                 const uint32_t from = static_cast<uint32_t>(t0 - lo), seen = static_cast<uint32_t>(max(hi - lo, 0));  // key e of the tile: from + e < seen
-                uint32_t x[2][32];
-                float top = -INFINITY;
+                uint32_t x[4][32];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) tmem_ld32(s_at + 32 * q, x[q]);
+                tmem_wait_ld();
+                if (masked) {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            if (from + static_cast<uint32_t>(32 * q + e) >= seen) x[q][e] = 0xFF800000u;  // -inf
+                }
                 // Missing keys are zeros with log_v = -inf; the factor of a group's scores is not negative: the largest score is the largest exponent.
-                auto largest = [&](const bool MASKED) __attribute__((always_inline)) {
-                    tmem_ld32(s_at, x[0]);
+                float top = -INFINITY;
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        tmem_wait_ld();
-                        if (q < 3) tmem_ld32(s_at + 32 * (q + 1), x[(q + 1) % 2]);
-                        uint32_t(&v)[32] = x[q % 2];
+                for (int i = 0; i < 8; ++i) {
+                    const GroupScale s = sc[i];
+                    const uint32_t* v = &x[i / 2][i % 2 * 16];
+                    float m = fmaxf(__uint_as_float(v[0]), __uint_as_float(v[1]));
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            const GroupScale s = sc[2 * q + i];
-                            float y[16];
-#pragma unroll
-                            for (int e = 0; e < 16; ++e) {
-                                y[e] = __uint_as_float(v[16 * i + e]);
-                                if (MASKED) y[e] = from + static_cast<uint32_t>(32 * q + 16 * i + e) < seen ? y[e] : -INFINITY;
-                            }
-                            float m = fmaxf(y[0], y[1]);
-#pragma unroll
-                            for (int e = 2; e < 16; e += 2) m = fmaxf(fmaxf(m, y[e]), y[e + 1]);
-                            const float z = fmaf(m, s.k * qs, s.log_v);
-                            top = fmaxf(top, MASKED && m == -INFINITY ? m : z);
-                        }
-                    }
-                };
-                if (masked) largest(true);
-                else largest(false);
+                    for (int e = 2; e < 16; e += 2) m = fmaxf(fmaxf(m, __uint_as_float(v[e])), __uint_as_float(v[e + 1]));
+                    top = fmaxf(top, m == -INFINITY ? m : fmaf(m, s.k * qs, s.log_v));
+                }
                 const float next = fmaxf(ref, top);
                 const bool first = ref == -INFINITY, grows = !first && next > ref + 8.0f;
                 if (__any_sync(0xFFFFFFFFu, grows)) {
@@ -488,41 +519,30 @@ __global__ void __launch_bounds__(TilesShape<D>::kThreads, 1) tiles_kernel(const
                 }
                 if (first || grows) ref = next;
                 const float base = ref == -INFINITY ? 0.0f : ref - 6.0f;
-                auto weigh = [&](const bool MASKED) __attribute__((always_inline)) {
-                    tmem_ld32(s_at, x[0]);
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        tmem_wait_ld();
-                        if (q < 3) tmem_ld32(s_at + 32 * (q + 1), x[(q + 1) % 2]);
-                        uint32_t(&v)[32] = x[q % 2];
-                        uint32_t weights[16];
+                for (int q = 0; q < 4; ++q) {
+                    uint32_t weights[16];
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            const GroupScale s = sc[2 * q + i];
-                            const float by = s.k * qs, add = s.log_v - base;
-                            const uint64_t by2 = pair(by, by), add2 = pair(add, add);
-                            uint64_t sum = 0;
+                    for (int i = 0; i < 2; ++i) {
+                        const GroupScale s = sc[2 * q + i];
+                        // an unseen key's score of -inf times a factor of zero would be NaN; the factor is zero where every score counts for nothing
+                        const float by = fmaxf(s.k * qs, 0x1p-126f), add = s.log_v - base;
+                        const uint64_t by2 = pair(by, by), add2 = pair(add, add);
+                        uint64_t sum = 0;
 #pragma unroll
-                            for (int e = 0; e < 16; e += 2) {
-                                float y0, y1;
-                                unpair(fma_pair(pair(__uint_as_float(v[16 * i + e]), __uint_as_float(v[16 * i + e + 1])), by2, add2), y0, y1);
-                                if (MASKED) {
-                                    y0 = from + static_cast<uint32_t>(32 * q + 16 * i + e) < seen ? y0 : -INFINITY;
-                                    y1 = from + static_cast<uint32_t>(32 * q + 16 * i + e + 1) < seen ? y1 : -INFINITY;
-                                }
-                                y0 = exp2_approx(y0), y1 = exp2_approx(y1);
-                                sum = add_pair(sum, pair(y0, y1));
-                                weights[8 * i + e / 2] = half2_bits(y0, y1);
-                            }
-                            float s0, s1;
-                            unpair(sum, s0, s1);
-                            l = fmaf(s0 + s1, s.inv_v, l);
+                        for (int e = 0; e < 16; e += 2) {
+                            float y0, y1;
+                            unpair(fma_pair(pair(__uint_as_float(x[q][16 * i + e]), __uint_as_float(x[q][16 * i + e + 1])), by2, add2), y0, y1);
+                            y0 = exp2_approx(y0), y1 = exp2_approx(y1);
+                            sum = add_pair(sum, pair(y0, y1));
+                            weights[8 * i + e / 2] = half2_bits(y0, y1);
                         }
-                        tmem_st16(s_at + 16 * q, weights);  // columns whose scores have been read
+                        float s0, s1;
+                        unpair(sum, s0, s1);
+                        l = fmaf(s0 + s1, s.inv_v, l);
                     }
-                };
-                if (masked) weigh(true);
-                else weigh(false);
+                    tmem_st16(s_at + 16 * q, weights);  // (all scores have been read)
+                }
                 tmem_wait_st();
                 tmem_before();
                 __syncwarp();
@@ -577,7 +597,7 @@ __global__ void __launch_bounds__(TilesShape<D>::kThreads, 1) tiles_kernel(const
             tmem_before();
             bar_sync(1, kSoft);
             if (nan_seen != 0) {  // stays set: the conversion is ahead, and what it saw may belong to a segment to come
-                spread_nan(c, w, walk.u, walk.g, 256, kSoft, [&](uint32_t row, uint32_t d) {
+                spread_nan(c, w, walk.u, walk.g, S::kSoftWarp * 32, kSoft, [&](uint32_t row, uint32_t d) {
                     if (walk.g.whole()) out_at(row)[d] = from_f32<T>(NAN);
                     else partial_slot(w, D, blockIdx.x, walk.g.from_start)[row * D + d] = NAN;
                 });
@@ -595,7 +615,7 @@ __global__ void __launch_bounds__(TilesShape<D>::kThreads, 1) tiles_kernel(const
                 bar_sync(1, kSoft);
                 if (is_last != 0) {
                     __threadfence();
-                    join_partials<T, D>(c, w, walk.u.s.row0, walk.u.head, walk.r0, walk.rows, c0, shares, 8, S::kSoftWarps);
+                    join_partials<T, D>(c, w, walk, c0, shares, S::kSoftWarp, S::kSoftWarps, joined_ml);
                 }
             }
             const bool more = walks[turn ^ 1].more != 0;
