@@ -38,8 +38,9 @@ struct TilesShape {
     // Slot number i of a CTA (the parts of K of its first tile, those of V, those of K of the second, ...) has place i % kSlots.  A place's user waits for
     // its last use by the parity of that use, so all of a place's uses are to be one warp's: 2 * kParts * kEvery of convert_slots divides kSlots.
     static_assert(kSlots % kConvWarps == 0);
-    // 128 registers a thread at launch; the warpgroups hand each other what they leave: (56 + conversion's and softmax's groups) = 4 * 128
-    static constexpr int kIdleRegs = 56, kConvRegs = 104, kSoftRegs = kStreams == 2 ? 176 : 248;
+    static constexpr uint32_t kAhead = D == 256 ? 16 : 8;  // 16-byte pieces that a conversion thread has under way
+    // 128 registers a thread at launch; the warpgroups hand each other what they leave
+    static constexpr int kIdleRegs = D == 256 ? 80 : 72, kConvRegs = D == 256 ? 104 : 88, kSoftRegs = kStreams == 2 ? 176 : 224;
     static_assert(kIdleRegs + kConvRegs * (kConvWarps / 4) + kSoftRegs * kStreams <= 512);
     static constexpr uint32_t kO = 256;                 // first accumulator column; scores are columns 0 .. 255
 };
@@ -111,150 +112,163 @@ __device__ __forceinline__ void sts128(uint32_t at, uint32_t a, uint32_t b, uint
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
+/// Where a conversion warp's loads are: in shared memory, so that the pieces under way have the registers.
+struct Cursor {
+    Unit u;
+    Segment g;
+};
+
 /// The slots of one part of K or V, of every `every`-th tile from `turn` on, over a CTA's whole range, by one warp: 16-byte pieces straight from the
-/// pages, half a slot ahead of the half that is converted.  The warp of K's part 0 publishes the tile's scales with its slot.
+/// pages to registers, kAhead of the slot's 16 accesses under way in front of the one that is converted.  The warp of K's part 0 publishes the tile's scales
+/// with its slot.
 template <int D, bool IS_V>
-__device__ __forceinline__ void convert_slots(const AttentionCall& c, const Work& w, const Range& range, uint32_t part, uint32_t turn, uint32_t every, uint32_t ring, uint32_t full,
-                                              uint32_t empty, GroupScale (*scales)[8], uint32_t* nan_seen, bool& alive) {
+__device__ __forceinline__ void convert_slots(const AttentionCall& c, const Work& w, const Range& range, Cursor& cursor, uint32_t part, uint32_t turn, uint32_t every, uint32_t ring,
+                                              uint32_t full, uint32_t empty, GroupScale (*scales)[8], uint32_t* nan_seen, bool& alive) {
     using S = TilesShape<D>;
     constexpr uint32_t kBlocks = IS_V ? S::kParts : 1;                   // 64-dim blocks of a slot's rows
     constexpr uint32_t kRows = IS_V ? S::kVTokens : 128, kStep = 8 / kBlocks;  // rows of a slot; of one access of the warp
-    constexpr int kHalf = 8;                                             // accesses of half a slot
-    constexpr uint32_t kGroups = kRows / 16, kPerGroup = 16 / kStep;     // groups of 16 rows; accesses of one
+    constexpr uint32_t kAccesses = 16, kAhead = S::kAhead;
+    constexpr uint32_t kPerGroup = 16 / kStep;                           // accesses of 16 rows
     const uint32_t lane = threadIdx.x % 32;
     // a quarter warp has four pieces of two rows: its eight 16-byte stores lie in different banks
     const uint32_t lane_row = lane / 8 / kBlocks * 2 + lane / 4 % 2, block = lane / 8 % kBlocks;
     const uint32_t from = lane_row * D + (IS_V ? block * 64 : part * 64) + lane % 4 * 16;             // of a group's first row
     const uint32_t to = block * (kRows * 128) + lane_row * 128 + ((lane % 4 * 2 ^ (lane_row & 7)) << 4);  // second half: the same ^ 16
-    const float scale = fabsf(c.scale) * 1.4426950408889634f;  // its sign is q's
-    auto wait = [&](uint32_t bar, uint32_t parity) {
-        if (alive) alive = __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity));
-    };
-    // where the loads are: a tile of a segment; lane i < 8 knows page and scale bytes of its i-th 16 keys, and those of the next tile to come
-    Unit u = range.unit;
-    Segment g = segment(range, u, range.unit_begin);
-    int32_t tile = g.lo, any_lo, any_hi, all_lo, all_hi, page = -1, page_next = -1;
-    uint32_t k_byte = 0, v_byte = 0, k_next = 0, v_next = 0, count = 0;  // count: tiles of the CTA before this one
-    auto limits = [&] {
-        const uint32_t first = u.row0(w) / c.group, last = (u.row0(w) + u.rows(w) - 1) / c.group;
-        any_lo = first_key(u.s, w.window, first), any_hi = end_key(u.s, c.causal, last);
-        all_lo = first_key(u.s, w.window, last), all_hi = end_key(u.s, c.causal, first);
-    };
+    // the tile that is loaded: of the CTA's tiles number `count`, keys from t0 on; lane i < 8 knows page and scale bytes of its i-th 16 keys, and those of
+    // this warp's next tile
+    int32_t tile, last, any_lo, any_hi, page = -1, page_next = -1;
+    uint32_t bytes = 0, bytes_next = 0, count = 0;
+    uint64_t group_at = 0;              // lane i < 8: where its keys' codes begin in the pool
+    bool plain = false, whole = false;  // every key is there and seen by some row; by all rows
+    const uint8_t* pool = nullptr;
     auto fetch = [&](int32_t of) {
         const int32_t t = of * 128 + static_cast<int32_t>(lane) * 16;
         page_next = -1;
-        if (lane < 8 && of < g.hi && t < any_hi && t + 16 > any_lo) {
-            const int32_t p = page_of(c.cache, u.seq, t >> c.cache.page_shift);
+        if (lane < 8 && of < last && t < any_hi && t + 16 > any_lo) {
+            const int32_t p = page_of(c.cache, cursor.u.seq, t >> c.cache.page_shift);
             page_next = static_cast<uint32_t>(p) < c.cache.n_pages ? p : -2;  // -2: a visible key's page is not there
             if (!IS_V && part == 0 && page_next >= 0) {
-                const uint64_t at = p * c.cache.scale_stride + u.head;
-                k_next = __ldg(c.cache.k_scale + at);
-                v_next = __ldg(c.cache.v_scale + at);
+                const uint64_t at = p * c.cache.scale_stride + cursor.u.head;
+                bytes_next = __ldg(c.cache.k_scale + at) | static_cast<uint32_t>(__ldg(c.cache.v_scale + at)) << 8;
             }
         }
     };
-    auto take = [&] { page = page_next, k_byte = k_next, v_byte = v_next; };
-    /// On to this warp's next tile; false at the end of the range.
-    auto advance = [&]() -> bool {
-        const int32_t by = static_cast<int32_t>(every);
-        if (tile + by < g.hi) {
-            tile += by, count += every;
-            take();
-            fetch(tile + by);
-            return true;
-        }
-        // tiles that the segments in between leave behind count towards `every`
-        uint32_t ahead = every;
+    auto take = [&] {  // the fetched tile becomes the one that is loaded
+        page = page_next, bytes = bytes_next;
+        const Unit& u = cursor.u;
+        const uint32_t first = u.row0(w) / c.group, final = (u.row0(w) + u.rows(w) - 1) / c.group;
+        const int32_t t0 = tile * 128;
+        plain = t0 >= any_lo && t0 + 128 <= any_hi && __all_sync(0xFFFFFFFFu, page >= 0 || lane >= 8);
+        whole = plain && t0 >= first_key(u.s, w.window, final) && t0 + 128 <= end_key(u.s, c.causal, first);
+        group_at = static_cast<uint32_t>(max(page, 0)) * c.cache.page_stride + (lane * 16 & (c.cache.page_tokens - 1)) * D;
+        fetch(tile + static_cast<int32_t>(every));
+    };
+    /// Enters the cursor's segment at its tile number `skip`, or a later one's at what is left of it; false at the end of the range.
+    auto enter = [&](uint32_t skip) -> bool {
         for (;;) {
-            const uint32_t left = static_cast<uint32_t>(g.hi - tile);
-            if (ahead < left) break;
-            ahead -= left, count += left;
-            if (g.unit_end >= range.end) return false;
-            const uint64_t begin = g.unit_end;
-            if (!next_unit(c, w, u)) return false;
-            g = segment(range, u, begin);
-            tile = g.lo;
+            const uint32_t n = static_cast<uint32_t>(cursor.g.hi - cursor.g.lo);
+            if (skip < n) break;
+            skip -= n, count += n;
+            const uint64_t begin = cursor.g.unit_end;
+            bool more = begin < range.end;
+            if (more) {
+                Unit u = cursor.u;
+                more = next_unit(c, w, u);
+                const Segment g = segment(range, u, begin);
+                __syncwarp();
+                if (lane == 0) cursor.u = u, cursor.g = g;
+                __syncwarp();
+            }
+            if (!more) return false;
         }
-        tile += static_cast<int32_t>(ahead), count += ahead;
-        limits();
+        const Unit& u = cursor.u;
+        const uint32_t first = u.row0(w) / c.group, final = (u.row0(w) + u.rows(w) - 1) / c.group;
+        any_lo = first_key(u.s, w.window, first), any_hi = end_key(u.s, c.causal, final);
+        tile = cursor.g.lo + static_cast<int32_t>(skip), last = cursor.g.hi, count += skip;
+        pool = (IS_V ? c.cache.v : c.cache.k) + (uint64_t{u.head} << c.cache.page_shift) * D + from;
         fetch(tile);
         take();
-        fetch(tile + by);
         return true;
     };
-    auto load = [&](uint32_t half, uint4 (&x)[kHalf]) {
-        const int32_t t0 = tile * 128 + (IS_V ? static_cast<int32_t>(part * kRows) : 0);
-        const bool inside = t0 >= any_lo && t0 + static_cast<int32_t>(kRows) <= any_hi;
-        const uint8_t* pool = (IS_V ? c.cache.v : c.cache.k) + (uint64_t{u.head} << c.cache.page_shift) * D + from;
-        constexpr uint32_t kLoadGroups = kGroups / 2;  // of a half
+    auto advance = [&]() -> bool {  // to this warp's next tile
+        if (tile + static_cast<int32_t>(every) < last) {
+            tile += static_cast<int32_t>(every), count += every;
+            take();
+            return true;
+        }
+        const uint32_t done = static_cast<uint32_t>(tile - cursor.g.lo);
+        count -= done;
+        return enter(done + every);
+    };
+    uint4 x[kAhead];
+    constexpr uint32_t kLot = kAhead / 2;  // accesses that are converted, and asked for, together
+    auto load = [&](uint32_t lot) __attribute__((always_inline)) {  // accesses lot * kLot .. of the tile that is loaded
+        constexpr uint32_t kFirst = IS_V ? kRows / 16 : 0;  // groups of a part of V
+        if (plain) {
+            constexpr uint32_t kSpan = kLot > kPerGroup ? kLot / kPerGroup : 1, kIn = kLot / kSpan;  // groups of a lot; accesses of each
 #pragma unroll
-        for (uint32_t i = 0; i < kLoadGroups; ++i) {
-            const uint32_t group = half * kLoadGroups + i, row = group * 16, in_tile = (IS_V ? part * kGroups : 0) + group;
-            const int32_t p = __shfl_sync(0xFFFFFFFFu, page, in_tile);
-            const uint8_t* src = pool + static_cast<uint32_t>(max(p, 0)) * c.cache.page_stride + ((IS_V ? part * kRows : 0) + row & (c.cache.page_tokens - 1)) * D;
+            for (uint32_t n = 0; n < kSpan; ++n) {
+                const uint32_t i0 = lot * kLot + n * kIn;
+                const uint8_t* src = pool + __shfl_sync(0xFFFFFFFFu, group_at, i0 / kPerGroup + part * kFirst);
 #pragma unroll
-            for (uint32_t k = 0; k < kPerGroup; ++k) {
-                uint4& v = x[i * kPerGroup + k];
-                const int32_t t = t0 + static_cast<int32_t>(row + k * kStep + lane_row);
-                v = make_uint4(0, 0, 0, 0);
-                if (p >= 0 && (inside || (t >= any_lo && t < any_hi))) v = __ldg(reinterpret_cast<const uint4*>(src + k * kStep * D));
+                for (uint32_t j = 0; j < kIn; ++j) x[(i0 + j) % kAhead] = __ldg(reinterpret_cast<const uint4*>(src + (i0 + j) % kPerGroup * kStep * D));
+            }
+        } else {
+#pragma unroll
+            for (uint32_t j = 0; j < kLot; ++j) x[(lot * kLot + j) % kAhead] = make_uint4(0, 0, 0, 0);
+#pragma unroll 1
+            for (uint32_t g = lot * kLot / kPerGroup; g <= (lot * kLot + kLot - 1) / kPerGroup; ++g) {
+                const uint32_t group = g + (IS_V ? part * (kRows / 16) : 0);
+                const uint8_t* from_group = pool + __shfl_sync(0xFFFFFFFFu, group_at, group);
+                const bool there = __shfl_sync(0xFFFFFFFFu, page, group) >= 0;
+#pragma unroll
+                for (uint32_t j = 0; j < kLot; ++j) {
+                    const uint32_t i = lot * kLot + j, k = i % kPerGroup * kStep;
+                    const int32_t t = tile * 128 + static_cast<int32_t>(group * 16 + k + lane_row);
+                    if (i / kPerGroup == g && there && t >= any_lo && t < any_hi) x[i % kAhead] = __ldg(reinterpret_cast<const uint4*>(from_group + k * D));
+                }
             }
         }
     };
-    auto store = [&](uint32_t half, uint4 (&x)[kHalf], uint32_t slot, bool check) {
-        if (check) {  // some row does not see some key: a NaN among the values would spread through a weight of zero
-            bool nan = false;
-#pragma unroll
-            for (int i = 0; i < kHalf; ++i) nan |= drop_nan(x[i].x) | drop_nan(x[i].y) | drop_nan(x[i].z) | drop_nan(x[i].w);
-            if (nan) *nan_seen = 1;
-        }
-#pragma unroll
-        for (uint32_t i = 0; i < kHalf; ++i) {
-            const uint32_t row = (half * kHalf + i) * kStep, at = (slot + to + row * 128) ^ ((row & 7) << 4);
-            sts128(at, widen_lo(x[i].x), widen_hi(x[i].x), widen_lo(x[i].y), widen_hi(x[i].y));
-            sts128(at ^ 16, widen_lo(x[i].z), widen_hi(x[i].z), widen_lo(x[i].w), widen_hi(x[i].w));
-        }
-    };
-    limits();
-    fetch(tile);
-    take();
-    fetch(tile + static_cast<int32_t>(every));
-    if (turn != 0) {
-        // the first tile of this warp is the CTA's tile number `turn`
-        uint32_t skip = turn;
-        while (skip >= static_cast<uint32_t>(g.hi - tile)) {
-            const uint32_t left = static_cast<uint32_t>(g.hi - tile);
-            skip -= left, count += left;
-            const uint64_t begin = g.unit_end;
-            if (begin >= range.end || !next_unit(c, w, u)) return;
-            g = segment(range, u, begin);
-            tile = g.lo;
-        }
-        tile += static_cast<int32_t>(skip), count += skip;
-        limits();
-        fetch(tile);
-        take();
-        fetch(tile + static_cast<int32_t>(every));
-    }
-    uint4 a[kHalf], b[kHalf];
-    load(0, a);
+    if (!enter(turn)) return;
+    load(0);
+    load(1);
+    const float scale = fabsf(c.scale) * 1.4426950408889634f;  // its sign is q's
     for (bool more = true; more;) {
-        load(1, b);
         const uint32_t number = (2 * count + (IS_V ? 1 : 0)) * S::kParts + part, at = number % S::kSlots, slot = ring + at * S::kSlot;
-        const bool check = IS_V && (tile * 128 < all_lo || tile * 128 + 128 > all_hi);
-        wait(empty + 8 * at, (number / S::kSlots & 1) ^ 1);
+        const bool check = IS_V && !whole;
+        if (alive) alive = __all_sync(0xFFFFFFFFu, mbar_wait(empty + 8 * at, (number / S::kSlots & 1) ^ 1));
         if (!IS_V && part == 0 && lane < 8) {
             GroupScale& s = scales[count % 8][lane];
-            const int32_t v = scale_byte(v_byte) - 127;
-            s.k = page >= 0 ? exp2_int(scale_byte(k_byte) - 127) * scale : 0.0f;
+            const int32_t v = scale_byte(bytes >> 8) - 127;
+            s.k = page >= 0 ? exp2_int(scale_byte(bytes & 255u) - 127) * scale : 0.0f;
             s.log_v = page >= 0 ? static_cast<float>(v) : -INFINITY;
             s.inv_v = page >= 0 ? exp2_int(-v) : 0.0f;
             if (page == -2 && c.status != nullptr) atomicOr(c.status, 8u);  // kStatusBadIndex
         }
-        store(0, a, slot, check);
-        more = advance();
-        if (more) load(0, a);
-        store(1, b, slot, check);
+#pragma unroll
+        for (uint32_t lot = 0; lot < kAccesses / kLot; ++lot) {
+            if (check) {  // a weight of zero would spread a NaN to rows that do not see it
+                bool nan = false;
+#pragma unroll
+                for (uint32_t j = 0; j < kLot; ++j) {
+                    uint4& v = x[(lot * kLot + j) % kAhead];
+                    nan |= drop_nan(v.x) | drop_nan(v.y) | drop_nan(v.z) | drop_nan(v.w);
+                }
+                if (nan) *nan_seen = 1;
+            }
+#pragma unroll
+            for (uint32_t j = 0; j < kLot; ++j) {
+                const uint32_t i = lot * kLot + j, row = i * kStep, to_row = (slot + to + row * 128) ^ ((row & 7) << 4);
+                const uint4 v = x[i % kAhead];
+                sts128(to_row, widen_lo(v.x), widen_hi(v.x), widen_lo(v.y), widen_hi(v.y));
+                sts128(to_row ^ 16, widen_lo(v.z), widen_hi(v.z), widen_lo(v.w), widen_hi(v.w));
+            }
+            constexpr uint32_t kTurn = (kAccesses - kAhead) / kLot;  // from this lot on the next tile is loaded
+            if (lot == kTurn) more = advance();
+            if (lot < kTurn) load(lot + 2);
+            else if (more) load(lot - kTurn);
+        }
         proxy_fence();
         __syncwarp();
         if (lane == 0) mbar_arrive(full + 8 * at);
@@ -267,23 +281,25 @@ __global__ void __launch_bounds__(TilesShape<D>::kThreads, 1) tiles_kernel(const
     constexpr int kStreams = S::kStreams, kParts = S::kParts, kSlots = S::kSlots, kScaleTiles = 8;
     extern __shared__ uint8_t raw_smem[];
     __shared__ PlanSmem plan;
-    __shared__ uint64_t bars[2 * kSlots + 3 * 2 + 2];
+    __shared__ uint64_t bars[2 * kSlots + 3 * 2 + 2 + 1];
     __shared__ GroupScale scales[kScaleTiles][8];  // a tile's stay until the slots' ring has gone round behind it: at most six tiles ahead are written
     __shared__ float q_unscale[S::kRows];
     __shared__ float2 joined_ml[S::kRows];
     __shared__ uint32_t nan_seen, is_last, tmem_word;
+    __shared__ Cursor cursors[S::kConvWarps];
     __shared__ Walk walks[2];  // the segment at hand and the next one, in turn
 
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
     const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     const uint32_t q_at = (smem_u32(raw_smem) + 1023u) & ~1023u, ring = q_at + S::kQ;
-    const uint32_t full = smem_u32(bars), empty = full + 8 * kSlots, s_full = empty + 8 * kSlots, p_ready = s_full + 16, pv_done = p_ready + 16, q_ready = pv_done + 16;
+    const uint32_t full = smem_u32(bars), empty = full + 8 * kSlots, s_full = empty + 8 * kSlots, p_ready = s_full + 16, pv_done = p_ready + 16, q_ready = pv_done + 16, idle = q_ready + 16;
     if (threadIdx.x == 0) {
         for (int i = 0; i < kSlots; ++i) {
             mbar_init(full + 8 * i, 1);
             mbar_init(empty + 8 * i, 1);
         }
+        mbar_init(idle, 1);
         for (int i = 0; i < 2; ++i) {
             mbar_init(s_full + 8 * i, 1);
             mbar_init(p_ready + 8 * i, 4);
@@ -300,6 +316,7 @@ __global__ void __launch_bounds__(TilesShape<D>::kThreads, 1) tiles_kernel(const
             walks[0].range = range;
             walks[0].u = range.unit;
             walks[0].enter(c, w, range.unit_begin);
+            for (Cursor& x : cursors) x = Cursor{range.unit, walks[0].g};
         }
     }
     if (warp == 1) {
@@ -321,63 +338,76 @@ __global__ void __launch_bounds__(TilesShape<D>::kThreads, 1) tiles_kernel(const
     if (warp == 0) {
         // ---- products --------------------------------------------------------------------------------------------------------------------
         constexpr uint32_t kScores = (1u << 4) | (128u / 8 << 17) | (128u / 16 << 24), kRowsOut = (1u << 4) | (1u << 16) | (static_cast<uint32_t>(D) / 8 << 17) | (128u / 16 << 24);
+        // What the issue needs is in uniform registers: the slots' places follow from the tile's number alone, and nothing but elect_one() guards it.
         Unit u = range.unit;
         uint64_t unit_begin = range.unit_begin;
-        uint32_t base = 0, segments = 0;
-        uint32_t uses[2] = {0, 0};  // of the score buffers, whose weights have been waited for
+        uint32_t count = 0, segments = 0, uses[2] = {0, 0};  // tiles; segments; waits for the weights in either score buffer
+        constexpr uint32_t kRounds = kSlots / (2 * kParts);  // tiles that fill the ring
+        const uint64_t q_desc = desc_k(q_at), k_desc = desc_k(ring), v_desc = desc_mn(ring, S::kVTokens * 128);
+        constexpr uint32_t kSlotDesc = S::kSlot / 16, kSteps = S::kVTokens / 16;
+        auto scores = [&](uint32_t tile, uint32_t s, uint32_t buffer) {  // tile: its number in the CTA
+            const uint32_t place = __shfl_sync(0xFFFFFFFFu, tile % kRounds * (2 * kParts), 0), parity = tile / kRounds & 1;
+#pragma unroll
+            for (uint32_t part = 0; part < kParts; ++part) {
+                if (s == 0) wait(full + 8 * (place + part), parity);
+                tmem_after();
+                if (elect_one()) {
+                    const uint64_t a = q_desc + (s * kParts + part) * 1024u, b = k_desc + (place + part) * kSlotDesc;
+#pragma unroll
+                    for (uint32_t k = 0; k < 4; ++k) mma_ss(tmem + buffer * 128, a + k * 2, b + k * 2, kScores, part + k != 0);
+                    if (s == kStreams - 1) mma_commit(empty + 8 * (place + part));
+                    if (part == kParts - 1) mma_commit(s_full + 8 * buffer);
+                }
+            }
+        };
+        auto rows = [&](uint32_t tile, uint32_t s, uint32_t buffer, bool add) {
+            const uint32_t place = __shfl_sync(0xFFFFFFFFu, tile % kRounds * (2 * kParts) + kParts, 0), parity = tile / kRounds & 1;
+            wait(p_ready + 8 * buffer, (buffer == 0 ? uses[0]++ : uses[1]++) & 1);
+            const uint32_t first = __shfl_sync(0xFFFFFFFFu, add ? 1u : 0u, 0);
+#pragma unroll
+            for (uint32_t part = 0; part < kParts; ++part) {
+                if (s == 0) wait(full + 8 * (place + part), parity);
+                tmem_after();
+                if (elect_one()) {
+                    const uint64_t v = v_desc + (place + part) * kSlotDesc;
+#pragma unroll
+                    for (uint32_t k = 0; k < kSteps; ++k)
+                        mma_ts(tmem + S::kO + s * D, tmem + buffer * 128 + (part * kSteps + k) * 8, v + k * 128, kRowsOut, part + k != 0 ? 1u : first);
+                    if (s == kStreams - 1) mma_commit(empty + 8 * (place + part));
+                    if (part == kParts - 1) mma_commit(pv_done + 8 * buffer);
+                }
+            }
+        };
         for (;;) {
             const Segment g = segment(range, u, unit_begin);
-            const uint32_t n = static_cast<uint32_t>(g.hi - g.lo), steps = n * kStreams;
-            auto scores = [&](uint32_t i) {
-                const uint32_t t = i / kStreams, s = i % kStreams;
-                if (t == 0) wait(q_ready + 8 * s, segments & 1);
-                const uint32_t first = base + 2 * t * kParts;
+            const uint32_t n = static_cast<uint32_t>(g.hi - g.lo);
 #pragma unroll
-                for (int part = 0; part < kParts; ++part) {
-                    const uint32_t slot = (first + part) % kSlots;
-                    if (s == 0) wait(full + 8 * slot, (first + part) / kSlots & 1);
-                    tmem_after();
-                    if (alive && elect_one()) {
-                        const uint64_t a = desc_k(q_at + (s * kParts + part) * 16384), b = desc_k(ring + slot * S::kSlot);
-#pragma unroll
-                        for (uint32_t k = 0; k < 4; ++k) mma_ss(tmem + i % 2 * 128, a + k * 2, b + k * 2, kScores, part + k != 0);
-                        if (s == kStreams - 1) mma_commit(empty + 8 * slot);
-                        if (part == kParts - 1) mma_commit(s_full + 8 * (i % 2));
-                    }
-                    __syncwarp();
-                }
-            };
-            auto rows = [&](uint32_t i) {
-                const uint32_t t = i / kStreams, s = i % kStreams, b = i % 2, use = b == 0 ? uses[0]++ : uses[1]++;
-                wait(p_ready + 8 * b, use & 1);
-                const uint32_t first = base + (2 * t + 1) * kParts;
-#pragma unroll
-                for (int part = 0; part < kParts; ++part) {
-                    const uint32_t slot = (first + part) % kSlots;
-                    if (s == 0) wait(full + 8 * slot, (first + part) / kSlots & 1);
-                    tmem_after();
-                    if (alive && elect_one()) {
-                        constexpr uint32_t kSteps = S::kVTokens / 16;
-                        const uint64_t v = desc_mn(ring + slot * S::kSlot, S::kVTokens * 128);
-#pragma unroll
-                        for (uint32_t k = 0; k < kSteps; ++k)
-                            mma_ts(tmem + S::kO + s * D, tmem + b * 128 + (part * kSteps + k) * 8, v + k * 128, kRowsOut, t + part + k != 0);
-                        if (s == kStreams - 1) mma_commit(empty + 8 * slot);
-                        if (part == kParts - 1) mma_commit(pv_done + 8 * b);
-                    }
-                    __syncwarp();
-                }
-            };
-            scores(0);
-            if (steps > 1) scores(1);
-            for (uint32_t i = 0; i < steps; ++i) {
-                rows(i);
-                if (i + 2 < steps) scores(i + 2);
+            for (uint32_t s = 0; s < kStreams; ++s) {
+                wait(q_ready + 8 * s, segments & 1);
+                scores(count, s, s);
             }
-            base += 2 * n * kParts;
+            if (kStreams == 1 && n > 1) scores(count + 1, 0, 1);
+            for (uint32_t t = 0; t < n; ++t) {
+                if constexpr (kStreams == 2) {
+#pragma unroll
+                    for (uint32_t s = 0; s < kStreams; ++s) {
+                        rows(count + t, s, s, t != 0);
+                        if (t + 1 < n) scores(count + t + 1, s, s);
+                    }
+                } else {
+                    const uint32_t buffer = __shfl_sync(0xFFFFFFFFu, t & 1, 0);
+                    rows(count + t, 0, buffer, t != 0);
+                    if (t + 2 < n) scores(count + t + 2, 0, buffer);
+                }
+            }
+            count += n;
             ++segments;
             unit_begin = g.unit_end;
             if (unit_begin >= range.end || !next_unit(c, w, u)) break;
+        }
+        if (!alive) {  // products may still be under way: TMEM and shared memory are given back when they are done
+            if (elect_one()) mma_commit(idle);
+            mbar_wait(idle, 0);
         }
     } else if (warp >= 4 && warp < S::kSoftWarp) {
         // ---- conversion ------------------------------------------------------------------------------------------------------------------
@@ -386,8 +416,8 @@ __global__ void __launch_bounds__(TilesShape<D>::kThreads, 1) tiles_kernel(const
         constexpr uint32_t kEvery = S::kConvWarps / (2 * kParts);
         const uint32_t role = (warp - 4) % (2 * kParts), turn = (warp - 4) / (2 * kParts), part = role % kParts;
         const bool is_v = role >= kParts;
-        if (is_v) convert_slots<D, true>(c, w, range, part, turn, kEvery, ring, full, empty, scales, &nan_seen, alive);
-        else convert_slots<D, false>(c, w, range, part, turn, kEvery, ring, full, empty, scales, &nan_seen, alive);
+        if (is_v) convert_slots<D, true>(c, w, range, cursors[warp - 4], part, turn, kEvery, ring, full, empty, scales, &nan_seen, alive);
+        else convert_slots<D, false>(c, w, range, cursors[warp - 4], part, turn, kEvery, ring, full, empty, scales, &nan_seen, alive);
     } else if (warp >= S::kSoftWarp) {
         // ---- softmax ---------------------------------------------------------------------------------------------------------------------
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::kSoftRegs));
