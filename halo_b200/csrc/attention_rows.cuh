@@ -243,7 +243,7 @@ __global__ void __launch_bounds__(RowsShape<D, TS, RG, TILE, CPS, sizeof(T) == 4
         Unit u = range.unit;
         uint64_t unit_begin = range.unit_begin;
         __syncthreads();  // the consumers move `walk` on from here
-        for (uint64_t pos = range.begin; pos < range.end;) {
+        for (;;) {
             const Segment g = segment(range, u, unit_begin);
             const int32_t first = first_key(u.s, w.window, u.row0(w) / c.group), end = end_key(u.s, c.causal, (u.row0(w) + u.rows(w) - 1) / c.group);
             // a lane knows the page and the scale bytes of one group of 16 tokens, for as many tiles as 32 lanes cover; the next lot is on its way
@@ -307,9 +307,8 @@ __global__ void __launch_bounds__(RowsShape<D, TS, RG, TILE, CPS, sizeof(T) == 4
                 }
                 if (!alive) break;
             }
-            pos = g.to_end ? g.unit_end : range.end;
             unit_begin = g.unit_end;
-            if (!alive || pos >= range.end || !next_unit(c, w, u)) break;
+            if (!alive || !range.reaches(unit_begin) || !next_unit(c, w, u)) break;
         }
         if (!alive) {
             if (lane == 0) atomicOr(w.error_word, 1u);
@@ -678,6 +677,7 @@ int launch_rows_kernel(HaloCudaCtx* ctx, const AttentionCall& c, Work w, cudaStr
     using S = RowsShape<D, TS, RG, TILE, CPS, sizeof(T) == 4 ? 2 : 1>;
     w.rows = S::kRows;
     w.tile = S::kTile;
+    w.pad = 4;
     w.least = 1;
     w.group = c.group;
     w.group_inverse = static_cast<uint32_t>((0xFFFFFFFFull + c.group) / c.group);

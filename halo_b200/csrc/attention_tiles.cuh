@@ -11,11 +11,12 @@
 // is (tile of 128 keys, row tile) and takes score buffer step % 2: while the softmax of one step runs, the tensor cores run the other's products.  The
 // weights overwrite the scores in TMEM as fp16 and are the A operand of P V from there.
 // Warps:
-//   0       tcgen05.mma issue;  1: TMEM allocation
+//   0       tcgen05.mma issue
+//   1-3     q -> fp16 in shared memory, of the next segment while the last one's rows are stored (and TMEM's allocation)
 //   4-7     conversion (4-11 where D is 256): each warp makes one part of K or V of every tile in a ring of eight 16 KiB slots (a K slot: 128 keys x
 //           64 dims; a V slot: 8192 / D keys x all dims, the N operand with dims contiguous); keys that no row of the CTA sees, missing pages and,
 //           in tiles that some row does not see whole, NaN codes of values become zeros (spread_nan puts the latter back)
-//   last 8  softmax, a thread to a row (the last 4 where NS is 1); also q -> fp16 in shared memory, the epilogue, and the joining of shares
+//   last 8  softmax, a thread to a row (the last 4 where NS is 1); also the epilogue and the joining of shares
 // Work is dealt as in attention_work.cuh, so a causal prompt's long and short rows and a short chunk behind a long context fill the device alike.
 //
 // What bounds it: the tensor pipe and, for D = 128, the exponentials (256 x 128 of them per 2048 clocks of products at 16 a clock); shared memory
@@ -170,7 +171,7 @@ __device__ __forceinline__ void convert_slots(const AttentionCall& c, const Work
             if (skip < n) break;
             skip -= n, count += n;
             const uint64_t begin = cursor.g.unit_end;
-            bool more = begin < range.end;
+            bool more = range.reaches(begin);
             if (more) {
                 Unit u = cursor.u;
                 more = next_unit(c, w, u);
@@ -281,9 +282,9 @@ __global__ void __launch_bounds__(TilesShape<D>::kThreads, 1) tiles_kernel(const
     constexpr int kStreams = S::kStreams, kParts = S::kParts, kSlots = S::kSlots, kScaleTiles = 8;
     extern __shared__ uint8_t raw_smem[];
     __shared__ PlanSmem plan;
-    __shared__ uint64_t bars[2 * kSlots + 3 * 2 + 2 + 1];
+    __shared__ uint64_t bars[2 * kSlots + 3 * 2 + 3];
     __shared__ GroupScale scales[kScaleTiles][8];  // a tile's stay until the slots' ring has gone round behind it: at most six tiles ahead are written
-    __shared__ float q_unscale[S::kRows];
+    __shared__ float q_unscale[2][S::kRows];  // of a segment and the next
     __shared__ float2 joined_ml[S::kRows];
     __shared__ uint32_t nan_seen, is_last, tmem_word;
     __shared__ Cursor cursors[S::kConvWarps];
@@ -293,18 +294,19 @@ __global__ void __launch_bounds__(TilesShape<D>::kThreads, 1) tiles_kernel(const
     asm volatile("griddepcontrol.launch_dependents;");
     const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     const uint32_t q_at = (smem_u32(raw_smem) + 1023u) & ~1023u, ring = q_at + S::kQ;
-    const uint32_t full = smem_u32(bars), empty = full + 8 * kSlots, s_full = empty + 8 * kSlots, p_ready = s_full + 16, pv_done = p_ready + 16, q_ready = pv_done + 16, idle = q_ready + 16;
+    const uint32_t full = smem_u32(bars), empty = full + 8 * kSlots, s_full = empty + 8 * kSlots, p_ready = s_full + 16, pv_done = p_ready + 16, q_ready = pv_done + 16, q_free = q_ready + 8, idle = q_free + 8;
     if (threadIdx.x == 0) {
         for (int i = 0; i < kSlots; ++i) {
             mbar_init(full + 8 * i, 1);
             mbar_init(empty + 8 * i, 1);
         }
+        mbar_init(q_ready, 3);
+        mbar_init(q_free, 1);
         mbar_init(idle, 1);
         for (int i = 0; i < 2; ++i) {
             mbar_init(s_full + 8 * i, 1);
             mbar_init(p_ready + 8 * i, 4);
             mbar_init(pv_done + 8 * i, 1);
-            mbar_init(q_ready + 8 * i, 4);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         nan_seen = 0;
@@ -381,11 +383,9 @@ __global__ void __launch_bounds__(TilesShape<D>::kThreads, 1) tiles_kernel(const
         for (;;) {
             const Segment g = segment(range, u, unit_begin);
             const uint32_t n = static_cast<uint32_t>(g.hi - g.lo);
+            wait(q_ready, segments & 1);
 #pragma unroll
-            for (uint32_t s = 0; s < kStreams; ++s) {
-                wait(q_ready + 8 * s, segments & 1);
-                scores(count, s, s);
-            }
+            for (uint32_t s = 0; s < kStreams; ++s) scores(count, s, s);
             if (kStreams == 1 && n > 1) scores(count + 1, 0, 1);
             for (uint32_t t = 0; t < n; ++t) {
                 if constexpr (kStreams == 2) {
@@ -402,12 +402,99 @@ __global__ void __launch_bounds__(TilesShape<D>::kThreads, 1) tiles_kernel(const
             }
             count += n;
             ++segments;
+            if (elect_one()) mma_commit(q_free);
             unit_begin = g.unit_end;
-            if (unit_begin >= range.end || !next_unit(c, w, u)) break;
+            if (!range.reaches(unit_begin) || !next_unit(c, w, u)) break;
         }
         if (!alive) {  // products may still be under way: TMEM and shared memory are given back when they are done
             if (elect_one()) mma_commit(idle);
             mbar_wait(idle, 0);
+        }
+    } else if (warp < 4) {
+        // ---- q: eight lanes to a row, four rows of a warp at a time, the next four rows' loads under way --------------------------------------------
+        constexpr uint32_t E = D / 8, kVecs = E * 2 / 16, kWarps = 3, kStride = 4 * kWarps;
+        const uint32_t l8 = lane % 8, first = (warp - 1) * 4 + lane / 8;
+        Unit u = range.unit;
+        uint64_t unit_begin = range.unit_begin;
+        for (uint32_t segments = 0;; ++segments) {
+            const Segment g = segment(range, u, unit_begin);
+            const uint32_t rows = u.rows(w), r0 = u.row0(w), token0 = r0 / c.group, behind = r0 - token0 * c.group;
+            const uint8_t* base = c.q.p + uint64_t{u.s.row0 + token0} * c.q.token_stride + uint64_t{u.head} * c.group * c.q.head_stride + l8 * (E * 2);
+            auto load = [&](uint32_t row, uint4 (&v)[kVecs]) {
+                const uint32_t p = behind + min(row, rows - 1), t = w.group == 1 ? p : __umulhi(p, w.group_inverse);
+                const uint8_t* q = base + t * c.q.token_stride + (p - t * w.group) * c.q.head_stride;
+                if (c.q.vec) {
+#pragma unroll
+                    for (uint32_t k = 0; k < kVecs; ++k) v[k] = __ldg(reinterpret_cast<const uint4*>(q) + k);
+                } else {
+#pragma unroll
+                    for (uint32_t k = 0; k < kVecs; ++k) {
+                        uint32_t x[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const uint16_t* at = reinterpret_cast<const uint16_t*>(q) + 8 * k + 2 * e;
+                            x[e] = at[0] | static_cast<uint32_t>(at[1]) << 16;
+                        }
+                        v[k] = make_uint4(x[0], x[1], x[2], x[3]);
+                    }
+                }
+            };
+            auto store = [&](uint32_t row, const uint4 (&v)[kVecs]) {
+                // the largest finite magnitude: as integers the magnitudes of either type have their order, infinities and NaN above
+                constexpr uint32_t kInf = std::is_same_v<T, __half> ? 0x7C00u : 0x7F80u;
+                uint32_t word[4 * kVecs], top2 = 0;
+                __builtin_memcpy(word, v, sizeof word);
+#pragma unroll
+                for (uint32_t k = 0; k < 4 * kVecs; ++k) top2 = __vmaxu2(top2, word[k] & 0x7FFF7FFFu);
+                uint32_t top = max(top2 & 0xFFFFu, top2 >> 16);
+                if (top >= kInf) {  // leave them out
+                    top = 0;
+#pragma unroll
+                    for (uint32_t k = 0; k < 4 * kVecs; ++k) {
+                        const uint32_t lo = word[k] & 0x7FFFu, hi = word[k] >> 16 & 0x7FFFu;
+                        top = max(top, max(lo < kInf ? lo : 0u, hi < kInf ? hi : 0u));
+                    }
+                }
+#pragma unroll
+                for (int d = 4; d != 0; d /= 2) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+                const uint16_t top16 = static_cast<uint16_t>(top);
+                T largest;
+                __builtin_memcpy(&largest, &top16, 2);
+                const int32_t exponent = row < rows ? max(static_cast<int32_t>(__float_as_uint(to_f32(largest)) >> 23) - 127, -100) : 0;
+                const float by = row >= rows ? 0.0f : c.scale < 0 ? -exp2_int(14 - exponent) : exp2_int(14 - exponent);
+                if (row >= static_cast<uint32_t>(S::kRows)) return;
+                if (l8 == 0) q_unscale[segments & 1][row] = exp2_int(exponent - 14);
+                const uint32_t in_tile = row % 128;
+#pragma unroll
+                for (uint32_t k = 0; k < kVecs; ++k) {
+                    uint32_t h[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        T x2[2];
+                        __builtin_memcpy(x2, &word[4 * k + e], 4);
+                        h[e] = half2_bits(to_f32(x2[0]) * by, to_f32(x2[1]) * by);
+                    }
+                    const uint32_t d = l8 * E + 8 * k;  // 64-element blocks of [128 rows][128 bytes]
+                    sts128(q_at + (row / 128 * kParts + d / 64) * 16384 + in_tile * 128 + ((d % 64 / 8 ^ (in_tile & 7)) << 4), h[0], h[1], h[2], h[3]);
+                }
+            };
+            uint4 v[2][kVecs];
+            load(first, v[0]);
+            load(first + kStride, v[1]);
+            if (segments != 0) wait(q_free, (segments - 1) & 1);  // the segment before has its last scores
+#pragma unroll 1
+            for (uint32_t row = first; row < static_cast<uint32_t>(S::kRows) + first - lane / 8; row += 2 * kStride) {
+#pragma unroll
+                for (uint32_t i = 0; i < 2; ++i) {
+                    store(row + i * kStride, v[i]);
+                    load(row + (i + 2) * kStride, v[i]);
+                }
+            }
+            proxy_fence();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_ready);
+            unit_begin = g.unit_end;
+            if (!range.reaches(unit_begin) || !next_unit(c, w, u)) break;
         }
     } else if (warp >= 4 && warp < S::kSoftWarp) {
         // ---- conversion ------------------------------------------------------------------------------------------------------------------
@@ -426,69 +513,15 @@ __global__ void __launch_bounds__(TilesShape<D>::kThreads, 1) tiles_kernel(const
         const uint32_t lanes = quarter * 32 << 16, o_at = tmem + lanes + S::kO + stream * D;
         uint32_t uses[2] = {0, 0}, tiles = 0;
         const bool leader = threadIdx.x == S::kSoftWarp * 32;
-        // q: eight lanes to a row
-        auto load_q = [&](const Walk& walk) {
-            constexpr int E = D / 8, kVecs = E * 2 / 16, kBatch = 16 / kVecs < 4 ? 16 / kVecs : 4;
-            const uint32_t l8 = lane % 8, rows = walk.rows;
-            for (int it = 0; it < 8; it += kBatch) {
-                uint4 v[kBatch][kVecs];
-#pragma unroll
-                for (int b = 0; b < kBatch; ++b) {
-                    const uint32_t row = stream * 128 + quarter * 32 + (it + b) * 4 + lane / 8;
-                    const uint8_t* q = walk.at(c, w, c.q, min(row, rows - 1)) + l8 * (E * 2);
-#pragma unroll
-                    for (int k = 0; k < kVecs; ++k) {
-                        if (c.q.vec) v[b][k] = __ldg(reinterpret_cast<const uint4*>(q) + k);
-                        else {
-                            uint32_t x[4];
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                const uint16_t* at = reinterpret_cast<const uint16_t*>(q) + 8 * k + 2 * e;
-                                x[e] = at[0] | static_cast<uint32_t>(at[1]) << 16;
-                            }
-                            v[b][k] = make_uint4(x[0], x[1], x[2], x[3]);
-                        }
-                    }
-                }
-#pragma unroll
-                for (int b = 0; b < kBatch; ++b) {
-                    const uint32_t in_tile = quarter * 32 + (it + b) * 4 + lane / 8, row = stream * 128 + in_tile;
-                    float x[E], top = 0;
-#pragma unroll
-                    for (int k = 0; k < kVecs; ++k) {
-                        T e8[8];
-                        __builtin_memcpy(e8, &v[b][k], 16);
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            x[8 * k + e] = row < rows ? to_f32(e8[e]) : 0.0f;
-                            top = fmaxf(top, fabsf(x[8 * k + e]) < INFINITY ? fabsf(x[8 * k + e]) : 0.0f);
-                        }
-                    }
-#pragma unroll
-                    for (int d = 4; d != 0; d /= 2) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
-                    const int32_t exponent = max(static_cast<int32_t>(__float_as_uint(top) >> 23) - 127, -100);
-                    const float by = c.scale < 0 ? -exp2_int(14 - exponent) : exp2_int(14 - exponent);
-                    if (l8 == 0) q_unscale[row] = exp2_int(exponent - 14);
-#pragma unroll
-                    for (int k = 0; k < kVecs; ++k) {
-                        const uint32_t d = l8 * E + 8 * k;  // 64-element blocks of [128 rows][128 bytes]
-                        sts128(q_at + (stream * kParts + d / 64) * 16384 + in_tile * 128 + ((d % 64 / 8 ^ (in_tile & 7)) << 4), half2_bits(x[8 * k] * by, x[8 * k + 1] * by),
-                               half2_bits(x[8 * k + 2] * by, x[8 * k + 3] * by), half2_bits(x[8 * k + 4] * by, x[8 * k + 5] * by), half2_bits(x[8 * k + 6] * by, x[8 * k + 7] * by));
-                    }
-                }
-            }
-            proxy_fence();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(q_ready + 8 * stream);
-        };
-        load_q(walks[0]);
+        uint32_t segments = 0;
         for (uint32_t turn = 0;; turn ^= 1) {
             const Walk& walk = walks[turn];
             if (leader) {
                 walks[turn ^ 1] = walk;
                 walks[turn ^ 1].advance(c, w);
             }
-            const float qs = q_unscale[r];
+            wait(q_ready, segments & 1);
+            const float qs = q_unscale[segments++ & 1][r];
             const uint32_t j = walk.token(w, min(r, walk.rows - 1));
             const int32_t lo = first_key(walk.u.s, w.window, j), hi = end_key(walk.u.s, c.causal, j);
             // keys that every row of this row tile sees (a tile without rows: of its last row's; nothing of it is kept)
@@ -512,10 +545,13 @@ __global__ void __launch_bounds__(TilesShape<D>::kThreads, 1) tiles_kernel(const
                 tmem_wait_ld();
                 if (masked) {
 #pragma unroll
-                    for (int q = 0; q < 4; ++q)
+                    for (int q = 0; q < 4; ++q) {
+                        const uint32_t at = from + static_cast<uint32_t>(32 * q);
+                        if (__all_sync(0xFFFFFFFFu, at < seen && seen - at >= 32u)) continue;  // every row of the warp sees these keys
 #pragma unroll
                         for (int e = 0; e < 32; ++e)
-                            if (from + static_cast<uint32_t>(32 * q + e) >= seen) x[q][e] = 0xFF800000u;  // -inf
+                            if (at + static_cast<uint32_t>(e) >= seen) x[q][e] = 0xFF800000u;  // -inf
+                    }
                 }
                 // Missing keys are zeros with log_v = -inf; the factor of a group's scores is not negative: the largest score is the largest exponent.
                 float top = -INFINITY;
@@ -581,9 +617,6 @@ __global__ void __launch_bounds__(TilesShape<D>::kThreads, 1) tiles_kernel(const
                 if (kStreams == 1) b ^= 1;
                 ++tiles;
             }
-            bar_sync(1, kSoft);  // the next segment is known
-            // q is free with this segment's last scores; the next one's goes in front of the rows, so that its products begin
-            if (walks[turn ^ 1].more != 0) load_q(walks[turn ^ 1]);
             wait(prev_bar, prev_parity);
             tmem_after();
             // ---- the segment's rows ------------------------------------------------------------------------------------------------------
@@ -667,6 +700,7 @@ int launch_tiles_kernel(HaloCudaCtx* ctx, const AttentionCall& c, Work w, cudaSt
     using S = TilesShape<D>;
     w.rows = S::kRows;
     w.tile = S::kTile;
+    w.pad = 3;
     w.least = 1;
     w.group = c.group;
     w.group_inverse = static_cast<uint32_t>((0xFFFFFFFFull + c.group) / c.group);

@@ -2,9 +2,10 @@
 //
 // A unit is (sequence, tile of packed rows, kv head): the packed rows of a sequence under one kv head are its (token, query head of the group)
 // pairs, token-major, so that a group's heads share every key and value that is fetched.  A unit walks the key tiles that any of its rows sees.  The key tiles
-// of all units, one unit after the other, are cut into gridDim.x equal ranges: no CTA has more than one tile more than another whatever
-// the lengths, and only the units at the ends of a range are shared with other CTAs.  Every CTA finds its range by itself from the lengths on the
-// device, so that a captured call follows them.
+// of all units, one unit after the other and `pad` positions without a tile in front of each (what a unit costs besides its tiles), are cut into gridDim.x
+// equal ranges: the CTAs' work is alike whatever the lengths, and only the units at the ends of a range are shared with other CTAs.  An end among
+// the positions without a tile counts as the unit's beginning.  Every CTA finds its range by itself from the lengths on the device, so that a captured
+// call follows them.
 //
 // A shared unit's CTAs store (maximum, sum, weighted row) per row in scratch; the last one to arrive (a counter in scratch, left at zero) joins them in
 // CTA order, so the result does not depend on who was last.
@@ -16,7 +17,8 @@ namespace attn {
 
 struct Work {  // what every kernel of a call is told besides the call
     uint32_t rows, tile;          // packed rows of a unit, keys of a tile
-    uint32_t least;               // tiles of a CTA, where a call has few
+    uint32_t pad;                 // what a unit costs besides its tiles, in tiles
+    uint32_t least;               // positions of a CTA, where a call has few
     uint32_t group, group_inverse;  // query heads of a kv head; ceil(2^32 / group)
     uint32_t row_tiles;           // of the longest sequence at most
     uint32_t lanes;               // of a warp that look at one sequence when the tiles are counted: a power of two
@@ -91,10 +93,11 @@ __device__ __forceinline__ uint64_t quotient(uint64_t a, uint64_t b) {
 __device__ __forceinline__ uint32_t owner(uint64_t x, uint64_t total, uint32_t n) { return static_cast<uint32_t>(quotient((x + 1) * n - 1, total)); }
 
 struct Range {
-    uint64_t begin, end, total;  // this CTA's tiles
-    uint32_t ctas;               // that have a range
-    uint64_t unit_begin;         // position of the first unit's first tile
-    Unit unit;                   // of tile `begin`
+    uint64_t begin, end, total;  // this CTA's positions
+    uint32_t ctas, pad;          // CTAs that have a range
+    uint64_t unit_begin;         // position that the first unit begins at
+    Unit unit;                   // of position `begin`
+    __device__ __forceinline__ bool reaches(uint64_t unit) const { return end > unit + pad; }  // a tile of the unit that begins at this position
 };
 
 struct PlanSmem {
@@ -113,7 +116,7 @@ __device__ inline bool find_range(const AttentionCall& c, const Work& w, PlanSme
         if (i < n_seq) {
             const Seq s = sequence(c.rows, c.cache, i);
             const uint32_t packed = packed_rows(c, w, s);
-            for (uint32_t r0 = sub * w.rows; r0 < packed; r0 += w.lanes * w.rows) n += span_of(c, w, s, r0, min(r0 + w.rows, packed) - 1).tiles();
+            for (uint32_t r0 = sub * w.rows; r0 < packed; r0 += w.lanes * w.rows) n += span_of(c, w, s, r0, min(r0 + w.rows, packed) - 1).tiles() + w.pad;
         }
         for (uint32_t d = w.lanes / 2; d != 0; d /= 2) n += __shfl_xor_sync(0xFFFFFFFFu, n, d);
         return n * c.cache.n_kv;
@@ -149,6 +152,7 @@ __device__ inline bool find_range(const AttentionCall& c, const Work& w, PlanSme
     const uint32_t ctas = static_cast<uint32_t>(min(uint64_t{gridDim.x}, max(total / w.least, uint64_t{1})));
     if (blockIdx.x >= ctas) return false;
     out->ctas = ctas;
+    out->pad = w.pad;
     out->begin = quotient(total * blockIdx.x, ctas);
     out->end = quotient(total * (blockIdx.x + 1), ctas);
     uint64_t before = 0;
@@ -177,7 +181,7 @@ __device__ inline bool find_range(const AttentionCall& c, const Work& w, PlanSme
     for (uint32_t base = 0; base < row_tiles; base += 32) {
         const uint32_t r = base + lane;
         uint64_t x = 0;
-        if (r < row_tiles) x = uint64_t{span_of(c, w, u.s, r * w.rows, min((r + 1) * w.rows, u.packed) - 1).tiles()} * c.cache.n_kv;
+        if (r < row_tiles) x = uint64_t{span_of(c, w, u.s, r * w.rows, min((r + 1) * w.rows, u.packed) - 1).tiles() + w.pad} * c.cache.n_kv;
         const uint64_t mine = x;
         for (uint32_t d = 1; d < 32; d *= 2) {
             const uint64_t y = __shfl_up_sync(0xFFFFFFFFu, x, d);
@@ -194,26 +198,27 @@ __device__ inline bool find_range(const AttentionCall& c, const Work& w, PlanSme
     }
     set_row_tile(c, w, u, row_tile);
     at -= front;
-    u.head = static_cast<uint32_t>(quotient(at, u.span.tiles()));
-    out->unit_begin = out->begin - (at - uint64_t{u.head} * u.span.tiles());
-    return true;
+    u.head = static_cast<uint32_t>(quotient(at, u.span.tiles() + w.pad));
+    out->unit_begin = out->begin - (at - uint64_t{u.head} * (u.span.tiles() + w.pad));
+    return out->reaches(out->unit_begin);
 }
 
 /// A stretch of a unit's tiles that one CTA walks.
 struct Segment {
     int32_t lo, hi;            // tiles of keys
-    uint64_t unit_begin, unit_end;
+    uint64_t unit_begin, unit_end;  // positions of the unit's tiles
     bool from_start, to_end;
     __device__ __forceinline__ bool whole() const { return from_start && to_end; }
 };
 __device__ __forceinline__ Segment segment(const Range& r, const Unit& u, uint64_t unit_begin) {
     Segment g;
-    g.unit_begin = unit_begin;
-    g.unit_end = unit_begin + u.span.tiles();
-    g.from_start = unit_begin >= r.begin;
+    const uint64_t first = unit_begin + r.pad;  // position of the unit's first tile
+    g.unit_begin = first;
+    g.unit_end = first + u.span.tiles();
+    g.from_start = first >= r.begin;
     g.to_end = g.unit_end <= r.end;
-    g.lo = u.span.lo + (g.from_start ? 0 : static_cast<int32_t>(r.begin - unit_begin));
-    g.hi = g.to_end ? u.span.hi : u.span.lo + static_cast<int32_t>(r.end - unit_begin);
+    g.lo = u.span.lo + (g.from_start ? 0 : static_cast<int32_t>(r.begin - first));
+    g.hi = g.to_end ? u.span.hi : u.span.lo + static_cast<int32_t>(r.end - first);
     return g;
 }
 
@@ -232,7 +237,7 @@ struct Walk {
         more = 1;
     }
     __device__ void advance(const AttentionCall& c, const Work& w) {
-        more = g.unit_end < range.end && next_unit(c, w, u);
+        more = range.reaches(g.unit_end) && next_unit(c, w, u);
         if (more) enter(c, w, g.unit_end);
     }
     /// The token of row r < 256 of the unit (group_inverse = ceil(2^32 / group): exact while (group + 256) * group < 2^32).
