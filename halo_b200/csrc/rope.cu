@@ -5,7 +5,7 @@
 // sincospif, whose argument is then in [-1, 1).
 //
 // What bounds it: HBM, 2 * size bytes an element.  A block takes a few tokens and a share of their heads: it computes the tokens' cosines and
-// sines once into shared memory, then every thread has four units in flight, a unit being the 16-byte vectors of both halves of 16 / size
+// sines into shared memory while its first loads are under way; a thread has two units in flight, a unit being the 16-byte vectors of both halves of 16 / size
 // pairs (one vector where pairs are adjacent), or a vector to copy.
 #include "rope.h"
 
@@ -13,13 +13,14 @@ namespace halo_cuda {
 namespace attn {
 namespace {
 
-constexpr uint32_t kThreads = 256, kUnroll = 4, kMaxTokens = 4;
+constexpr uint32_t kThreads = 256, kUnroll = 2, kMaxTokens = 4;
 
 struct RopeArgs {
     const int32_t* positions;
     Heads q, k, q_out, k_out;
     uint32_t n_tokens, n_q, heads, dim;     // heads: n_q + n_kv
-    uint32_t tokens_per_block, heads_per_block;
+    uint32_t tokens_per_block, heads_per_block;  // (of a warp, in rope_warp_kernel)
+    uint32_t shares;                             // of a token's heads, in rope_warp_kernel
     uint32_t pairs, turn_units, units;      // units of a row: those that turn, then those that copy
     uint32_t q_copies, k_copies;            // out of place: elements behind the pairs are copied
     float magnitude;
@@ -34,26 +35,20 @@ struct alignas(sizeof(T) * N) Vec {
 /// V: elements of an access, 16 bytes or (misaligned operands, odd numbers of pairs) one.  A turning unit is V pairs of the half layout, V / 2 adjacent
 /// pairs, or one pair.
 template <class T, int V, bool INTERLEAVED>
-__global__ void __launch_bounds__(kThreads) rope_kernel(const __grid_constant__ RopeArgs a) {
-    __shared__ float2 spin[kMaxTokens * HALO_CUDA_ROPE_MAX_PAIRS];
+__global__ void __launch_bounds__(kThreads, 4) rope_kernel(const __grid_constant__ RopeArgs a) {
+    constexpr int kPairs = INTERLEAVED ? (V > 1 ? V / 2 : 1) : V;  // of a unit
+    using Factors = Vec<float, kPairs>;
+    __shared__ alignas(16) float cosine[kMaxTokens * HALO_CUDA_ROPE_MAX_PAIRS], sine[kMaxTokens * HALO_CUDA_ROPE_MAX_PAIRS];
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
     const uint32_t t0 = blockIdx.x * a.tokens_per_block, nt = min(a.tokens_per_block, a.n_tokens - t0);
     const uint32_t h0 = blockIdx.y * a.heads_per_block, nh = min(a.heads_per_block, a.heads - h0);
-    for (uint32_t i = threadIdx.x; i < nt * a.pairs; i += kThreads) {
-        const uint32_t t = i / a.pairs, j = i - t * a.pairs;
-        const uint64_t phase = static_cast<uint64_t>(static_cast<int64_t>(__ldg(a.positions + t0 + t))) * a.turns[j];
-        float s, c;
-        sincospif(static_cast<float>(static_cast<int32_t>(phase >> 32)) * 0x1p-31f, &s, &c);
-        spin[i] = make_float2(c * a.magnitude, s * a.magnitude);
-    }
-    __syncthreads();
     using Word = Vec<T, V>;
     const uint32_t total = nt * nh * a.units;
-    for (uint32_t base = threadIdx.x; base < total; base += kThreads * kUnroll) {
+    for (uint32_t base = threadIdx.x, turn = 0; turn == 0 || base - threadIdx.x < total; base += kThreads * kUnroll, ++turn) {
         Word x[kUnroll], z[kUnroll];
         Word *px[kUnroll], *pz[kUnroll];  // where the results go
-        uint32_t pair[kUnroll];           // index of the unit's first pair in `spin`; ~0: copy; ~1: nothing
+        uint32_t pair[kUnroll];           // index of the unit's first pair in the factors; ~0: copy; ~1: nothing
 #pragma unroll
         for (uint32_t r = 0; r < kUnroll; ++r) {
             const uint32_t i = base + r * kThreads;
@@ -66,7 +61,6 @@ __global__ void __launch_bounds__(kThreads) rope_kernel(const __grid_constant__ 
             const uint8_t* src = in.p + uint64_t{t0 + t} * in.token_stride + uint64_t{hh} * in.head_stride;
             uint8_t* dst = out.p + uint64_t{t0 + t} * out.token_stride + uint64_t{hh} * out.head_stride;
             if (u < a.turn_units) {
-                constexpr uint32_t kPairs = INTERLEAVED ? (V > 1 ? V / 2 : 1) : V;
                 const uint32_t first = INTERLEAVED ? u * 2 * kPairs : u * V, second = INTERLEAVED ? first + 1 : first + a.pairs;
                 pair[r] = t * a.pairs + u * kPairs;
                 x[r] = *reinterpret_cast<const Word*>(src + first * sizeof(T));
@@ -82,6 +76,16 @@ __global__ void __launch_bounds__(kThreads) rope_kernel(const __grid_constant__ 
                 px[r] = reinterpret_cast<Word*>(dst + at * sizeof(T));
             }
         }
+        if (turn == 0) {  // behind the first loads, which are under way meanwhile
+            for (uint32_t i = threadIdx.x; i < nt * a.pairs; i += kThreads) {
+                const uint32_t t = i / a.pairs, j = i - t * a.pairs;
+                const uint64_t phase = static_cast<uint64_t>(static_cast<int64_t>(__ldg(a.positions + t0 + t))) * a.turns[j];
+                float s, c;
+                sincospif(static_cast<float>(static_cast<int32_t>(phase >> 32)) * 0x1p-31f, &s, &c);
+                cosine[i] = c * a.magnitude, sine[i] = s * a.magnitude;
+            }
+            __syncthreads();
+        }
 #pragma unroll
         for (uint32_t r = 0; r < kUnroll; ++r) {
             if (pair[r] == ~1u) continue;
@@ -89,22 +93,21 @@ __global__ void __launch_bounds__(kThreads) rope_kernel(const __grid_constant__ 
                 *px[r] = x[r];
                 continue;
             }
+            const Factors c = *reinterpret_cast<const Factors*>(cosine + pair[r]), s = *reinterpret_cast<const Factors*>(sine + pair[r]);
             if constexpr (INTERLEAVED && V > 1) {
 #pragma unroll
-                for (int j = 0; j < V / 2; ++j) {
-                    const float2 cs = spin[pair[r] + j];
+                for (int j = 0; j < kPairs; ++j) {
                     const float p = to_f32(x[r].v[2 * j]), q = to_f32(x[r].v[2 * j + 1]);
-                    x[r].v[2 * j] = from_f32<T>(p * cs.x - q * cs.y);
-                    x[r].v[2 * j + 1] = from_f32<T>(q * cs.x + p * cs.y);
+                    x[r].v[2 * j] = from_f32<T>(p * c.v[j] - q * s.v[j]);
+                    x[r].v[2 * j + 1] = from_f32<T>(q * c.v[j] + p * s.v[j]);
                 }
                 *px[r] = x[r];
             } else {
 #pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    const float2 cs = spin[pair[r] + j];
+                for (int j = 0; j < kPairs; ++j) {
                     const float p = to_f32(x[r].v[j]), q = to_f32(z[r].v[j]);
-                    x[r].v[j] = from_f32<T>(p * cs.x - q * cs.y);
-                    z[r].v[j] = from_f32<T>(q * cs.x + p * cs.y);
+                    x[r].v[j] = from_f32<T>(p * c.v[j] - q * s.v[j]);
+                    z[r].v[j] = from_f32<T>(q * c.v[j] + p * s.v[j]);
                 }
                 *px[r] = x[r];
                 *pz[r] = z[r];
@@ -113,20 +116,86 @@ __global__ void __launch_bounds__(kThreads) rope_kernel(const __grid_constant__ 
     }
 }
 
+/// Wide operands whose heads have a power of two of turning units, at most 32: a warp for a share of one token's heads, a lane for one unit of every
+/// 32 / units-th of them, so that its factors stay in registers.  Lanes that share a unit share out its sines and cosines; nothing is waited for but loads.
+template <class T, int V, bool INTERLEAVED>
+__global__ void __launch_bounds__(kThreads) rope_warp_kernel(const __grid_constant__ RopeArgs a) {
+    constexpr int kPairs = INTERLEAVED ? V / 2 : V, kAhead = 4;
+    using Word = Vec<T, V>;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;");
+    const uint32_t lane = threadIdx.x % 32, item = blockIdx.x * (kThreads / 32) + threadIdx.x / 32;
+    const uint32_t t = item / a.shares, share = item - t * a.shares;
+    if (t >= a.n_tokens) return;
+    const uint32_t h0 = share * a.heads_per_block, h1 = min(h0 + a.heads_per_block, a.heads);
+    const uint32_t units = a.turn_units, u = lane & (units - 1), sub = lane / units, step = 32 / units;
+    auto row = [&](uint32_t h, bool to) {
+        const bool is_q = h < a.n_q;
+        const Heads& x = to ? (is_q ? a.q_out : a.k_out) : (is_q ? a.q : a.k);
+        return x.p + uint64_t{t} * x.token_stride + uint64_t{is_q ? h : h - a.n_q} * x.head_stride;
+    };
+    const uint32_t first = INTERLEAVED ? u * 2 * kPairs : u * V, second = first + a.pairs;
+    Word x[kAhead], z[kAhead];
+    auto load = [&](uint32_t h) {
+#pragma unroll
+        for (uint32_t r = 0; r < kAhead; ++r) {
+            if (h + r * step >= h1) break;
+            const uint8_t* src = row(h + r * step, false);
+            x[r] = *reinterpret_cast<const Word*>(src + first * sizeof(T));
+            if constexpr (!INTERLEAVED) z[r] = *reinterpret_cast<const Word*>(src + second * sizeof(T));
+        }
+    };
+    load(h0 + sub);
+    const uint64_t position = static_cast<uint64_t>(static_cast<int64_t>(__ldg(a.positions + t)));
+    float c[kPairs], s[kPairs];
+    // pair p of the unit is made by the unit's lane p % step
+#pragma unroll
+    for (int m = 0; m < kPairs; ++m) {
+        if (m * step >= kPairs) break;
+        const uint64_t phase = position * a.turns[u * kPairs + min(sub + m * step, static_cast<uint32_t>(kPairs - 1))];
+        sincospif(static_cast<float>(static_cast<int32_t>(phase >> 32)) * 0x1p-31f, &s[m], &c[m]);
+    }
+    float cosine[kPairs], sine[kPairs];
+#pragma unroll
+    for (uint32_t p = 0; p < kPairs; ++p) {
+        const uint32_t from = u + units * (p & (step - 1)), m = p / step;
+        float cm = c[0], sm = s[0];
+#pragma unroll
+        for (uint32_t k = 1; k < kPairs; ++k)
+            if (m == k) cm = c[k], sm = s[k];
+        cosine[p] = __shfl_sync(0xFFFFFFFFu, cm, from) * a.magnitude;
+        sine[p] = __shfl_sync(0xFFFFFFFFu, sm, from) * a.magnitude;
+    }
+    for (uint32_t h = h0 + sub; h - sub < h1; h += kAhead * step) {
+        if (h - sub != h0) load(h);
+#pragma unroll
+        for (uint32_t r = 0; r < kAhead; ++r) {
+            if (h + r * step >= h1) break;
+            uint8_t* dst = row(h + r * step, true);
+#pragma unroll
+            for (int j = 0; j < kPairs; ++j) {
+                T &e0 = x[r].v[INTERLEAVED ? 2 * j : j], &e1 = INTERLEAVED ? x[r].v[2 * j + 1] : z[r].v[j];
+                const float p = to_f32(e0), q = to_f32(e1);
+                e0 = from_f32<T>(p * cosine[j] - q * sine[j]);
+                e1 = from_f32<T>(q * cosine[j] + p * sine[j]);
+            }
+            *reinterpret_cast<Word*>(dst + first * sizeof(T)) = x[r];
+            if constexpr (!INTERLEAVED) *reinterpret_cast<Word*>(dst + second * sizeof(T)) = z[r];
+        }
+    }
+    const uint32_t copies = a.units - a.turn_units;
+    for (uint32_t i = lane; i < (h1 - h0) * copies; i += 32) {
+        const uint32_t h = h0 + i / copies, at = 2 * a.pairs + i % copies * V;
+        if (h < a.n_q ? a.q_copies : a.k_copies) *reinterpret_cast<Word*>(row(h, true) + at * sizeof(T)) = *reinterpret_cast<const Word*>(row(h, false) + at * sizeof(T));
+    }
+}
+
 template <class T, int V, bool INTERLEAVED>
 int launch(RopeArgs a, cudaStream_t s) {
     const bool copies = a.q_copies || a.k_copies;
     a.turn_units = INTERLEAVED ? a.pairs * 2 / (V > 1 ? V : 2) : a.pairs / V;
     a.units = a.turn_units + (copies ? (a.dim - 2 * a.pairs) / V : 0);
-    // One pass of the loop a block where there is enough for it: first whole tokens, then shares of one token's heads.
-    const uint32_t room = kThreads * kUnroll, per_token = a.heads * a.units;
-    a.tokens_per_block = per_token == 0 ? 1 : std::min(std::max(room / per_token, 1u), kMaxTokens);
-    a.heads_per_block = a.tokens_per_block > 1 ? a.heads : std::min(a.heads, std::max(room / a.units, 1u));
-    const uint32_t shares = (a.heads + a.heads_per_block - 1) / a.heads_per_block;  // <= 131070
-    a.heads_per_block = (a.heads + shares - 1) / shares;
-    if (shares > 65535u) a.heads_per_block = (a.heads + 65534u) / 65535u;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((a.n_tokens + a.tokens_per_block - 1) / a.tokens_per_block, (a.heads + a.heads_per_block - 1) / a.heads_per_block);
     cfg.blockDim = dim3(kThreads);
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
@@ -134,6 +203,30 @@ int launch(RopeArgs a, cudaStream_t s) {
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
+    if constexpr (V > 1) {
+        if (a.turn_units <= 32 && (a.turn_units & (a.turn_units - 1)) == 0) {
+            // A token's heads to one warp, for its factors' sake, unless that leaves the device without warps; at least one step of heads each.
+            constexpr uint32_t kWarps = 148 * 16;
+            const uint32_t step = 32 / a.turn_units, most = (a.heads + step - 1) / step;
+            a.shares = std::min(most, (kWarps + a.n_tokens - 1) / a.n_tokens);
+            a.heads_per_block = (a.heads + a.shares - 1) / a.shares;
+            a.shares = (a.heads + a.heads_per_block - 1) / a.heads_per_block;
+            const uint64_t blocks = (uint64_t{a.n_tokens} * a.shares + kThreads / 32 - 1) / (kThreads / 32);
+            if (uint64_t{a.n_tokens} * a.shares <= 0x7FFFFFFFu) {
+                cfg.gridDim = dim3(static_cast<uint32_t>(blocks));
+                HC_CUDA(cudaLaunchKernelEx(&cfg, rope_warp_kernel<T, V, INTERLEAVED>, a));
+                return 0;
+            }
+        }
+    }
+    // One pass of the loop a block where there is enough for it: first whole tokens, then shares of one token's heads.
+    const uint32_t room = kThreads * kUnroll, per_token = a.heads * a.units;
+    a.tokens_per_block = per_token == 0 ? 1 : std::min(std::max(room / per_token, 1u), kMaxTokens);
+    a.heads_per_block = a.tokens_per_block > 1 ? a.heads : std::min(a.heads, std::max(room / a.units, 1u));
+    const uint32_t shares = (a.heads + a.heads_per_block - 1) / a.heads_per_block;  // <= 131070
+    a.heads_per_block = (a.heads + shares - 1) / shares;
+    if (shares > 65535u) a.heads_per_block = (a.heads + 65534u) / 65535u;
+    cfg.gridDim = dim3((a.n_tokens + a.tokens_per_block - 1) / a.tokens_per_block, (a.heads + a.heads_per_block - 1) / a.heads_per_block);
     HC_CUDA(cudaLaunchKernelEx(&cfg, rope_kernel<T, V, INTERLEAVED>, a));
     return 0;
 }
