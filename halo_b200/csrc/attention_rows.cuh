@@ -114,69 +114,107 @@ __device__ void spread_nan(const AttentionCall& c, const Work& w, const Unit& u,
 /// (maximum, 1 / sum).
 template <class T, int D>
 __device__ __forceinline__ void join_partials(const AttentionCall& c, const Work& w, const Walk& walk, uint32_t c0, uint32_t shares, uint32_t warp0, uint32_t warps, float2* row_ml) {
-    constexpr uint32_t kAhead = 4;  // shares whose loads are under way together
-    const uint32_t thread = threadIdx.x - warp0 * 32, threads = warps * 32, rows = walk.rows;
+    const uint32_t thread = threadIdx.x - warp0 * 32, threads = warps * 32, lane = thread % 32, rows = walk.rows;
     auto slot = [&](uint32_t k) { return partial_slot(w, D, c0 + min(k, shares - 1), k == 0); };
+    // Without a maximum a share's sum and row are zero, or NaN: they count as they are.
+    if (shares <= 4) {
 #pragma unroll 1
-    for (uint32_t r = thread; r < rows; r += threads) {
-        float m = -INFINITY, l = 0;
-#pragma unroll 1
-        for (uint32_t k0 = 0; k0 < shares; k0 += 2 * kAhead) {
-            float2 ml[2 * kAhead];
+        for (uint32_t r = thread; r < rows; r += threads) {
+            float2 ml[4];
+            float m = -INFINITY, l = 0;
 #pragma unroll
-            for (uint32_t k = 0; k < 2 * kAhead; ++k) ml[k] = __ldcg(reinterpret_cast<const float2*>(slot(k0 + k) + w.rows * D + 2 * r));
-            float top = m;
+            for (uint32_t k = 0; k < 4; ++k) ml[k] = __ldcg(reinterpret_cast<const float2*>(slot(k) + w.rows * D + 2 * r));
 #pragma unroll
-            for (uint32_t k = 0; k < 2 * kAhead; ++k) top = fmaxf(top, ml[k].x);
-            l *= m == -INFINITY ? 1.0f : exp2_approx(m - top);  // without a maximum sum and row are zero, or NaN
-            m = top;
+            for (uint32_t k = 0; k < 4; ++k) m = fmaxf(m, ml[k].x);
 #pragma unroll
-            for (uint32_t k = 0; k < 2 * kAhead; ++k)
-                if (k0 + k < shares) l += ml[k].x == -INFINITY ? ml[k].y : exp2_approx(ml[k].x - top) * ml[k].y;
+            for (uint32_t k = 0; k < 4; ++k)
+                if (k < shares) l += ml[k].x == -INFINITY ? ml[k].y : exp2_approx(ml[k].x - m) * ml[k].y;
+            row_ml[r] = make_float2(m, l != 0 ? 1.0f / l : 0.0f);
         }
-        row_ml[r] = make_float2(m, l != 0 ? 1.0f / l : 0.0f);
-    }
-    bar_sync(1, threads);
+    } else {  // a warp to four rows, a lane to every 32nd share
 #pragma unroll 1
-    for (uint32_t i = thread; i < rows * (D / 4); i += 2 * threads) {
-        float4 o[2];
-        float m[2];
-        uint32_t row[2], dim[2];
+        for (uint32_t r0 = thread / 32 * 4; r0 < rows; r0 += warps * 4) {
+            float m[4], l[4] = {};
 #pragma unroll
-        for (uint32_t h = 0; h < 2; ++h) {
-            const uint32_t at = min(i + h * threads, rows * (D / 4) - 1);
-            row[h] = at / (D / 4), dim[h] = at % (D / 4) * 4;
-            m[h] = row_ml[row[h]].x;
-            o[h] = make_float4(0, 0, 0, 0);
-        }
+            for (uint32_t i = 0; i < 4; ++i) m[i] = -INFINITY;
 #pragma unroll 1
-        for (uint32_t k0 = 0; k0 < shares; k0 += kAhead) {
-            float f[2][kAhead];
-            float4 x[2][kAhead];
+            for (uint32_t k = lane; k < shares; k += 32) {
+                float2 ml[4];
 #pragma unroll
-            for (uint32_t k = 0; k < kAhead; ++k) {
-                const float* s = slot(k0 + k);
+                for (uint32_t i = 0; i < 4; ++i) ml[i] = __ldcg(reinterpret_cast<const float2*>(slot(k) + w.rows * D + 2 * min(r0 + i, rows - 1)));
 #pragma unroll
-                for (uint32_t h = 0; h < 2; ++h) {
-                    f[h][k] = __ldcg(s + w.rows * D + 2 * row[h]);
-                    x[h][k] = __ldcg(reinterpret_cast<const float4*>(s + row[h] * D + dim[h]));
+                for (uint32_t i = 0; i < 4; ++i) {
+                    const float top = fmaxf(m[i], ml[i].x);
+                    l[i] = (m[i] == -INFINITY ? l[i] : exp2_approx(m[i] - top) * l[i]) + (ml[i].x == -INFINITY ? ml[i].y : exp2_approx(ml[i].x - top) * ml[i].y);
+                    m[i] = top;
                 }
             }
 #pragma unroll
-            for (uint32_t k = 0; k < kAhead; ++k)
+            for (uint32_t i = 0; i < 4; ++i) {
+                float top = m[i];
 #pragma unroll
-                for (uint32_t h = 0; h < 2; ++h) {
-                    // a share of weight zero adds nothing, but a NaN in it is one of a token that the row sees; behind the last share: the last again
-                    const float by = k0 + k >= shares ? 0.0f : f[h][k] == -INFINITY ? 1.0f : exp2_approx(f[h][k] - m[h]);
-                    o[h].x += by * x[h][k].x, o[h].y += by * x[h][k].y, o[h].z += by * x[h][k].z, o[h].w += by * x[h][k].w;
-                }
+                for (uint32_t d = 16; d != 0; d /= 2) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+                l[i] = m[i] == -INFINITY ? l[i] : exp2_approx(m[i] - top) * l[i];
+#pragma unroll
+                for (uint32_t d = 16; d != 0; d /= 2) l[i] += __shfl_xor_sync(0xFFFFFFFFu, l[i], d);
+                if (lane == 0 && r0 + i < rows) row_ml[r0 + i] = make_float2(top, l[i] != 0 ? 1.0f / l[i] : 0.0f);
+            }
         }
+    }
+    bar_sync(1, threads);
+    // a share of weight zero adds nothing, but a NaN in it is one of a token that the row sees; behind the last share: the last again, with weight zero
+    auto weight = [&](uint32_t k, float of, float m) { return k >= shares ? 0.0f : of == -INFINITY ? 1.0f : exp2_approx(of - m); };
+    auto add = [&](float4& o, float by, const float4& x) { o.x += by * x.x, o.y += by * x.y, o.z += by * x.z, o.w += by * x.w; };
+    auto put = [&](uint32_t r, uint32_t d, const float4& o) {
+        const float inv = row_ml[r].y;
+        T* out = reinterpret_cast<T*>(walk.at(c, w, c.out, r)) + d;
+        out[0] = from_f32<T>(o.x * inv), out[1] = from_f32<T>(o.y * inv), out[2] = from_f32<T>(o.z * inv), out[3] = from_f32<T>(o.w * inv);
+    };
+    const uint32_t pieces = rows * (D / 4);
+    if (shares <= 4) {  // loads of two pieces under way together
+#pragma unroll 1
+        for (uint32_t i = thread; i < pieces; i += 2 * threads) {
+            float f[2][4];
+            float4 x[2][4];
 #pragma unroll
-        for (uint32_t h = 0; h < 2; ++h) {
-            if (i + h * threads >= rows * (D / 4)) break;
-            const float inv = row_ml[row[h]].y;
-            T* out = reinterpret_cast<T*>(walk.at(c, w, c.out, row[h])) + dim[h];
-            out[0] = from_f32<T>(o[h].x * inv), out[1] = from_f32<T>(o[h].y * inv), out[2] = from_f32<T>(o[h].z * inv), out[3] = from_f32<T>(o[h].w * inv);
+            for (uint32_t h = 0; h < 2; ++h)
+#pragma unroll
+                for (uint32_t k = 0; k < 4; ++k) {
+                    const uint32_t at = min(i + h * threads, pieces - 1), r = at / (D / 4);
+                    f[h][k] = __ldcg(slot(k) + w.rows * D + 2 * r);
+                    x[h][k] = __ldcg(reinterpret_cast<const float4*>(slot(k) + at * 4));
+                }
+#pragma unroll
+            for (uint32_t h = 0; h < 2; ++h) {
+                const uint32_t at = i + h * threads;
+                if (at >= pieces) break;
+                const uint32_t r = at / (D / 4);
+                float4 o = make_float4(0, 0, 0, 0);
+#pragma unroll
+                for (uint32_t k = 0; k < 4; ++k) add(o, weight(k, f[h][k], row_ml[r].x), x[h][k]);
+                put(r, at % (D / 4) * 4, o);
+            }
+        }
+    } else {  // of a piece's next ten shares
+        constexpr uint32_t kAhead = 10;
+#pragma unroll 1
+        for (uint32_t i = thread; i < pieces; i += threads) {
+            const uint32_t r = i / (D / 4);
+            const float m = row_ml[r].x;
+            float4 o = make_float4(0, 0, 0, 0);
+#pragma unroll 1
+            for (uint32_t k0 = 0; k0 < shares; k0 += kAhead) {
+                float f[kAhead];
+                float4 x[kAhead];
+#pragma unroll
+                for (uint32_t k = 0; k < kAhead; ++k) {
+                    f[k] = __ldcg(slot(k0 + k) + w.rows * D + 2 * r);
+                    x[k] = __ldcg(reinterpret_cast<const float4*>(slot(k0 + k) + i * 4));
+                }
+#pragma unroll
+                for (uint32_t k = 0; k < kAhead; ++k) add(o, weight(k0 + k, f[k], m), x[k]);
+            }
+            put(r, i % (D / 4) * 4, o);
         }
     }
 }

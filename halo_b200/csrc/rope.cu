@@ -119,8 +119,8 @@ __global__ void __launch_bounds__(kThreads, 4) rope_kernel(const __grid_constant
 /// Wide operands whose heads have a power of two of turning units, at most 32: a warp for a share of one token's heads, a lane for one unit of every
 /// 32 / units-th of them, so that its factors stay in registers.  Lanes that share a unit share out its sines and cosines; nothing is waited for but loads.
 template <class T, int V, bool INTERLEAVED>
-__global__ void __launch_bounds__(kThreads) rope_warp_kernel(const __grid_constant__ RopeArgs a) {
-    constexpr int kPairs = INTERLEAVED ? V / 2 : V, kAhead = 4;
+__global__ void __launch_bounds__(kThreads, 4) rope_warp_kernel(const __grid_constant__ RopeArgs a) {
+    constexpr int kPairs = INTERLEAVED ? V / 2 : V, kAhead = 2;
     using Word = Vec<T, V>;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
