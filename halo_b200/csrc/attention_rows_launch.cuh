@@ -10,9 +10,7 @@ int launch_rows(HaloCudaCtx* ctx, const AttentionCall& c, const Work& w, cudaStr
     return with_type(c.type, [&](auto t) {
         using T = decltype(t);
         if (w.max_rows <= 16) return launch_rows_kernel<T, D, 4, 1, 64, D == 256 ? 2 : 3>(ctx, c, w, s);
-        if constexpr (sizeof(T) == 2) return launch_tiles_kernel<T, D>(ctx, c, w, s);
-        if (w.max_rows <= 32) return launch_rows_kernel<T, D, 4, 2, 64, 1>(ctx, c, w, s);
-        return launch_rows_kernel<T, D, 2, 4, 64, 1>(ctx, c, w, s);
+        return launch_tiles_kernel<T, D>(ctx, c, w, s);
     });
 }
 

@@ -1,5 +1,5 @@
-// ATTENTION for 16-bit operands and many rows to a sequence (prompts, chunks of prompts): tcgen05 products with fp16 operands, the cache's codes
-// converted to fp16 once for 256 packed rows (128 for heads of 256 elements).
+// ATTENTION for many rows to a sequence (prompts, chunks of prompts): tcgen05 products with fp16 operands, the cache's codes converted to fp16 once
+// for 256 packed rows (128 for heads of 256 elements, and for fp32 operands, whose q and weights are two fp16 terms each).
 //
 //   x_t = q . k_t * (s_K(t) * scale * log2 e) + log2 s_V(t),   p_t = 2^(x_t - r + 6),   o = sum p_t code(v_t),   l = sum p_t / s_V(t),   out = o / l
 //
@@ -7,8 +7,8 @@
 // passes r by 8, so p_t is at most 2^14 and keeps 11 bits down to 2^-20 of the reference.
 //
 // Packed rows are the M side (a TMEM lane each), keys the N side of S = Q K^T, dims the N side of O = P V.  A CTA (one an SM) holds NS tiles of
-// 128 rows: two, each with scores, weights and accumulators of its own (128 + D columns), or one with two score buffers where D is 256.  A step
-// is (tile of 128 keys, row tile) and takes score buffer step % 2: while the softmax of one step runs, the tensor cores run the other's products.  The
+// 128 rows: two, each with scores, weights and accumulators of its own (128 + D columns), or one with two score buffers.  A step
+// is (tile of 128 keys, or of 64 for fp32 rows of 256 elements; row tile) and takes score buffer step % 2: while the softmax of one step runs, the tensor cores run the other's products.  The
 // weights overwrite the scores in TMEM as fp16 and are the A operand of P V from there.
 // Warps:
 //   0       tcgen05.mma issue
@@ -27,23 +27,27 @@
 namespace halo_cuda {
 namespace attn {
 
-template <int D>
+/// TERMS: fp16 terms of q and of the weights (1: 16-bit operands, 2: fp32 operands).
+template <int D, int TERMS>
 struct TilesShape {
-    static constexpr int kStreams = D == 256 ? 1 : 2, kTile = 128, kRows = 128 * kStreams, kSlots = 8;
-    static constexpr uint32_t kSlot = 16384, kQ = kRows * D * 2;
-    static constexpr int kParts = D / 64;               // slots of a tile of K, and of V
-    static constexpr int kVTokens = 128 * 64 / D;       // keys of a V slot
+    static constexpr int kStreams = D == 256 || TERMS == 2 ? 1 : 2, kRows = 128 * kStreams, kSlots = 8;
+    static constexpr int kTile = D == 256 && TERMS == 2 ? 64 : 128;  // keys: both terms of q leave room for half
+    static constexpr int kParts = D / 64;                  // slots of a tile of K, and of V
+    static constexpr int kVTokens = kTile * 64 / D;        // keys of a V slot
+    static constexpr uint32_t kSlot = kTile * 128, kQ = kRows * D * 2 * TERMS;
     static constexpr uint32_t kSmem = 1024 + kQ + kSlots * kSlot;
-    static constexpr int kConvWarps = D == 256 ? 8 : 4, kSoftWarp = 4 + kConvWarps, kSoftWarps = 4 * kStreams, kThreads = 512;
-    static_assert((kSoftWarp + kSoftWarps) * 32 == kThreads);
+    static constexpr uint32_t kBuffer = kTile;             // columns of a score buffer, which the terms of the weights (kTile / 2 columns each) overwrite
+    static constexpr uint32_t kO = 256;                    // first accumulator column
+    static constexpr int kConvWarps = D == 256 ? 8 : 4, kSoftWarp = 4 + kConvWarps, kSoftWarps = 4 * kStreams, kThreads = (kSoftWarp + kSoftWarps) * 32;
     // Slot number i of a CTA (the parts of K of its first tile, those of V, those of K of the second, ...) has place i % kSlots.  A place's user waits for
     // its last use by the parity of that use, so all of a place's uses are to be one warp's: 2 * kParts * kEvery of convert_slots divides kSlots.
     static_assert(kSlots % kConvWarps == 0);
-    static constexpr uint32_t kAhead = D == 256 ? 16 : 8;  // 16-byte pieces that a conversion thread has under way
-    // 128 registers a thread at launch; the warpgroups hand each other what they leave
-    static constexpr int kIdleRegs = D == 256 ? 80 : 72, kConvRegs = D == 256 ? 104 : 88, kSoftRegs = kStreams == 2 ? 176 : 224;
-    static_assert(kIdleRegs + kConvRegs * (kConvWarps / 4) + kSoftRegs * kStreams <= 512);
-    static constexpr uint32_t kO = 256;                 // first accumulator column; scores are columns 0 .. 255
+    static constexpr uint32_t kAccesses = kSlot / 1024;    // 16-byte pieces of a slot that a conversion thread makes
+    static constexpr uint32_t kAhead = D == 256 ? kAccesses : 8;  // that it has under way
+    // What a thread has at launch; the warpgroups hand each other what they leave.
+    static constexpr int kLaunchRegs = kThreads == 512 ? 128 : 168;
+    static constexpr int kIdleRegs = D == 256 || TERMS == 2 ? 80 : 72, kConvRegs = D == 256 ? 104 : 88, kSoftRegs = kStreams == 2 ? 176 : 224;
+    static_assert(kIdleRegs + kConvRegs * (kConvWarps / 4) + kSoftRegs * kStreams <= kLaunchRegs * (kThreads / 128));
 };
 
 __device__ __forceinline__ uint64_t desc_k(uint32_t addr) {  // K-major, 128-byte rows and swizzle: atoms of 8 rows, 1024 bytes apart
@@ -122,30 +126,31 @@ struct Cursor {
 /// The slots of one part of K or V, of every `every`-th tile from `turn` on, over a CTA's whole range, by one warp: 16-byte pieces straight from the
 /// pages to registers, kAhead of the slot's 16 accesses under way in front of the one that is converted.  The warp of K's part 0 publishes the tile's scales
 /// with its slot.
-template <int D, bool IS_V>
+template <int D, int TERMS, bool IS_V>
 __device__ __forceinline__ void convert_slots(const AttentionCall& c, const Work& w, const Range& range, Cursor& cursor, uint32_t part, uint32_t turn, uint32_t every, uint32_t ring,
                                               uint32_t full, uint32_t empty, GroupScale (*scales)[8], uint32_t* nan_seen, bool& alive) {
-    using S = TilesShape<D>;
+    using S = TilesShape<D, TERMS>;
     constexpr uint32_t kBlocks = IS_V ? S::kParts : 1;                   // 64-dim blocks of a slot's rows
-    constexpr uint32_t kRows = IS_V ? S::kVTokens : 128, kStep = 8 / kBlocks;  // rows of a slot; of one access of the warp
-    constexpr uint32_t kAccesses = 16, kAhead = S::kAhead;
+    constexpr int32_t kTile = S::kTile;
+    constexpr uint32_t kRows = IS_V ? S::kVTokens : kTile, kStep = 8 / kBlocks;  // rows of a slot; of one access of the warp
+    constexpr uint32_t kAccesses = S::kAccesses, kAhead = S::kAhead;
     constexpr uint32_t kPerGroup = 16 / kStep;                           // accesses of 16 rows
     const uint32_t lane = threadIdx.x % 32;
     // a quarter warp has four pieces of two rows: its eight 16-byte stores lie in different banks
     const uint32_t lane_row = lane / 8 / kBlocks * 2 + lane / 4 % 2, block = lane / 8 % kBlocks;
     const uint32_t from = lane_row * D + (IS_V ? block * 64 : part * 64) + lane % 4 * 16;             // of a group's first row
     const uint32_t to = block * (kRows * 128) + lane_row * 128 + ((lane % 4 * 2 ^ (lane_row & 7)) << 4);  // second half: the same ^ 16
-    // the tile that is loaded: of the CTA's tiles number `count`, keys from t0 on; lane i < 8 knows page and scale bytes of its i-th 16 keys, and those of
+    // the tile that is loaded: of the CTA's tiles number `count`, keys from t0 on; lane i knows page and scale bytes of its i-th 16 keys, and those of
     // this warp's next tile
     int32_t tile, last, any_lo, any_hi, page = -1, page_next = -1;
     uint32_t bytes = 0, bytes_next = 0, count = 0;
-    uint64_t group_at = 0;              // lane i < 8: where its keys' codes begin in the pool
+    uint64_t group_at = 0;              // lane i: where its keys' codes begin in the pool
     bool plain = false, whole = false;  // every key is there and seen by some row; by all rows
     const uint8_t* pool = nullptr;
     auto fetch = [&](int32_t of) {
-        const int32_t t = of * 128 + static_cast<int32_t>(lane) * 16;
+        const int32_t t = of * kTile + static_cast<int32_t>(lane) * 16;
         page_next = -1;
-        if (lane < 8 && of < last && t < any_hi && t + 16 > any_lo) {
+        if (lane < kTile / 16 && of < last && t < any_hi && t + 16 > any_lo) {
             const int32_t p = page_of(c.cache, cursor.u.seq, t >> c.cache.page_shift);
             page_next = static_cast<uint32_t>(p) < c.cache.n_pages ? p : -2;  // -2: a visible key's page is not there
             if (!IS_V && part == 0 && page_next >= 0) {
@@ -158,10 +163,10 @@ __device__ __forceinline__ void convert_slots(const AttentionCall& c, const Work
         page = page_next, bytes = bytes_next;
         const Unit& u = cursor.u;
         const uint32_t first = u.row0(w) / c.group, final = (u.row0(w) + u.rows(w) - 1) / c.group;
-        const int32_t t0 = tile * 128;
-        plain = t0 >= any_lo && t0 + 128 <= any_hi && __all_sync(0xFFFFFFFFu, page >= 0 || lane >= 8);
-        whole = plain && t0 >= first_key(u.s, w.window, final) && t0 + 128 <= end_key(u.s, c.causal, first);
-        group_at = static_cast<uint32_t>(max(page, 0)) * c.cache.page_stride + (lane * 16 & (c.cache.page_tokens - 1)) * D;
+        const int32_t t0 = tile * kTile;
+        plain = t0 >= any_lo && t0 + kTile <= any_hi && __all_sync(0xFFFFFFFFu, page >= 0 || lane >= kTile / 16);
+        whole = plain && t0 >= first_key(u.s, w.window, final) && t0 + kTile <= end_key(u.s, c.causal, first);
+        group_at = static_cast<uint32_t>(max(page, 0)) * c.cache.page_stride + ((static_cast<uint32_t>(t0) + lane * 16) & (c.cache.page_tokens - 1)) * D;
         fetch(tile + static_cast<int32_t>(every));
     };
     /// Enters the cursor's segment at its tile number `skip`, or a later one's at what is left of it; false at the end of the range.
@@ -225,7 +230,7 @@ __device__ __forceinline__ void convert_slots(const AttentionCall& c, const Work
 #pragma unroll
                 for (uint32_t j = 0; j < kLot; ++j) {
                     const uint32_t i = lot * kLot + j, k = i % kPerGroup * kStep;
-                    const int32_t t = tile * 128 + static_cast<int32_t>(group * 16 + k + lane_row);
+                    const int32_t t = tile * kTile + static_cast<int32_t>(group * 16 + k + lane_row);
                     if (i / kPerGroup == g && there && t >= any_lo && t < any_hi) x[i % kAhead] = __ldg(reinterpret_cast<const uint4*>(from_group + k * D));
                 }
             }
@@ -239,7 +244,7 @@ __device__ __forceinline__ void convert_slots(const AttentionCall& c, const Work
         const uint32_t number = (2 * count + (IS_V ? 1 : 0)) * S::kParts + part, at = number % S::kSlots, slot = ring + at * S::kSlot;
         const bool check = IS_V && !whole;
         if (alive) alive = __all_sync(0xFFFFFFFFu, mbar_wait(empty + 8 * at, (number / S::kSlots & 1) ^ 1));
-        if (!IS_V && part == 0 && lane < 8) {
+        if (!IS_V && part == 0 && lane < kTile / 16) {
             GroupScale& s = scales[count % 8][lane];
             const int32_t v = scale_byte(bytes >> 8) - 127;
             s.k = page >= 0 ? exp2_int(scale_byte(bytes & 255u) - 127) * scale : 0.0f;
@@ -277,8 +282,10 @@ __device__ __forceinline__ void convert_slots(const AttentionCall& c, const Work
 }
 
 template <class T, int D>
-__global__ void __launch_bounds__(TilesShape<D>::kThreads, 1) tiles_kernel(const __grid_constant__ AttentionCall c, const __grid_constant__ Work w) {
-    using S = TilesShape<D>;
+__global__ void __launch_bounds__(TilesShape<D, sizeof(T) == 4 ? 2 : 1>::kThreads, 1) tiles_kernel(const __grid_constant__ AttentionCall c, const __grid_constant__ Work w) {
+    constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;
+    using S = TilesShape<D, TERMS>;
+    constexpr int kTile = S::kTile;
     constexpr int kStreams = S::kStreams, kParts = S::kParts, kSlots = S::kSlots, kScaleTiles = 8;
     extern __shared__ uint8_t raw_smem[];
     __shared__ PlanSmem plan;
@@ -339,7 +346,7 @@ __global__ void __launch_bounds__(TilesShape<D>::kThreads, 1) tiles_kernel(const
     if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::kIdleRegs));
     if (warp == 0) {
         // ---- products --------------------------------------------------------------------------------------------------------------------
-        constexpr uint32_t kScores = (1u << 4) | (128u / 8 << 17) | (128u / 16 << 24), kRowsOut = (1u << 4) | (1u << 16) | (static_cast<uint32_t>(D) / 8 << 17) | (128u / 16 << 24);
+        constexpr uint32_t kScores = (1u << 4) | (static_cast<uint32_t>(kTile) / 8 << 17) | (128u / 16 << 24), kRowsOut = (1u << 4) | (1u << 16) | (static_cast<uint32_t>(D) / 8 << 17) | (128u / 16 << 24);
         // What the issue needs is in uniform registers: the slots' places follow from the tile's number alone, and nothing but elect_one() guards it.
         Unit u = range.unit;
         uint64_t unit_begin = range.unit_begin;
@@ -354,9 +361,13 @@ __global__ void __launch_bounds__(TilesShape<D>::kThreads, 1) tiles_kernel(const
                 if (s == 0) wait(full + 8 * (place + part), parity);
                 tmem_after();
                 if (elect_one()) {
-                    const uint64_t a = q_desc + (s * kParts + part) * 1024u, b = k_desc + (place + part) * kSlotDesc;
+                    const uint64_t b = k_desc + (place + part) * kSlotDesc;
 #pragma unroll
-                    for (uint32_t k = 0; k < 4; ++k) mma_ss(tmem + buffer * 128, a + k * 2, b + k * 2, kScores, part + k != 0);
+                    for (uint32_t term = 0; term < TERMS; ++term) {
+                        const uint64_t a = q_desc + ((term + s) * kParts + part) * 1024u;
+#pragma unroll
+                        for (uint32_t k = 0; k < 4; ++k) mma_ss(tmem + buffer * S::kBuffer, a + k * 2, b + k * 2, kScores, part + term + k != 0);
+                    }
                     if (s == kStreams - 1) mma_commit(empty + 8 * (place + part));
                     if (part == kParts - 1) mma_commit(s_full + 8 * buffer);
                 }
@@ -373,8 +384,11 @@ __global__ void __launch_bounds__(TilesShape<D>::kThreads, 1) tiles_kernel(const
                 if (elect_one()) {
                     const uint64_t v = v_desc + (place + part) * kSlotDesc;
 #pragma unroll
-                    for (uint32_t k = 0; k < kSteps; ++k)
-                        mma_ts(tmem + S::kO + s * D, tmem + buffer * 128 + (part * kSteps + k) * 8, v + k * 128, kRowsOut, part + k != 0 ? 1u : first);
+                    for (uint32_t term = 0; term < TERMS; ++term)
+#pragma unroll
+                        for (uint32_t k = 0; k < kSteps; ++k)
+                            mma_ts(tmem + S::kO + s * D, tmem + buffer * S::kBuffer + term * (kTile / 2) + (part * kSteps + k) * 8, v + k * 128, kRowsOut,
+                                   part + term + k != 0 ? 1u : first);
                     if (s == kStreams - 1) mma_commit(empty + 8 * (place + part));
                     if (part == kParts - 1) mma_commit(pv_done + 8 * buffer);
                 }
@@ -412,14 +426,14 @@ __global__ void __launch_bounds__(TilesShape<D>::kThreads, 1) tiles_kernel(const
         }
     } else if (warp < 4) {
         // ---- q: eight lanes to a row, four rows of a warp at a time, the next four rows' loads under way --------------------------------------------
-        constexpr uint32_t E = D / 8, kVecs = E * 2 / 16, kWarps = 3, kStride = 4 * kWarps;
+        constexpr uint32_t E = D / 8, kVecs = E * sizeof(T) / 16, kWarps = 3, kStride = 4 * kWarps, kLoads = TERMS == 2 ? 1 : 2;
         const uint32_t l8 = lane % 8, first = (warp - 1) * 4 + lane / 8;
         Unit u = range.unit;
         uint64_t unit_begin = range.unit_begin;
         for (uint32_t segments = 0;; ++segments) {
             const Segment g = segment(range, u, unit_begin);
             const uint32_t rows = u.rows(w), r0 = u.row0(w), token0 = r0 / c.group, behind = r0 - token0 * c.group;
-            const uint8_t* base = c.q.p + uint64_t{u.s.row0 + token0} * c.q.token_stride + uint64_t{u.head} * c.group * c.q.head_stride + l8 * (E * 2);
+            const uint8_t* base = c.q.p + uint64_t{u.s.row0 + token0} * c.q.token_stride + uint64_t{u.head} * c.group * c.q.head_stride + l8 * (E * sizeof(T));
             auto load = [&](uint32_t row, uint4 (&v)[kVecs]) {
                 const uint32_t p = behind + min(row, rows - 1), t = w.group == 1 ? p : __umulhi(p, w.group_inverse);
                 const uint8_t* q = base + t * c.q.token_stride + (p - t * w.group) * c.q.head_stride;
@@ -432,62 +446,91 @@ __global__ void __launch_bounds__(TilesShape<D>::kThreads, 1) tiles_kernel(const
                         uint32_t x[4];
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            const uint16_t* at = reinterpret_cast<const uint16_t*>(q) + 8 * k + 2 * e;
-                            x[e] = at[0] | static_cast<uint32_t>(at[1]) << 16;
+                            if constexpr (TERMS == 2) {
+                                x[e] = reinterpret_cast<const uint32_t*>(q)[4 * k + e];
+                            } else {
+                                const uint16_t* at = reinterpret_cast<const uint16_t*>(q) + 8 * k + 2 * e;
+                                x[e] = at[0] | static_cast<uint32_t>(at[1]) << 16;
+                            }
                         }
                         v[k] = make_uint4(x[0], x[1], x[2], x[3]);
                     }
                 }
             };
             auto store = [&](uint32_t row, const uint4 (&v)[kVecs]) {
-                // the largest finite magnitude: as integers the magnitudes of either type have their order, infinities and NaN above
-                constexpr uint32_t kInf = std::is_same_v<T, __half> ? 0x7C00u : 0x7F80u;
-                uint32_t word[4 * kVecs], top2 = 0;
+                // the largest finite magnitude: as integers the magnitudes of every type have their order, infinities and NaN above
+                uint32_t word[4 * kVecs], top = 0;
                 __builtin_memcpy(word, v, sizeof word);
-#pragma unroll
-                for (uint32_t k = 0; k < 4 * kVecs; ++k) top2 = __vmaxu2(top2, word[k] & 0x7FFF7FFFu);
-                uint32_t top = max(top2 & 0xFFFFu, top2 >> 16);
-                if (top >= kInf) {  // leave them out
-                    top = 0;
+                int32_t exponent;
+                if constexpr (TERMS == 2) {
 #pragma unroll
                     for (uint32_t k = 0; k < 4 * kVecs; ++k) {
-                        const uint32_t lo = word[k] & 0x7FFFu, hi = word[k] >> 16 & 0x7FFFu;
-                        top = max(top, max(lo < kInf ? lo : 0u, hi < kInf ? hi : 0u));
+                        const uint32_t m = word[k] & 0x7FFFFFFFu;
+                        top = max(top, m < 0x7F800000u ? m : 0u);
+                    }
+                } else {
+                    constexpr uint32_t kInf = std::is_same_v<T, __half> ? 0x7C00u : 0x7F80u;
+                    uint32_t top2 = 0;
+#pragma unroll
+                    for (uint32_t k = 0; k < 4 * kVecs; ++k) top2 = __vmaxu2(top2, word[k] & 0x7FFF7FFFu);
+                    top = max(top2 & 0xFFFFu, top2 >> 16);
+                    if (top >= kInf) {  // leave them out
+                        top = 0;
+#pragma unroll
+                        for (uint32_t k = 0; k < 4 * kVecs; ++k) {
+                            const uint32_t lo = word[k] & 0x7FFFu, hi = word[k] >> 16 & 0x7FFFu;
+                            top = max(top, max(lo < kInf ? lo : 0u, hi < kInf ? hi : 0u));
+                        }
                     }
                 }
 #pragma unroll
                 for (int d = 4; d != 0; d /= 2) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
-                const uint16_t top16 = static_cast<uint16_t>(top);
-                T largest;
-                __builtin_memcpy(&largest, &top16, 2);
-                const int32_t exponent = row < rows ? max(static_cast<int32_t>(__float_as_uint(to_f32(largest)) >> 23) - 127, -100) : 0;
+                if constexpr (TERMS == 2) {
+                    exponent = static_cast<int32_t>(top >> 23) - 127;
+                } else {
+                    const uint16_t top16 = static_cast<uint16_t>(top);
+                    T largest;
+                    __builtin_memcpy(&largest, &top16, 2);
+                    exponent = static_cast<int32_t>(__float_as_uint(to_f32(largest)) >> 23) - 127;
+                }
+                exponent = row < rows ? max(exponent, -100) : 0;
                 const float by = row >= rows ? 0.0f : c.scale < 0 ? -exp2_int(14 - exponent) : exp2_int(14 - exponent);
                 if (row >= static_cast<uint32_t>(S::kRows)) return;
                 if (l8 == 0) q_unscale[segments & 1][row] = exp2_int(exponent - 14);
                 const uint32_t in_tile = row % 128;
 #pragma unroll
-                for (uint32_t k = 0; k < kVecs; ++k) {
-                    uint32_t h[4];
+                for (uint32_t k = 0; k < E / 8; ++k) {
+                    uint32_t h[4], rest[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        T x2[2];
-                        __builtin_memcpy(x2, &word[4 * k + e], 4);
-                        h[e] = half2_bits(to_f32(x2[0]) * by, to_f32(x2[1]) * by);
+                        float p, q;
+                        if constexpr (TERMS == 2) {
+                            p = __uint_as_float(word[8 * k + 2 * e]) * by, q = __uint_as_float(word[8 * k + 2 * e + 1]) * by;
+                        } else {
+                            T x2[2];
+                            __builtin_memcpy(x2, &word[4 * k + e], 4);
+                            p = to_f32(x2[0]) * by, q = to_f32(x2[1]) * by;
+                        }
+                        h[e] = half2_bits(p, q);
+                        if constexpr (TERMS == 2) rest[e] = half2_rest(p, q, h[e]);
                     }
                     const uint32_t d = l8 * E + 8 * k;  // 64-element blocks of [128 rows][128 bytes]
-                    sts128(q_at + (row / 128 * kParts + d / 64) * 16384 + in_tile * 128 + ((d % 64 / 8 ^ (in_tile & 7)) << 4), h[0], h[1], h[2], h[3]);
+                    const uint32_t at = q_at + (row / 128 * kParts + d / 64) * 16384 + in_tile * 128 + ((d % 64 / 8 ^ (in_tile & 7)) << 4);
+                    sts128(at, h[0], h[1], h[2], h[3]);
+                    if constexpr (TERMS == 2) sts128(at + kParts * 16384, rest[0], rest[1], rest[2], rest[3]);
                 }
             };
-            uint4 v[2][kVecs];
-            load(first, v[0]);
-            load(first + kStride, v[1]);
+            uint4 v[kLoads][kVecs];
+#pragma unroll
+            for (uint32_t i = 0; i < kLoads; ++i) load(first + i * kStride, v[i]);
             if (segments != 0) wait(q_free, (segments - 1) & 1);  // the segment before has its last scores
 #pragma unroll 1
-            for (uint32_t row = first; row < static_cast<uint32_t>(S::kRows) + first - lane / 8; row += 2 * kStride) {
+            for (uint32_t at = 0; at < static_cast<uint32_t>(S::kRows); at += kLoads * kStride) {
 #pragma unroll
-                for (uint32_t i = 0; i < 2; ++i) {
-                    store(row + i * kStride, v[i]);
-                    load(row + (i + 2) * kStride, v[i]);
+                for (uint32_t i = 0; i < kLoads; ++i) {
+                    const uint32_t row = at + first + i * kStride;
+                    store(row, v[i]);
+                    load(row + kLoads * kStride, v[i]);
                 }
             }
             proxy_fence();
@@ -503,8 +546,8 @@ __global__ void __launch_bounds__(TilesShape<D>::kThreads, 1) tiles_kernel(const
         constexpr uint32_t kEvery = S::kConvWarps / (2 * kParts);
         const uint32_t role = (warp - 4) % (2 * kParts), turn = (warp - 4) / (2 * kParts), part = role % kParts;
         const bool is_v = role >= kParts;
-        if (is_v) convert_slots<D, true>(c, w, range, cursors[warp - 4], part, turn, kEvery, ring, full, empty, scales, &nan_seen, alive);
-        else convert_slots<D, false>(c, w, range, cursors[warp - 4], part, turn, kEvery, ring, full, empty, scales, &nan_seen, alive);
+        if (is_v) convert_slots<D, TERMS, true>(c, w, range, cursors[warp - 4], part, turn, kEvery, ring, full, empty, scales, &nan_seen, alive);
+        else convert_slots<D, TERMS, false>(c, w, range, cursors[warp - 4], part, turn, kEvery, ring, full, empty, scales, &nan_seen, alive);
     } else if (warp >= S::kSoftWarp) {
         // ---- softmax ---------------------------------------------------------------------------------------------------------------------
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::kSoftRegs));
@@ -532,20 +575,21 @@ __global__ void __launch_bounds__(TilesShape<D>::kThreads, 1) tiles_kernel(const
             uint32_t prev_bar = 0, prev_parity = 0;
             uint32_t b = kStreams == 2 ? stream : 0;
             for (int32_t tile = walk.g.lo; tile < last_tile; ++tile) {
-                const uint32_t use = b == 0 ? uses[0]++ : uses[1]++, s_at = tmem + lanes + b * 128;
+                const uint32_t use = b == 0 ? uses[0]++ : uses[1]++, s_at = tmem + lanes + b * S::kBuffer;
                 wait(s_full + 8 * b, use & 1);
                 tmem_after();
                 const GroupScale* sc = scales[tiles % kScaleTiles];
-                const int32_t t0 = tile * 128;
-                const bool masked = t0 < all_lo || t0 + 128 > all_hi;
+                const int32_t t0 = tile * kTile;
+                const bool masked = t0 < all_lo || t0 + kTile > all_hi;
                 const uint32_t from = static_cast<uint32_t>(t0 - lo), seen = static_cast<uint32_t>(max(hi - lo, 0));  // key e of the tile: from + e < seen
-                uint32_t x[4][32];
+                constexpr int kChunks = kTile / 32;
+                uint32_t x[kChunks][32];
 #pragma unroll
-                for (int q = 0; q < 4; ++q) tmem_ld32(s_at + 32 * q, x[q]);
+                for (int q = 0; q < kChunks; ++q) tmem_ld32(s_at + 32 * q, x[q]);
                 tmem_wait_ld();
                 if (masked) {
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
+                    for (int q = 0; q < kChunks; ++q) {
                         const uint32_t at = from + static_cast<uint32_t>(32 * q);
                         if (__all_sync(0xFFFFFFFFu, at < seen && seen - at >= 32u)) continue;  // every row of the warp sees these keys
 #pragma unroll
@@ -556,7 +600,7 @@ __global__ void __launch_bounds__(TilesShape<D>::kThreads, 1) tiles_kernel(const
                 // Missing keys are zeros with log_v = -inf; the factor of a group's scores is not negative: the largest score is the largest exponent.
                 float top = -INFINITY;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
+                for (int i = 0; i < 2 * kChunks; ++i) {
                     const GroupScale s = sc[i];
                     const uint32_t* v = &x[i / 2][i % 2 * 16];
                     float m = fmaxf(__uint_as_float(v[0]), __uint_as_float(v[1]));
@@ -586,8 +630,8 @@ __global__ void __launch_bounds__(TilesShape<D>::kThreads, 1) tiles_kernel(const
                 if (first || grows) ref = next;
                 const float base = ref == -INFINITY ? 0.0f : ref - 6.0f;
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    uint32_t weights[16];
+                for (int q = 0; q < kChunks; ++q) {
+                    uint32_t weights[16], rest[16];
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         const GroupScale s = sc[2 * q + i];
@@ -602,12 +646,14 @@ __global__ void __launch_bounds__(TilesShape<D>::kThreads, 1) tiles_kernel(const
                             y0 = exp2_approx(y0), y1 = exp2_approx(y1);
                             sum = add_pair(sum, pair(y0, y1));
                             weights[8 * i + e / 2] = half2_bits(y0, y1);
+                            if constexpr (TERMS == 2) rest[8 * i + e / 2] = half2_rest(y0, y1, weights[8 * i + e / 2]);
                         }
                         float s0, s1;
                         unpair(sum, s0, s1);
                         l = fmaf(s0 + s1, s.inv_v, l);
                     }
                     tmem_st16(s_at + 16 * q, weights);  // (all scores have been read)
+                    if constexpr (TERMS == 2) tmem_st16(s_at + kTile / 2 + 16 * q, rest);
                 }
                 tmem_wait_st();
                 tmem_before();
@@ -640,9 +686,10 @@ __global__ void __launch_bounds__(TilesShape<D>::kThreads, 1) tiles_kernel(const
                     T y[32];
 #pragma unroll
                     for (int e = 0; e < 32; ++e) y[e] = from_f32<T>(__uint_as_float(o[e]) * inv);
+                    constexpr int kPer = 16 / sizeof(T);
                     if (c.out.vec) {
 #pragma unroll
-                        for (int e = 0; e < 32; e += 8) {
+                        for (int e = 0; e < 32; e += kPer) {
                             uint4 v;
                             __builtin_memcpy(&v, &y[e], 16);
                             *reinterpret_cast<uint4*>(out + d + e) = v;
@@ -697,7 +744,7 @@ __global__ void __launch_bounds__(TilesShape<D>::kThreads, 1) tiles_kernel(const
 
 template <class T, int D>
 int launch_tiles_kernel(HaloCudaCtx* ctx, const AttentionCall& c, Work w, cudaStream_t s) {
-    using S = TilesShape<D>;
+    using S = TilesShape<D, sizeof(T) == 4 ? 2 : 1>;
     w.rows = S::kRows;
     w.tile = S::kTile;
     w.pad = 3;

@@ -165,9 +165,10 @@ def test_a_prompt_of_several_tiles(be, kind, dim):
 
 @pytest.mark.parametrize("dim", [64, 128, 256])
 @pytest.mark.parametrize("q_len,kv_len", [([150, 40, 260], [2900, 1700, 260]), ([700], [2100])])
-def test_prompts_of_many_tiles_to_a_block(be, dim, q_len, kv_len):
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_prompts_of_many_tiles_to_a_block(be, kind, dim, q_len, kv_len):
     """More tiles of keys than the device has blocks by an order: blocks walk the ends of several units."""
-    c = Case(23, "bf16", dim, 64, 6, 3, q_len, kv_len)
+    c = Case(23, kind, dim, 64, 6, 3, q_len, kv_len)
     c.compare(c.run(be))
 
 
