@@ -249,6 +249,8 @@ __global__ void __launch_bounds__(RowsShape<D, TS, RG, TILE, CPS, sizeof(T) == 4
     float* join = reinterpret_cast<float*>(raw_smem + (smem - smem_u32(raw_smem)) + S::kStages * S::kStage + S::kQ);
     const uint32_t full = smem_u32(bars), empty = full + 8 * S::kStages;
     if (threadIdx.x == 0) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&k_map) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&v_map) : "memory");
         for (int i = 0; i < S::kStages; ++i) {
             mbar_init(full + 8 * i, 1);
             mbar_init(empty + 8 * i, S::kWarps);
@@ -719,7 +721,7 @@ int launch_rows_kernel(HaloCudaCtx* ctx, const AttentionCall& c, Work w, cudaStr
     w.least = 1;
     w.group = c.group;
     w.group_inverse = static_cast<uint32_t>((0xFFFFFFFFull + c.group) / c.group);
-    w.row_tiles = (c.rows.max_tokens * c.group + S::kRows - 1) / S::kRows;
+    w.row_tiles = (w.max_rows + S::kRows - 1) / S::kRows;
     w.lanes = 1;
     while (w.lanes < 32 && w.lanes < w.row_tiles) w.lanes *= 2;
     CUtensorMap k_map, v_map;

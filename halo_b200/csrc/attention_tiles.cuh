@@ -117,6 +117,13 @@ __device__ __forceinline__ void sts128(uint32_t at, uint32_t a, uint32_t b, uint
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
+/// 16 bytes that this SM reads once: no place in what shared memory leaves of the L1 cache.
+__device__ __forceinline__ uint4 load_once(const uint8_t* p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+
 /// Where a conversion warp's loads are: in shared memory, so that the pieces under way have the registers.
 struct Cursor {
     Unit u;
@@ -142,30 +149,30 @@ __device__ __forceinline__ void convert_slots(const AttentionCall& c, const Work
     const uint32_t to = block * (kRows * 128) + lane_row * 128 + ((lane % 4 * 2 ^ (lane_row & 7)) << 4);  // second half: the same ^ 16
     // the tile that is loaded: of the CTA's tiles number `count`, keys from t0 on; lane i knows page and scale bytes of its i-th 16 keys, and those of
     // this warp's next tile
-    int32_t tile, last, any_lo, any_hi, page = -1, page_next = -1;
-    uint32_t bytes = 0, bytes_next = 0, count = 0;
+    int32_t tile, last, any_lo, any_hi, all_lo, all_hi, page = -1;
+    int32_t entry = -1;                 // of the page table, for this warp's next tile; not looked at before that tile's turn
+    uint32_t k_byte = 0, v_byte = 0, count = 0;
     uint64_t group_at = 0;              // lane i: where its keys' codes begin in the pool
     bool plain = false, whole = false;  // every key is there and seen by some row; by all rows
     const uint8_t* pool = nullptr;
     auto fetch = [&](int32_t of) {
         const int32_t t = of * kTile + static_cast<int32_t>(lane) * 16;
-        page_next = -1;
+        entry = -1;
         if (lane < kTile / 16 && of < last && t < any_hi && t + 16 > any_lo) {
-            const int32_t p = page_of(c.cache, cursor.u.seq, t >> c.cache.page_shift);
-            page_next = static_cast<uint32_t>(p) < c.cache.n_pages ? p : -2;  // -2: a visible key's page is not there
-            if (!IS_V && part == 0 && page_next >= 0) {
-                const uint64_t at = p * c.cache.scale_stride + cursor.u.head;
-                bytes_next = __ldg(c.cache.k_scale + at) | static_cast<uint32_t>(__ldg(c.cache.v_scale + at)) << 8;
-            }
+            entry = page_of(c.cache, cursor.u.seq, t >> c.cache.page_shift);
         }
     };
     auto take = [&] {  // the fetched tile becomes the one that is loaded
-        page = page_next, bytes = bytes_next;
-        const Unit& u = cursor.u;
-        const uint32_t first = u.row0(w) / c.group, final = (u.row0(w) + u.rows(w) - 1) / c.group;
-        const int32_t t0 = tile * kTile;
+        const int32_t t0 = tile * kTile, t = t0 + static_cast<int32_t>(lane) * 16;
+        const bool wanted = lane < kTile / 16 && t < any_hi && t + 16 > any_lo;
+        page = !wanted ? -1 : static_cast<uint32_t>(entry) < c.cache.n_pages ? entry : -2;  // -2: a visible key's page is not there
+        if (!IS_V && part == 0 && page >= 0) {
+            const uint64_t at = page * c.cache.scale_stride + cursor.u.head;
+            k_byte = __ldg(c.cache.k_scale + at);
+            v_byte = __ldg(c.cache.v_scale + at);
+        }
         plain = t0 >= any_lo && t0 + kTile <= any_hi && __all_sync(0xFFFFFFFFu, page >= 0 || lane >= kTile / 16);
-        whole = plain && t0 >= first_key(u.s, w.window, final) && t0 + kTile <= end_key(u.s, c.causal, first);
+        whole = plain && t0 >= all_lo && t0 + kTile <= all_hi;
         group_at = static_cast<uint32_t>(max(page, 0)) * c.cache.page_stride + ((static_cast<uint32_t>(t0) + lane * 16) & (c.cache.page_tokens - 1)) * D;
         fetch(tile + static_cast<int32_t>(every));
     };
@@ -190,6 +197,7 @@ __device__ __forceinline__ void convert_slots(const AttentionCall& c, const Work
         const Unit& u = cursor.u;
         const uint32_t first = u.row0(w) / c.group, final = (u.row0(w) + u.rows(w) - 1) / c.group;
         any_lo = first_key(u.s, w.window, first), any_hi = end_key(u.s, c.causal, final);
+        all_lo = first_key(u.s, w.window, final), all_hi = end_key(u.s, c.causal, first);
         tile = cursor.g.lo + static_cast<int32_t>(skip), last = cursor.g.hi, count += skip;
         pool = (IS_V ? c.cache.v : c.cache.k) + (uint64_t{u.head} << c.cache.page_shift) * D + from;
         fetch(tile);
@@ -217,7 +225,7 @@ __device__ __forceinline__ void convert_slots(const AttentionCall& c, const Work
                 const uint32_t i0 = lot * kLot + n * kIn;
                 const uint8_t* src = pool + __shfl_sync(0xFFFFFFFFu, group_at, i0 / kPerGroup + part * kFirst);
 #pragma unroll
-                for (uint32_t j = 0; j < kIn; ++j) x[(i0 + j) % kAhead] = __ldg(reinterpret_cast<const uint4*>(src + (i0 + j) % kPerGroup * kStep * D));
+                for (uint32_t j = 0; j < kIn; ++j) x[(i0 + j) % kAhead] = load_once(src + (i0 + j) % kPerGroup * kStep * D);
             }
         } else {
 #pragma unroll
@@ -231,7 +239,7 @@ __device__ __forceinline__ void convert_slots(const AttentionCall& c, const Work
                 for (uint32_t j = 0; j < kLot; ++j) {
                     const uint32_t i = lot * kLot + j, k = i % kPerGroup * kStep;
                     const int32_t t = tile * kTile + static_cast<int32_t>(group * 16 + k + lane_row);
-                    if (i / kPerGroup == g && there && t >= any_lo && t < any_hi) x[i % kAhead] = __ldg(reinterpret_cast<const uint4*>(from_group + k * D));
+                    if (i / kPerGroup == g && there && t >= any_lo && t < any_hi) x[i % kAhead] = load_once(from_group + k * D);
                 }
             }
         }
@@ -246,8 +254,8 @@ __device__ __forceinline__ void convert_slots(const AttentionCall& c, const Work
         if (alive) alive = __all_sync(0xFFFFFFFFu, mbar_wait(empty + 8 * at, (number / S::kSlots & 1) ^ 1));
         if (!IS_V && part == 0 && lane < kTile / 16) {
             GroupScale& s = scales[count % 8][lane];
-            const int32_t v = scale_byte(bytes >> 8) - 127;
-            s.k = page >= 0 ? exp2_int(scale_byte(bytes & 255u) - 127) * scale : 0.0f;
+            const int32_t v = scale_byte(v_byte) - 127;
+            s.k = page >= 0 ? exp2_int(scale_byte(k_byte) - 127) * scale : 0.0f;
             s.log_v = page >= 0 ? static_cast<float>(v) : -INFINITY;
             s.inv_v = page >= 0 ? exp2_int(-v) : 0.0f;
             if (page == -2 && c.status != nullptr) atomicOr(c.status, 8u);  // kStatusBadIndex
@@ -525,7 +533,7 @@ __global__ void __launch_bounds__(TilesShape<D, sizeof(T) == 4 ? 2 : 1>::kThread
             for (uint32_t i = 0; i < kLoads; ++i) load(first + i * kStride, v[i]);
             if (segments != 0) wait(q_free, (segments - 1) & 1);  // the segment before has its last scores
 #pragma unroll 1
-            for (uint32_t at = 0; at < static_cast<uint32_t>(S::kRows); at += kLoads * kStride) {
+            for (uint32_t at = 0; at < rows; at += kLoads * kStride) {  // what lies behind the last row is never kept
 #pragma unroll
                 for (uint32_t i = 0; i < kLoads; ++i) {
                     const uint32_t row = at + first + i * kStride;
@@ -571,6 +579,7 @@ __global__ void __launch_bounds__(TilesShape<D, sizeof(T) == 4 ? 2 : 1>::kThread
             const int32_t all_lo = first_key(walk.u.s, w.window, walk.token(w, min(stream * 128 + 127, walk.rows - 1)));
             const int32_t all_hi = end_key(walk.u.s, c.causal, walk.token(w, min(stream * 128, walk.rows - 1)));
             const int32_t last_tile = walk.g.hi;
+            const bool any_row = stream * 128 + quarter * 32 < walk.rows;
             float ref = -INFINITY, l = 0;
             uint32_t prev_bar = 0, prev_parity = 0;
             uint32_t b = kStreams == 2 ? stream : 0;
@@ -578,6 +587,15 @@ __global__ void __launch_bounds__(TilesShape<D, sizeof(T) == 4 ? 2 : 1>::kThread
                 const uint32_t use = b == 0 ? uses[0]++ : uses[1]++, s_at = tmem + lanes + b * S::kBuffer;
                 wait(s_full + 8 * b, use & 1);
                 tmem_after();
+                if (!any_row) {  // nothing of this warp's rows is kept
+                    tmem_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(p_ready + 8 * b);
+                    prev_bar = pv_done + 8 * b, prev_parity = use & 1;
+                    if (kStreams == 1) b ^= 1;
+                    ++tiles;
+                    continue;
+                }
                 const GroupScale* sc = scales[tiles % kScaleTiles];
                 const int32_t t0 = tile * kTile;
                 const bool masked = t0 < all_lo || t0 + kTile > all_hi;
@@ -751,7 +769,7 @@ int launch_tiles_kernel(HaloCudaCtx* ctx, const AttentionCall& c, Work w, cudaSt
     w.least = 1;
     w.group = c.group;
     w.group_inverse = static_cast<uint32_t>((0xFFFFFFFFull + c.group) / c.group);
-    w.row_tiles = (c.rows.max_tokens * c.group + S::kRows - 1) / S::kRows;
+    w.row_tiles = (w.max_rows + S::kRows - 1) / S::kRows;
     w.lanes = 1;
     while (w.lanes < 32 && w.lanes < w.row_tiles) w.lanes *= 2;
     const uint32_t ctas = static_cast<uint32_t>(ctx->prop.multiProcessorCount);

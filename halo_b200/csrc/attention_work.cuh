@@ -106,11 +106,70 @@ struct PlanSmem {
     uint32_t seq;
 };
 
+/// The CTA's positions out of `total`; false if it has none.
+__device__ __forceinline__ bool cut_range(const Work& w, uint64_t total, Range* out) {
+    out->total = total;
+    if (total == 0) return false;
+    // where a call has few tiles, a share of a unit has at least `least`: it costs its CTA, and the one that joins the shares, as much as a few
+    const uint32_t ctas = static_cast<uint32_t>(min(uint64_t{gridDim.x}, max(quotient(total, w.least), uint64_t{1})));
+    if (blockIdx.x >= ctas) return false;
+    out->ctas = ctas;
+    out->pad = w.pad;
+    out->begin = quotient(total * blockIdx.x, ctas);
+    out->end = quotient(total * (blockIdx.x + 1), ctas);
+    return true;
+}
+
+/// find_range where no sequence has more than one row tile: every warp for itself, a lane to a sequence, without a barrier.
+__device__ inline bool find_range_by_warps(const AttentionCall& c, const Work& w, Range* out) {
+    const uint32_t lane = threadIdx.x % 32, n_seq = c.cache.n_seq;
+    uint64_t total = 0, n = 0, upto = 0;
+    auto count = [&](uint32_t i) {  // this lane's sequence's positions, and the sum up to it
+        n = 0;
+        if (i < n_seq) {
+            const Seq s = sequence(c.rows, c.cache, i);
+            const uint32_t packed = packed_rows(c, w, s);
+            if (packed != 0) n = uint64_t{span_of(c, w, s, 0, packed - 1).tiles() + w.pad} * c.cache.n_kv;
+        }
+        upto = n;
+        for (uint32_t d = 1; d < 32; d *= 2) {
+            const uint64_t y = __shfl_up_sync(0xFFFFFFFFu, upto, d);
+            if (lane >= d) upto += y;
+        }
+    };
+    for (uint32_t base = 0; base < n_seq; base += 32) {
+        count(base + lane);
+        total += __shfl_sync(0xFFFFFFFFu, upto, 31);
+    }
+    if (!cut_range(w, total, out)) return false;
+    uint64_t before = 0;
+    for (uint32_t base = 0; base < n_seq; base += 32) {
+        if (n_seq > 32) count(base + lane);
+        const uint32_t hit = __ballot_sync(0xFFFFFFFFu, out->begin < before + upto);
+        if (hit != 0) {
+            const uint32_t l = __ffs(hit) - 1;
+            before += __shfl_sync(0xFFFFFFFFu, upto - n, l);
+            Unit& u = out->unit;
+            u.seq = base + l;
+            u.s = sequence(c.rows, c.cache, u.seq);
+            u.packed = packed_rows(c, w, u.s);
+            set_row_tile(c, w, u, 0);
+            const uint64_t at = out->begin - before, length = u.span.tiles() + w.pad;
+            u.head = static_cast<uint32_t>(quotient(at, length));
+            out->unit_begin = before + u.head * length;
+            break;
+        }
+        before += __shfl_sync(0xFFFFFFFFu, upto, 31);
+    }
+    return out->reaches(out->unit_begin);
+}
+
 /// All threads of the CTA (a multiple of a warp).  `lanes` lanes share a sequence; a pass over the sequences sums their tiles, another finds
 /// the one that this CTA's range begins in (one pass does both where the CTA sees all sequences at once).
 __device__ inline bool find_range(const AttentionCall& c, const Work& w, PlanSmem& sm, Range* out) {
     const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32, warps = blockDim.x / 32;
     const uint32_t per_pass = blockDim.x / w.lanes, sub = threadIdx.x % w.lanes, n_seq = c.cache.n_seq;
+    if (w.row_tiles == 1) return find_range_by_warps(c, w, out);
     auto tiles_of = [&](uint32_t i) {  // all lanes of the group get the sum
         uint64_t n = 0;
         if (i < n_seq) {
@@ -146,15 +205,7 @@ __device__ inline bool find_range(const AttentionCall& c, const Work& w, PlanSme
         upto = scan(n, &all);
         total += all;
     }
-    out->total = total;
-    if (total == 0) return false;
-    // where a call has few tiles, a share of a unit has at least `least`: it costs its CTA, and the one that joins the shares, as much as a few
-    const uint32_t ctas = static_cast<uint32_t>(min(uint64_t{gridDim.x}, max(total / w.least, uint64_t{1})));
-    if (blockIdx.x >= ctas) return false;
-    out->ctas = ctas;
-    out->pad = w.pad;
-    out->begin = quotient(total * blockIdx.x, ctas);
-    out->end = quotient(total * (blockIdx.x + 1), ctas);
+    if (!cut_range(w, total, out)) return false;
     uint64_t before = 0;
     for (uint32_t base = 0; base < n_seq; base += per_pass) {
         uint64_t all = total;
