@@ -16,7 +16,7 @@
 //   4-7     conversion (4-11 where D is 256): each warp makes one part of K or V of every tile in a ring of eight 16 KiB slots (a K slot: 128 keys x
 //           64 dims; a V slot: 8192 / D keys x all dims, the N operand with dims contiguous); keys that no row of the CTA sees, missing pages and,
 //           in tiles that some row does not see whole, NaN codes of values become zeros (spread_nan puts the latter back)
-//   last 8  softmax, a thread to a row (the last 4 where NS is 1); also the epilogue and the joining of shares
+//   last 8  softmax, a thread to a row and a tile's keys, or to half of them where NS is 1; also the epilogue, and the joining of shares
 // Work is dealt as in attention_work.cuh, so a causal prompt's long and short rows and a short chunk behind a long context fill the device alike.
 //
 // What bounds it: the tensor pipe and, for D = 128, the exponentials (256 x 128 of them per 2048 clocks of products at 16 a clock); shared memory
@@ -38,16 +38,18 @@ struct TilesShape {
     static constexpr uint32_t kSmem = 1024 + kQ + kSlots * kSlot;
     static constexpr uint32_t kBuffer = kTile;             // columns of a score buffer, which the terms of the weights (kTile / 2 columns each) overwrite
     static constexpr uint32_t kO = 256;                    // first accumulator column
-    static constexpr int kConvWarps = D == 256 ? 8 : 4, kSoftWarp = 4 + kConvWarps, kSoftWarps = 4 * kStreams, kThreads = (kSoftWarp + kSoftWarps) * 32;
+    static constexpr int kHalves = 2 / kStreams;           // softmax warpgroups that share a row tile's keys
+    static constexpr int kKeys = kTile / kHalves;          // of a tile that one of them has
+    static constexpr int kConvWarps = D == 256 ? 8 : 4, kSoftWarp = 4 + kConvWarps, kSoftWarps = 8, kThreads = (kSoftWarp + kSoftWarps) * 32;
     // Slot number i of a CTA (the parts of K of its first tile, those of V, those of K of the second, ...) has place i % kSlots.  A place's user waits for
     // its last use by the parity of that use, so all of a place's uses are to be one warp's: 2 * kParts * kEvery of convert_slots divides kSlots.
     static_assert(kSlots % kConvWarps == 0);
     static constexpr uint32_t kAccesses = kSlot / 1024;    // 16-byte pieces of a slot that a conversion thread makes
-    static constexpr uint32_t kAhead = D == 256 ? kAccesses : 8;  // that it has under way
+    static constexpr uint32_t kAhead = 8;                  // that it has under way (all 16 of D = 256: 1672 -> 2147 us for 2048 tokens behind 28000)
     // What a thread has at launch; the warpgroups hand each other what they leave.
-    static constexpr int kLaunchRegs = kThreads == 512 ? 128 : 168;
-    static constexpr int kIdleRegs = D == 256 || TERMS == 2 ? 80 : 72, kConvRegs = D == 256 ? 104 : 88, kSoftRegs = kStreams == 2 ? 176 : 224;
-    static_assert(kIdleRegs + kConvRegs * (kConvWarps / 4) + kSoftRegs * kStreams <= kLaunchRegs * (kThreads / 128));
+    static constexpr int kLaunchRegs = kThreads == 512 ? 128 : 96;
+    static constexpr int kIdleRegs = D == 256 ? 72 : kStreams == 1 ? 80 : 72, kConvRegs = D == 256 ? 80 : 88, kSoftRegs = D == 256 ? 120 : kStreams == 1 ? 168 : 176;
+    static_assert(kIdleRegs + kConvRegs * (kConvWarps / 4) + 2 * kSoftRegs <= kLaunchRegs * (kThreads / 128));
 };
 
 __device__ __forceinline__ uint64_t desc_k(uint32_t addr) {  // K-major, 128-byte rows and swizzle: atoms of 8 rows, 1024 bytes apart
@@ -115,13 +117,6 @@ __device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
 }
 __device__ __forceinline__ void sts128(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
-}
-
-/// 16 bytes that this SM reads once: no place in what shared memory leaves of the L1 cache.
-__device__ __forceinline__ uint4 load_once(const uint8_t* p) {
-    uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-    return v;
 }
 
 /// Where a conversion warp's loads are: in shared memory, so that the pieces under way have the registers.
@@ -225,7 +220,7 @@ __device__ __forceinline__ void convert_slots(const AttentionCall& c, const Work
                 const uint32_t i0 = lot * kLot + n * kIn;
                 const uint8_t* src = pool + __shfl_sync(0xFFFFFFFFu, group_at, i0 / kPerGroup + part * kFirst);
 #pragma unroll
-                for (uint32_t j = 0; j < kIn; ++j) x[(i0 + j) % kAhead] = load_once(src + (i0 + j) % kPerGroup * kStep * D);
+                for (uint32_t j = 0; j < kIn; ++j) x[(i0 + j) % kAhead] = __ldg(reinterpret_cast<const uint4*>(src + (i0 + j) % kPerGroup * kStep * D));
             }
         } else {
 #pragma unroll
@@ -239,7 +234,7 @@ __device__ __forceinline__ void convert_slots(const AttentionCall& c, const Work
                 for (uint32_t j = 0; j < kLot; ++j) {
                     const uint32_t i = lot * kLot + j, k = i % kPerGroup * kStep;
                     const int32_t t = tile * kTile + static_cast<int32_t>(group * 16 + k + lane_row);
-                    if (i / kPerGroup == g && there && t >= any_lo && t < any_hi) x[i % kAhead] = load_once(from_group + k * D);
+                    if (i / kPerGroup == g && there && t >= any_lo && t < any_hi) x[i % kAhead] = __ldg(reinterpret_cast<const uint4*>(from_group + k * D));
                 }
             }
         }
@@ -301,6 +296,7 @@ __global__ void __launch_bounds__(TilesShape<D, sizeof(T) == 4 ? 2 : 1>::kThread
     __shared__ GroupScale scales[kScaleTiles][8];  // a tile's stay until the slots' ring has gone round behind it: at most six tiles ahead are written
     __shared__ float q_unscale[2][S::kRows];  // of a segment and the next
     __shared__ float2 joined_ml[S::kRows];
+    __shared__ float shared_top[2][S::kHalves][128];  // of a tile and the next: the maxima that a row tile's warpgroups tell each other
     __shared__ uint32_t nan_seen, is_last, tmem_word;
     __shared__ Cursor cursors[S::kConvWarps];
     __shared__ Walk walks[2];  // the segment at hand and the next one, in turn
@@ -320,7 +316,7 @@ __global__ void __launch_bounds__(TilesShape<D, sizeof(T) == 4 ? 2 : 1>::kThread
         mbar_init(idle, 1);
         for (int i = 0; i < 2; ++i) {
             mbar_init(s_full + 8 * i, 1);
-            mbar_init(p_ready + 8 * i, 4);
+            mbar_init(p_ready + 8 * i, 4 * S::kHalves);
             mbar_init(pv_done + 8 * i, 1);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -560,7 +556,8 @@ __global__ void __launch_bounds__(TilesShape<D, sizeof(T) == 4 ? 2 : 1>::kThread
         // ---- softmax ---------------------------------------------------------------------------------------------------------------------
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::kSoftRegs));
         constexpr uint32_t kSoft = S::kSoftWarps * 32;
-        const uint32_t stream = (warp - S::kSoftWarp) / 4, quarter = warp % 4, r = stream * 128 + quarter * 32 + lane;  // this thread's row of the unit
+        const uint32_t group = (warp - S::kSoftWarp) / 4, stream = kStreams == 2 ? group : 0, half = kStreams == 2 ? 0 : group;
+        const uint32_t quarter = warp % 4, r = stream * 128 + quarter * 32 + lane;  // this thread's row of the unit
         const uint32_t lanes = quarter * 32 << 16, o_at = tmem + lanes + S::kO + stream * D;
         uint32_t uses[2] = {0, 0}, tiles = 0;
         const bool leader = threadIdx.x == S::kSoftWarp * 32;
@@ -596,14 +593,14 @@ __global__ void __launch_bounds__(TilesShape<D, sizeof(T) == 4 ? 2 : 1>::kThread
                     ++tiles;
                     continue;
                 }
-                const GroupScale* sc = scales[tiles % kScaleTiles];
+                const GroupScale* sc = scales[tiles % kScaleTiles] + half * (S::kKeys / 16);
                 const int32_t t0 = tile * kTile;
                 const bool masked = t0 < all_lo || t0 + kTile > all_hi;
-                const uint32_t from = static_cast<uint32_t>(t0 - lo), seen = static_cast<uint32_t>(max(hi - lo, 0));  // key e of the tile: from + e < seen
-                constexpr int kChunks = kTile / 32;
+                const uint32_t from = static_cast<uint32_t>(t0 - lo) + half * S::kKeys, seen = static_cast<uint32_t>(max(hi - lo, 0));  // key e of this thread's: from + e < seen
+                constexpr int kChunks = S::kKeys / 32;
                 uint32_t x[kChunks][32];
 #pragma unroll
-                for (int q = 0; q < kChunks; ++q) tmem_ld32(s_at + 32 * q, x[q]);
+                for (int q = 0; q < kChunks; ++q) tmem_ld32(s_at + half * S::kKeys + 32 * q, x[q]);
                 tmem_wait_ld();
                 if (masked) {
 #pragma unroll
@@ -626,6 +623,11 @@ __global__ void __launch_bounds__(TilesShape<D, sizeof(T) == 4 ? 2 : 1>::kThread
                     for (int e = 2; e < 16; e += 2) m = fmaxf(fmaxf(m, __uint_as_float(v[e])), __uint_as_float(v[e + 1]));
                     top = fmaxf(top, m == -INFINITY ? m : fmaf(m, s.k * qs, s.log_v));
                 }
+                if constexpr (S::kHalves == 2) {  // the warp that has the other keys of these rows; both have read their scores behind this
+                    shared_top[tiles & 1][half][r] = top;
+                    bar_sync(2 + quarter, 64);
+                    top = fmaxf(top, shared_top[tiles & 1][half ^ 1][r]);
+                }
                 const float next = fmaxf(ref, top);
                 const bool first = ref == -INFINITY, grows = !first && next > ref + 8.0f;
                 if (__any_sync(0xFFFFFFFFu, grows)) {
@@ -634,7 +636,7 @@ __global__ void __launch_bounds__(TilesShape<D, sizeof(T) == 4 ? 2 : 1>::kThread
                     wait(prev_bar, prev_parity);
                     tmem_after();
 #pragma unroll 1
-                    for (int d = 0; d < D; d += 32) {
+                    for (int d = half * (D / S::kHalves); d < static_cast<int>(half + 1) * (D / S::kHalves); d += 32) {
                         uint32_t o[32];
                         tmem_ld32(o_at + d, o);
                         tmem_wait_ld();
@@ -670,8 +672,8 @@ __global__ void __launch_bounds__(TilesShape<D, sizeof(T) == 4 ? 2 : 1>::kThread
                         unpair(sum, s0, s1);
                         l = fmaf(s0 + s1, s.inv_v, l);
                     }
-                    tmem_st16(s_at + 16 * q, weights);  // (all scores have been read)
-                    if constexpr (TERMS == 2) tmem_st16(s_at + kTile / 2 + 16 * q, rest);
+                    tmem_st16(s_at + half * (S::kKeys / 2) + 16 * q, weights);  // (all scores have been read)
+                    if constexpr (TERMS == 2) tmem_st16(s_at + kTile / 2 + half * (S::kKeys / 2) + 16 * q, rest);
                 }
                 tmem_wait_st();
                 tmem_before();
@@ -685,6 +687,12 @@ __global__ void __launch_bounds__(TilesShape<D, sizeof(T) == 4 ? 2 : 1>::kThread
             tmem_after();
             // ---- the segment's rows ------------------------------------------------------------------------------------------------------
             const bool keep = r < walk.rows;
+            if constexpr (S::kHalves == 2) {
+                shared_top[tiles & 1][half][r] = l;
+                bar_sync(2 + quarter, 64);
+                l += shared_top[tiles & 1][half ^ 1][r];
+                bar_sync(2 + quarter, 64);  // read, before the next segment's first tile writes there
+            }
             float* slot = walk.g.whole() ? nullptr : partial_slot(w, D, blockIdx.x, walk.g.from_start) + r * D;
             auto out_at = [&](uint32_t row) {
                 return reinterpret_cast<T*>(walk.at(c, w, c.out, row));
@@ -692,7 +700,7 @@ __global__ void __launch_bounds__(TilesShape<D, sizeof(T) == 4 ? 2 : 1>::kThread
             T* out = out_at(min(r, walk.rows - 1));
             const float inv = l != 0 ? 1.0f / l : 0.0f;
 #pragma unroll 1
-            for (int d = 0; d < D; d += 32) {
+            for (int d = half * (D / S::kHalves); d < static_cast<int>(half + 1) * (D / S::kHalves); d += 32) {
                 uint32_t o[32];
                 tmem_ld32(o_at + d, o);
                 tmem_wait_ld();
@@ -718,7 +726,7 @@ __global__ void __launch_bounds__(TilesShape<D, sizeof(T) == 4 ? 2 : 1>::kThread
                     }
                 }
             }
-            if (keep && slot != nullptr) {
+            if (keep && half == 0 && slot != nullptr) {
                 float* ml = partial_slot(w, D, blockIdx.x, walk.g.from_start) + w.rows * D + 2 * r;
                 *reinterpret_cast<float2*>(ml) = make_float2(ref, l);
             }
