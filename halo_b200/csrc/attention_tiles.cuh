@@ -38,6 +38,9 @@ struct TilesShape {
     static constexpr uint32_t kSmem = 1024 + kQ + kSlots * kSlot;
     static constexpr uint32_t kBuffer = kTile;             // columns of a score buffer, which the terms of the weights (kTile / 2 columns each) overwrite
     static constexpr uint32_t kO = 256;                    // first accumulator column
+    // The tensor cores cut sums off instead of rounding them, always towards zero: a chain of n of them is n * 2^-25 too small in the mean.  fp32 operands'
+    // rows are added up in fp32 outside after every 32 (4 tiles of 64 keys, 2 of 128); 0: never.
+    static constexpr uint32_t kSettle = TERMS == 2 ? 32 / (kTile / 8) : 0;
     static constexpr int kHalves = 2 / kStreams;           // softmax warpgroups that share a row tile's keys
     static constexpr int kKeys = kTile / kHalves;          // of a tile that one of them has
     static constexpr int kConvWarps = D == 256 ? 8 : 4, kSoftWarp = 4 + kConvWarps, kSoftWarps = 8, kThreads = (kSoftWarp + kSoftWarps) * 32;
@@ -360,20 +363,18 @@ __global__ void __launch_bounds__(TilesShape<D, sizeof(T) == 4 ? 2 : 1>::kThread
         constexpr uint32_t kSlotDesc = S::kSlot / 16, kSteps = S::kVTokens / 16;
         auto scores = [&](uint32_t tile, uint32_t s, uint32_t buffer) {  // tile: its number in the CTA
             const uint32_t place = __shfl_sync(0xFFFFFFFFu, tile % kRounds * (2 * kParts), 0), parity = tile / kRounds & 1;
+            // the small terms first: sums are cut off at the size they have by then
 #pragma unroll
-            for (uint32_t part = 0; part < kParts; ++part) {
-                if (s == 0) wait(full + 8 * (place + part), parity);
+            for (uint32_t i = 0; i < TERMS * kParts; ++i) {
+                const uint32_t term = TERMS - 1 - i / kParts, part = i % kParts;
+                if (s == 0 && i < kParts) wait(full + 8 * (place + part), parity);
                 tmem_after();
                 if (elect_one()) {
-                    const uint64_t b = k_desc + (place + part) * kSlotDesc;
+                    const uint64_t a = q_desc + ((term + s) * kParts + part) * 1024u, b = k_desc + (place + part) * kSlotDesc;
 #pragma unroll
-                    for (uint32_t term = 0; term < TERMS; ++term) {
-                        const uint64_t a = q_desc + ((term + s) * kParts + part) * 1024u;
-#pragma unroll
-                        for (uint32_t k = 0; k < 4; ++k) mma_ss(tmem + buffer * S::kBuffer, a + k * 2, b + k * 2, kScores, part + term + k != 0);
-                    }
-                    if (s == kStreams - 1) mma_commit(empty + 8 * (place + part));
-                    if (part == kParts - 1) mma_commit(s_full + 8 * buffer);
+                    for (uint32_t k = 0; k < 4; ++k) mma_ss(tmem + buffer * S::kBuffer, a + k * 2, b + k * 2, kScores, i + k != 0);
+                    if (term == 0 && s == kStreams - 1) mma_commit(empty + 8 * (place + part));
+                    if (i == TERMS * kParts - 1) mma_commit(s_full + 8 * buffer);
                 }
             }
         };
@@ -414,7 +415,7 @@ __global__ void __launch_bounds__(TilesShape<D, sizeof(T) == 4 ? 2 : 1>::kThread
                     }
                 } else {
                     const uint32_t buffer = __shfl_sync(0xFFFFFFFFu, t & 1, 0);
-                    rows(count + t, 0, buffer, t != 0);
+                    rows(count + t, 0, buffer, TERMS == 2 ? t % S::kSettle != 0 : t != 0);
                     if (t + 2 < n) scores(count + t + 2, 0, buffer);
                 }
             }
@@ -576,6 +577,28 @@ __global__ void __launch_bounds__(TilesShape<D, sizeof(T) == 4 ? 2 : 1>::kThread
             const int32_t all_lo = first_key(walk.u.s, w.window, walk.token(w, min(stream * 128 + 127, walk.rows - 1)));
             const int32_t all_hi = end_key(walk.u.s, c.causal, walk.token(w, min(stream * 128, walk.rows - 1)));
             const int32_t last_tile = walk.g.hi;
+            // fp32 operands: this thread's part of the row as far as it is added up outside, four dims at a time, the rows of a warp side by side
+            uint32_t settled = 0;
+            float4* outside = reinterpret_cast<float4*>(w.settled) + blockIdx.x * (128u * D / 4) + r;
+            auto settle = [&](float fade, bool take) {  // outside = outside * fade, or outside + the accumulators
+#pragma unroll 1
+                for (uint32_t d = half * (D / S::kHalves); d < (half + 1) * (D / S::kHalves); d += 32) {
+                    uint32_t o[32];
+                    if (take) {
+                        tmem_ld32(o_at + d, o);
+                        tmem_wait_ld();
+                    }
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4) {
+                        float4* at = outside + (d + e) / 4 * 128;
+                        float4 v = settled != 0 ? *at : make_float4(0, 0, 0, 0);
+                        if (take) v.x += __uint_as_float(o[e]), v.y += __uint_as_float(o[e + 1]), v.z += __uint_as_float(o[e + 2]), v.w += __uint_as_float(o[e + 3]);
+                        else v.x *= fade, v.y *= fade, v.z *= fade, v.w *= fade;
+                        *at = v;
+                    }
+                }
+                if (take) ++settled;
+            };
             const bool any_row = stream * 128 + quarter * 32 < walk.rows;
             float ref = -INFINITY, l = 0;
             uint32_t prev_bar = 0, prev_parity = 0;
@@ -646,8 +669,19 @@ __global__ void __launch_bounds__(TilesShape<D, sizeof(T) == 4 ? 2 : 1>::kThread
                     }
                     tmem_wait_st();
                     l *= fade;
+                    if constexpr (TERMS == 2) {
+                        if (settled != 0) settle(fade, false);
+                    }
                 }
                 if (first || grows) ref = next;
+                if constexpr (TERMS == 2) {
+                    const uint32_t t = static_cast<uint32_t>(tile - walk.g.lo);
+                    if (t != 0 && t % S::kSettle == 0) {  // this tile's products begin anew
+                        wait(prev_bar, prev_parity);
+                        tmem_after();
+                        settle(1.0f, true);
+                    }
+                }
                 const float base = ref == -INFINITY ? 0.0f : ref - 6.0f;
 #pragma unroll
                 for (int q = 0; q < kChunks; ++q) {
@@ -704,6 +738,16 @@ __global__ void __launch_bounds__(TilesShape<D, sizeof(T) == 4 ? 2 : 1>::kThread
                 uint32_t o[32];
                 tmem_ld32(o_at + d, o);
                 tmem_wait_ld();
+                if constexpr (TERMS == 2) {
+                    if (settled != 0) {
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4) {
+                            const float4 v = outside[(d + e) / 4 * 128];
+                            o[e] = __float_as_uint(__uint_as_float(o[e]) + v.x), o[e + 1] = __float_as_uint(__uint_as_float(o[e + 1]) + v.y);
+                            o[e + 2] = __float_as_uint(__uint_as_float(o[e + 2]) + v.z), o[e + 3] = __float_as_uint(__uint_as_float(o[e + 3]) + v.w);
+                        }
+                    }
+                }
                 if (!keep) continue;
                 if (slot != nullptr) {
 #pragma unroll
@@ -784,8 +828,10 @@ int launch_tiles_kernel(HaloCudaCtx* ctx, const AttentionCall& c, Work w, cudaSt
     void* p = nullptr;
     if (int rc = workspace(ctx, 5, ctas * sizeof(uint32_t), s, &p, true)) return rc;
     w.counters = static_cast<uint32_t*>(p);
-    if (int rc = workspace(ctx, 6, partial_bytes(S::kRows, D, ctas), s, &p)) return rc;
+    const uint64_t partials = partial_bytes(S::kRows, D, ctas);
+    if (int rc = workspace(ctx, 6, partials + (S::kSettle != 0 ? uint64_t{ctas} * S::kRows * D * 4 : 0), s, &p)) return rc;
     w.partials = static_cast<float*>(p);
+    w.settled = w.partials + partials / 4;
     w.error_word = ctx->error_word_dev;
     auto kernel = tiles_kernel<T, D>;
     if (int rc = allow_dynamic_smem(ctx, reinterpret_cast<const void*>(kernel), S::kSmem)) return rc;
