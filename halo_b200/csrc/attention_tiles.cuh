@@ -39,8 +39,8 @@ struct TilesShape {
     static constexpr uint32_t kBuffer = kTile;             // columns of a score buffer, which the terms of the weights (kTile / 2 columns each) overwrite
     static constexpr uint32_t kO = 256;                    // first accumulator column
     // The tensor cores cut sums off instead of rounding them, always towards zero: a chain of n of them is n * 2^-25 too small in the mean.  fp32 operands'
-    // rows are added up in fp32 outside after every 32 (4 tiles of 64 keys, 2 of 128); 0: never.
-    static constexpr uint32_t kSettle = TERMS == 2 ? 32 / (kTile / 8) : 0;
+    // rows are added up in fp32 outside after every 64 (8 tiles of 64 keys, 4 of 128); 0: never.
+    static constexpr uint32_t kSettle = TERMS == 2 ? 64 / (kTile / 8) : 0;
     static constexpr int kHalves = 2 / kStreams;           // softmax warpgroups that share a row tile's keys
     static constexpr int kKeys = kTile / kHalves;          // of a tile that one of them has
     static constexpr int kConvWarps = D == 256 ? 8 : 4, kSoftWarp = 4 + kConvWarps, kSoftWarps = 8, kThreads = (kSoftWarp + kSoftWarps) * 32;
@@ -51,7 +51,7 @@ struct TilesShape {
     static constexpr uint32_t kAhead = 8;                  // that it has under way (all 16 of D = 256: 1672 -> 2147 us for 2048 tokens behind 28000)
     // What a thread has at launch; the warpgroups hand each other what they leave.
     static constexpr int kLaunchRegs = kThreads == 512 ? 128 : 96;
-    static constexpr int kIdleRegs = D == 256 ? 72 : kStreams == 1 ? 80 : 72, kConvRegs = D == 256 ? 80 : 88, kSoftRegs = D == 256 ? 120 : kStreams == 1 ? 168 : 176;
+    static constexpr int kIdleRegs = kStreams == 1 ? 80 : 72, kConvRegs = D == 256 ? 80 : 88, kSoftRegs = D == 256 ? 120 : kStreams == 1 ? 168 : 176;
     static_assert(kIdleRegs + kConvRegs * (kConvWarps / 4) + 2 * kSoftRegs <= kLaunchRegs * (kThreads / 128));
 };
 
