@@ -596,13 +596,8 @@ __global__ void __launch_bounds__(RowsShape<D, TS, RG, TILE, CPS, sizeof(T) == 4
             const int32_t t0 = tile * static_cast<int32_t>(kTile);
             const bool masked = t0 < all_lo || t0 + static_cast<int32_t>(kTile) > all_hi || partly[stage] != 0;
             float ahead[NT][4];
-            if (masked) {
-                scores(next, ahead);
-                weigh(true, t0, x);
-            } else {
-                scores(next, ahead);
-                weigh(false, t0, x);
-            }
+            scores(next, ahead);
+            weigh(masked, t0, x);
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
