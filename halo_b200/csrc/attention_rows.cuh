@@ -9,8 +9,9 @@
 // into [2^14, 2^15) and rounded to fp16: exact for fp16 and bf16 operands (but for elements below 2^-29 of the row's largest);
 // fp32 operands are taken as two fp16 terms, and so are their p_t.  Accumulators, maxima and sums are fp32.
 //
-// A CTA has RG groups of TS warps.  A group has 16 packed rows (attention_work.cuh); its warps share the keys of a tile, each with a running maximum,
-// sum and accumulators of its own that are joined at the end of a segment, so no warp waits for another inside the walk.  A producer warp
+// A CTA has 16 packed rows (attention_work.cuh).  Its warps share the keys of a tile, each with a running maximum, sum and accumulators of its own
+// that are joined at the end of a segment, so no warp waits for another inside the walk.  Heads of 256 elements would take 128 registers of accumulators a
+// thread: there two warps share the same keys, each makes half of the scores and all of the weights, and has half of the dims.  A producer warp
 // brings the tiles' codes by TMA, a box for each page, into a ring, and with them the scales of every 16 tokens (a page is at least 16).
 //
 // What bounds it: HBM.  A byte of the cache costs a warp half a conversion, and a sixteenth of a 16 x 8 x 16 product for 16 rows.
@@ -27,20 +28,21 @@ struct GroupScale {
     float pad;
 };
 
-/// TILE: keys of a tile.  CPS: CTAs that share an SM.
-template <int D, int TS, int RG, int TILE, int CPS, int TERMS>
+/// TS: warps, or pairs of them, that share a tile's keys.  TILE: keys of a tile.  CPS: CTAs that share an SM.
+template <int D, int TS, int TILE, int CPS, int TERMS>
 struct RowsShape {
     static constexpr uint32_t kTile = TILE, kGroups = TILE / 16;  // groups of 16 tokens, each inside one page
     static_assert(TILE % 64 == 0 && TILE % (16 * TS) == 0 && kGroups <= 32);
-    static constexpr int kWarps = TS * RG, kThreads = (kWarps + 1) * 32, kRows = 16 * RG;
+    static constexpr int kSplit = D == 256 ? 2 : 1;               // warps that share the dims of the same keys
+    static constexpr int kWarps = TS * kSplit, kThreads = (kWarps + 1) * 32, kRows = 16;
     static constexpr uint32_t kHalfTile = kTile * D;  // K or V of a tile
     static constexpr uint32_t kStage = 2 * kHalfTile;
-    static constexpr uint32_t kQ = RG * (D / 16) * TERMS * 512;
+    static constexpr uint32_t kQ = (D / 16) * TERMS * 512;
     static constexpr uint32_t kJoinRow = D + D / 8 + (D == 256 ? 16 : 0);  // floats of a row of the warps' joined rows
-    static constexpr uint32_t kJoin = RG * 16 * kJoinRow * 4;
+    static constexpr uint32_t kJoin = 16 * kJoinRow * 4;
     static constexpr uint32_t kFixed = 1024 + kQ + kJoin;  // alignment, q, the warps' joined rows
-    // an SM's 228 KiB, less 1 KiB a CTA for the system and 3 KiB for what is declared in the kernel
-    static constexpr uint32_t kStagesRoom = (228 / CPS * 1024 - 4096 - kFixed) / kStage;
+    // an SM's 228 KiB, less 1 KiB a CTA for the system and what is declared in the kernel (up to 8 KiB with pairs of warps, else 3)
+    static constexpr uint32_t kStagesRoom = (228 / CPS * 1024 - (kSplit == 2 ? 9216 : 4096) - kFixed) / kStage;
     static constexpr int kStages = kStagesRoom > 6 ? 6 : kStagesRoom;
     static constexpr uint32_t kSmem = kFixed + kStages * kStage;
     static_assert(kStages >= 2);
@@ -219,14 +221,15 @@ __device__ __forceinline__ void join_partials(const AttentionCall& c, const Work
     }
 }
 
-template <class T, int D, int TS, int RG, int TILE, int CPS>
-__global__ void __launch_bounds__(RowsShape<D, TS, RG, TILE, CPS, sizeof(T) == 4 ? 2 : 1>::kThreads, CPS)
+template <class T, int D, int TS, int TILE, int CPS>
+__global__ void __launch_bounds__(RowsShape<D, TS, TILE, CPS, sizeof(T) == 4 ? 2 : 1>::kThreads, CPS)
     rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const __grid_constant__ AttentionCall c,
                 const __grid_constant__ Work w) {
     constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;
-    using S = RowsShape<D, TS, RG, TILE, CPS, TERMS>;
+    using S = RowsShape<D, TS, TILE, CPS, TERMS>;
     constexpr int kParts = D > 128 ? D / 128 : 1, kPartDim = D / kParts;  // 128-byte columns of a tile
-    constexpr int kChunk = kPartDim / 8;                                  // dims of a lane group in a part: 16, or 8
+    constexpr int kOwn = kParts / S::kSplit, NO = TILE / TS / 8 / S::kSplit;  // parts, and blocks of 8 tokens' scores, of a warp
+    constexpr int kChunk = kPartDim / 8;    // dims of a lane group in a part: 16, or 8
     constexpr uint32_t kTile = S::kTile, kGroups = S::kGroups;
     constexpr int NT = TILE / TS / 8;                                        // blocks of 8 tokens of a warp
     constexpr bool kKeepQ = TERMS == 1 && D <= 64;                        // a row group's q in registers
@@ -235,7 +238,8 @@ __global__ void __launch_bounds__(RowsShape<D, TS, RG, TILE, CPS, sizeof(T) == 4
     __shared__ uint64_t bars[2 * S::kStages];
     __shared__ GroupScale scales[S::kStages][kGroups];
     __shared__ uint32_t partly[S::kStages];  // a page of the stage's tile is missing
-    __shared__ float2 row_ml[RG][TS][16];
+    __shared__ float2 row_ml[TS][16];
+    __shared__ float4 told[S::kSplit == 2 ? 2 : 1][TS][S::kSplit][NO][32];  // scores that a pair's warps tell each other, of a tile and the next
     __shared__ float q_unscale[S::kRows];
     __shared__ uint32_t nan_seen, is_last;
     __shared__ Walk walk;
@@ -365,8 +369,8 @@ __global__ void __launch_bounds__(RowsShape<D, TS, RG, TILE, CPS, sizeof(T) == 4
 
     // ---- consumers -------------------------------------------------------------------------------------------------------------------
     constexpr uint32_t kConsumers = S::kWarps * 32;
-    const uint32_t rg = warp / TS, ts = warp % TS, g8 = lane / 4, t4 = lane % 4;
-    const uint32_t my_q = q_at + rg * (D / 16) * TERMS * 512 + lane * 16;
+    const uint32_t ds = warp % S::kSplit, ts = warp / S::kSplit, g8 = lane / 4, t4 = lane % 4;
+    const uint32_t my_q = q_at + lane * 16;
     auto tau = [](uint32_t n) { return n ^ ((n & 1) << 2); };  // token of column n of a block of 8: spreads a quarter warp's reads over the banks
     __syncthreads();
     do {
@@ -412,7 +416,7 @@ __global__ void __launch_bounds__(RowsShape<D, TS, RG, TILE, CPS, sizeof(T) == 4
                 for (int e = 0; e < E; e += 2) {
                     // dim 64 a + 16 t + 4 s + 2 p + {0, 1}: k step 4 a + s, lane t of a quad, register 2 p (+ 1 for the rows 8 and up)
                     const uint32_t d = lane * E + e, step = d / 64 * 4 + d % 16 / 4, t = d % 64 / 16, p = d % 4 / 2;
-                    const uint32_t at = q_at + (r / 16) * (D / 16) * TERMS * 512 + step * TERMS * 512 + (r % 8 * 4 + t) * 16 + (2 * p + r / 8 % 2) * 4;
+                    const uint32_t at = q_at + step * TERMS * 512 + (r % 8 * 4 + t) * 16 + (2 * p + r / 8 % 2) * 4;
                     const float a = x[e] * by, b = x[e + 1] * by;
                     const uint32_t hi = half2_bits(a, b);
                     asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(hi) : "memory");
@@ -431,7 +435,7 @@ __global__ void __launch_bounds__(RowsShape<D, TS, RG, TILE, CPS, sizeof(T) == 4
         float qs[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const uint32_t r = rg * 16 + g8 + 8 * i, j = walk.token(w, min(r, rows - 1));
+            const uint32_t r = g8 + 8 * i, j = walk.token(w, min(r, rows - 1));
             lo[i] = first_key(u.s, w.window, j);
             hi[i] = end_key(u.s, c.causal, j);
             qs[i] = q_unscale[r];
@@ -441,24 +445,28 @@ __global__ void __launch_bounds__(RowsShape<D, TS, RG, TILE, CPS, sizeof(T) == 4
         const int32_t all_lo = first_key(u.s, w.window, last_token), all_hi = end_key(u.s, c.causal, first_token);
         const int32_t any_lo = first_key(u.s, w.window, first_token), any_hi = end_key(u.s, c.causal, last_token);
 
-        float o[kParts][kChunk][4];
+        float o[kOwn][kChunk][4];
 #pragma unroll
-        for (int a = 0; a < kParts; ++a)
+        for (int a = 0; a < kOwn; ++a)
 #pragma unroll
             for (int b = 0; b < kChunk; ++b) o[a][b][0] = o[a][b][1] = o[a][b][2] = o[a][b][3] = 0;
         float m[2] = {-INFINITY, -INFINITY}, l[2] = {0, 0};
 
         const uint32_t tok = ts * (NT * 8);  // this warp's first token of a tile
-        auto scores = [&](uint32_t st, float (&x)[NT][4]) {  // q . k of a stage's tile
-            const uint32_t k_at = ring + st * S::kStage;
+        auto scores = [&](uint32_t st, float (&x)[NO][4]) {  // q . k of this warp's tokens of a stage's tile
+            const uint32_t k_at = ring + st * S::kStage, first = tok + ds * (NO * 8);
+            constexpr int kChains = NO == 1 ? 2 : 1;  // sums of every other step, where one block of tokens would be one chain of products
+            float y[kChains][NO][4];
 #pragma unroll
-            for (int n = 0; n < NT; ++n) x[n][0] = x[n][1] = x[n][2] = x[n][3] = 0;
+            for (int h = 0; h < kChains; ++h)
+#pragma unroll
+                for (int n = 0; n < NO; ++n) y[h][n][0] = y[h][n][1] = y[h][n][2] = y[h][n][3] = 0;
 #pragma unroll
             for (int a = 0; a < D / 64; ++a) {
-                uint4 kw[NT];
+                uint4 kw[NO];
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
-                    kw[n] = lds128(k_at + (D > 64 ? a / 2 * kTile * 128 : 0) + swizzled(tok + 8 * n + tau(g8), (D > 64 ? a % 2 * 4 : 0) + t4, D));
+                for (int n = 0; n < NO; ++n)
+                    kw[n] = lds128(k_at + (D > 64 ? a / 2 * kTile * 128 : 0) + swizzled(first + 8 * n + tau(g8), (D > 64 ? a % 2 * 4 : 0) + t4, D));
 #pragma unroll
                 for (int s = 0; s < 4; ++s) {
                     uint4 q[TERMS];
@@ -468,13 +476,23 @@ __global__ void __launch_bounds__(RowsShape<D, TS, RG, TILE, CPS, sizeof(T) == 4
                         for (int term = 0; term < TERMS; ++term) q[term] = lds128(my_q + ((a * 4 + s) * TERMS + term) * 512);
                     }
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) {
+                    for (int n = 0; n < NO; ++n) {
                         const uint32_t word = s == 0 ? kw[n].x : s == 1 ? kw[n].y : s == 2 ? kw[n].z : kw[n].w;
                         const uint32_t b0 = widen_lo(word), b1 = widen_hi(word);
 #pragma unroll
-                        for (int term = 0; term < TERMS; ++term) mma16816(x[n], q[term].x, q[term].y, q[term].z, q[term].w, b0, b1);
+                        for (int term = 0; term < TERMS; ++term) mma16816(y[s % kChains][n], q[term].x, q[term].y, q[term].z, q[term].w, b0, b1);
                     }
                 }
+            }
+#pragma unroll
+            for (int n = 0; n < NO; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[n][e] = kChains == 2 ? y[0][n][e] + y[kChains - 1][n][e] : y[0][n][e];
+        };
+        auto tell = [&](uint32_t turn, const float (&x)[NO][4]) {
+            if constexpr (S::kSplit == 2) {
+#pragma unroll
+                for (int n = 0; n < NO; ++n) told[turn & 1][ts][ds][n][lane] = make_float4(x[n][0], x[n][1], x[n][2], x[n][3]);
             }
         };
         // the weights of a tile's scores, and what they add to the sums and rows.  MASKED: some row does not see some token of the tile.
@@ -518,7 +536,7 @@ __global__ void __launch_bounds__(RowsShape<D, TS, RG, TILE, CPS, sizeof(T) == 4
                 for (int i = 0; i < 2; ++i) {
                     l[i] *= fade[i];
 #pragma unroll
-                    for (int a = 0; a < kParts; ++a)
+                    for (int a = 0; a < kOwn; ++a)
 #pragma unroll
                         for (int b = 0; b < kChunk; ++b) o[a][b][2 * i] *= fade[i], o[a][b][2 * i + 1] *= fade[i];
                 }
@@ -544,12 +562,12 @@ __global__ void __launch_bounds__(RowsShape<D, TS, RG, TILE, CPS, sizeof(T) == 4
 #pragma unroll
                 for (int i = 0; i < 4; ++i) row[i] = tok + 16 * s + 8 * (i / 2) + tau(2 * t4 + i % 2);
 #pragma unroll
-                for (int a = 0; a < kParts; ++a) {
+                for (int a = 0; a < kOwn; ++a) {
                     uint32_t vw[4][kChunk / 4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         if constexpr (D > 64) {
-                            const uint4 v = lds128(v_at + a * kTile * 128 + swizzled(row[i], g8, D));
+                            const uint4 v = lds128(v_at + (ds * kOwn + a) * kTile * 128 + swizzled(row[i], g8, D));
                             vw[i][0] = v.x, vw[i][1] = v.y, vw[i][2] = v.z, vw[i][3] = v.w;
                         } else {
                             const uint2 v = lds64(v_at + swizzled(row[i], g8 / 2, D) + g8 % 2 * 8);
@@ -586,22 +604,34 @@ __global__ void __launch_bounds__(RowsShape<D, TS, RG, TILE, CPS, sizeof(T) == 4
         // The next tile's scores are issued in front of this tile's weights: two independent chains for a warp that has few neighbours.  Behind the last
         // tile they are those of whatever the next stage holds, and unused.
         if (alive) alive = __all_sync(0xFFFFFFFFu, mbar_wait(full + 8 * stage, parity));
-        float x[NT][4];
-        scores(stage, x);
+        float mine[NO][4];
+        scores(stage, mine);
+        tell(0, mine);
         const int32_t last = walk.g.hi;
-        for (int32_t tile = walk.g.lo; tile < last; ++tile) {
+        uint32_t turn = 0;
+        for (int32_t tile = walk.g.lo; tile < last; ++tile, ++turn) {
             const bool wraps = stage + 1 == S::kStages;
             const uint32_t next = wraps ? 0 : stage + 1;
             if (alive && tile + 1 < last) alive = __all_sync(0xFFFFFFFFu, mbar_wait(full + 8 * next, parity ^ (wraps ? 1 : 0)));
             const int32_t t0 = tile * static_cast<int32_t>(kTile);
             const bool masked = t0 < all_lo || t0 + static_cast<int32_t>(kTile) > all_hi || partly[stage] != 0;
-            float ahead[NT][4];
-            scores(next, ahead);
+            float x[NT][4];
+            if constexpr (S::kSplit == 2) {  // what is told of the next tile goes beside this one's: one barrier a tile
+                bar_sync(2 + ts, 64);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const float4 v = told[turn & 1][ts][n / NO][n % NO][lane];
+                    x[n][0] = v.x, x[n][1] = v.y, x[n][2] = v.z, x[n][3] = v.w;
+                }
+            } else {
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[n][e] = mine[n][e];
+            }
+            scores(next, mine);
+            tell(turn + 1, mine);
             weigh(masked, t0, x);
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) x[n][e] = ahead[n][e];
             __syncwarp();
             if (lane == 0) mbar_arrive(empty + 8 * stage);
             advance();
@@ -618,34 +648,34 @@ __global__ void __launch_bounds__(RowsShape<D, TS, RG, TILE, CPS, sizeof(T) == 4
         auto out_at = [&](uint32_t r) {
             return reinterpret_cast<T*>(walk.at(c, w, c.out, r));
         };
-        if (t4 == 0) row_ml[rg][ts][g8] = make_float2(m[0], l[0]), row_ml[rg][ts][g8 + 8] = make_float2(m[1], l[1]);
+        if (t4 == 0 && ds == 0) row_ml[ts][g8] = make_float2(m[0], l[0]), row_ml[ts][g8 + 8] = make_float2(m[1], l[1]);
         bar_sync(1, kConsumers);
         float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0, 0}, f[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
 #pragma unroll
-            for (int k = 0; k < TS; ++k) top[i] = fmaxf(top[i], row_ml[rg][k][g8 + 8 * i].x);
+            for (int k = 0; k < TS; ++k) top[i] = fmaxf(top[i], row_ml[k][g8 + 8 * i].x);
 #pragma unroll
             for (int k = 0; k < TS; ++k) {
-                const float2 ml = row_ml[rg][k][g8 + 8 * i];
+                const float2 ml = row_ml[k][g8 + 8 * i];
                 sum[i] += ml.x == -INFINITY ? ml.y : exp2_approx(ml.x - top[i]) * ml.y;
             }
             f[i] = m[i] == -INFINITY ? 1.0f : exp2_approx(m[i] - top[i]);
         }
         // Dim d of a row lies at d + d / 32 * 4: the lanes of a 16-byte store spread over the banks.
-        float* mine = join + (rg * 16 + g8) * S::kJoinRow + t4 * (2 * kChunk) + t4 * (2 * kChunk) / 32 * 4;
+        float* into = join + g8 * S::kJoinRow + t4 * (2 * kChunk) + t4 * (2 * kChunk) / 32 * 4;
 #pragma unroll 1
         for (int k = 0; k < TS; ++k) {
             if (ts == static_cast<uint32_t>(k)) {
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
-                    for (int a = 0; a < kParts; ++a)
+                    for (int a = 0; a < kOwn; ++a)
 #pragma unroll
                         for (int e = 0; e < 2; ++e)
 #pragma unroll
                             for (int b = 0; b < kChunk; b += 4) {
-                                float4* to = reinterpret_cast<float4*>(mine + 8 * i * S::kJoinRow + a * (kPartDim / 32 * 36) + e * kChunk + b);
+                                float4* to = reinterpret_cast<float4*>(into + 8 * i * S::kJoinRow + (ds * kOwn + a) * (kPartDim / 32 * 36) + e * kChunk + b);
                                 float4 v = make_float4(o[a][b][2 * i + e] * f[i], o[a][b + 1][2 * i + e] * f[i], o[a][b + 2][2 * i + e] * f[i], o[a][b + 3][2 * i + e] * f[i]);
                                 if (k != 0) {
                                     const float4 x = *to;
@@ -656,10 +686,10 @@ __global__ void __launch_bounds__(RowsShape<D, TS, RG, TILE, CPS, sizeof(T) == 4
             }
             bar_sync(1, kConsumers);
         }
-        if (ts == 0 && t4 == 0) row_ml[rg][0][g8] = make_float2(top[0], sum[0]), row_ml[rg][0][g8 + 8] = make_float2(top[1], sum[1]);
+        if (warp == 0 && t4 == 0) row_ml[0][g8] = make_float2(top[0], sum[0]), row_ml[0][g8 + 8] = make_float2(top[1], sum[1]);
         bar_sync(1, kConsumers);
         for (uint32_t r = warp; r < walk.rows; r += S::kWarps) {
-            const float2 ml = row_ml[r / 16][0][r % 16];
+            const float2 ml = row_ml[0][r];
             const float inv = ml.y != 0 ? 1.0f / ml.y : 0.0f;
             T* out = out_at(r);
 #pragma unroll
@@ -707,9 +737,9 @@ __global__ void __launch_bounds__(RowsShape<D, TS, RG, TILE, CPS, sizeof(T) == 4
 /// The cache's pool as {dim, rows of all heads of a page, pages}, a box of one page's rows of one head.
 int pool_map(const Cache& c, const uint8_t* pool, uint32_t box_rows, CUtensorMap* out);
 
-template <class T, int D, int TS, int RG, int TILE, int CPS>
+template <class T, int D, int TS, int TILE, int CPS>
 int launch_rows_kernel(HaloCudaCtx* ctx, const AttentionCall& c, Work w, cudaStream_t s) {
-    using S = RowsShape<D, TS, RG, TILE, CPS, sizeof(T) == 4 ? 2 : 1>;
+    using S = RowsShape<D, TS, TILE, CPS, sizeof(T) == 4 ? 2 : 1>;
     w.rows = S::kRows;
     w.tile = S::kTile;
     w.pad = 4;
@@ -730,7 +760,7 @@ int launch_rows_kernel(HaloCudaCtx* ctx, const AttentionCall& c, Work w, cudaStr
     if (int rc = workspace(ctx, 6, partial_bytes(S::kRows, D, ctas), s, &p)) return rc;
     w.partials = static_cast<float*>(p);
     w.error_word = ctx->error_word_dev;
-    auto kernel = rows_kernel<T, D, TS, RG, TILE, CPS>;
+    auto kernel = rows_kernel<T, D, TS, TILE, CPS>;
     if (int rc = allow_dynamic_smem(ctx, reinterpret_cast<const void*>(kernel), S::kSmem)) return rc;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(ctas);
