@@ -29,10 +29,6 @@ int pool_map(const Cache& c, const uint8_t* pool, uint32_t box_rows, CUtensorMap
     return 0;
 }
 
-
-
-
-
 int launch_attention(HaloCudaCtx* ctx, const AttentionCall& c, cudaStream_t s) {
     if (c.cache.n_pages == 0 || c.cache.max_pages == 0) return fail(HALO_CUDA_E_UNSUPPORTED, "ATTENTION: a cache without pages");
     auto run = [&](uint32_t min_rows, uint32_t max_rows) {
@@ -40,15 +36,14 @@ int launch_attention(HaloCudaCtx* ctx, const AttentionCall& c, cudaStream_t s) {
         w.window = static_cast<int32_t>(std::min(c.window, 0x7FFFFFFFu));
         w.min_rows = min_rows;
         w.max_rows = max_rows;
-        return c.cache.head_dim == 64 ? launch_rows<64>(ctx, c, w, s) : c.cache.head_dim == 128 ? launch_rows<128>(ctx, c, w, s) : launch_rows<256>(ctx, c, w, s);
+        return c.cache.head_dim == 64 ? launch_kernel<64>(ctx, c, w, s) : c.cache.head_dim == 128 ? launch_kernel<128>(ctx, c, w, s) : launch_kernel<256>(ctx, c, w, s);
     };
-    // Sequences of few rows among others run in a launch of their own: under the tiles of long ones each would fetch its cache alone.
-    const uint32_t most = c.rows.max_tokens * c.group;
+    // Sequences of few rows among others run in a launch of their own.
+    const uint32_t most = c.rows.max_tokens * c.group, few = few_rows(c);
     const bool ragged = c.rows.n_tokens < uint64_t{c.cache.n_seq} * c.rows.max_tokens;
-    constexpr uint32_t kFew = 16;
-    if (most <= kFew || !ragged) return run(1, most);
-    if (int rc = run(1, kFew)) return rc;
-    return run(kFew + 1, most);
+    if (most <= few || !ragged) return run(1, most);
+    if (int rc = run(1, few)) return rc;
+    return run(few + 1, most);
 }
 
 }  // namespace attn

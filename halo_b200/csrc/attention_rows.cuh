@@ -776,9 +776,14 @@ int launch_rows_kernel(HaloCudaCtx* ctx, const AttentionCall& c, Work w, cudaStr
     return 0;
 }
 
-/// One of the kernels above by operand type; instantiated for each head size in a file of its own.
+/// One of the kernels by operand type and rows; instantiated for each head size in a file of its own.
 template <int D>
-int launch_rows(HaloCudaCtx* ctx, const AttentionCall& c, const Work& w, cudaStream_t s);
+int launch_kernel(HaloCudaCtx* ctx, const AttentionCall& c, const Work& w, cudaStream_t s);
+
+/// Up to how many packed rows of a sequence the row kernel takes.  12 sequences of 2000 - 4700 tokens, row kernel / tcgen05 kernel, us: heads of 256, 24
+/// rows: fp32 66 / 81, bf16 56 / 58; 36 rows: 89 / 88, 75 / 64.  Heads of 128, 40 rows: fp32 79 / 81, bf16 61 / 93; 64 rows: 100 / 84, 76 / 93.  Heads of
+/// 64, 64 rows: 63 / 67, 55 / 74.
+inline uint32_t few_rows(const AttentionCall& c) { return c.cache.head_dim == 256 ? 32 : c.type == HALO_CUDA_T_F32 ? 48 : 64; }
 
 }  // namespace attn
 }  // namespace halo_cuda
