@@ -74,7 +74,8 @@ int take_cache(const HaloCudaKvCache& c, const char* op, Cache* out, CacheSpans*
         return fail(HALO_CUDA_E_UNSUPPORTED, "%s: pages of %u tokens (16, 32, 64 or 128)", op, c.page_tokens);
     if (c.n_kv == 0 || c.n_kv > 65535u) return fail(HALO_CUDA_E_KERNEL, "%s: %u kv heads", op, c.n_kv);
     if (c.n_pages > 0x7FFFFFFFu) return fail(HALO_CUDA_E_KERNEL, "%s: %u pages", op, c.n_pages);
-    if (uint64_t{c.max_pages} * c.page_tokens >= (1ull << 31)) return fail(HALO_CUDA_E_KERNEL, "%s: sequences of %u pages of %u tokens", op, c.max_pages, c.page_tokens);
+    if (c.n_seq > 0x7FFFFFFFu) return fail(HALO_CUDA_E_KERNEL, "%s: %u sequences", op, c.n_seq);
+    if (uint64_t{c.max_pages} * c.page_tokens > (1ull << 30)) return fail(HALO_CUDA_E_KERNEL, "%s: sequences of %u pages of %u tokens", op, c.max_pages, c.page_tokens);
     const uint64_t page = uint64_t{c.n_kv} * c.page_tokens * c.head_dim;
     *out = Cache{static_cast<uint8_t*>(c.k), static_cast<uint8_t*>(c.v), c.k_scale, c.v_scale, c.table, c.page_stride != 0 ? c.page_stride : page,
                  c.scale_stride != 0 ? c.scale_stride : c.n_kv, c.table_stride != 0 ? c.table_stride : uint64_t{c.max_pages} * 4,

@@ -20,23 +20,36 @@ namespace {
 
 constexpr uint32_t kUnit = 16;  // elements of a thread's unit: one 16-byte store of codes
 
+/// A thread's unit as it lies in memory: 16-bit elements stay packed until they are needed, for the sake of registers.
 template <class T>
-__device__ __forceinline__ void load_unit(const uint8_t* p, bool vec, float (&x)[kUnit]) {
-    constexpr uint32_t per = 16 / sizeof(T);
-    if (vec) {
+struct Raw {
+    uint32_t word[kUnit * sizeof(T) / 4];
+    __device__ __forceinline__ void load(const uint8_t* p, bool vec) {
+        if (vec) {
 #pragma unroll
-        for (uint32_t i = 0; i < kUnit / per; ++i) {
-            const uint4 w = __ldg(reinterpret_cast<const uint4*>(p) + i);
-            T v[per];
-            __builtin_memcpy(v, &w, 16);
+            for (uint32_t i = 0; i < kUnit * sizeof(T) / 16; ++i) {
+                const uint4 w = __ldg(reinterpret_cast<const uint4*>(p) + i);
+                word[4 * i] = w.x, word[4 * i + 1] = w.y, word[4 * i + 2] = w.z, word[4 * i + 3] = w.w;
+            }
+        } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
-            for (uint32_t j = 0; j < per; ++j) x[i * per + j] = to_f32(v[j]);
+            for (uint32_t i = 0; i < kUnit; ++i) word[i] = reinterpret_cast<const uint32_t*>(p)[i];
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < kUnit / 2; ++i) word[i] = reinterpret_cast<const uint16_t*>(p)[2 * i] | static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(p)[2 * i + 1]) << 16;
         }
-    } else {
-#pragma unroll
-        for (uint32_t j = 0; j < kUnit; ++j) x[j] = to_f32(reinterpret_cast<const T*>(p)[j]);
     }
-}
+    __device__ __forceinline__ float operator[](uint32_t j) const {
+        T v;
+        if constexpr (sizeof(T) == 4) {
+            v = __uint_as_float(word[j]);
+        } else {
+            const uint16_t h = static_cast<uint16_t>(j % 2 != 0 ? word[j / 2] >> 16 : word[j / 2] & 0xFFFFu);
+            __builtin_memcpy(&v, &h, 2);
+        }
+        return to_f32(v);
+    }
+};
 __device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
     const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
     const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
@@ -73,14 +86,18 @@ __global__ void __launch_bounds__(512) kv_write_kernel(const WriteCall c) {
     uint8_t* dst = (is_v ? kv.v : kv.k) + page * kv.page_stride + uint64_t{head} * kv.page_tokens * kv.head_dim;
     uint8_t* scale = (is_v ? kv.v_scale : kv.k_scale) + page * kv.scale_stride + head;
 
-    float x[UNITS][kUnit];
+    Raw<T> x[UNITS];
     float top = 0;
 #pragma unroll
     for (uint32_t i = 0; i < UNITS; ++i) {
         const uint32_t u = threadIdx.x + i * blockDim.x;
         if (u >= units) break;
         const uint32_t row = u / row_units, at = u - row * row_units;
-        load_unit<T>(src + row * in.token_stride + at * kUnit * sizeof(T), in.vec != 0, x[i]);
+        x[i].load(src + row * in.token_stride + at * kUnit * sizeof(T), in.vec != 0);
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < UNITS; ++i) {
+        if (threadIdx.x + i * blockDim.x >= units) break;
 #pragma unroll
         for (uint32_t j = 0; j < kUnit; ++j) {
             const float m = fabsf(x[i][j]);

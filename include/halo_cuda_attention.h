@@ -89,12 +89,12 @@ typedef struct HaloCudaKvCache {
     const int32_t* table;                           /* n_seq rows of max_pages page numbers (device) */
     uint64_t page_stride, scale_stride, table_stride; /* bytes; 0 = dense: n_kv * page_tokens * head_dim, n_kv, max_pages * 4 */
     uint32_t type;        /* HALO_CUDA_KV_E4M3 */
-    uint32_t n_pages;     /* in the pools */
+    uint32_t n_pages;     /* in the pools; below 2^31 */
     uint32_t n_kv;
     uint32_t head_dim;    /* 64, 128 or 256 */
     uint32_t page_tokens; /* 16, 32, 64 or 128 */
-    uint32_t max_pages;   /* of one sequence; max_pages * page_tokens < 2^31 */
-    uint32_t n_seq, reserved;
+    uint32_t max_pages;   /* of one sequence; max_pages * page_tokens at most 2^30 */
+    uint32_t n_seq, reserved; /* n_seq below 2^31 */
 } HaloCudaKvCache;
 
 /* Whose the token rows of a call are: sequence i has rows start[i] .. start[i + 1] - 1 of the operands (device, n_seq + 1 values, never
@@ -111,8 +111,9 @@ typedef struct HaloCudaKvRows {
  * the largest finite magnitude of its new rows is at most 448, or the scale it had if that is larger and slots in front of the new rows hold
  * the sequence's earlier tokens: those are then rounded again to the new scale.  Codes are rounded to nearest, ties to even; infinities become
  * +-448, a NaN stays one.  Slots behind the new rows keep their bytes (and no meaning).  Rows at negative positions are skipped.  A page
- * number outside [0, n_pages) sets bit 8 (kStatusBadIndex) of *status (device word, optional) and nothing is written for it.  Two sequences of one call
- * must not write into the same page: a forked page is copied first (halo_cuda_memcpy_d2d_async of its codes and scale bytes). */
+ * number outside [0, n_pages) sets bit 8 (kStatusBadIndex) of *status (device word, optional) and nothing is written for it.  At most 65535
+ * sequences and 32767 kv heads.  Two sequences of one call must not write into the same page: a forked page is copied first
+ * (halo_cuda_memcpy_d2d_async of its codes and scale bytes). */
 typedef struct HaloCudaKvWrite {
     uint32_t type, reserved; /* of k and v: HALO_CUDA_T_F32, _F16, _BF16 */
     HaloCudaKvCache cache;
@@ -127,10 +128,12 @@ int halo_cuda_kv_write(HaloCudaCtx* ctx, const HaloCudaKvWrite* args, HaloCudaSt
  * those t > p - window.  A row that sees none gets zeros.  What a row does not see has no influence on it, whatever it holds.  Tokens of a page whose
  * number is outside [0, n_pages) are left out and set bit 8 of *status (device word, optional).
  * Type F32 computes to fp32 accuracy (both factors of the products in two fp16 terms); F16 and BF16 take q exactly and round the weights to 11
- * bits; sums and softmax are fp32 throughout.  The order of the sums goes with the shape and the lengths of the whole call, and the same call
- * gives the same bits.  Uses context scratch, whose size goes with the operands' shapes alone: run a call once before capturing it. */
+ * bits; sums and softmax are fp32 throughout.  Weights (times their values' scale) below 2^-20 of the row's largest are rounded to multiples of
+ * 2^-30 of it, for all types.  The order of the sums goes with the shape and the lengths of the whole call, and the same call gives the same bits.
+ * The cache has at least one page, and the table a column.  Uses context scratch, whose size goes with the operands' shapes alone: run a call once
+ * before capturing it. */
 typedef struct HaloCudaAttention {
-    uint32_t type, n_q; /* of q and out; n_q: a multiple of n_kv */
+    uint32_t type, n_q; /* of q and out; n_q: a multiple of n_kv, at most 32768 */
     HaloCudaKvCache cache;
     HaloCudaKvRows rows;
     HaloCudaHeads q, out; /* n_tokens x n_q x head_dim; out overlaps neither q nor the cache */

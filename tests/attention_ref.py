@@ -77,8 +77,12 @@ def kv_write(cache: dict, k: np.ndarray, v: np.ndarray, start, length) -> bool:
     return bad
 
 
-def attention(q: np.ndarray, cache: dict, start, length, scale: float, causal: bool = True, window: int = 0, out: np.ndarray | None = None):
-    """(out, sum of weights * |v|, largest sum of |q_d k_d| * |scale| of a seen token, number of seen tokens); rows of no sequence keep `out`."""
+def attention(q: np.ndarray, cache: dict, start, length, scale: float, causal: bool = True, window: int = 0, out: np.ndarray | None = None,
+              floor: np.ndarray | None = None):
+    """(out, sum of weights * |v|, largest sum of |q_d k_d| * |scale| of a seen token, number of seen tokens); rows of no sequence keep `out`.
+    `floor` gets what the smallest weights may be off by.  A kernel holds weight * s_V as fp16 numbers (fp32 operands: as two, the second of the first's
+    remainder) scaled so that the row's largest is at least 2^6.  fp16's smallest step is 2^-24, so a rounding is off by at most half a step, 2^-25,
+    where the 2^-11 of attention_bound does not cover it: at most 2^-31 of the largest weight * s_V, for each token, times the code it multiplies."""
     n_pages, n_kv, page_tokens, dim = cache["k"].shape
     n_q = q.shape[1]
     g = n_q // n_kv
@@ -113,6 +117,9 @@ def attention(q: np.ndarray, cache: dict, start, length, scale: float, causal: b
                     w /= w.sum(axis=1, keepdims=True)
                     y[lo + r, h * g:h * g + g] = w @ v[m]
                     weight[lo + r, h * g:h * g + g] = w @ np.abs(v[m])
+                    if floor is not None:
+                        s_v = scale_of(cache["v_scale"][at, h])[m]
+                        floor[lo + r, h * g:h * g + g] = 2.0 ** -31 * (w * s_v).max(axis=1)[:, None] * np.abs(v[m] / s_v[:, None]).sum(axis=0)
                     top[lo + r, h * g:h * g + g] = (np.abs(qs) @ np.abs(k[m]).T * abs(scale)).max(axis=1)
                 count[lo + r, h * g:h * g + g] = m.sum()
     return y, weight, top, count

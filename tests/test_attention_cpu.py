@@ -230,3 +230,9 @@ def test_the_backends_operands_are_checked_on_the_host():
     a.head_dim, a.q.ref.buffer.writable = 128, False
     with pytest.raises(hb.HaloError, match="read-only"):
         be.partial_rope(hb.Stream(be, 0), a)
+
+
+@pytest.mark.parametrize("call", [write_call, attention_call])
+def test_positions_and_sequences_stay_below_what_the_device_counts_in(call):
+    last(call(cache=cache(max_pages=2 ** 25, page_tokens=64, table_stride=2 ** 27)), capi.E_KERNEL, "sequences of")
+    last(call(cache=cache(n_seq=2 ** 31)), capi.E_KERNEL, "2147483648 sequences")

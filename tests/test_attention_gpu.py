@@ -110,10 +110,11 @@ class Case:
 
     def compare(self, out, causal=True, window=0, scale=None, bad=0):
         s = self.dim ** -0.5 if scale is None else scale
-        want, weight, top, count = ref.attention(self.q, self.cache, self.start, self.length, s, causal, window, out=np.full(self.q.shape, 77.0))
+        floor = np.zeros(self.q.shape)
+        want, weight, top, count = ref.attention(self.q, self.cache, self.start, self.length, s, causal, window, np.full(self.q.shape, 77.0), floor)
         got = out.double().cpu().numpy()
         assert np.array_equal(np.isnan(got), np.isnan(want))
-        bound = ref.attention_bound(self.kind, self.dim, want, weight, top, count)
+        bound = ref.attention_bound(self.kind, self.dim, want, weight, top, count) + floor
         with np.errstate(invalid="ignore"):
             off = np.abs(got - want) / np.where(np.isnan(want), 1, bound)
         worst = np.nanmax(off, initial=0.0)
@@ -400,6 +401,57 @@ def test_a_batch_of_hundreds(be):
     c.compare(c.run(be))
 
 
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("rows", [1, 50])
+def test_query_rows_of_any_magnitude(be, kind, dim, rows):
+    """Neighbouring rows from 2^-14 to 2^12 times the ordinary size, with loudly and faintly scaled keys."""
+    c = Case(24, kind, dim, 32, 2, 3, [rows] * 3, [rows + 90, rows + 20, rows + 200])
+    c.q *= 2.0 ** (np.arange(c.q.shape[0] * c.n_q).reshape(c.q.shape[0], c.n_q, 1) * 5 % 27 - 14)
+    c.q[0, 1] = 0
+    c.cache["k_scale"][:] = c.rng.integers(108, 118, c.cache["k_scale"].shape)
+    c.to_device()
+    c.compare(c.run(be))
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("rows", [1, 50])
+def test_shared_pages(be, kind, rows):
+    """Sequences with a common beginning in the same pages, and a page that a sequence holds twice."""
+    c = Case(25, kind, 128, 16, 2, 4, [rows] * 3, [rows + 64, rows + 80, rows + 48])
+    t = c.cache["table"]
+    t[1, :3] = t[0, :3]
+    t[2, 1] = t[2, 0]
+    c.to_device()
+    c.compare(c.run(be))
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("q_len", [[1, 2, 1], [80, 1, 200]])
+def test_two_graphs_replayed_at_once(be, kind, q_len):
+    """Each of a stream of its own: their shares of units do not meet."""
+    cs = [Case(26 + i, kind, 128, 32, 2, 4, q_len, [2000, 700 + i, 3000]) for i in range(2)]
+    want = [c.run(be) for c in cs]
+    outs = [torch.zeros_like(w) for w in want]
+    streams, graphs = [torch.cuda.Stream() for _ in cs], [torch.cuda.CUDAGraph() for _ in cs]
+    args = [c.call(o) for c, o in zip(cs, outs)]
+    for a, s, g in zip(args, streams, graphs):
+        check(be.lib.halo_cuda_attention(be.ctx, C.byref(a), s.cuda_stream))
+        torch.cuda.synchronize()
+        with torch.cuda.graph(g, stream=s):
+            check(be.lib.halo_cuda_attention(be.ctx, C.byref(a), s.cuda_stream))
+    for o in outs:
+        o.zero_()
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for o, w in zip(outs, want):
+        assert torch.equal(o, w)
+
+
 # ---- KV_WRITE --------------------------------------------------------------------------------------------------------------------------------
 def write(be, c, k, v, status=None, **kw):
     a = dict(type=c.type, cache=c.kv(), rows=c.rows(), k=heads(k), v=heads(v), status=(c.status if status is None else status).data_ptr())
@@ -530,6 +582,17 @@ def test_kv_write_captured(be):
         torch.cuda.synchronize()
         ref.kv_write(c.cache, kh, vh, c.start, length)
         same_cache(c)
+
+
+def test_kv_write_padded_rows_and_rows_behind_the_last_sequence(be):
+    """Rows that belong to no sequence, or lie beyond max_tokens, are not written anywhere."""
+    c = Case(38, "bf16", 128, 16, 2, 1, [2, 5, 1], [20, 33, 1])
+    (k, v), (kh, vh) = new_rows(c)
+    pad = [torch.full((6, c.n_kv, c.dim), 300.0, dtype=c.dtype, device="cuda") for _ in range(2)]
+    k, v = (torch.cat([t, p]) for t, p in zip((k, v), pad))
+    write(be, c, k, v, rows=c.rows(n_tokens=c.n_tokens + 6))
+    ref.kv_write(c.cache, kh, vh, c.start, c.length)
+    same_cache(c)
 
 
 # ---- PARTIAL_ROPE ----------------------------------------------------------------------------------------------------------------------------
