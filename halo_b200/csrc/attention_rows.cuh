@@ -1,5 +1,4 @@
-// ATTENTION for few rows to a sequence (decoded tokens, drafts), and for fp32 operands of any number of rows: warp-level fp16 tensor-core products
-// over the cache's codes, converted in registers.
+// ATTENTION for few rows to a sequence (decoded tokens, drafts): warp-level fp16 tensor-core products over the cache's codes, converted in registers.
 //
 //   x_t = q . k_t * (s_K(t) * scale * log2 e) + log2 s_V(t),   m = max x_t,   p_t = 2^(x_t - m + 14)
 //   o = sum p_t code(v_t),   l = sum p_t / s_V(t),   out = o / l
@@ -14,7 +13,9 @@
 // thread: there two warps share the same keys, each makes half of the scores and all of the weights, and has half of the dims.  A producer warp
 // brings the tiles' codes by TMA, a box for each page, into a ring, and with them the scales of every 16 tokens (a page is at least 16).
 //
-// What bounds it: HBM.  A byte of the cache costs a warp half a conversion, and a sixteenth of a 16 x 8 x 16 product for 16 rows.
+// What bounds it: HBM while the walk lasts (131071 tokens of 8 heads of 128, 268 MB, take 64 us, 4.2 TB/s; of a CTA's 92 thousand clocks the walk has 80,
+// which is 6.2 TB/s, the search for its share 4, the first tile 6).  A byte of the cache costs a warp half a conversion, and a sixteenth of a
+// 16 x 8 x 16 product for 16 rows.  Heads of 256 with fp32 operands, four products for one: issue slots (2.1 TB/s).
 #pragma once
 #include <cuda.h>
 
@@ -743,7 +744,6 @@ int launch_rows_kernel(HaloCudaCtx* ctx, const AttentionCall& c, Work w, cudaStr
     w.rows = S::kRows;
     w.tile = S::kTile;
     w.pad = 4;
-    w.least = 1;
     w.group = c.group;
     w.group_inverse = static_cast<uint32_t>((0xFFFFFFFFull + c.group) / c.group);
     w.row_tiles = (w.max_rows + S::kRows - 1) / S::kRows;

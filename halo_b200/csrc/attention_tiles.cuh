@@ -818,7 +818,6 @@ int launch_tiles_kernel(HaloCudaCtx* ctx, const AttentionCall& c, Work w, cudaSt
     w.rows = S::kRows;
     w.tile = S::kTile;
     w.pad = 3;
-    w.least = 1;
     w.group = c.group;
     w.group_inverse = static_cast<uint32_t>((0xFFFFFFFFull + c.group) / c.group);
     w.row_tiles = (w.max_rows + S::kRows - 1) / S::kRows;

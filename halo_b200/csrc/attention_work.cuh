@@ -18,7 +18,6 @@ namespace attn {
 struct Work {  // what every kernel of a call is told besides the call
     uint32_t rows, tile;          // packed rows of a unit, keys of a tile
     uint32_t pad;                 // what a unit costs besides its tiles, in tiles
-    uint32_t least;               // positions of a CTA, where a call has few
     uint32_t group, group_inverse;  // query heads of a kv head; ceil(2^32 / group)
     uint32_t row_tiles;           // of the longest sequence at most
     uint32_t lanes;               // of a warp that look at one sequence when the tiles are counted: a power of two
@@ -111,8 +110,7 @@ struct PlanSmem {
 __device__ __forceinline__ bool cut_range(const Work& w, uint64_t total, Range* out) {
     out->total = total;
     if (total == 0) return false;
-    // where a call has few tiles, a share of a unit has at least `least`: it costs its CTA, and the one that joins the shares, as much as a few
-    const uint32_t ctas = static_cast<uint32_t>(min(uint64_t{gridDim.x}, max(quotient(total, w.least), uint64_t{1})));
+    const uint32_t ctas = static_cast<uint32_t>(min(uint64_t{gridDim.x}, total));
     if (blockIdx.x >= ctas) return false;
     out->ctas = ctas;
     out->pad = w.pad;
