@@ -97,15 +97,16 @@ __device__ __forceinline__ bool drop_nan(uint32_t& w) {
 /// Writes NaN over the results of rows that see a token whose value is NaN there: the walk left those codes out in tiles that some rows do not see
 /// whole, where a product with weight zero would have spread them.  `at(row, d)` is the result's address.
 template <class At>
-__device__ void spread_nan(const AttentionCall& c, const Work& w, const Unit& u, const Segment& g, uint32_t thread0, uint32_t threads, At&& at) {
-    const uint32_t rows = u.rows(w), r0 = u.row0(w), dim = c.cache.head_dim;
+__device__ void spread_nan(const AttentionCall& c, const Work& w, const Unit& u, const Segment& g, uint32_t first_row, uint32_t end_row, uint32_t first_dim, uint32_t end_dim,
+                           uint32_t dim_step, At&& at) {
+    const uint32_t r0 = u.row0(w);
     for (int32_t t = g.lo * static_cast<int32_t>(w.tile); t < min(g.hi * static_cast<int32_t>(w.tile), u.s.length); ++t) {
         const int32_t page = page_of(c.cache, u.seq, t >> c.cache.page_shift);
         if (static_cast<uint32_t>(page) >= c.cache.n_pages) continue;
-        const uint8_t* v = c.cache.v + page * c.cache.page_stride + (uint64_t{u.head} * c.cache.page_tokens + (t & (c.cache.page_tokens - 1))) * dim;
-        for (uint32_t d = threadIdx.x - thread0; d < dim; d += threads) {
+        const uint8_t* v = c.cache.v + page * c.cache.page_stride + (uint64_t{u.head} * c.cache.page_tokens + (t & (c.cache.page_tokens - 1))) * c.cache.head_dim;
+        for (uint32_t d = first_dim; d < end_dim; d += dim_step) {
             if ((v[d] & 127) != 127) continue;
-            for (uint32_t r = 0; r < rows; ++r) {
+            for (uint32_t r = first_row; r < end_row; ++r) {
                 const uint32_t j = (r0 + r) / c.group;
                 if (t >= first_key(u.s, w.window, j) && t < end_key(u.s, c.causal, j)) at(r, d);
             }
@@ -113,9 +114,37 @@ __device__ void spread_nan(const AttentionCall& c, const Work& w, const Unit& u,
     }
 }
 
+template <class T, int D, int SHARES, int AHEAD, class Slot, class Weight, class Add, class Put>
+__device__ __forceinline__ void join_few(uint32_t pieces, uint32_t thread, uint32_t threads, const Work& w, Slot& slot, Weight& weight, Add& add, Put& put, const float2* row_ml) {
+#pragma unroll 1
+    for (uint32_t i = thread; i < pieces; i += AHEAD * threads) {
+        float f[AHEAD][SHARES];
+        float4 x[AHEAD][SHARES];
+#pragma unroll
+        for (uint32_t h = 0; h < AHEAD; ++h)
+#pragma unroll
+            for (uint32_t k = 0; k < SHARES; ++k) {
+                const uint32_t at = min(i + h * threads, pieces - 1), r = at / (D / 4);
+                f[h][k] = __ldcg(slot(k) + w.rows * D + 2 * r);
+                x[h][k] = __ldcg(reinterpret_cast<const float4*>(slot(k) + at * 4));
+            }
+#pragma unroll
+        for (uint32_t h = 0; h < AHEAD; ++h) {
+            const uint32_t at = i + h * threads;
+            if (at >= pieces) break;
+            const uint32_t r = at / (D / 4);
+            float4 o = make_float4(0, 0, 0, 0);
+#pragma unroll
+            for (uint32_t k = 0; k < SHARES; ++k) add(o, weight(k, f[h][k], row_ml[r].x), x[h][k]);
+            put(r, at % (D / 4) * 4, o);
+        }
+    }
+}
+
 /// Joins the shares of a unit in CTA order and stores its rows.  All `warps` of the caller, from warp0 on, take part; `row_ml` has room for every row's
-/// (maximum, 1 / sum).
-template <class T, int D>
+/// (maximum, 1 / sum).  FEW, AHEAD: up to FEW shares, loads of AHEAD pieces of a row are under way together (a caller whose walk has the registers to
+/// spare: 4 pieces, 8 of up to two shares, for 7 prompts of 360 - 1570 tokens 10 us of 250).
+template <class T, int D, int AHEAD>
 __device__ __forceinline__ void join_partials(const AttentionCall& c, const Work& w, const Walk& walk, uint32_t c0, uint32_t shares, uint32_t warp0, uint32_t warps, float2* row_ml) {
     const uint32_t thread = threadIdx.x - warp0 * 32, threads = warps * 32, lane = thread % 32, rows = walk.rows;
     auto slot = [&](uint32_t k) { return partial_slot(w, D, c0 + min(k, shares - 1), k == 0); };
@@ -174,30 +203,9 @@ __device__ __forceinline__ void join_partials(const AttentionCall& c, const Work
         out[0] = from_f32<T>(o.x * inv), out[1] = from_f32<T>(o.y * inv), out[2] = from_f32<T>(o.z * inv), out[3] = from_f32<T>(o.w * inv);
     };
     const uint32_t pieces = rows * (D / 4);
-    if (shares <= 4) {  // loads of two pieces under way together
-#pragma unroll 1
-        for (uint32_t i = thread; i < pieces; i += 2 * threads) {
-            float f[2][4];
-            float4 x[2][4];
-#pragma unroll
-            for (uint32_t h = 0; h < 2; ++h)
-#pragma unroll
-                for (uint32_t k = 0; k < 4; ++k) {
-                    const uint32_t at = min(i + h * threads, pieces - 1), r = at / (D / 4);
-                    f[h][k] = __ldcg(slot(k) + w.rows * D + 2 * r);
-                    x[h][k] = __ldcg(reinterpret_cast<const float4*>(slot(k) + at * 4));
-                }
-#pragma unroll
-            for (uint32_t h = 0; h < 2; ++h) {
-                const uint32_t at = i + h * threads;
-                if (at >= pieces) break;
-                const uint32_t r = at / (D / 4);
-                float4 o = make_float4(0, 0, 0, 0);
-#pragma unroll
-                for (uint32_t k = 0; k < 4; ++k) add(o, weight(k, f[h][k], row_ml[r].x), x[h][k]);
-                put(r, at % (D / 4) * 4, o);
-            }
-        }
+    if (AHEAD > 2 && shares <= 2) join_few<T, D, 2, 2 * AHEAD>(pieces, thread, threads, w, slot, weight, add, put, row_ml);
+    else if (shares <= 4) {
+        join_few<T, D, 4, AHEAD>(pieces, thread, threads, w, slot, weight, add, put, row_ml);
     } else {  // of a piece's next ten shares
         constexpr uint32_t kAhead = 10;
 #pragma unroll 1
@@ -704,7 +712,7 @@ __global__ void __launch_bounds__(RowsShape<D, TS, TILE, CPS, sizeof(T) == 4 ? 2
         }
         bar_sync(1, kConsumers);
         if (nan_seen != 0) {
-            spread_nan(c, w, walk.u, walk.g, 0, kConsumers, [&](uint32_t r, uint32_t d) {
+            spread_nan(c, w, walk.u, walk.g, 0, walk.u.rows(w), threadIdx.x, c.cache.head_dim, kConsumers, [&](uint32_t r, uint32_t d) {
                 if (slot == nullptr) out_at(r)[d] = from_f32<T>(NAN);
                 else slot[r * D + d] = NAN;
             });
@@ -724,7 +732,7 @@ __global__ void __launch_bounds__(RowsShape<D, TS, TILE, CPS, sizeof(T) == 4 ? 2
             bar_sync(1, kConsumers);
             if (is_last != 0) {
                 __threadfence();
-                join_partials<T, D>(c, w, walk, c0, shares, 0, S::kWarps, joined_ml);
+                join_partials<T, D, 2>(c, w, walk, c0, shares, 0, S::kWarps, joined_ml);
             }
         }
         bar_sync(1, kConsumers);  // nobody reads q, the joined rows or `walk` any more

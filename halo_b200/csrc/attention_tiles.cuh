@@ -43,6 +43,10 @@ struct TilesShape {
     static constexpr uint32_t kSettle = TERMS == 2 ? 64 / (kTile / 8) : 0;
     static constexpr int kHalves = 2 / kStreams;           // softmax warpgroups that share a row tile's keys
     static constexpr int kKeys = kTile / kHalves;          // of a tile that one of them has
+    /// Column of a score buffer that the weights of a tile's 16 keys from 16 * i on begin at: a warpgroup's lie where its scores were.
+    static constexpr uint32_t weights_at(uint32_t term, uint32_t i) {
+        return TERMS == 2 ? term * (kTile / 2) + i * 8 : i / (kKeys / 16) * kKeys + i % (kKeys / 16) * 8;
+    }
     static constexpr int kConvWarps = D == 256 ? 8 : 4, kSoftWarp = 4 + kConvWarps, kSoftWarps = 8, kThreads = (kSoftWarp + kSoftWarps) * 32;
     // Slot number i of a CTA (the parts of K of its first tile, those of V, those of K of the second, ...) has place i % kSlots.  A place's user waits for
     // its last use by the parity of that use, so all of a place's uses are to be one warp's: 2 * kParts * kEvery of convert_slots divides kSlots.
@@ -214,7 +218,7 @@ __device__ __forceinline__ void convert_slots(const AttentionCall& c, const Work
     };
     uint4 x[kAhead];
     constexpr uint32_t kLot = kAhead / 2;  // accesses that are converted, and asked for, together
-    auto load = [&](uint32_t lot) __attribute__((always_inline)) {  // accesses lot * kLot .. of the tile that is loaded
+    auto load = [&](uint32_t lot, uint32_t p) __attribute__((always_inline)) {  // accesses lot * kLot .. of the tile that is loaded; lot % 2 == p
         constexpr uint32_t kFirst = IS_V ? kRows / 16 : 0;  // groups of a part of V
         if (plain) {
             constexpr uint32_t kSpan = kLot > kPerGroup ? kLot / kPerGroup : 1, kIn = kLot / kSpan;  // groups of a lot; accesses of each
@@ -223,11 +227,11 @@ __device__ __forceinline__ void convert_slots(const AttentionCall& c, const Work
                 const uint32_t i0 = lot * kLot + n * kIn;
                 const uint8_t* src = pool + __shfl_sync(0xFFFFFFFFu, group_at, i0 / kPerGroup + part * kFirst);
 #pragma unroll
-                for (uint32_t j = 0; j < kIn; ++j) x[(i0 + j) % kAhead] = __ldg(reinterpret_cast<const uint4*>(src + (i0 + j) % kPerGroup * kStep * D));
+                for (uint32_t j = 0; j < kIn; ++j) x[p * kLot + n * kIn + j] = __ldg(reinterpret_cast<const uint4*>(src + (i0 + j) % kPerGroup * kStep * D));
             }
         } else {
 #pragma unroll
-            for (uint32_t j = 0; j < kLot; ++j) x[(lot * kLot + j) % kAhead] = make_uint4(0, 0, 0, 0);
+            for (uint32_t j = 0; j < kLot; ++j) x[p * kLot + j] = make_uint4(0, 0, 0, 0);
 #pragma unroll 1
             for (uint32_t g = lot * kLot / kPerGroup; g <= (lot * kLot + kLot - 1) / kPerGroup; ++g) {
                 const uint32_t group = g + (IS_V ? part * (kRows / 16) : 0);
@@ -237,14 +241,14 @@ __device__ __forceinline__ void convert_slots(const AttentionCall& c, const Work
                 for (uint32_t j = 0; j < kLot; ++j) {
                     const uint32_t i = lot * kLot + j, k = i % kPerGroup * kStep;
                     const int32_t t = tile * kTile + static_cast<int32_t>(group * 16 + k + lane_row);
-                    if (i / kPerGroup == g && there && t >= any_lo && t < any_hi) x[i % kAhead] = __ldg(reinterpret_cast<const uint4*>(from_group + k * D));
+                    if (i / kPerGroup == g && there && t >= any_lo && t < any_hi) x[p * kLot + j] = __ldg(reinterpret_cast<const uint4*>(from_group + k * D));
                 }
             }
         }
     };
     if (!enter(turn)) return;
-    load(0);
-    load(1);
+    load(0, 0);
+    load(1, 1);
     const float scale = fabsf(c.scale) * 1.4426950408889634f;  // its sign is q's
     for (bool more = true; more;) {
         const uint32_t number = (2 * count + (IS_V ? 1 : 0)) * S::kParts + part, at = number % S::kSlots, slot = ring + at * S::kSlot;
@@ -258,28 +262,32 @@ __device__ __forceinline__ void convert_slots(const AttentionCall& c, const Work
             s.inv_v = page >= 0 ? exp2_int(-v) : 0.0f;
             if (page == -2 && c.status != nullptr) atomicOr(c.status, 8u);  // kStatusBadIndex
         }
+        // two lots' worth of code for all: unrolled, the warps waited for instructions (2048 tokens behind 28000, heads of 256: 1520 us, so 1440)
+#pragma unroll 1
+        for (uint32_t o = 0; o < kAccesses / kAhead; ++o) {
+            const bool last_ones = o + 1 == kAccesses / kAhead;  // behind them the next tile is loaded
 #pragma unroll
-        for (uint32_t lot = 0; lot < kAccesses / kLot; ++lot) {
-            if (check) {  // a weight of zero would spread a NaN to rows that do not see it
-                bool nan = false;
+            for (uint32_t p = 0; p < 2; ++p) {
+                const uint32_t lot = 2 * o + p;
+                if (check) {  // a weight of zero would spread a NaN to rows that do not see it
+                    bool nan = false;
+#pragma unroll
+                    for (uint32_t j = 0; j < kLot; ++j) {
+                        uint4& v = x[p * kLot + j];
+                        nan |= drop_nan(v.x) | drop_nan(v.y) | drop_nan(v.z) | drop_nan(v.w);
+                    }
+                    if (nan) *nan_seen = 1;
+                }
 #pragma unroll
                 for (uint32_t j = 0; j < kLot; ++j) {
-                    uint4& v = x[(lot * kLot + j) % kAhead];
-                    nan |= drop_nan(v.x) | drop_nan(v.y) | drop_nan(v.z) | drop_nan(v.w);
+                    const uint32_t row = (lot * kLot + j) * kStep, to_row = (slot + to + row * 128) ^ ((row & 7) << 4);
+                    const uint4 v = x[p * kLot + j];
+                    sts128(to_row, widen_lo(v.x), widen_hi(v.x), widen_lo(v.y), widen_hi(v.y));
+                    sts128(to_row ^ 16, widen_lo(v.z), widen_hi(v.z), widen_lo(v.w), widen_hi(v.w));
                 }
-                if (nan) *nan_seen = 1;
+                if (p == 0 && last_ones) more = advance();
+                if (!last_ones || more) load(last_ones ? p : lot + 2, p);
             }
-#pragma unroll
-            for (uint32_t j = 0; j < kLot; ++j) {
-                const uint32_t i = lot * kLot + j, row = i * kStep, to_row = (slot + to + row * 128) ^ ((row & 7) << 4);
-                const uint4 v = x[i % kAhead];
-                sts128(to_row, widen_lo(v.x), widen_hi(v.x), widen_lo(v.y), widen_hi(v.y));
-                sts128(to_row ^ 16, widen_lo(v.z), widen_hi(v.z), widen_lo(v.w), widen_hi(v.w));
-            }
-            constexpr uint32_t kTurn = (kAccesses - kAhead) / kLot;  // from this lot on the next tile is loaded
-            if (lot == kTurn) more = advance();
-            if (lot < kTurn) load(lot + 2);
-            else if (more) load(lot - kTurn);
         }
         proxy_fence();
         __syncwarp();
@@ -302,7 +310,7 @@ __global__ void __launch_bounds__(TilesShape<D, sizeof(T) == 4 ? 2 : 1>::kThread
     __shared__ float shared_top[2][S::kHalves][128];  // of a tile and the next: the maxima that a row tile's warpgroups tell each other
     __shared__ uint32_t nan_seen, is_last, tmem_word;
     __shared__ Cursor cursors[S::kConvWarps];
-    __shared__ Walk walks[2];  // the segment at hand and the next one, in turn
+    __shared__ Walk walks[2];  // of a segment and the next, in turn: from the warps that stage q
 
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
@@ -330,9 +338,7 @@ __global__ void __launch_bounds__(TilesShape<D, sizeof(T) == 4 ? 2 : 1>::kThread
         if (!find_range(c, w, plan, &range)) return;
         if (threadIdx.x == 0) {
             walks[0].range = range;
-            walks[0].u = range.unit;
-            walks[0].enter(c, w, range.unit_begin);
-            for (Cursor& x : cursors) x = Cursor{range.unit, walks[0].g};
+            for (Cursor& x : cursors) x = Cursor{range.unit, segment(range, range.unit, range.unit_begin)};
         }
     }
     if (warp == 1) {
@@ -348,7 +354,7 @@ __global__ void __launch_bounds__(TilesShape<D, sizeof(T) == 4 ? 2 : 1>::kThread
         if (alive) alive = __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity));
     };
     const Range range = walks[0].range;
-    __syncthreads();  // `walks` belong to the softmax warps from here
+    __syncthreads();  // `walks` belong to the warps that stage q from here
 
     if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::kIdleRegs));
     if (warp == 0) {
@@ -392,12 +398,17 @@ __global__ void __launch_bounds__(TilesShape<D, sizeof(T) == 4 ? 2 : 1>::kThread
                     for (uint32_t term = 0; term < TERMS; ++term)
 #pragma unroll
                         for (uint32_t k = 0; k < kSteps; ++k)
-                            mma_ts(tmem + S::kO + s * D, tmem + buffer * S::kBuffer + term * (kTile / 2) + (part * kSteps + k) * 8, v + k * 128, kRowsOut,
+                            mma_ts(tmem + S::kO + s * D, tmem + buffer * S::kBuffer + S::weights_at(term, part * kSteps + k), v + k * 128, kRowsOut,
                                    part + term + k != 0 ? 1u : first);
                     if (s == kStreams - 1) mma_commit(empty + 8 * (place + part));
                     if (part == kParts - 1) mma_commit(pv_done + 8 * buffer);
                 }
             }
+        };
+        // Behind the segment's last scores the next one's q may be written, while the last weights are still to come.  Not before weights of this segment
+        // were there, though: all softmax warps are past their look at q_ready then, and it can go on by a phase.
+        auto release_q = [&] {
+            if (elect_one()) mma_commit(q_free);
         };
         for (;;) {
             const Segment g = segment(range, u, unit_begin);
@@ -412,16 +423,18 @@ __global__ void __launch_bounds__(TilesShape<D, sizeof(T) == 4 ? 2 : 1>::kThread
                     for (uint32_t s = 0; s < kStreams; ++s) {
                         rows(count + t, s, s, t != 0);
                         if (t + 1 < n) scores(count + t + 1, s, s);
+                        if (s == kStreams - 1 && t + 2 == n) release_q();
                     }
                 } else {
                     const uint32_t buffer = __shfl_sync(0xFFFFFFFFu, t & 1, 0);
                     rows(count + t, 0, buffer, TERMS == 2 ? t % S::kSettle != 0 : t != 0);
                     if (t + 2 < n) scores(count + t + 2, 0, buffer);
+                    if (t + 3 == n) release_q();
                 }
             }
             count += n;
             ++segments;
-            if (elect_one()) mma_commit(q_free);
+            if (n < 4 - kStreams) release_q();
             unit_begin = g.unit_end;
             if (!range.reaches(unit_begin) || !next_unit(c, w, u)) break;
         }
@@ -430,46 +443,72 @@ __global__ void __launch_bounds__(TilesShape<D, sizeof(T) == 4 ? 2 : 1>::kThread
             mbar_wait(idle, 0);
         }
     } else if (warp < 4) {
-        // ---- q: eight lanes to a row, four rows of a warp at a time, the next four rows' loads under way --------------------------------------------
-        constexpr uint32_t E = D / 8, kVecs = E * sizeof(T) / 16, kWarps = 3, kStride = 4 * kWarps, kLoads = TERMS == 2 ? 1 : 2;
+        // ---- q: eight lanes to a row.  The operand's bits take as much room as the fp16 terms that they become: all rows are copied to where their terms
+        // go, so that their latency shows once, and converted in place, every lane what it has copied. ------------------------------------------------------
+        constexpr uint32_t kPieces = D / 64, kWords = 4 * TERMS, kStride = 12;  // pieces of 8 elements of a lane, 64 elements apart; rows of the three warps
         const uint32_t l8 = lane % 8, first = (warp - 1) * 4 + lane / 8;
         Unit u = range.unit;
         uint64_t unit_begin = range.unit_begin;
         for (uint32_t segments = 0;; ++segments) {
             const Segment g = segment(range, u, unit_begin);
             const uint32_t rows = u.rows(w), r0 = u.row0(w), token0 = r0 / c.group, behind = r0 - token0 * c.group;
-            const uint8_t* base = c.q.p + uint64_t{u.s.row0 + token0} * c.q.token_stride + uint64_t{u.head} * c.group * c.q.head_stride + l8 * (E * sizeof(T));
-            auto load = [&](uint32_t row, uint4 (&v)[kVecs]) {
-                const uint32_t p = behind + min(row, rows - 1), t = w.group == 1 ? p : __umulhi(p, w.group_inverse);
-                const uint8_t* q = base + t * c.q.token_stride + (p - t * w.group) * c.q.head_stride;
+            Unit next = u;
+            const bool more = range.reaches(g.unit_end) && next_unit(c, w, next);
+            const uint8_t* base = c.q.p + uint64_t{u.s.row0 + token0} * c.q.token_stride + uint64_t{u.head} * c.group * c.q.head_stride + l8 * (8 * sizeof(T));
+            auto source = [&](uint32_t row) {
+                const uint32_t p = behind + row, t = w.group == 1 ? p : __umulhi(p, w.group_inverse);
+                return base + t * c.q.token_stride + (p - t * w.group) * c.q.head_stride;
+            };
+            auto place = [&](uint32_t row) {  // 64-element blocks of [128 rows][128 bytes]; a second term's are behind the first's
+                return q_at + row / 128 * (kParts * 16384) + row % 128 * 128 + ((l8 ^ (row & 7)) << 4);
+            };
+            for (uint32_t row = first; row < rows; row += kStride) {
+                const uint8_t* q = source(row);
+#pragma unroll
+                for (uint32_t k = 0; k < kPieces; ++k) asm volatile("prefetch.global.L2 [%0];" ::"l"(q + k * (64 * sizeof(T))));
+            }
+            if (segments != 0) wait(q_free, (segments - 1) & 1);  // the segment before has its last scores, and the softmax is not behind it
+            if (warp == 1 && lane == 0) {
+                Walk& walk = walks[segments & 1];
+                walk.u = u, walk.g = g, walk.rows = rows, walk.r0 = r0, walk.token0 = token0, walk.behind = behind, walk.more = more;
+            }
+#pragma unroll 1
+            for (uint32_t row = first; row < rows; row += kStride) {
+                const uint8_t* q = source(row);
+                const uint32_t to = place(row);
                 if (c.q.vec) {
 #pragma unroll
-                    for (uint32_t k = 0; k < kVecs; ++k) v[k] = __ldg(reinterpret_cast<const uint4*>(q) + k);
+                    for (uint32_t k = 0; k < kPieces * TERMS; ++k)
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + (k / TERMS + k % TERMS * kParts) * 16384), "l"(q + k / TERMS * (64 * sizeof(T)) + k % TERMS * 16) : "memory");
                 } else {
-#pragma unroll
-                    for (uint32_t k = 0; k < kVecs; ++k) {
+#pragma unroll 1
+                    for (uint32_t k = 0; k < kPieces * TERMS; ++k) {
+                        const uint8_t* from = q + k / TERMS * (64 * sizeof(T)) + k % TERMS * 16;
                         uint32_t x[4];
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            if constexpr (TERMS == 2) {
-                                x[e] = reinterpret_cast<const uint32_t*>(q)[4 * k + e];
-                            } else {
-                                const uint16_t* at = reinterpret_cast<const uint16_t*>(q) + 8 * k + 2 * e;
-                                x[e] = at[0] | static_cast<uint32_t>(at[1]) << 16;
-                            }
+                            if constexpr (TERMS == 2) x[e] = reinterpret_cast<const uint32_t*>(from)[e];
+                            else x[e] = reinterpret_cast<const uint16_t*>(from)[2 * e] | static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(from)[2 * e + 1]) << 16;
                         }
-                        v[k] = make_uint4(x[0], x[1], x[2], x[3]);
+                        sts128(to + (k / TERMS + k % TERMS * kParts) * 16384, x[0], x[1], x[2], x[3]);
                     }
                 }
-            };
-            auto store = [&](uint32_t row, const uint4 (&v)[kVecs]) {
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+#pragma unroll 2
+            for (uint32_t row = first; row - first % 4 < rows; row += kStride) {  // all of a warp's rows or none
+                const uint32_t at = place(min(row, static_cast<uint32_t>(S::kRows) - 1));
+                uint32_t word[kPieces * kWords];
+#pragma unroll
+                for (uint32_t k = 0; k < kPieces * TERMS; ++k) {
+                    const uint4 v = lds128(at + (k / TERMS + k % TERMS * kParts) * 16384);
+                    word[4 * k] = v.x, word[4 * k + 1] = v.y, word[4 * k + 2] = v.z, word[4 * k + 3] = v.w;
+                }
                 // the largest finite magnitude: as integers the magnitudes of every type have their order, infinities and NaN above
-                uint32_t word[4 * kVecs], top = 0;
-                __builtin_memcpy(word, v, sizeof word);
-                int32_t exponent;
+                uint32_t top = 0;
                 if constexpr (TERMS == 2) {
 #pragma unroll
-                    for (uint32_t k = 0; k < 4 * kVecs; ++k) {
+                    for (uint32_t k = 0; k < kPieces * kWords; ++k) {
                         const uint32_t m = word[k] & 0x7FFFFFFFu;
                         top = max(top, m < 0x7F800000u ? m : 0u);
                     }
@@ -477,12 +516,12 @@ __global__ void __launch_bounds__(TilesShape<D, sizeof(T) == 4 ? 2 : 1>::kThread
                     constexpr uint32_t kInf = std::is_same_v<T, __half> ? 0x7C00u : 0x7F80u;
                     uint32_t top2 = 0;
 #pragma unroll
-                    for (uint32_t k = 0; k < 4 * kVecs; ++k) top2 = __vmaxu2(top2, word[k] & 0x7FFF7FFFu);
+                    for (uint32_t k = 0; k < kPieces * kWords; ++k) top2 = __vmaxu2(top2, word[k] & 0x7FFF7FFFu);
                     top = max(top2 & 0xFFFFu, top2 >> 16);
                     if (top >= kInf) {  // leave them out
                         top = 0;
 #pragma unroll
-                        for (uint32_t k = 0; k < 4 * kVecs; ++k) {
+                        for (uint32_t k = 0; k < kPieces * kWords; ++k) {
                             const uint32_t lo = word[k] & 0x7FFFu, hi = word[k] >> 16 & 0x7FFFu;
                             top = max(top, max(lo < kInf ? lo : 0u, hi < kInf ? hi : 0u));
                         }
@@ -490,6 +529,7 @@ __global__ void __launch_bounds__(TilesShape<D, sizeof(T) == 4 ? 2 : 1>::kThread
                 }
 #pragma unroll
                 for (int d = 4; d != 0; d /= 2) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+                int32_t exponent;
                 if constexpr (TERMS == 2) {
                     exponent = static_cast<int32_t>(top >> 23) - 127;
                 } else {
@@ -498,13 +538,12 @@ __global__ void __launch_bounds__(TilesShape<D, sizeof(T) == 4 ? 2 : 1>::kThread
                     __builtin_memcpy(&largest, &top16, 2);
                     exponent = static_cast<int32_t>(__float_as_uint(to_f32(largest)) >> 23) - 127;
                 }
-                exponent = row < rows ? max(exponent, -100) : 0;
-                const float by = row >= rows ? 0.0f : c.scale < 0 ? -exp2_int(14 - exponent) : exp2_int(14 - exponent);
-                if (row >= static_cast<uint32_t>(S::kRows)) return;
+                if (row >= rows) continue;
+                exponent = max(exponent, -100);
+                const float by = c.scale < 0 ? -exp2_int(14 - exponent) : exp2_int(14 - exponent);
                 if (l8 == 0) q_unscale[segments & 1][row] = exp2_int(exponent - 14);
-                const uint32_t in_tile = row % 128;
 #pragma unroll
-                for (uint32_t k = 0; k < E / 8; ++k) {
+                for (uint32_t k = 0; k < kPieces; ++k) {
                     uint32_t h[4], rest[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
@@ -519,30 +558,15 @@ __global__ void __launch_bounds__(TilesShape<D, sizeof(T) == 4 ? 2 : 1>::kThread
                         h[e] = half2_bits(p, q);
                         if constexpr (TERMS == 2) rest[e] = half2_rest(p, q, h[e]);
                     }
-                    const uint32_t d = l8 * E + 8 * k;  // 64-element blocks of [128 rows][128 bytes]
-                    const uint32_t at = q_at + (row / 128 * kParts + d / 64) * 16384 + in_tile * 128 + ((d % 64 / 8 ^ (in_tile & 7)) << 4);
-                    sts128(at, h[0], h[1], h[2], h[3]);
-                    if constexpr (TERMS == 2) sts128(at + kParts * 16384, rest[0], rest[1], rest[2], rest[3]);
-                }
-            };
-            uint4 v[kLoads][kVecs];
-#pragma unroll
-            for (uint32_t i = 0; i < kLoads; ++i) load(first + i * kStride, v[i]);
-            if (segments != 0) wait(q_free, (segments - 1) & 1);  // the segment before has its last scores
-#pragma unroll 1
-            for (uint32_t at = 0; at < rows; at += kLoads * kStride) {  // what lies behind the last row is never kept
-#pragma unroll
-                for (uint32_t i = 0; i < kLoads; ++i) {
-                    const uint32_t row = at + first + i * kStride;
-                    store(row, v[i]);
-                    load(row + kLoads * kStride, v[i]);
+                    sts128(at + k * 16384, h[0], h[1], h[2], h[3]);
+                    if constexpr (TERMS == 2) sts128(at + (k + kParts) * 16384, rest[0], rest[1], rest[2], rest[3]);
                 }
             }
             proxy_fence();
             __syncwarp();
             if (lane == 0) mbar_arrive(q_ready);
-            unit_begin = g.unit_end;
-            if (!range.reaches(unit_begin) || !next_unit(c, w, u)) break;
+            if (!more) break;
+            u = next, unit_begin = g.unit_end;
         }
     } else if (warp >= 4 && warp < S::kSoftWarp) {
         // ---- conversion ------------------------------------------------------------------------------------------------------------------
@@ -562,15 +586,10 @@ __global__ void __launch_bounds__(TilesShape<D, sizeof(T) == 4 ? 2 : 1>::kThread
         const uint32_t lanes = quarter * 32 << 16, o_at = tmem + lanes + S::kO + stream * D;
         uint32_t uses[2] = {0, 0}, tiles = 0;
         const bool leader = threadIdx.x == S::kSoftWarp * 32;
-        uint32_t segments = 0;
-        for (uint32_t turn = 0;; turn ^= 1) {
-            const Walk& walk = walks[turn];
-            if (leader) {
-                walks[turn ^ 1] = walk;
-                walks[turn ^ 1].advance(c, w);
-            }
+        for (uint32_t segments = 0;; ++segments) {
+            const Walk& walk = walks[segments & 1];
             wait(q_ready, segments & 1);
-            const float qs = q_unscale[segments++ & 1][r];
+            const float qs = q_unscale[segments & 1][r];
             const uint32_t j = walk.token(w, min(r, walk.rows - 1));
             const int32_t lo = first_key(walk.u.s, w.window, j), hi = end_key(walk.u.s, c.causal, j);
             // keys that every row of this row tile sees (a tile without rows: of its last row's; nothing of it is kept)
@@ -621,30 +640,42 @@ __global__ void __launch_bounds__(TilesShape<D, sizeof(T) == 4 ? 2 : 1>::kThread
                 const bool masked = t0 < all_lo || t0 + kTile > all_hi;
                 const uint32_t from = static_cast<uint32_t>(t0 - lo) + half * S::kKeys, seen = static_cast<uint32_t>(max(hi - lo, 0));  // key e of this thread's: from + e < seen
                 constexpr int kChunks = S::kKeys / 32;
-                uint32_t x[kChunks][32];
+                // The scores are read again for the weights, 32 at a time: a loop's worth of code for both passes, and of registers.  (Unrolled over 128 keys the
+                // warps waited for instructions: prompts of 360 - 1570 tokens 245 us, with 64 keys 232, with 32 215.)  Two terms of the weights take
+                // the room of scores that are still to be read: there the scores are held.
+                constexpr bool kHold = TERMS == 2;
+                constexpr int kUnrolled = kHold ? kChunks : 1;
+                uint32_t x[kHold ? kChunks : 1][32];
+                auto mask = [&](int q, uint32_t (&v)[32]) __attribute__((always_inline)) {
+                    const uint32_t at = from + static_cast<uint32_t>(32 * q);
+                    if (__all_sync(0xFFFFFFFFu, at < seen && seen - at >= 32u)) return;  // every row of the warp sees these keys
 #pragma unroll
-                for (int q = 0; q < kChunks; ++q) tmem_ld32(s_at + half * S::kKeys + 32 * q, x[q]);
-                tmem_wait_ld();
-                if (masked) {
+                    for (int e = 0; e < 32; ++e)
+                        if (at + static_cast<uint32_t>(e) >= seen) v[e] = 0xFF800000u;  // -inf
+                };
+                if (kHold) {
 #pragma unroll
-                    for (int q = 0; q < kChunks; ++q) {
-                        const uint32_t at = from + static_cast<uint32_t>(32 * q);
-                        if (__all_sync(0xFFFFFFFFu, at < seen && seen - at >= 32u)) continue;  // every row of the warp sees these keys
-#pragma unroll
-                        for (int e = 0; e < 32; ++e)
-                            if (at + static_cast<uint32_t>(e) >= seen) x[q][e] = 0xFF800000u;  // -inf
-                    }
+                    for (int q = 0; q < kChunks; ++q) tmem_ld32(s_at + half * S::kKeys + 32 * q, x[kHold ? q : 0]);
+                    tmem_wait_ld();
                 }
                 // Missing keys are zeros with log_v = -inf; the factor of a group's scores is not negative: the largest score is the largest exponent.
                 float top = -INFINITY;
+#pragma unroll kUnrolled
+                for (int q = 0; q < kChunks; ++q) {
+                    uint32_t (&v)[32] = x[kHold ? q : 0];
+                    if (!kHold) {
+                        tmem_ld32(s_at + half * S::kKeys + 32 * q, v);
+                        tmem_wait_ld();
+                    }
+                    if (masked) mask(q, v);
 #pragma unroll
-                for (int i = 0; i < 2 * kChunks; ++i) {
-                    const GroupScale s = sc[i];
-                    const uint32_t* v = &x[i / 2][i % 2 * 16];
-                    float m = fmaxf(__uint_as_float(v[0]), __uint_as_float(v[1]));
+                    for (int i = 0; i < 2; ++i) {
+                        const GroupScale s = sc[2 * q + i];
+                        float m = fmaxf(__uint_as_float(v[16 * i]), __uint_as_float(v[16 * i + 1]));
 #pragma unroll
-                    for (int e = 2; e < 16; e += 2) m = fmaxf(fmaxf(m, __uint_as_float(v[e])), __uint_as_float(v[e + 1]));
-                    top = fmaxf(top, m == -INFINITY ? m : fmaf(m, s.k * qs, s.log_v));
+                        for (int e = 2; e < 16; e += 2) m = fmaxf(fmaxf(m, __uint_as_float(v[16 * i + e])), __uint_as_float(v[16 * i + e + 1]));
+                        top = fmaxf(top, m == -INFINITY ? m : fmaf(m, s.k * qs, s.log_v));
+                    }
                 }
                 if constexpr (S::kHalves == 2) {  // the warp that has the other keys of these rows; both have read their scores behind this
                     shared_top[tiles & 1][half][r] = top;
@@ -683,9 +714,15 @@ __global__ void __launch_bounds__(TilesShape<D, sizeof(T) == 4 ? 2 : 1>::kThread
                     }
                 }
                 const float base = ref == -INFINITY ? 0.0f : ref - 6.0f;
-#pragma unroll
+#pragma unroll kUnrolled
                 for (int q = 0; q < kChunks; ++q) {
                     uint32_t weights[16], rest[16];
+                    uint32_t (&v)[32] = x[kHold ? q : 0];
+                    if (!kHold) {
+                        tmem_ld32(s_at + half * S::kKeys + 32 * q, v);
+                        tmem_wait_ld();
+                        if (masked) mask(q, v);
+                    }
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         const GroupScale s = sc[2 * q + i];
@@ -696,7 +733,7 @@ __global__ void __launch_bounds__(TilesShape<D, sizeof(T) == 4 ? 2 : 1>::kThread
 #pragma unroll
                         for (int e = 0; e < 16; e += 2) {
                             float y0, y1;
-                            unpair(fma_pair(pair(__uint_as_float(x[q][16 * i + e]), __uint_as_float(x[q][16 * i + e + 1])), by2, add2), y0, y1);
+                            unpair(fma_pair(pair(__uint_as_float(v[16 * i + e]), __uint_as_float(v[16 * i + e + 1])), by2, add2), y0, y1);
                             y0 = exp2_approx(y0), y1 = exp2_approx(y1);
                             sum = add_pair(sum, pair(y0, y1));
                             weights[8 * i + e / 2] = half2_bits(y0, y1);
@@ -706,7 +743,7 @@ __global__ void __launch_bounds__(TilesShape<D, sizeof(T) == 4 ? 2 : 1>::kThread
                         unpair(sum, s0, s1);
                         l = fmaf(s0 + s1, s.inv_v, l);
                     }
-                    tmem_st16(s_at + half * (S::kKeys / 2) + 16 * q, weights);  // (all scores have been read)
+                    tmem_st16(s_at + half * (TERMS == 2 ? S::kKeys / 2 : S::kKeys) + 16 * q, weights);  // over scores that have been read
                     if constexpr (TERMS == 2) tmem_st16(s_at + kTile / 2 + half * (S::kKeys / 2) + 16 * q, rest);
                 }
                 tmem_wait_st();
@@ -775,13 +812,14 @@ __global__ void __launch_bounds__(TilesShape<D, sizeof(T) == 4 ? 2 : 1>::kThread
                 *reinterpret_cast<float2*>(ml) = make_float2(ref, l);
             }
             tmem_before();
-            bar_sync(1, kSoft);
-            if (nan_seen != 0) {  // stays set: the conversion is ahead, and what it saw may belong to a segment to come
-                spread_nan(c, w, walk.u, walk.g, S::kSoftWarp * 32, kSoft, [&](uint32_t row, uint32_t d) {
+            // every warp for what it stored; a flag stays set: the conversion is ahead, and what it saw may belong to a segment to come
+            if (any_row && __any_sync(0xFFFFFFFFu, *static_cast<volatile uint32_t*>(&nan_seen) != 0)) {
+                __syncwarp();
+                const uint32_t top = stream * 128 + quarter * 32, dims = D / S::kHalves;
+                spread_nan(c, w, walk.u, walk.g, top, min(top + 32, walk.rows), half * dims + lane, (half + 1) * dims, 32, [&](uint32_t row, uint32_t d) {
                     if (walk.g.whole()) out_at(row)[d] = from_f32<T>(NAN);
                     else partial_slot(w, D, blockIdx.x, walk.g.from_start)[row * D + d] = NAN;
                 });
-                bar_sync(1, kSoft);
             }
             if (!walk.g.whole()) {
                 const uint32_t c0 = owner(walk.g.unit_begin, range.total, range.ctas), shares = owner(walk.g.unit_end - 1, range.total, range.ctas) - c0 + 1;
@@ -795,12 +833,11 @@ __global__ void __launch_bounds__(TilesShape<D, sizeof(T) == 4 ? 2 : 1>::kThread
                 bar_sync(1, kSoft);
                 if (is_last != 0) {
                     __threadfence();
-                    join_partials<T, D>(c, w, walk, c0, shares, S::kSoftWarp, S::kSoftWarps, joined_ml);
+                    join_partials<T, D, 4>(c, w, walk, c0, shares, S::kSoftWarp, S::kSoftWarps, joined_ml);
                 }
+                bar_sync(1, kSoft);  // nobody reads `is_last` or `joined_ml` any more
             }
-            const bool more = walks[turn ^ 1].more != 0;
-            bar_sync(1, kSoft);  // nobody reads `walk` any more
-            if (!more) break;
+            if (walk.more == 0) break;
         }
     }
     if (!alive && lane == 0) atomicOr(w.error_word, 1u);
