@@ -7,20 +7,23 @@
 // passes r by 8, so p_t is at most 2^14 and keeps 11 bits down to 2^-20 of the reference.
 //
 // Packed rows are the M side (a TMEM lane each), keys the N side of S = Q K^T, dims the N side of O = P V.  A CTA (one an SM) holds NS tiles of
-// 128 rows: two, each with scores, weights and accumulators of its own (128 + D columns), or one with two score buffers.  A step
-// is (tile of 128 keys, or of 64 for fp32 rows of 256 elements; row tile) and takes score buffer step % 2: while the softmax of one step runs, the tensor cores run the other's products.  The
-// weights overwrite the scores in TMEM as fp16 and are the A operand of P V from there.
+// 128 rows: two, each with scores, weights and accumulators of its own (128 + D columns), or one (D = 256, and fp32 operands) with two score
+// buffers.  A step is (tile of 128 keys, or of 64 for fp32 rows of 256 elements; row tile) and takes score buffer step % 2: while the softmax of one step
+// runs, the tensor cores run the other's products.  The weights overwrite the scores in TMEM as fp16 and are the A operand of P V from there.
 // Warps:
 //   0       tcgen05.mma issue
-//   1-3     q -> fp16 in shared memory, of the next segment while the last one's rows are stored (and TMEM's allocation)
+//   1-3     q -> fp16 in shared memory, of the next segment while the last one's last weights are made (and TMEM's allocation)
 //   4-7     conversion (4-11 where D is 256): each warp makes one part of K or V of every tile in a ring of eight 16 KiB slots (a K slot: 128 keys x
 //           64 dims; a V slot: 8192 / D keys x all dims, the N operand with dims contiguous); keys that no row of the CTA sees, missing pages and,
 //           in tiles that some row does not see whole, NaN codes of values become zeros (spread_nan puts the latter back)
 //   last 8  softmax, a thread to a row and a tile's keys, or to half of them where NS is 1; also the epilogue, and the joining of shares
 // Work is dealt as in attention_work.cuh, so a causal prompt's long and short rows and a short chunk behind a long context fill the device alike.
 //
-// What bounds it: the tensor pipe and, for D = 128, the exponentials (256 x 128 of them per 2048 clocks of products at 16 a clock); shared memory
-// carries 128 bytes a clock, of which the products' operands take about 96.
+// What bounds it.  For D = 128 256 rows x 128 keys are 2100 clocks of products, and as many of exponentials (16 a clock).  Prompts of 364 - 1568 tokens (76.6
+// GFLOP, 720 units) take 207 us, 370 TFLOP/s: the two row tiles' chains of scores, maximum, weights and products overlap only in part, and a unit's ends
+// (q, first scores, last rows) cost as much as two or three tiles.  Code size counts as much as instructions: the warps of an SM run five different loops,
+// and unrolled ones waited for instructions more than for anything else.  2048 tokens behind 28000 with D = 256 (1459 GFLOP) take 1430 us, 1020 TFLOP/s:
+// the tensor pipe is busy for 0.6 of it at that; the conversion of the codes, once for 128 rows, holds it up.
 #pragma once
 #include "attention_rows.cuh"
 
@@ -854,7 +857,7 @@ int launch_tiles_kernel(HaloCudaCtx* ctx, const AttentionCall& c, Work w, cudaSt
     using S = TilesShape<D, sizeof(T) == 4 ? 2 : 1>;
     w.rows = S::kRows;
     w.tile = S::kTile;
-    w.pad = 3;
+    w.pad = 3;  // prompts of 364 - 1568 tokens 245 us with 2 or 3, 309 with 1, and 1 % more with 5 than with 3
     w.group = c.group;
     w.group_inverse = static_cast<uint32_t>((0xFFFFFFFFull + c.group) / c.group);
     w.row_tiles = (w.max_rows + S::kRows - 1) / S::kRows;
