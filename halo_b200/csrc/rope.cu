@@ -4,7 +4,7 @@
 // 2^31 is as exact as that of position 1 (an fp32 product would be off by a tenth of a radian at a million).  Its leading 32 bits go through
 // sincospif, whose argument is then in [-1, 1).
 //
-// What bounds it: HBM, 2 * size bytes an element (8192 tokens of 40 heads of 128 in bf16, 168 MB, 39 us, 4.3 TB/s); for few tokens the launch.  A block takes a few tokens and a share of their heads: it computes the tokens' cosines and
+// What bounds it: HBM, 2 * size bytes an element (8192 tokens of 40 heads of 128 in bf16, 168 MB, 34 us, 4.9 TB/s); for few tokens the launch.  A block takes a few tokens and a share of their heads: it computes the tokens' cosines and
 // sines into shared memory while its first loads are under way; a thread has two units in flight, a unit being the 16-byte vectors of both halves of 16 / size
 // pairs (one vector where pairs are adjacent), or a vector to copy.
 #include "rope.h"
@@ -120,7 +120,7 @@ __global__ void __launch_bounds__(kThreads, 4) rope_kernel(const __grid_constant
 /// 32 / units-th of them, so that its factors stay in registers.  Lanes that share a unit share out its sines and cosines; nothing is waited for but loads.
 template <class T, int V, bool INTERLEAVED>
 __global__ void __launch_bounds__(kThreads, 4) rope_warp_kernel(const __grid_constant__ RopeArgs a) {
-    constexpr int kPairs = INTERLEAVED ? V / 2 : V, kAhead = 2;
+    constexpr int kPairs = INTERLEAVED ? V / 2 : V;
     using Word = Vec<T, V>;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
@@ -135,17 +135,14 @@ __global__ void __launch_bounds__(kThreads, 4) rope_warp_kernel(const __grid_con
         return x.p + uint64_t{t} * x.token_stride + uint64_t{is_q ? h : h - a.n_q} * x.head_stride;
     };
     const uint32_t first = INTERLEAVED ? u * 2 * kPairs : u * V, second = first + a.pairs;
-    Word x[kAhead], z[kAhead];
-    auto load = [&](uint32_t h) {
-#pragma unroll
-        for (uint32_t r = 0; r < kAhead; ++r) {
-            if (h + r * step >= h1) break;
-            const uint8_t* src = row(h + r * step, false);
-            x[r] = *reinterpret_cast<const Word*>(src + first * sizeof(T));
-            if constexpr (!INTERLEAVED) z[r] = *reinterpret_cast<const Word*>(src + second * sizeof(T));
-        }
+    Word x, z;
+    auto load = [&](uint32_t h, Word& x, Word& z) {
+        if (h >= h1) return;
+        const uint8_t* src = row(h, false);
+        x = *reinterpret_cast<const Word*>(src + first * sizeof(T));
+        if constexpr (!INTERLEAVED) z = *reinterpret_cast<const Word*>(src + second * sizeof(T));
     };
-    load(h0 + sub);
+    load(h0 + sub, x, z);
     const uint64_t position = static_cast<uint64_t>(static_cast<int64_t>(__ldg(a.positions + t)));
     float c[kPairs], s[kPairs];
     // pair p of the unit is made by the unit's lane p % step
@@ -166,22 +163,22 @@ __global__ void __launch_bounds__(kThreads, 4) rope_warp_kernel(const __grid_con
         cosine[p] = __shfl_sync(0xFFFFFFFFu, cm, from) * a.magnitude;
         sine[p] = __shfl_sync(0xFFFFFFFFu, sm, from) * a.magnitude;
     }
-    for (uint32_t h = h0 + sub; h - sub < h1; h += kAhead * step) {
-        if (h - sub != h0) load(h);
+    // the next head under way while one is turned (two heads at a time, each pair waited for: 39 us for 8192 tokens of 40 heads of 128 in bf16, so 34)
+    for (uint32_t h = h0 + sub; h < h1; h += step) {
+        Word next_x, next_z;
+        load(h + step, next_x, next_z);
+        uint8_t* dst = row(h, true);
 #pragma unroll
-        for (uint32_t r = 0; r < kAhead; ++r) {
-            if (h + r * step >= h1) break;
-            uint8_t* dst = row(h + r * step, true);
-#pragma unroll
-            for (int j = 0; j < kPairs; ++j) {
-                T &e0 = x[r].v[INTERLEAVED ? 2 * j : j], &e1 = INTERLEAVED ? x[r].v[2 * j + 1] : z[r].v[j];
-                const float p = to_f32(e0), q = to_f32(e1);
-                e0 = from_f32<T>(p * cosine[j] - q * sine[j]);
-                e1 = from_f32<T>(q * cosine[j] + p * sine[j]);
-            }
-            *reinterpret_cast<Word*>(dst + first * sizeof(T)) = x[r];
-            if constexpr (!INTERLEAVED) *reinterpret_cast<Word*>(dst + second * sizeof(T)) = z[r];
+        for (int j = 0; j < kPairs; ++j) {
+            T &e0 = x.v[INTERLEAVED ? 2 * j : j], &e1 = INTERLEAVED ? x.v[2 * j + 1] : z.v[j];
+            const float p = to_f32(e0), q = to_f32(e1);
+            e0 = from_f32<T>(p * cosine[j] - q * sine[j]);
+            e1 = from_f32<T>(q * cosine[j] + p * sine[j]);
         }
+        *reinterpret_cast<Word*>(dst + first * sizeof(T)) = x;
+        if constexpr (!INTERLEAVED) *reinterpret_cast<Word*>(dst + second * sizeof(T)) = z;
+        x = next_x;
+        if constexpr (!INTERLEAVED) z = next_z;
     }
     const uint32_t copies = a.units - a.turn_units;
     for (uint32_t i = lane; i < (h1 - h0) * copies; i += 32) {
