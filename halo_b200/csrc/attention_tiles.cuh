@@ -313,7 +313,7 @@ __global__ void __launch_bounds__(TilesShape<D, sizeof(T) == 4 ? 2 : 1>::kThread
     __shared__ float shared_top[2][S::kHalves][128];  // of a tile and the next: the maxima that a row tile's warpgroups tell each other
     __shared__ uint32_t nan_seen, is_last, tmem_word;
     __shared__ Cursor cursors[S::kConvWarps];
-    __shared__ Walk walks[2];  // of a segment and the next, in turn: from the warps that stage q
+    __shared__ Walk walks[2];  // the segment at hand and the next one, in turn
 
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
@@ -341,7 +341,9 @@ __global__ void __launch_bounds__(TilesShape<D, sizeof(T) == 4 ? 2 : 1>::kThread
         if (!find_range(c, w, plan, &range)) return;
         if (threadIdx.x == 0) {
             walks[0].range = range;
-            for (Cursor& x : cursors) x = Cursor{range.unit, segment(range, range.unit, range.unit_begin)};
+            walks[0].u = range.unit;
+            walks[0].enter(c, w, range.unit_begin);
+            for (Cursor& x : cursors) x = Cursor{range.unit, walks[0].g};
         }
     }
     if (warp == 1) {
@@ -357,7 +359,7 @@ __global__ void __launch_bounds__(TilesShape<D, sizeof(T) == 4 ? 2 : 1>::kThread
         if (alive) alive = __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity));
     };
     const Range range = walks[0].range;
-    __syncthreads();  // `walks` belong to the warps that stage q from here
+    __syncthreads();  // `walks` belong to the softmax warps from here
 
     if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::kIdleRegs));
     if (warp == 0) {
@@ -455,8 +457,6 @@ __global__ void __launch_bounds__(TilesShape<D, sizeof(T) == 4 ? 2 : 1>::kThread
         for (uint32_t segments = 0;; ++segments) {
             const Segment g = segment(range, u, unit_begin);
             const uint32_t rows = u.rows(w), r0 = u.row0(w), token0 = r0 / c.group, behind = r0 - token0 * c.group;
-            Unit next = u;
-            const bool more = range.reaches(g.unit_end) && next_unit(c, w, next);
             const uint8_t* base = c.q.p + uint64_t{u.s.row0 + token0} * c.q.token_stride + uint64_t{u.head} * c.group * c.q.head_stride + l8 * (8 * sizeof(T));
             auto source = [&](uint32_t row) {
                 const uint32_t p = behind + row, t = w.group == 1 ? p : __umulhi(p, w.group_inverse);
@@ -471,10 +471,6 @@ __global__ void __launch_bounds__(TilesShape<D, sizeof(T) == 4 ? 2 : 1>::kThread
                 for (uint32_t k = 0; k < kPieces; ++k) asm volatile("prefetch.global.L2 [%0];" ::"l"(q + k * (64 * sizeof(T))));
             }
             if (segments != 0) wait(q_free, (segments - 1) & 1);  // the segment before has its last scores, and the softmax is not behind it
-            if (warp == 1 && lane == 0) {
-                Walk& walk = walks[segments & 1];
-                walk.u = u, walk.g = g, walk.rows = rows, walk.r0 = r0, walk.token0 = token0, walk.behind = behind, walk.more = more;
-            }
 #pragma unroll 1
             for (uint32_t row = first; row < rows; row += kStride) {
                 const uint8_t* q = source(row);
@@ -568,8 +564,8 @@ __global__ void __launch_bounds__(TilesShape<D, sizeof(T) == 4 ? 2 : 1>::kThread
             proxy_fence();
             __syncwarp();
             if (lane == 0) mbar_arrive(q_ready);
-            if (!more) break;
-            u = next, unit_begin = g.unit_end;
+            unit_begin = g.unit_end;
+            if (!range.reaches(unit_begin) || !next_unit(c, w, u)) break;
         }
     } else if (warp >= 4 && warp < S::kSoftWarp) {
         // ---- conversion ------------------------------------------------------------------------------------------------------------------
@@ -590,7 +586,13 @@ __global__ void __launch_bounds__(TilesShape<D, sizeof(T) == 4 ? 2 : 1>::kThread
         uint32_t uses[2] = {0, 0}, tiles = 0;
         const bool leader = threadIdx.x == S::kSoftWarp * 32;
         for (uint32_t segments = 0;; ++segments) {
+            // The warps' way from segment to segment, and so the barriers that they meet at, follows from the lengths alone: also when a wait has run out.
             const Walk& walk = walks[segments & 1];
+            if (leader) {
+                Walk& next = walks[(segments & 1) ^ 1];
+                next = walk;
+                next.advance(c, w);
+            }
             wait(q_ready, segments & 1);
             const float qs = q_unscale[segments & 1][r];
             const uint32_t j = walk.token(w, min(r, walk.rows - 1));
@@ -838,9 +840,9 @@ __global__ void __launch_bounds__(TilesShape<D, sizeof(T) == 4 ? 2 : 1>::kThread
                     __threadfence();
                     join_partials<T, D, 4>(c, w, walk, c0, shares, S::kSoftWarp, S::kSoftWarps, joined_ml);
                 }
-                bar_sync(1, kSoft);  // nobody reads `is_last` or `joined_ml` any more
             }
-            if (walk.more == 0) break;
+            bar_sync(1, kSoft);  // nobody reads `walk`, `is_last` or `joined_ml` any more; the next walk is there
+            if (walks[(segments & 1) ^ 1].more == 0) break;
         }
     }
     if (!alive && lane == 0) atomicOr(w.error_word, 1u);
