@@ -365,7 +365,7 @@ __global__ void __launch_bounds__(RowsShape<D, TS, TILE, CPS, sizeof(T) == 4 ? 2
             if (!alive || !range.reaches(unit_begin) || !next_unit(c, w, u)) break;
         }
         if (!alive) {
-            if (lane == 0) atomicOr(w.error_word, 1u);
+            if (lane == 0) report_lost(w.error_word);
             // nothing may land in this CTA's shared memory once it is gone
             for (uint32_t i = 0; i < min(issued, static_cast<uint32_t>(S::kStages)); ++i) {
                 stage = stage == 0 ? S::kStages - 1 : stage - 1;
@@ -740,7 +740,7 @@ __global__ void __launch_bounds__(RowsShape<D, TS, TILE, CPS, sizeof(T) == 4 ? 2
         if (threadIdx.x == 0) walk.advance(c, w);
         bar_sync(1, kConsumers);
     } while (walk.more != 0);
-    if (!alive && lane == 0) atomicOr(w.error_word, 1u);
+    if (!alive && lane == 0) report_lost(w.error_word);
     __syncthreads();
 }
 

@@ -845,7 +845,7 @@ __global__ void __launch_bounds__(TilesShape<D, sizeof(T) == 4 ? 2 : 1>::kThread
             if (walks[(segments & 1) ^ 1].more == 0) break;
         }
     }
-    if (!alive && lane == 0) atomicOr(w.error_word, 1u);
+    if (!alive && lane == 0) report_lost(w.error_word);
     tmem_before();
     __syncthreads();
     if (warp == 1) {

@@ -327,6 +327,10 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
     }
     return false;
 }
+/// A wait has run out: the host finds the context lost at its next synchronisation.  A context without pinned host memory has no word for it.
+__device__ __forceinline__ void report_lost(uint32_t* error_word) {
+    if (error_word != nullptr) atomicOr(error_word, 1u);
+}
 __device__ __forceinline__ void tma_3d(uint32_t dst, const void* map, int32_t x, int32_t y, int32_t z, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(map),
                  "r"(x), "r"(y), "r"(z), "r"(bar)
