@@ -48,6 +48,13 @@ struct RowsShape {
     static constexpr int kStages = kStagesRoom > 6 ? 6 : kStagesRoom;
     static constexpr uint32_t kSmem = kFixed + kStages * kStage;
     static_assert(kStages >= 2);
+    // The tensor cores cut a sum off where they add a product to it, always towards zero, by up to an ulp (fp32 operands, a chain of 8192 products: 4e-4 too
+    // small).  After so many tiles a thread's rows and sums are added up in fp32 outside: 64 products of 16 keys for fp32 operands (262144 positions: 1.5e-6
+    // off), 512 for 16-bit ones (2^-15 in the mean, a sixteenth of fp16's half step).  A chain begun anew with every tile and added up in registers cost
+    // more: 32 sequences of 3000 - 9000 tokens, 24 rows of 256, fp32: 109 us with no settling, 115 so, 129.
+    static constexpr int32_t kSettle = (TERMS == 2 ? 64 : 512) / (TERMS * (TILE / TS / 16));
+    static constexpr uint32_t kPieces = D / 8 / kSplit;  // float4 of a thread's part of the rows
+    static constexpr uint64_t kSettledBytes = uint64_t{kWarps} * 32 * (kPieces + 1) * 16;
 };
 
 __device__ __forceinline__ uint32_t swizzled(uint32_t row, uint32_t chunk, int dim) {  // of a tile's half: 128-byte rows, or 64-byte rows of 64 elements
@@ -461,6 +468,35 @@ __global__ void __launch_bounds__(RowsShape<D, TS, TILE, CPS, sizeof(T) == 4 ? 2
 #pragma unroll
             for (int b = 0; b < kChunk; ++b) o[a][b][0] = o[a][b][1] = o[a][b][2] = o[a][b][3] = 0;
         float m[2] = {-INFINITY, -INFINITY}, l[2] = {0, 0};
+        // Adds the rows and sums to what lies outside, and begins them anew; behind the last tile the other way round.
+        auto settle = [&](bool first, bool last) __attribute__((always_inline)) {
+            // Outside: this thread's rows, the threads of a piece side by side, and behind them (maximum that they refer to, sum) of either row.
+            float4* outside = reinterpret_cast<float4*>(w.settled) + blockIdx.x * (kConsumers * (S::kPieces + 1)) + threadIdx.x;
+            float4 ml = make_float4(-INFINITY, 0, -INFINITY, 0);
+            if (!first) ml = outside[S::kPieces * kConsumers];
+            // without a maximum what lies outside is zero, or NaN
+            const float f[2] = {ml.x == -INFINITY ? 1.0f : exp2_approx(ml.x - m[0]), ml.z == -INFINITY ? 1.0f : exp2_approx(ml.z - m[1])};
+            l[0] = fmaf(ml.y, f[0], l[0]), l[1] = fmaf(ml.w, f[1], l[1]);
+#pragma unroll
+            for (int a = 0; a < kOwn; ++a)
+#pragma unroll
+                for (int b = 0; b < kChunk; ++b) {
+                    float4* at = outside + (a * kChunk + b) * kConsumers;
+                    float (&v)[4] = o[a][b];
+                    if (!first) {
+                        const float4 x = *at;
+                        v[0] = fmaf(x.x, f[0], v[0]), v[1] = fmaf(x.y, f[0], v[1]), v[2] = fmaf(x.z, f[1], v[2]), v[3] = fmaf(x.w, f[1], v[3]);
+                    }
+                    if (!last) {
+                        *at = make_float4(v[0], v[1], v[2], v[3]);
+                        v[0] = v[1] = v[2] = v[3] = 0;
+                    }
+                }
+            if (!last) {
+                outside[S::kPieces * kConsumers] = make_float4(m[0], l[0], m[1], l[1]);
+                l[0] = l[1] = 0;
+            }
+        };
 
         const uint32_t tok = ts * (NT * 8);  // this warp's first token of a tile
         auto scores = [&](uint32_t st, float (&x)[NO][4]) {  // q . k of this warp's tokens of a stage's tile
@@ -499,10 +535,10 @@ __global__ void __launch_bounds__(RowsShape<D, TS, TILE, CPS, sizeof(T) == 4 ? 2
 #pragma unroll
                 for (int e = 0; e < 4; ++e) x[n][e] = kChains == 2 ? y[0][n][e] + y[kChains - 1][n][e] : y[0][n][e];
         };
-        auto tell = [&](uint32_t turn, const float (&x)[NO][4]) {
+        auto tell = [&](int32_t tile, const float (&x)[NO][4]) {
             if constexpr (S::kSplit == 2) {
 #pragma unroll
-                for (int n = 0; n < NO; ++n) told[turn & 1][ts][ds][n][lane] = make_float4(x[n][0], x[n][1], x[n][2], x[n][3]);
+                for (int n = 0; n < NO; ++n) told[tile & 1][ts][ds][n][lane] = make_float4(x[n][0], x[n][1], x[n][2], x[n][3]);
             }
         };
         // the weights of a tile's scores, and what they add to the sums and rows.  MASKED: some row does not see some token of the tile.
@@ -616,36 +652,41 @@ __global__ void __launch_bounds__(RowsShape<D, TS, TILE, CPS, sizeof(T) == 4 ? 2
         if (alive) alive = __all_sync(0xFFFFFFFFu, mbar_wait(full + 8 * stage, parity));
         float mine[NO][4];
         scores(stage, mine);
-        tell(0, mine);
+        tell(walk.g.lo, mine);
         const int32_t last = walk.g.hi;
-        uint32_t turn = 0;
-        for (int32_t tile = walk.g.lo; tile < last; ++tile, ++turn) {
-            const bool wraps = stage + 1 == S::kStages;
-            const uint32_t next = wraps ? 0 : stage + 1;
-            if (alive && tile + 1 < last) alive = __all_sync(0xFFFFFFFFu, mbar_wait(full + 8 * next, parity ^ (wraps ? 1 : 0)));
-            const int32_t t0 = tile * static_cast<int32_t>(kTile);
-            const bool masked = t0 < all_lo || t0 + static_cast<int32_t>(kTile) > all_hi || partly[stage] != 0;
-            float x[NT][4];
-            if constexpr (S::kSplit == 2) {  // what is told of the next tile goes beside this one's: one barrier a tile
-                bar_sync(2 + ts, 64);
+        for (int32_t tile = walk.g.lo;;) {
+            const int32_t until = min(last, tile + S::kSettle);
+            for (; tile < until; ++tile) {
+                const bool wraps = stage + 1 == S::kStages;
+                const uint32_t next = wraps ? 0 : stage + 1;
+                if (alive && tile + 1 < last) alive = __all_sync(0xFFFFFFFFu, mbar_wait(full + 8 * next, parity ^ (wraps ? 1 : 0)));
+                const int32_t t0 = tile * static_cast<int32_t>(kTile);
+                const bool masked = t0 < all_lo || t0 + static_cast<int32_t>(kTile) > all_hi || partly[stage] != 0;
+                float x[NT][4];
+                if constexpr (S::kSplit == 2) {  // what is told of the next tile goes beside this one's: one barrier a tile
+                    bar_sync(2 + ts, 64);
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    const float4 v = told[turn & 1][ts][n / NO][n % NO][lane];
-                    x[n][0] = v.x, x[n][1] = v.y, x[n][2] = v.z, x[n][3] = v.w;
+                    for (int n = 0; n < NT; ++n) {
+                        const float4 v = told[tile & 1][ts][n / NO][n % NO][lane];
+                        x[n][0] = v.x, x[n][1] = v.y, x[n][2] = v.z, x[n][3] = v.w;
+                    }
+                } else {
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) x[n][e] = mine[n][e];
                 }
-            } else {
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) x[n][e] = mine[n][e];
+                scores(next, mine);
+                tell(tile + 1, mine);
+                weigh(masked, t0, x);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(empty + 8 * stage);
+                advance();
             }
-            scores(next, mine);
-            tell(turn + 1, mine);
-            weigh(masked, t0, x);
-            __syncwarp();
-            if (lane == 0) mbar_arrive(empty + 8 * stage);
-            advance();
+            if (tile == last) break;
+            settle(tile - walk.g.lo == S::kSettle, false);
         }
+        if (last - walk.g.lo > S::kSettle) settle(false, true);
 
         // ---- the segment's rows: joined over the group's warps, then stored or left in scratch ---------------------------------------------------
 #pragma unroll
@@ -766,8 +807,10 @@ int launch_rows_kernel(HaloCudaCtx* ctx, const AttentionCall& c, Work w, cudaStr
     void* p = nullptr;
     if (int rc = workspace(ctx, 5, ctas * sizeof(uint32_t), s, &p, true)) return rc;
     w.counters = static_cast<uint32_t*>(p);
-    if (int rc = workspace(ctx, 6, partial_bytes(S::kRows, D, ctas), s, &p)) return rc;
+    const uint64_t partials = partial_bytes(S::kRows, D, ctas);
+    if (int rc = workspace(ctx, 6, partials + ctas * S::kSettledBytes, s, &p)) return rc;
     w.partials = static_cast<float*>(p);
+    w.settled = w.partials + partials / 4;
     w.error_word = ctx->error_word_dev;
     auto kernel = rows_kernel<T, D, TS, TILE, CPS>;
     if (int rc = allow_dynamic_smem(ctx, reinterpret_cast<const void*>(kernel), S::kSmem)) return rc;

@@ -24,7 +24,7 @@ struct Work {  // what every kernel of a call is told besides the call
     int32_t window;               // 0: none
     uint32_t* counters;           // one for each CTA
     float* partials;              // two slots for each CTA
-    float* settled;               // fp32 operands of the tiles kernel: a row tile for each CTA, 16-byte aligned
+    float* settled;               // what a CTA has taken out of the tensor cores of the segment at hand, 16-byte aligned
     uint32_t* error_word;
     uint32_t min_rows, max_rows;  // packed rows of the sequences that this launch answers for
 };

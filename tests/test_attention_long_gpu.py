@@ -1,0 +1,87 @@
+"""ATTENTION over long contexts: sequences of up to a hundred million positions whose tables name a few pages again and again, so that a block
+walks a long way, the cache stays small, and the answer is known from the pages alone."""
+from __future__ import annotations
+
+import ctypes as C
+
+import attention_ref as ref
+import numpy as np
+import pytest
+import torch
+
+from halo_b200 import backend as hb
+from halo_b200 import capi
+
+pytestmark = pytest.mark.gpu
+
+KINDS = {"f32": (torch.float32, capi.T_F32), "f16": (torch.float16, capi.T_F16), "bf16": (torch.bfloat16, capi.T_BF16)}
+STEP = {"f32": 2.0 ** -24, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}  # half a step of a rounding
+PAGE, PAGES = 128, 3
+
+
+@pytest.fixture(scope="module")
+def be():
+    return hb.CudaBackend(0)
+
+
+class Repeated:
+    """One sequence of `n` positions, n_kv heads with a query head each, `rows` rows that all see the whole of it."""
+
+    def __init__(self, seed, kind, dim, n_kv, rows, n):
+        rng = np.random.default_rng(seed)
+        self.dtype, self.type = KINDS[kind]
+        self.dim, self.n_kv, self.rows, self.n = dim, n_kv, rows, n
+        shape = (PAGES, n_kv, PAGE, dim)
+        # values of one sign, 0.5 to 1.875: what is lost of a sum does not cancel
+        self.k = rng.integers(0x20, 0x40, shape).astype(np.uint8)
+        self.v = rng.integers(0x30, 0x40, shape).astype(np.uint8)
+        self.table = rng.integers(0, PAGES, -(-n // PAGE)).astype(np.int32)
+        self.dev = {name: torch.from_numpy(x).cuda() for name, x in (("k", self.k), ("v", self.v), ("table", self.table))}
+        self.scales = torch.full((PAGES, n_kv), 127, dtype=torch.uint8, device="cuda")
+        self.q = torch.from_numpy(rng.normal(size=(rows, n_kv, dim)).astype(np.float32)).to(self.dtype).cuda()
+        self.length = torch.tensor([n], dtype=torch.int32, device="cuda")
+
+    def run(self, be, scale=0.0):
+        out = torch.full_like(self.q, 77.0)
+        cache = capi.KvCache(k=self.dev["k"].data_ptr(), v=self.dev["v"].data_ptr(), k_scale=self.scales.data_ptr(), v_scale=self.scales.data_ptr(),
+                             table=self.dev["table"].data_ptr(), type=capi.KV_E4M3, n_pages=PAGES, n_kv=self.n_kv, head_dim=self.dim, page_tokens=PAGE,
+                             max_pages=len(self.table), n_seq=1)
+        heads = [capi.Heads(t.data_ptr(), 0, 0) for t in (self.q, out)]
+        a = capi.Attention(type=self.type, n_q=self.n_kv, cache=cache, rows=capi.KvRows(None, self.length.data_ptr(), self.rows, self.rows), q=heads[0],
+                           out=heads[1], causal=0, window=0, scale=scale)
+        assert be.lib.halo_cuda_attention(be.ctx, C.byref(a), torch.cuda.current_stream().cuda_stream) == 0, capi.last_error()
+        assert be.lib.halo_cuda_stream_sync(be.ctx, torch.cuda.current_stream().cuda_stream, 0) == 0, capi.last_error()
+        return out.double().cpu().numpy()
+
+    def want(self, scale=0.0):
+        """([row][kv head][dim], largest sum of |q_d k_d| * |scale|), every key of a page counted as often as the table names the page."""
+        times = np.zeros((PAGES, PAGE))
+        np.add.at(times, self.table[:-1], 1)
+        times[self.table[-1], :(self.n - 1) % PAGE + 1] += 1
+        k, v, q = ref.VALUES[self.k], ref.VALUES[self.v], self.q.double().cpu().numpy()
+        w = np.exp(np.einsum("rhd,phtd->rhpt", q, k) * scale) * times
+        return np.einsum("rhpt,phtd->rhd", w, v) / w.sum(axis=(2, 3))[..., None], np.einsum("rhd,phtd->rhpt", np.abs(q), np.abs(k)).max() * abs(scale)
+
+
+# How many products of 16 keys follow one another in the tensor cores before their sum is taken out (rows: attention_rows.cuh, few rows to a sequence).
+RUN = {("rows", "f32"): 64, ("rows", "f16"): 512}
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("kernel,kind,n", [("rows", "f32", (1 << 18) + 5), ("rows", "f16", (1 << 23) + 70)])
+def test_sums_of_a_long_context(be, kernel, kind, n, dim):
+    """u = 2^-24.  The tensor cores cut a sum off where they add a product of 16 keys, by an ulp (2u) at most, RUN times before it is taken out; the weights'
+    sum takes twice as many additions, half an ulp (u) each, in that stretch.  What was taken out is added up in fp32, u for either sum and stretch.  Joining a
+    block's warps, up to 17 blocks, and the quotient: under 64 u.  Everything has one sign, so no sum on the way is larger than the last.  16-bit operands:
+    a scale of zero, every weight is the same power of two and nothing but the sums can be off.  fp32: weights that differ (sums of equal ones would be exact),
+    each off by what attention_ref.attention_bound says.  Then the output's own rounding."""
+    run, u = RUN[kernel, kind], 2.0 ** -24
+    c = Repeated(1, kind, dim, 512, 1 if kernel == "rows" else 100, n)  # more units than the device has blocks: one walks whole units
+    scale = 0.0 if kind == "f16" else 0.25 / dim
+    got, (want, top) = c.run(be, scale), c.want(scale)
+    keys = run // (2 if kind == "f32" else 1) * (16 if kernel == "tiles" else 64)
+    weights = 0.0 if kind == "f16" else 2 * ((dim + 16) * u * top + 4 * u + 2.0 ** -22 * top) + 2.0 ** -22
+    bound = 4 * run * u + 2 * (n / keys + 1) * u + 64 * u + weights + STEP[kind]
+    off = np.abs(got / want - 1).max()
+    print(f"{kernel} {kind} {dim}: off by {off:.3g}, bound {bound:.3g}")
+    assert off <= bound
