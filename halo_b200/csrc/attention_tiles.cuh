@@ -41,9 +41,10 @@ struct TilesShape {
     static constexpr uint32_t kSmem = 1024 + kQ + kSlots * kSlot;
     static constexpr uint32_t kBuffer = kTile;             // columns of a score buffer, which the terms of the weights (kTile / 2 columns each) overwrite
     static constexpr uint32_t kO = 256;                    // first accumulator column
-    // The tensor cores cut sums off instead of rounding them, always towards zero: a chain of n of them is n * 2^-25 too small in the mean.  fp32 operands'
-    // rows are added up in fp32 outside after every 64 (8 tiles of 64 keys, 4 of 128); 0: never.
-    static constexpr uint32_t kSettle = TERMS == 2 ? 64 / (kTile / 8) : 0;
+    // The tensor cores cut sums off instead of rounding them, always towards zero.  After so many tiles a row's products, and its sum of weights, are added up
+    // in fp32 outside: 64 products of 16 keys for fp32 operands (8 tiles of 64 keys, 4 of 128; 262144 positions to a block: 1e-5 off), 1024 for 16-bit ones
+    // (128 tiles; 4 million positions to a block: 7e-3 too small without, within fp16's half step with it, for 2 % of short prompts' time).
+    static constexpr int32_t kSettle = (TERMS == 2 ? 64 : 1024) / (kTile / 16 * TERMS);
     static constexpr int kHalves = 2 / kStreams;           // softmax warpgroups that share a row tile's keys
     static constexpr int kKeys = kTile / kHalves;          // of a tile that one of them has
     /// Column of a score buffer that the weights of a tile's 16 keys from 16 * i on begin at: a warpgroup's lie where its scores were.
@@ -426,13 +427,13 @@ __global__ void __launch_bounds__(TilesShape<D, sizeof(T) == 4 ? 2 : 1>::kThread
                 if constexpr (kStreams == 2) {
 #pragma unroll
                     for (uint32_t s = 0; s < kStreams; ++s) {
-                        rows(count + t, s, s, t != 0);
+                        rows(count + t, s, s, t % S::kSettle != 0);
                         if (t + 1 < n) scores(count + t + 1, s, s);
                         if (s == kStreams - 1 && t + 2 == n) release_q();
                     }
                 } else {
                     const uint32_t buffer = __shfl_sync(0xFFFFFFFFu, t & 1, 0);
-                    rows(count + t, 0, buffer, TERMS == 2 ? t % S::kSettle != 0 : t != 0);
+                    rows(count + t, 0, buffer, t % S::kSettle != 0);
                     if (t + 2 < n) scores(count + t + 2, 0, buffer);
                     if (t + 3 == n) release_q();
                 }
@@ -601,168 +602,186 @@ __global__ void __launch_bounds__(TilesShape<D, sizeof(T) == 4 ? 2 : 1>::kThread
             const int32_t all_lo = first_key(walk.u.s, w.window, walk.token(w, min(stream * 128 + 127, walk.rows - 1)));
             const int32_t all_hi = end_key(walk.u.s, c.causal, walk.token(w, min(stream * 128, walk.rows - 1)));
             const int32_t last_tile = walk.g.hi;
-            // fp32 operands: this thread's part of the row as far as it is added up outside, four dims at a time, the rows of a warp side by side
-            uint32_t settled = 0;
-            float4* outside = reinterpret_cast<float4*>(w.settled) + blockIdx.x * (128u * D / 4) + r;
-            auto settle = [&](float fade, bool take) {  // outside = outside * fade, or outside + the accumulators
+            float ref = -INFINITY, l = 0;
+            // This thread's part of the row as far as it is added up outside, four dims at a time, the rows of a warp side by side; (reference, sum of weights) of it.
+            constexpr uint32_t kOutside = S::kRows * D / 4;
+            auto outside = [&] { return reinterpret_cast<float4*>(w.settled) + blockIdx.x * kOutside + r; };
+            auto outside_l = [&] {
+                return reinterpret_cast<float2*>(reinterpret_cast<float4*>(w.settled) + gridDim.x * kOutside) + blockIdx.x * kSoft + threadIdx.x - S::kSoftWarp * 32;
+            };
+            auto fade_outside = [&](float2 of) { return of.x == -INFINITY ? 1.0f : exp2_approx(of.x - ref); };  // without a reference: zero, or NaN
+            auto settle = [&](bool first) {  // the accumulators and l go outside; the next products begin anew
+                const float2 of = first ? make_float2(-INFINITY, 0) : *outside_l();
+                const float fade = fade_outside(of);
 #pragma unroll 1
                 for (uint32_t d = half * (D / S::kHalves); d < (half + 1) * (D / S::kHalves); d += 32) {
                     uint32_t o[32];
-                    if (take) {
-                        tmem_ld32(o_at + d, o);
-                        tmem_wait_ld();
-                    }
+                    tmem_ld32(o_at + d, o);
+                    tmem_wait_ld();
 #pragma unroll
                     for (int e = 0; e < 32; e += 4) {
-                        float4* at = outside + (d + e) / 4 * 128;
-                        float4 v = settled != 0 ? *at : make_float4(0, 0, 0, 0);
-                        if (take) v.x += __uint_as_float(o[e]), v.y += __uint_as_float(o[e + 1]), v.z += __uint_as_float(o[e + 2]), v.w += __uint_as_float(o[e + 3]);
-                        else v.x *= fade, v.y *= fade, v.z *= fade, v.w *= fade;
+                        float4* at = outside() + (d + e) / 4 * S::kRows;
+                        float4 v = make_float4(0, 0, 0, 0);
+                        if (!first) v = *at;
+                        v.x = fmaf(v.x, fade, __uint_as_float(o[e])), v.y = fmaf(v.y, fade, __uint_as_float(o[e + 1]));
+                        v.z = fmaf(v.z, fade, __uint_as_float(o[e + 2])), v.w = fmaf(v.w, fade, __uint_as_float(o[e + 3]));
                         *at = v;
                     }
                 }
-                if (take) ++settled;
+                *outside_l() = make_float2(ref, fmaf(of.y, fade, l));
+                l = 0;
             };
             const bool any_row = stream * 128 + quarter * 32 < walk.rows;
-            float ref = -INFINITY, l = 0;
             uint32_t prev_bar = 0, prev_parity = 0;
             uint32_t b = kStreams == 2 ? stream : 0;
-            for (int32_t tile = walk.g.lo; tile < last_tile; ++tile) {
-                const uint32_t use = b == 0 ? uses[0]++ : uses[1]++, s_at = tmem + lanes + b * S::kBuffer;
-                wait(s_full + 8 * b, use & 1);
-                tmem_after();
-                if (!any_row) {  // nothing of this warp's rows is kept
+            for (int32_t tile = walk.g.lo;;) {
+                const int32_t until = TERMS == 2 ? last_tile : min(last_tile, tile + S::kSettle);
+                for (; tile < until; ++tile) {
+                    const uint32_t use = b == 0 ? uses[0]++ : uses[1]++, s_at = tmem + lanes + b * S::kBuffer;
+                    wait(s_full + 8 * b, use & 1);
+                    tmem_after();
+                    if (!any_row) {  // nothing of this warp's rows is kept
+                        tmem_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(p_ready + 8 * b);
+                        prev_bar = pv_done + 8 * b, prev_parity = use & 1;
+                        if (kStreams == 1) b ^= 1;
+                        ++tiles;
+                        continue;
+                    }
+                    const GroupScale* sc = scales[tiles % kScaleTiles] + half * (S::kKeys / 16);
+                    const int32_t t0 = tile * kTile;
+                    const bool masked = t0 < all_lo || t0 + kTile > all_hi;
+                    const uint32_t from = static_cast<uint32_t>(t0 - lo) + half * S::kKeys, seen = static_cast<uint32_t>(max(hi - lo, 0));  // key e of this thread's: from + e < seen
+                    constexpr int kChunks = S::kKeys / 32;
+                    // The scores are read again for the weights, 32 at a time: a loop's worth of code for both passes, and of registers.  (Unrolled over 128 keys the
+                    // warps waited for instructions: prompts of 360 - 1570 tokens 245 us, with 64 keys 232, with 32 215.)  Two terms of the weights take
+                    // the room of scores that are still to be read: there the scores are held.
+                    constexpr bool kHold = TERMS == 2;
+                    constexpr int kUnrolled = kHold ? kChunks : 1;
+                    uint32_t x[kHold ? kChunks : 1][32];
+                    auto mask = [&](int q, uint32_t (&v)[32]) __attribute__((always_inline)) {
+                        const uint32_t at = from + static_cast<uint32_t>(32 * q);
+                        if (__all_sync(0xFFFFFFFFu, at < seen && seen - at >= 32u)) return;  // every row of the warp sees these keys
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            if (at + static_cast<uint32_t>(e) >= seen) v[e] = 0xFF800000u;  // -inf
+                    };
+                    if (kHold) {
+#pragma unroll
+                        for (int q = 0; q < kChunks; ++q) tmem_ld32(s_at + half * S::kKeys + 32 * q, x[kHold ? q : 0]);
+                        tmem_wait_ld();
+                    }
+                    // Missing keys are zeros with log_v = -inf; the factor of a group's scores is not negative: the largest score is the largest exponent.
+                    float top = -INFINITY;
+#pragma unroll kUnrolled
+                    for (int q = 0; q < kChunks; ++q) {
+                        uint32_t (&v)[32] = x[kHold ? q : 0];
+                        if (!kHold) {
+                            tmem_ld32(s_at + half * S::kKeys + 32 * q, v);
+                            tmem_wait_ld();
+                        }
+                        if (masked) mask(q, v);
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const GroupScale s = sc[2 * q + i];
+                            float m = fmaxf(__uint_as_float(v[16 * i]), __uint_as_float(v[16 * i + 1]));
+#pragma unroll
+                            for (int e = 2; e < 16; e += 2) m = fmaxf(fmaxf(m, __uint_as_float(v[16 * i + e])), __uint_as_float(v[16 * i + e + 1]));
+                            top = fmaxf(top, m == -INFINITY ? m : fmaf(m, s.k * qs, s.log_v));
+                        }
+                    }
+                    if constexpr (S::kHalves == 2) {  // the warp that has the other keys of these rows; both have read their scores behind this
+                        shared_top[tiles & 1][half][r] = top;
+                        bar_sync(2 + quarter, 64);
+                        top = fmaxf(top, shared_top[tiles & 1][half ^ 1][r]);
+                    }
+                    const float next = fmaxf(ref, top);
+                    const bool first = ref == -INFINITY, grows = !first && next > ref + 8.0f;
+                    if (__any_sync(0xFFFFFFFFu, grows)) {
+                        // the products into the accumulators so far have to be done; a row without a reference has accumulators of zero, or NaN
+                        const float fade = grows ? exp2_approx(ref - next) : 1.0f;
+                        wait(prev_bar, prev_parity);
+                        tmem_after();
+#pragma unroll 1
+                        for (int d = half * (D / S::kHalves); d < static_cast<int>(half + 1) * (D / S::kHalves); d += 32) {
+                            uint32_t o[32];
+                            tmem_ld32(o_at + d, o);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * fade);
+                            tmem_st32(o_at + d, o);
+                        }
+                        tmem_wait_st();
+                        l *= fade;
+                    }
+                    if (first || grows) ref = next;
+                    if constexpr (TERMS == 2) {
+                        const int32_t t = tile - walk.g.lo;
+                        if (t != 0 && t % S::kSettle == 0) {  // (behind this tile's maximum, which need not wait)
+                            wait(prev_bar, prev_parity);
+                            tmem_after();
+                            settle(t == S::kSettle);
+                        }
+                    }
+                    const float base = ref == -INFINITY ? 0.0f : ref - 6.0f;
+#pragma unroll kUnrolled
+                    for (int q = 0; q < kChunks; ++q) {
+                        uint32_t weights[16], rest[16];
+                        uint32_t (&v)[32] = x[kHold ? q : 0];
+                        if (!kHold) {
+                            tmem_ld32(s_at + half * S::kKeys + 32 * q, v);
+                            tmem_wait_ld();
+                            if (masked) mask(q, v);
+                        }
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const GroupScale s = sc[2 * q + i];
+                            // an unseen key's score of -inf times a factor of zero would be NaN; the factor is zero where every score counts for nothing
+                            const float by = fmaxf(s.k * qs, 0x1p-126f), add = s.log_v - base;
+                            const uint64_t by2 = pair(by, by), add2 = pair(add, add);
+                            uint64_t sum = 0;
+#pragma unroll
+                            for (int e = 0; e < 16; e += 2) {
+                                float y0, y1;
+                                unpair(fma_pair(pair(__uint_as_float(v[16 * i + e]), __uint_as_float(v[16 * i + e + 1])), by2, add2), y0, y1);
+                                y0 = exp2_approx(y0), y1 = exp2_approx(y1);
+                                sum = add_pair(sum, pair(y0, y1));
+                                weights[8 * i + e / 2] = half2_bits(y0, y1);
+                                if constexpr (TERMS == 2) rest[8 * i + e / 2] = half2_rest(y0, y1, weights[8 * i + e / 2]);
+                            }
+                            float s0, s1;
+                            unpair(sum, s0, s1);
+                            l = fmaf(s0 + s1, s.inv_v, l);
+                        }
+                        tmem_st16(s_at + half * (TERMS == 2 ? S::kKeys / 2 : S::kKeys) + 16 * q, weights);  // over scores that have been read
+                        if constexpr (TERMS == 2) tmem_st16(s_at + kTile / 2 + half * (S::kKeys / 2) + 16 * q, rest);
+                    }
+                    tmem_wait_st();
                     tmem_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(p_ready + 8 * b);
                     prev_bar = pv_done + 8 * b, prev_parity = use & 1;
                     if (kStreams == 1) b ^= 1;
                     ++tiles;
-                    continue;
                 }
-                const GroupScale* sc = scales[tiles % kScaleTiles] + half * (S::kKeys / 16);
-                const int32_t t0 = tile * kTile;
-                const bool masked = t0 < all_lo || t0 + kTile > all_hi;
-                const uint32_t from = static_cast<uint32_t>(t0 - lo) + half * S::kKeys, seen = static_cast<uint32_t>(max(hi - lo, 0));  // key e of this thread's: from + e < seen
-                constexpr int kChunks = S::kKeys / 32;
-                // The scores are read again for the weights, 32 at a time: a loop's worth of code for both passes, and of registers.  (Unrolled over 128 keys the
-                // warps waited for instructions: prompts of 360 - 1570 tokens 245 us, with 64 keys 232, with 32 215.)  Two terms of the weights take
-                // the room of scores that are still to be read: there the scores are held.
-                constexpr bool kHold = TERMS == 2;
-                constexpr int kUnrolled = kHold ? kChunks : 1;
-                uint32_t x[kHold ? kChunks : 1][32];
-                auto mask = [&](int q, uint32_t (&v)[32]) __attribute__((always_inline)) {
-                    const uint32_t at = from + static_cast<uint32_t>(32 * q);
-                    if (__all_sync(0xFFFFFFFFu, at < seen && seen - at >= 32u)) return;  // every row of the warp sees these keys
-#pragma unroll
-                    for (int e = 0; e < 32; ++e)
-                        if (at + static_cast<uint32_t>(e) >= seen) v[e] = 0xFF800000u;  // -inf
-                };
-                if (kHold) {
-#pragma unroll
-                    for (int q = 0; q < kChunks; ++q) tmem_ld32(s_at + half * S::kKeys + 32 * q, x[kHold ? q : 0]);
-                    tmem_wait_ld();
-                }
-                // Missing keys are zeros with log_v = -inf; the factor of a group's scores is not negative: the largest score is the largest exponent.
-                float top = -INFINITY;
-#pragma unroll kUnrolled
-                for (int q = 0; q < kChunks; ++q) {
-                    uint32_t (&v)[32] = x[kHold ? q : 0];
-                    if (!kHold) {
-                        tmem_ld32(s_at + half * S::kKeys + 32 * q, v);
-                        tmem_wait_ld();
-                    }
-                    if (masked) mask(q, v);
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const GroupScale s = sc[2 * q + i];
-                        float m = fmaxf(__uint_as_float(v[16 * i]), __uint_as_float(v[16 * i + 1]));
-#pragma unroll
-                        for (int e = 2; e < 16; e += 2) m = fmaxf(fmaxf(m, __uint_as_float(v[16 * i + e])), __uint_as_float(v[16 * i + e + 1]));
-                        top = fmaxf(top, m == -INFINITY ? m : fmaf(m, s.k * qs, s.log_v));
-                    }
-                }
-                if constexpr (S::kHalves == 2) {  // the warp that has the other keys of these rows; both have read their scores behind this
-                    shared_top[tiles & 1][half][r] = top;
-                    bar_sync(2 + quarter, 64);
-                    top = fmaxf(top, shared_top[tiles & 1][half ^ 1][r]);
-                }
-                const float next = fmaxf(ref, top);
-                const bool first = ref == -INFINITY, grows = !first && next > ref + 8.0f;
-                if (__any_sync(0xFFFFFFFFu, grows)) {
-                    // the products into the accumulators so far have to be done; a row without a reference has accumulators of zero, or NaN
-                    const float fade = grows ? exp2_approx(ref - next) : 1.0f;
+                if (__builtin_expect(tile == last_tile, 1)) break;
+                if (any_row) {
                     wait(prev_bar, prev_parity);
                     tmem_after();
-#pragma unroll 1
-                    for (int d = half * (D / S::kHalves); d < static_cast<int>(half + 1) * (D / S::kHalves); d += 32) {
-                        uint32_t o[32];
-                        tmem_ld32(o_at + d, o);
-                        tmem_wait_ld();
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * fade);
-                        tmem_st32(o_at + d, o);
-                    }
-                    tmem_wait_st();
-                    l *= fade;
-                    if constexpr (TERMS == 2) {
-                        if (settled != 0) settle(fade, false);
-                    }
+                    settle(tile - walk.g.lo == S::kSettle);
                 }
-                if (first || grows) ref = next;
-                if constexpr (TERMS == 2) {
-                    const uint32_t t = static_cast<uint32_t>(tile - walk.g.lo);
-                    if (t != 0 && t % S::kSettle == 0) {  // this tile's products begin anew
-                        wait(prev_bar, prev_parity);
-                        tmem_after();
-                        settle(1.0f, true);
-                    }
-                }
-                const float base = ref == -INFINITY ? 0.0f : ref - 6.0f;
-#pragma unroll kUnrolled
-                for (int q = 0; q < kChunks; ++q) {
-                    uint32_t weights[16], rest[16];
-                    uint32_t (&v)[32] = x[kHold ? q : 0];
-                    if (!kHold) {
-                        tmem_ld32(s_at + half * S::kKeys + 32 * q, v);
-                        tmem_wait_ld();
-                        if (masked) mask(q, v);
-                    }
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const GroupScale s = sc[2 * q + i];
-                        // an unseen key's score of -inf times a factor of zero would be NaN; the factor is zero where every score counts for nothing
-                        const float by = fmaxf(s.k * qs, 0x1p-126f), add = s.log_v - base;
-                        const uint64_t by2 = pair(by, by), add2 = pair(add, add);
-                        uint64_t sum = 0;
-#pragma unroll
-                        for (int e = 0; e < 16; e += 2) {
-                            float y0, y1;
-                            unpair(fma_pair(pair(__uint_as_float(v[16 * i + e]), __uint_as_float(v[16 * i + e + 1])), by2, add2), y0, y1);
-                            y0 = exp2_approx(y0), y1 = exp2_approx(y1);
-                            sum = add_pair(sum, pair(y0, y1));
-                            weights[8 * i + e / 2] = half2_bits(y0, y1);
-                            if constexpr (TERMS == 2) rest[8 * i + e / 2] = half2_rest(y0, y1, weights[8 * i + e / 2]);
-                        }
-                        float s0, s1;
-                        unpair(sum, s0, s1);
-                        l = fmaf(s0 + s1, s.inv_v, l);
-                    }
-                    tmem_st16(s_at + half * (TERMS == 2 ? S::kKeys / 2 : S::kKeys) + 16 * q, weights);  // over scores that have been read
-                    if constexpr (TERMS == 2) tmem_st16(s_at + kTile / 2 + half * (S::kKeys / 2) + 16 * q, rest);
-                }
-                tmem_wait_st();
-                tmem_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(p_ready + 8 * b);
-                prev_bar = pv_done + 8 * b, prev_parity = use & 1;
-                if (kStreams == 1) b ^= 1;
-                ++tiles;
             }
             wait(prev_bar, prev_parity);
             tmem_after();
             // ---- the segment's rows ------------------------------------------------------------------------------------------------------
             const bool keep = r < walk.rows;
+            float fade = 0;
+            if (__builtin_expect(any_row && last_tile - walk.g.lo > S::kSettle, 0)) {
+                const float2 of = *outside_l();
+                fade = fade_outside(of);
+                l = fmaf(of.y, fade, l);
+            }
             if constexpr (S::kHalves == 2) {
                 shared_top[tiles & 1][half][r] = l;
                 bar_sync(2 + quarter, 64);
@@ -780,14 +799,12 @@ __global__ void __launch_bounds__(TilesShape<D, sizeof(T) == 4 ? 2 : 1>::kThread
                 uint32_t o[32];
                 tmem_ld32(o_at + d, o);
                 tmem_wait_ld();
-                if constexpr (TERMS == 2) {
-                    if (settled != 0) {
+                if (__builtin_expect(any_row && last_tile - walk.g.lo > S::kSettle, 0)) {
 #pragma unroll
-                        for (int e = 0; e < 32; e += 4) {
-                            const float4 v = outside[(d + e) / 4 * 128];
-                            o[e] = __float_as_uint(__uint_as_float(o[e]) + v.x), o[e + 1] = __float_as_uint(__uint_as_float(o[e + 1]) + v.y);
-                            o[e + 2] = __float_as_uint(__uint_as_float(o[e + 2]) + v.z), o[e + 3] = __float_as_uint(__uint_as_float(o[e + 3]) + v.w);
-                        }
+                    for (int e = 0; e < 32; e += 4) {
+                        const float4 v = outside()[(d + e) / 4 * S::kRows];
+                        o[e] = __float_as_uint(fmaf(v.x, fade, __uint_as_float(o[e]))), o[e + 1] = __float_as_uint(fmaf(v.y, fade, __uint_as_float(o[e + 1])));
+                        o[e + 2] = __float_as_uint(fmaf(v.z, fade, __uint_as_float(o[e + 2]))), o[e + 3] = __float_as_uint(fmaf(v.w, fade, __uint_as_float(o[e + 3])));
                     }
                 }
                 if (!keep) continue;
@@ -870,7 +887,7 @@ int launch_tiles_kernel(HaloCudaCtx* ctx, const AttentionCall& c, Work w, cudaSt
     if (int rc = workspace(ctx, 5, ctas * sizeof(uint32_t), s, &p, true)) return rc;
     w.counters = static_cast<uint32_t*>(p);
     const uint64_t partials = partial_bytes(S::kRows, D, ctas);
-    if (int rc = workspace(ctx, 6, partials + (S::kSettle != 0 ? uint64_t{ctas} * S::kRows * D * 4 : 0), s, &p)) return rc;
+    if (int rc = workspace(ctx, 6, partials + uint64_t{ctas} * (S::kRows * D * 4 + S::kSoftWarps * 32 * 8), s, &p)) return rc;
     w.partials = static_cast<float*>(p);
     w.settled = w.partials + partials / 4;
     w.error_word = ctx->error_word_dev;

@@ -127,9 +127,11 @@ int halo_cuda_kv_write(HaloCudaCtx* ctx, const HaloCudaKvWrite* args, HaloCudaSt
  * h / (n_q / n_kv) of the row's sequence.  A row at position p sees tokens t < length; causal = 1: of those t <= p; window > 0 (causal only): of
  * those t > p - window.  A row that sees none gets zeros.  What a row does not see has no influence on it, whatever it holds.  Tokens of a page whose
  * number is outside [0, n_pages) are left out and set bit 8 of *status (device word, optional).
- * Type F32 computes to fp32 accuracy (both factors of the products in two fp16 terms); F16 and BF16 take q exactly and round the weights to 11
- * bits; sums and softmax are fp32 throughout.  Weights (times their values' scale) below 2^-20 of the row's largest are rounded to multiples of
- * 2^-30 of it, for all types.  The order of the sums goes with the shape and the lengths of the whole call, and the same call gives the same bits.
+ * Type F32 computes to fp32 accuracy (both factors of the products in two fp16 terms, 22 bits); F16 and BF16 take q exactly and round the weights to
+ * 11 bits.  Softmax and sums are fp32; the tensor cores cut a sum off where they add 16 keys to it, so one is taken out and added up, rounded, after at most
+ * 64 (F32) or 1024 (F16, BF16) such steps: what is lost of it is below 2^-17 or 2^-13, however long the context.  Weights (times their values' scale)
+ * below 2^-20 of the row's largest are rounded to multiples of 2^-30 of it, for all types.  The order of the sums goes with the shape and the lengths of
+ * the whole call, and the same call gives the same bits.
  * The cache has at least one page, and the table a column.  Uses context scratch, whose size goes with the operands' shapes alone: run a call once
  * before capturing it. */
 typedef struct HaloCudaAttention {

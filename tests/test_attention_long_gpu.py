@@ -27,7 +27,7 @@ def be():
 class Repeated:
     """One sequence of `n` positions, n_kv heads with a query head each, `rows` rows that all see the whole of it."""
 
-    def __init__(self, seed, kind, dim, n_kv, rows, n):
+    def __init__(self, seed, kind, dim, n_kv, rows, n, table=None):
         rng = np.random.default_rng(seed)
         self.dtype, self.type = KINDS[kind]
         self.dim, self.n_kv, self.rows, self.n = dim, n_kv, rows, n
@@ -35,7 +35,7 @@ class Repeated:
         # values of one sign, 0.5 to 1.875: what is lost of a sum does not cancel
         self.k = rng.integers(0x20, 0x40, shape).astype(np.uint8)
         self.v = rng.integers(0x30, 0x40, shape).astype(np.uint8)
-        self.table = rng.integers(0, PAGES, -(-n // PAGE)).astype(np.int32)
+        self.table = (rng.integers(0, PAGES, -(-n // PAGE)) if table is None else np.array(table)).astype(np.int32)
         self.dev = {name: torch.from_numpy(x).cuda() for name, x in (("k", self.k), ("v", self.v), ("table", self.table))}
         self.scales = torch.full((PAGES, n_kv), 127, dtype=torch.uint8, device="cuda")
         self.q = torch.from_numpy(rng.normal(size=(rows, n_kv, dim)).astype(np.float32)).to(self.dtype).cuda()
@@ -59,16 +59,22 @@ class Repeated:
         np.add.at(times, self.table[:-1], 1)
         times[self.table[-1], :(self.n - 1) % PAGE + 1] += 1
         k, v, q = ref.VALUES[self.k], ref.VALUES[self.v], self.q.double().cpu().numpy()
-        w = np.exp(np.einsum("rhd,phtd->rhpt", q, k) * scale) * times
-        return np.einsum("rhpt,phtd->rhd", w, v) / w.sum(axis=(2, 3))[..., None], np.einsum("rhd,phtd->rhpt", np.abs(q), np.abs(k)).max() * abs(scale)
+        w = np.exp(np.einsum("rhd,phtd->rhpt", q, k, optimize=True) * scale) * times
+        return np.einsum("rhpt,phtd->rhd", w, v, optimize=True) / w.sum(axis=(2, 3))[..., None], np.einsum("rhd,phtd->rhpt", np.abs(q), np.abs(k), optimize=True).max() * abs(scale)
 
 
-# How many products of 16 keys follow one another in the tensor cores before their sum is taken out (rows: attention_rows.cuh, few rows to a sequence).
-RUN = {("rows", "f32"): 64, ("rows", "f16"): 512}
+# How many products of 16 keys follow one another in the tensor cores before their sum is taken out (rows: attention_rows.cuh, 64 rows of 16-bit operands
+# or 48 of fp32 at most; tiles: attention_tiles.cuh).
+RUN = {("rows", "f32"): 64, ("rows", "f16"): 512, ("tiles", "f32"): 64, ("tiles", "f16"): 1024}
+
+
+def few(kernel, dim):
+    """(kv heads, rows) of a call of the kernel with more units than the device has blocks (three on an SM, or one): a block walks whole units."""
+    return (460 if kernel == "rows" and dim < 256 else 160), (1 if kernel == "rows" else 70)
 
 
 @pytest.mark.parametrize("dim", [64, 128, 256])
-@pytest.mark.parametrize("kernel,kind,n", [("rows", "f32", (1 << 18) + 5), ("rows", "f16", (1 << 23) + 70)])
+@pytest.mark.parametrize("kernel,kind,n", [("rows", "f32", (1 << 18) + 5), ("rows", "f16", (1 << 23) + 70), ("tiles", "f32", (1 << 18) + 5), ("tiles", "f16", 1 << 22)])
 def test_sums_of_a_long_context(be, kernel, kind, n, dim):
     """u = 2^-24.  The tensor cores cut a sum off where they add a product of 16 keys, by an ulp (2u) at most, RUN times before it is taken out; the weights'
     sum takes twice as many additions, half an ulp (u) each, in that stretch.  What was taken out is added up in fp32, u for either sum and stretch.  Joining a
@@ -76,12 +82,37 @@ def test_sums_of_a_long_context(be, kernel, kind, n, dim):
     a scale of zero, every weight is the same power of two and nothing but the sums can be off.  fp32: weights that differ (sums of equal ones would be exact),
     each off by what attention_ref.attention_bound says.  Then the output's own rounding."""
     run, u = RUN[kernel, kind], 2.0 ** -24
-    c = Repeated(1, kind, dim, 512, 1 if kernel == "rows" else 100, n)  # more units than the device has blocks: one walks whole units
+    c = Repeated(1, kind, dim, *few(kernel, dim), n)
     scale = 0.0 if kind == "f16" else 0.25 / dim
     got, (want, top) = c.run(be, scale), c.want(scale)
     keys = run // (2 if kind == "f32" else 1) * (16 if kernel == "tiles" else 64)
     weights = 0.0 if kind == "f16" else 2 * ((dim + 16) * u * top + 4 * u + 2.0 ** -22 * top) + 2.0 ** -22
     bound = 4 * run * u + 2 * (n / keys + 1) * u + 64 * u + weights + STEP[kind]
+    off = np.abs(got / want - 1).max()
+    print(f"{kernel} {kind} {dim}: off by {off:.3g}, bound {bound:.3g}")
+    assert off <= bound
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("kernel,kind", [("rows", "f32"), ("rows", "f16"), ("rows", "bf16"), ("tiles", "f32"), ("tiles", "f16"), ("tiles", "bf16")])
+def test_a_maximum_that_grows_behind_sums_that_were_taken_out(be, kernel, kind, dim):
+    """40960 keys of one page's and 40960 of another's, then five of a third's whose scores are about 2^10 times the others' in weight, by which everything
+    before is multiplied down: the parts of the answer are of like size."""
+    pages = 320
+    c = Repeated(2, kind, dim, *few(kernel, dim), 2 * pages * PAGE + 5, [0] * pages + [1] * pages + [2])
+    # rows of ones: a score is the mean of the key's dims times 8
+    c.q = torch.ones_like(c.q)
+    rng = np.random.default_rng(3)
+    c.k[:] = rng.integers(0x28, 0x2A, c.k.shape)    # 0.25, 0.28: a score of about 2.1
+    c.k[2] = rng.integers(0x38, 0x3A, c.k[2].shape)  # 1, 1.125: about 8.5
+    c.v[1] += 8                                      # twice the first page's
+    c.dev = {name: torch.from_numpy(x).cuda() for name, x in (("k", c.k), ("v", c.v), ("table", c.table))}
+    scale = 8.0 / dim
+    got, (want, top) = c.run(be, scale), c.want(scale)
+    u, run = 2.0 ** -24, RUN[kernel, "f32" if kind == "f32" else "f16"]
+    keys = run // (2 if kind == "f32" else 1) * (16 if kernel == "tiles" else 64)
+    weights = 2 * ((dim + 16) * u * top + 4 * u + (2.0 ** -22 * top if kind == "f32" else 0)) + (2.0 ** -22 if kind == "f32" else 2.0 ** -11)
+    bound = 4 * run * u + 4 * (c.n / keys + 1) * u + 64 * u + weights + STEP[kind]  # (a stretch's multiplication too)
     off = np.abs(got / want - 1).max()
     print(f"{kernel} {kind} {dim}: off by {off:.3g}, bound {bound:.3g}")
     assert off <= bound
