@@ -103,20 +103,44 @@ __device__ __forceinline__ bool drop_nan(uint32_t& w) {
 }
 
 /// Writes NaN over the results of rows that see a token whose value is NaN there: the walk left those codes out in tiles that some rows do not see
-/// whole, where a product with weight zero would have spread them.  `at(row, d)` is the result's address.
+/// whole, or whose pages are not all there, since a product with weight zero would have spread them.  Only those tiles are looked at (every token of 60000, one
+/// after the other, took 300 to 9000 us).  Called by whole warps that share the segment's codes of dims [first_dim, first_dim + dims), 16 bytes to a thread at a
+/// time; `at(row, d)` is the result's address.
 template <class At>
-__device__ void spread_nan(const AttentionCall& c, const Work& w, const Unit& u, const Segment& g, uint32_t first_row, uint32_t end_row, uint32_t first_dim, uint32_t end_dim,
-                           uint32_t dim_step, At&& at) {
-    const uint32_t r0 = u.row0(w);
-    for (int32_t t = g.lo * static_cast<int32_t>(w.tile); t < min(g.hi * static_cast<int32_t>(w.tile), u.s.length); ++t) {
-        const int32_t page = page_of(c.cache, u.seq, t >> c.cache.page_shift);
-        if (static_cast<uint32_t>(page) >= c.cache.n_pages) continue;
-        const uint8_t* v = c.cache.v + page * c.cache.page_stride + (uint64_t{u.head} * c.cache.page_tokens + (t & (c.cache.page_tokens - 1))) * c.cache.head_dim;
-        for (uint32_t d = first_dim; d < end_dim; d += dim_step) {
-            if ((v[d] & 127) != 127) continue;
-            for (uint32_t r = first_row; r < end_row; ++r) {
-                const uint32_t j = (r0 + r) / c.group;
-                if (t >= first_key(u.s, w.window, j) && t < end_key(u.s, c.causal, j)) at(r, d);
+__device__ void spread_nan(const AttentionCall& c, const Work& w, const Unit& u, const Segment& g, uint32_t first_row, uint32_t end_row, uint32_t first_dim, uint32_t dims,
+                           uint32_t thread, uint32_t threads, At&& at) {
+    const uint32_t r0 = u.row0(w), lane = threadIdx.x % 32, chunks = dims / 16;
+    const int32_t tile_keys = static_cast<int32_t>(w.tile), page_tokens = static_cast<int32_t>(c.cache.page_tokens);
+    const int32_t all_lo = first_key(u.s, w.window, (r0 + u.rows(w) - 1) / c.group), all_hi = end_key(u.s, c.causal, r0 / c.group);
+    auto missing = [&](int32_t t) { return static_cast<uint32_t>(page_of(c.cache, u.seq, t >> c.cache.page_shift)) >= c.cache.n_pages; };
+    for (int32_t base = g.lo; base < g.hi; base += 32) {
+        const int32_t tile = base + static_cast<int32_t>(lane), t = tile * tile_keys;
+        bool look = false;
+        if (tile < g.hi) {
+            look = t < all_lo || t + tile_keys > all_hi;
+            for (int32_t k = 0; k < tile_keys && !look; k += page_tokens) look = missing(t + k);
+        }
+        for (uint32_t left = __ballot_sync(0xFFFFFFFFu, look); left != 0; left &= left - 1) {
+            const int32_t first = (base + __ffs(left) - 1) * tile_keys;
+            for (int32_t t0 = first; t0 < min(first + tile_keys, u.s.length); t0 += 16) {
+                if (missing(t0)) continue;
+                const int32_t page = page_of(c.cache, u.seq, t0 >> c.cache.page_shift);
+                const uint8_t* v = c.cache.v + page * c.cache.page_stride + (uint64_t{u.head} * c.cache.page_tokens + (t0 & (page_tokens - 1))) * c.cache.head_dim + first_dim;
+                for (uint32_t i = thread; i < dims; i += threads) {  // 16 tokens of `chunks` pieces each
+                    const int32_t key = t0 + static_cast<int32_t>(i / chunks);
+                    const uint4 codes = *reinterpret_cast<const uint4*>(v + i / chunks * c.cache.head_dim + i % chunks * 16);
+                    if (key >= u.s.length) continue;
+#pragma unroll
+                    for (uint32_t n = 0; n < 4; ++n) {
+                        for (uint32_t hit = nan_bits(n == 0 ? codes.x : n == 1 ? codes.y : n == 2 ? codes.z : codes.w); hit != 0; hit &= hit - 1) {
+                            const uint32_t d = first_dim + i % chunks * 16 + n * 4 + (__ffs(hit) - 1) / 8;
+                            for (uint32_t r = first_row; r < end_row; ++r) {
+                                const uint32_t j = (r0 + r) / c.group;
+                                if (key >= first_key(u.s, w.window, j) && key < end_key(u.s, c.causal, j)) at(r, d);
+                            }
+                        }
+                    }
+                }
             }
         }
     }
@@ -754,7 +778,7 @@ __global__ void __launch_bounds__(RowsShape<D, TS, TILE, CPS, sizeof(T) == 4 ? 2
         }
         bar_sync(1, kConsumers);
         if (nan_seen != 0) {
-            spread_nan(c, w, walk.u, walk.g, 0, walk.u.rows(w), threadIdx.x, c.cache.head_dim, kConsumers, [&](uint32_t r, uint32_t d) {
+            spread_nan(c, w, walk.u, walk.g, 0, walk.u.rows(w), 0, D, threadIdx.x, kConsumers, [&](uint32_t r, uint32_t d) {
                 if (slot == nullptr) out_at(r)[d] = from_f32<T>(NAN);
                 else slot[r * D + d] = NAN;
             });

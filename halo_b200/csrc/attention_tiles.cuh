@@ -141,7 +141,7 @@ struct Cursor {
 /// with its slot.
 template <int D, int TERMS, bool IS_V>
 __device__ __forceinline__ void convert_slots(const AttentionCall& c, const Work& w, const Range& range, Cursor& cursor, uint32_t part, uint32_t turn, uint32_t every, uint32_t ring,
-                                              uint32_t full, uint32_t empty, GroupScale (*scales)[8], uint32_t* nan_seen, bool& alive) {
+                                              uint32_t full, uint32_t empty, GroupScale (*scales)[8], uint32_t* nan_tiles, bool& alive) {
     using S = TilesShape<D, TERMS>;
     constexpr uint32_t kBlocks = IS_V ? S::kParts : 1;                   // 64-dim blocks of a slot's rows
     constexpr int32_t kTile = S::kTile;
@@ -280,7 +280,7 @@ __device__ __forceinline__ void convert_slots(const AttentionCall& c, const Work
                         uint4& v = x[p * kLot + j];
                         nan |= drop_nan(v.x) | drop_nan(v.y) | drop_nan(v.z) | drop_nan(v.w);
                     }
-                    if (nan) *nan_seen = 1;
+                    if (nan) atomicMax(nan_tiles, count + 1);  // (of the next tile where that is loaded already)
                 }
 #pragma unroll
                 for (uint32_t j = 0; j < kLot; ++j) {
@@ -312,7 +312,7 @@ __global__ void __launch_bounds__(TilesShape<D, sizeof(T) == 4 ? 2 : 1>::kThread
     __shared__ float q_unscale[2][S::kRows];  // of a segment and the next
     __shared__ float2 joined_ml[S::kRows];
     __shared__ float shared_top[2][S::kHalves][128];  // of a tile and the next: the maxima that a row tile's warpgroups tell each other
-    __shared__ uint32_t nan_seen, is_last, tmem_word;
+    __shared__ uint32_t nan_tiles, is_last, tmem_word;  // nan_tiles: of the CTA's tiles, how many the last one with a NaN code left out is in
     __shared__ Cursor cursors[S::kConvWarps];
     __shared__ Walk walks[2];  // the segment at hand and the next one, in turn
 
@@ -335,7 +335,7 @@ __global__ void __launch_bounds__(TilesShape<D, sizeof(T) == 4 ? 2 : 1>::kThread
             mbar_init(pv_done + 8 * i, 1);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        nan_seen = 0;
+        nan_tiles = 0;
     }
     {
         Range range;
@@ -575,8 +575,8 @@ __global__ void __launch_bounds__(TilesShape<D, sizeof(T) == 4 ? 2 : 1>::kThread
         constexpr uint32_t kEvery = S::kConvWarps / (2 * kParts);
         const uint32_t role = (warp - 4) % (2 * kParts), turn = (warp - 4) / (2 * kParts), part = role % kParts;
         const bool is_v = role >= kParts;
-        if (is_v) convert_slots<D, TERMS, true>(c, w, range, cursors[warp - 4], part, turn, kEvery, ring, full, empty, scales, &nan_seen, alive);
-        else convert_slots<D, TERMS, false>(c, w, range, cursors[warp - 4], part, turn, kEvery, ring, full, empty, scales, &nan_seen, alive);
+        if (is_v) convert_slots<D, TERMS, true>(c, w, range, cursors[warp - 4], part, turn, kEvery, ring, full, empty, scales, &nan_tiles, alive);
+        else convert_slots<D, TERMS, false>(c, w, range, cursors[warp - 4], part, turn, kEvery, ring, full, empty, scales, &nan_tiles, alive);
     } else if (warp >= S::kSoftWarp) {
         // ---- softmax ---------------------------------------------------------------------------------------------------------------------
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::kSoftRegs));
@@ -834,11 +834,11 @@ __global__ void __launch_bounds__(TilesShape<D, sizeof(T) == 4 ? 2 : 1>::kThread
                 *reinterpret_cast<float2*>(ml) = make_float2(ref, l);
             }
             tmem_before();
-            // every warp for what it stored; a flag stays set: the conversion is ahead, and what it saw may belong to a segment to come
-            if (any_row && __any_sync(0xFFFFFFFFu, *static_cast<volatile uint32_t*>(&nan_seen) != 0)) {
+            // every warp for what it stored; the conversion is ahead, and what it saw may belong to a segment to come
+            if (any_row && __any_sync(0xFFFFFFFFu, *static_cast<volatile uint32_t*>(&nan_tiles) > tiles - static_cast<uint32_t>(last_tile - walk.g.lo))) {
                 __syncwarp();
                 const uint32_t top = stream * 128 + quarter * 32, dims = D / S::kHalves;
-                spread_nan(c, w, walk.u, walk.g, top, min(top + 32, walk.rows), half * dims + lane, (half + 1) * dims, 32, [&](uint32_t row, uint32_t d) {
+                spread_nan(c, w, walk.u, walk.g, top, min(top + 32, walk.rows), half * dims, dims, lane, 32, [&](uint32_t row, uint32_t d) {
                     if (walk.g.whole()) out_at(row)[d] = from_f32<T>(NAN);
                     else partial_slot(w, D, blockIdx.x, walk.g.from_start)[row * D + d] = NAN;
                 });

@@ -11,6 +11,7 @@ import torch
 
 from halo_b200 import backend as hb
 from halo_b200 import capi
+from test_attention_gpu import Case
 
 pytestmark = pytest.mark.gpu
 
@@ -40,16 +41,32 @@ class Repeated:
         self.scales = torch.full((PAGES, n_kv), 127, dtype=torch.uint8, device="cuda")
         self.q = torch.from_numpy(rng.normal(size=(rows, n_kv, dim)).astype(np.float32)).to(self.dtype).cuda()
         self.length = torch.tensor([n], dtype=torch.int32, device="cuda")
+        self.causal = 0
 
-    def run(self, be, scale=0.0):
-        out = torch.full_like(self.q, 77.0)
+    def call(self, be, out, scale):
         cache = capi.KvCache(k=self.dev["k"].data_ptr(), v=self.dev["v"].data_ptr(), k_scale=self.scales.data_ptr(), v_scale=self.scales.data_ptr(),
                              table=self.dev["table"].data_ptr(), type=capi.KV_E4M3, n_pages=PAGES, n_kv=self.n_kv, head_dim=self.dim, page_tokens=PAGE,
                              max_pages=len(self.table), n_seq=1)
         heads = [capi.Heads(t.data_ptr(), 0, 0) for t in (self.q, out)]
         a = capi.Attention(type=self.type, n_q=self.n_kv, cache=cache, rows=capi.KvRows(None, self.length.data_ptr(), self.rows, self.rows), q=heads[0],
-                           out=heads[1], causal=0, window=0, scale=scale)
+                           out=heads[1], causal=self.causal, window=0, scale=scale)
         assert be.lib.halo_cuda_attention(be.ctx, C.byref(a), torch.cuda.current_stream().cuda_stream) == 0, capi.last_error()
+
+    def time(self, be, scale):
+        """Microseconds of a call on the device, of the fastest of five."""
+        out, best = torch.empty_like(self.q), float("inf")
+        for _ in range(5):
+            begin, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            begin.record()
+            self.call(be, out, scale)
+            end.record()
+            torch.cuda.synchronize()
+            best = min(best, begin.elapsed_time(end) * 1e3)
+        return best
+
+    def run(self, be, scale=0.0):
+        out = torch.full_like(self.q, 77.0)
+        self.call(be, out, scale)
         assert be.lib.halo_cuda_stream_sync(be.ctx, torch.cuda.current_stream().cuda_stream, 0) == 0, capi.last_error()
         return out.double().cpu().numpy()
 
@@ -116,3 +133,39 @@ def test_a_maximum_that_grows_behind_sums_that_were_taken_out(be, kernel, kind, 
     off = np.abs(got / want - 1).max()
     print(f"{kernel} {kind} {dim}: off by {off:.3g}, bound {bound:.3g}")
     assert off <= bound
+
+@pytest.mark.parametrize("kind,rows", [("f32", 4), ("bf16", 4), ("f32", 300), ("bf16", 300)])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_a_nan_among_the_last_keys_costs_a_few_tiles(be, kind, rows, dim):
+    """What a NaN that some rows do not see takes to come back is a look at the tiles at the edge of what they see, not at all that they see."""
+    n = 60000
+    c = Repeated(4, kind, dim, 8, rows, n, [0, 1] * (n // PAGE // 2) + [2])
+    c.causal = 1
+    clean = c.run(be, 0.5 / dim)
+    last = min(rows // 2, 40)  # rows that see it, in the last page
+    page, slot = c.table[(n - last) // PAGE], (n - last) % PAGE
+    assert page == 2
+    plain = c.time(be, 0.5 / dim)
+    c.dev["v"][page, 3, slot, 5] = 127
+    got, slow = c.run(be, 0.5 / dim), c.time(be, 0.5 / dim)
+    nan = np.zeros(got.shape, bool)
+    nan[rows - last:, 3, 5] = True
+    assert np.array_equal(np.isnan(got), nan)
+    assert np.array_equal(got[~nan], clean[~nan])
+    print(f"{kind} {rows} rows of {dim}: {plain:.0f} us, with a NaN {slow:.0f}")
+    assert slow < 1.5 * plain + 100
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("rows", [1, 150])
+@pytest.mark.parametrize("window", [0, 90])
+def test_a_nan_beside_a_missing_page(be, kind, dim, rows, window):
+    """In tiles without all of their pages NaN codes are left out of the products and put back behind them, for every row that sees them."""
+    c = Case(50, kind, dim, 16, 2, 3, [rows, rows], [rows + 700, rows + 400])
+    for i, at in ((0, 16 * 40 + 3), (1, 100)):
+        c.cache["table"][i, at // 16 - 1] = -1
+        c.cache["v"][c.cache["table"][i, at // 16], i, at % 16, 37 + i] = 255
+    c.cache["v"][c.cache["table"][0, (rows + 650) // 16], 1, (rows + 650) % 16, 1] = 127  # in a tile at the edge of what some rows see, or beside it
+    c.to_device()
+    c.compare(c.run(be, window=window), window=window, bad=8)  # the last row sees keys from rows + 700 - 90 on: 624 to 639, of the missing page, among them
