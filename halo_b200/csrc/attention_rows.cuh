@@ -105,10 +105,10 @@ __device__ __forceinline__ bool drop_nan(uint32_t& w) {
 /// Writes NaN over the results of rows that see a token whose value is NaN there: the walk left those codes out in tiles that some rows do not see
 /// whole, or whose pages are not all there, since a product with weight zero would have spread them.  Only those tiles are looked at (every token of 60000, one
 /// after the other, took 300 to 9000 us).  Called by whole warps that share the segment's codes of dims [first_dim, first_dim + dims), 16 bytes to a thread at a
-/// time; `at(row, d)` is the result's address.
+/// time; `at(row, d)` is the result's address.  Counts `moved` up, for those who wait for the warps meanwhile.
 template <class At>
 __device__ void spread_nan(const AttentionCall& c, const Work& w, const Unit& u, const Segment& g, uint32_t first_row, uint32_t end_row, uint32_t first_dim, uint32_t dims,
-                           uint32_t thread, uint32_t threads, At&& at) {
+                           uint32_t thread, uint32_t threads, volatile uint32_t* moved, At&& at) {
     const uint32_t r0 = u.row0(w), lane = threadIdx.x % 32, chunks = dims / 16;
     const int32_t tile_keys = static_cast<int32_t>(w.tile), page_tokens = static_cast<int32_t>(c.cache.page_tokens);
     const int32_t all_lo = first_key(u.s, w.window, (r0 + u.rows(w) - 1) / c.group), all_hi = end_key(u.s, c.causal, r0 / c.group);
@@ -120,6 +120,7 @@ __device__ void spread_nan(const AttentionCall& c, const Work& w, const Unit& u,
             look = t < all_lo || t + tile_keys > all_hi;
             for (int32_t k = 0; k < tile_keys && !look; k += page_tokens) look = missing(t + k);
         }
+        if (lane == 0) *moved = *moved + 1;
         for (uint32_t left = __ballot_sync(0xFFFFFFFFu, look); left != 0; left &= left - 1) {
             const int32_t first = (base + __ffs(left) - 1) * tile_keys;
             for (int32_t t0 = first; t0 < min(first + tile_keys, u.s.length); t0 += 16) {
@@ -282,7 +283,7 @@ __global__ void __launch_bounds__(RowsShape<D, TS, TILE, CPS, sizeof(T) == 4 ? 2
     __shared__ float2 row_ml[TS][16];
     __shared__ float4 told[S::kSplit == 2 ? 2 : 1][TS][S::kSplit][NO][32];  // scores that a pair's warps tell each other, of a tile and the next
     __shared__ float q_unscale[S::kRows];
-    __shared__ uint32_t nan_seen, is_last;
+    __shared__ uint32_t nan_seen, is_last, moved;
     __shared__ Walk walk;
     __shared__ float2 joined_ml[S::kRows];
 
@@ -302,6 +303,7 @@ __global__ void __launch_bounds__(RowsShape<D, TS, TILE, CPS, sizeof(T) == 4 ? 2
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         nan_seen = 0;
+        moved = 0;
     }
     {
         Range range;
@@ -358,7 +360,7 @@ __global__ void __launch_bounds__(RowsShape<D, TS, TILE, CPS, sizeof(T) == 4 ? 2
                 if (page == -2 && c.status != nullptr) atomicOr(c.status, 8u);  // kStatusBadIndex
                 const uint32_t present = __ballot_sync(0xFFFFFFFFu, page >= 0);
                 for (int32_t tile = base; tile < min(base + kLot, g.hi); ++tile) {
-                    if (alive) alive = __all_sync(0xFFFFFFFFu, mbar_wait(empty + 8 * stage, parity ^ 1));
+                    if (alive) alive = __all_sync(0xFFFFFFFFu, mbar_wait(empty + 8 * stage, parity ^ 1, &moved));
                     if (!alive) break;
                     const uint32_t in_tile = (tile - base) * kGroups, here = present >> in_tile & static_cast<uint32_t>((uint64_t{1} << kGroups) - 1);
                     const uint32_t step = page_rows / 16;  // groups of a box
@@ -778,7 +780,7 @@ __global__ void __launch_bounds__(RowsShape<D, TS, TILE, CPS, sizeof(T) == 4 ? 2
         }
         bar_sync(1, kConsumers);
         if (nan_seen != 0) {
-            spread_nan(c, w, walk.u, walk.g, 0, walk.u.rows(w), 0, D, threadIdx.x, kConsumers, [&](uint32_t r, uint32_t d) {
+            spread_nan(c, w, walk.u, walk.g, 0, walk.u.rows(w), 0, D, threadIdx.x, kConsumers, &moved, [&](uint32_t r, uint32_t d) {
                 if (slot == nullptr) out_at(r)[d] = from_f32<T>(NAN);
                 else slot[r * D + d] = NAN;
             });

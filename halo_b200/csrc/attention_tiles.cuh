@@ -313,6 +313,7 @@ __global__ void __launch_bounds__(TilesShape<D, sizeof(T) == 4 ? 2 : 1>::kThread
     __shared__ float2 joined_ml[S::kRows];
     __shared__ float shared_top[2][S::kHalves][128];  // of a tile and the next: the maxima that a row tile's warpgroups tell each other
     __shared__ uint32_t nan_tiles, is_last, tmem_word;  // nan_tiles: of the CTA's tiles, how many the last one with a NaN code left out is in
+    __shared__ uint32_t moved;                          // counted up by the softmax warps as they go on
     __shared__ Cursor cursors[S::kConvWarps];
     __shared__ Walk walks[2];  // the segment at hand and the next one, in turn
 
@@ -336,6 +337,7 @@ __global__ void __launch_bounds__(TilesShape<D, sizeof(T) == 4 ? 2 : 1>::kThread
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         nan_tiles = 0;
+        moved = 0;
     }
     {
         Range range;
@@ -471,7 +473,9 @@ __global__ void __launch_bounds__(TilesShape<D, sizeof(T) == 4 ? 2 : 1>::kThread
 #pragma unroll
                 for (uint32_t k = 0; k < kPieces; ++k) asm volatile("prefetch.global.L2 [%0];" ::"l"(q + k * (64 * sizeof(T))));
             }
-            if (segments != 0) wait(q_free, (segments - 1) & 1);  // the segment before has its last scores, and the softmax is not behind it
+            // The segment before has its last scores, and the softmax is not behind it.  That is as far away as the segment is long: on contexts of some tens of
+            // millions of positions a wait for one step would run out.  (The products' and conversion's waits are for a step, and looked at `moved` 2 - 4 % slower.)
+            if (segments != 0 && alive) alive = __all_sync(0xFFFFFFFFu, mbar_wait(q_free, (segments - 1) & 1, &moved));
 #pragma unroll 1
             for (uint32_t row = first; row < rows; row += kStride) {
                 const uint8_t* q = source(row);
@@ -764,6 +768,7 @@ __global__ void __launch_bounds__(TilesShape<D, sizeof(T) == 4 ? 2 : 1>::kThread
                     prev_bar = pv_done + 8 * b, prev_parity = use & 1;
                     if (kStreams == 1) b ^= 1;
                     ++tiles;
+                    if (leader) *static_cast<volatile uint32_t*>(&moved) = moved + 1;
                 }
                 if (__builtin_expect(tile == last_tile, 1)) break;
                 if (any_row) {
@@ -838,7 +843,7 @@ __global__ void __launch_bounds__(TilesShape<D, sizeof(T) == 4 ? 2 : 1>::kThread
             if (any_row && __any_sync(0xFFFFFFFFu, *static_cast<volatile uint32_t*>(&nan_tiles) > tiles - static_cast<uint32_t>(last_tile - walk.g.lo))) {
                 __syncwarp();
                 const uint32_t top = stream * 128 + quarter * 32, dims = D / S::kHalves;
-                spread_nan(c, w, walk.u, walk.g, top, min(top + 32, walk.rows), half * dims, dims, lane, 32, [&](uint32_t row, uint32_t d) {
+                spread_nan(c, w, walk.u, walk.g, top, min(top + 32, walk.rows), half * dims, dims, lane, 32, &moved, [&](uint32_t row, uint32_t d) {
                     if (walk.g.whole()) out_at(row)[d] = from_f32<T>(NAN);
                     else partial_slot(w, D, blockIdx.x, walk.g.from_start)[row * D + d] = NAN;
                 });

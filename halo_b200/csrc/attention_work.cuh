@@ -313,7 +313,7 @@ __device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) {
 }
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
 constexpr uint32_t kWaitSpins = 1u << 18;  // of a try_wait that sleeps in hardware: seconds
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {  // for what one step of another warp brings
     for (uint32_t i = 0; i < kWaitSpins; ++i) {
         uint32_t ok;
         asm volatile(
@@ -326,6 +326,17 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
         if (ok) return true;
     }
     return false;
+}
+/// For what more than a step may come in front of (a segment takes as long as its context): given up once `moved`, which the warps waited for count up as they
+/// go on, has stood still for as long as a step may take.
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, const volatile uint32_t* moved) {
+    uint32_t before = ~0u;
+    while (!mbar_wait(bar, parity)) {
+        const uint32_t now = *moved;
+        if (now == before) return false;
+        before = now;
+    }
+    return true;
 }
 /// A wait has run out: the host finds the context lost at its next synchronisation.  A context without pinned host memory has no word for it.
 __device__ __forceinline__ void report_lost(uint32_t* error_word) {

@@ -53,7 +53,7 @@ class Repeated:
         assert be.lib.halo_cuda_attention(be.ctx, C.byref(a), torch.cuda.current_stream().cuda_stream) == 0, capi.last_error()
 
     def time(self, be, scale):
-        """Microseconds of a call on the device, of the fastest of five."""
+        """Microseconds of the fastest of five calls on the device."""
         out, best = torch.empty_like(self.q), float("inf")
         for _ in range(5):
             begin, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
@@ -169,3 +169,13 @@ def test_a_nan_beside_a_missing_page(be, kind, dim, rows, window):
     c.cache["v"][c.cache["table"][0, (rows + 650) // 16], 1, (rows + 650) % 16, 1] = 127  # in a tile at the edge of what some rows see, or beside it
     c.to_device()
     c.compare(c.run(be, window=window), window=window, bad=8)  # the last row sees keys from rows + 700 - 90 on: 624 to 639, of the missing page, among them
+
+
+def test_a_block_may_walk_for_seconds(be):
+    """A unit of 134 million positions: q of the block's next one is waited for through all of it, which takes 2.3 s, longer than a wait for
+    a single step may (1.3 s)."""
+    c = Repeated(5, "f16", 64, 222, 70, 1 << 27)
+    got, (want, _) = c.run(be), c.want()
+    run, u = RUN["tiles", "f16"], 2.0 ** -24
+    assert np.abs(got / want - 1).max() <= 4 * run * u + 2 * (c.n / (run * 16) + 1) * u + 64 * u + STEP["f16"]  # as in test_sums_of_a_long_context
+    assert be.lib.halo_cuda_ctx_lost(be.ctx) == 0
