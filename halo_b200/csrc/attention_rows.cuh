@@ -27,7 +27,7 @@ namespace attn {
 
 struct GroupScale {
     float k, log_v, inv_v;  // s_K * scale * log2 e; log2 s_V, -inf for tokens of no page; 1 / s_V
-    float pad;
+    uint32_t gap;           // a visible key of the tile has no page (the prompts kernel)
 };
 
 /// TS: warps, or pairs of them, that share a tile's keys.  TILE: keys of a tile.  CPS: CTAs that share an SM.

@@ -258,8 +258,10 @@ __device__ __forceinline__ void convert_slots(const AttentionCall& c, const Work
         const uint32_t number = (2 * count + (IS_V ? 1 : 0)) * S::kParts + part, at = number % S::kSlots, slot = ring + at * S::kSlot;
         const bool check = IS_V && !whole;
         if (alive) alive = __all_sync(0xFFFFFFFFu, mbar_wait(empty + 8 * at, (number / S::kSlots & 1) ^ 1));
+        const bool gap = !IS_V && part == 0 && __any_sync(0xFFFFFFFFu, page == -2);
         if (!IS_V && part == 0 && lane < kTile / 16) {
             GroupScale& s = scales[count % 8][lane];
+            s.gap = gap;
             const int32_t v = scale_byte(v_byte) - 127;
             s.k = page >= 0 ? exp2_int(scale_byte(k_byte) - 127) * scale : 0.0f;
             s.log_v = page >= 0 ? static_cast<float>(v) : -INFINITY;
@@ -671,6 +673,17 @@ __global__ void __launch_bounds__(TilesShape<D, sizeof(T) == 4 ? 2 : 1>::kThread
                         for (int e = 0; e < 32; ++e)
                             if (at + static_cast<uint32_t>(e) >= seen) v[e] = 0xFF800000u;  // -inf
                     };
+                    if (sc->gap != 0) {  // keys that are not there are zeros: times a NaN or an infinity of q they would count
+#pragma unroll 1
+                        for (int i = 0; i < S::kKeys / 16; ++i) {
+                            if (sc[i].log_v != -INFINITY) continue;
+                            uint32_t none[16];
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) none[e] = 0xFF800000u;
+                            tmem_st16(s_at + half * S::kKeys + 16 * i, none);
+                        }
+                        tmem_wait_st();
+                    }
                     if (kHold) {
 #pragma unroll
                         for (int q = 0; q < kChunks; ++q) tmem_ld32(s_at + half * S::kKeys + 32 * q, x[kHold ? q : 0]);

@@ -126,7 +126,8 @@ int halo_cuda_kv_write(HaloCudaCtx* ctx, const HaloCudaKvWrite* args, HaloCudaSt
 /* out[row][h] = sum_t w_t V[t], w = softmax over the tokens t that the row sees of scale * q[row][h] . K[t], with K and V of kv head
  * h / (n_q / n_kv) of the row's sequence.  A row at position p sees tokens t < length; causal = 1: of those t <= p; window > 0 (causal only): of
  * those t > p - window.  A row that sees none gets zeros.  What a row does not see has no influence on it, whatever it holds.  Tokens of a page whose
- * number is outside [0, n_pages) are left out and set bit 8 of *status (device word, optional).
+ * number is outside [0, n_pages) are left out and set bit 8 of *status (device word, optional).  A row whose q holds a NaN or an infinity gets NaN, or
+ * zeros where it sees none or all of its scores are minus infinity; no other row is touched by it.
  * Type F32 computes to fp32 accuracy (both factors of the products in two fp16 terms, 22 bits); F16 and BF16 take q exactly and round the weights to
  * 11 bits.  Softmax and sums are fp32; the tensor cores cut a sum off where they add 16 keys to it, so one is taken out and added up, rounded, after at most
  * 64 (F32) or 1024 (F16, BF16) such steps: what is lost of it is below 2^-17 or 2^-13, however long the context.  Weights (times their values' scale)

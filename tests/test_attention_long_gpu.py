@@ -179,3 +179,21 @@ def test_a_block_may_walk_for_seconds(be):
     run, u = RUN["tiles", "f16"], 2.0 ** -24
     assert np.abs(got / want - 1).max() <= 4 * run * u + 2 * (c.n / (run * 16) + 1) * u + 64 * u + STEP["f16"]  # as in test_sums_of_a_long_context
     assert be.lib.halo_cuda_ctx_lost(be.ctx) == 0
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("rows", [1, 3, 150])
+def test_a_row_of_nan_that_sees_nothing_gets_zeros(be, kind, dim, rows):
+    """Rows of NaN, some of which see tokens of missing pages alone: a page that is not there counts for nothing whatever it is multiplied with."""
+    c = Case(51, kind, dim, 16, 2, 3, [rows] * 3, [rows, rows, rows + 300])
+    c.cache["table"][0, :] = -1                  # no page of it is there
+    c.cache["table"][1, :min(rows, 30) // 16 + 1] = c.n_pages  # none that its first rows see
+    c.cache["table"][2, 3:11] = -5               # a whole tile of keys and parts of others
+    c.to_device()
+    q = c.q_dev.clone()
+    q[::2, :, 5] = float("nan")
+    c.q_dev, c.q = q, q.double().cpu().numpy()
+    out = c.run(be)
+    want = c.compare(out, bad=8)
+    assert np.all(want[:rows + 1] == 0)
