@@ -79,7 +79,7 @@ __global__ void __launch_bounds__(kThreads, 4) rope_kernel(const __grid_constant
         if (turn == 0) {  // behind the first loads, which are under way meanwhile
             for (uint32_t i = threadIdx.x; i < nt * a.pairs; i += kThreads) {
                 const uint32_t t = i / a.pairs, j = i - t * a.pairs;
-                const uint64_t phase = static_cast<uint64_t>(static_cast<int64_t>(__ldg(a.positions + t0 + t))) * a.turns[j];
+                const uint64_t phase = static_cast<uint64_t>(static_cast<int64_t>(attn::load(a.positions + t0 + t))) * a.turns[j];
                 float s, c;
                 sincospif(static_cast<float>(static_cast<int32_t>(phase >> 32)) * 0x1p-31f, &s, &c);
                 cosine[i] = c * a.magnitude, sine[i] = s * a.magnitude;
@@ -143,7 +143,7 @@ __global__ void __launch_bounds__(kThreads, 4) rope_warp_kernel(const __grid_con
         if constexpr (!INTERLEAVED) z = *reinterpret_cast<const Word*>(src + second * sizeof(T));
     };
     load(h0 + sub, x, z);
-    const uint64_t position = static_cast<uint64_t>(static_cast<int64_t>(__ldg(a.positions + t)));
+    const uint64_t position = static_cast<uint64_t>(static_cast<int64_t>(attn::load(a.positions + t)));
     float c[kPairs], s[kPairs];
     // pair p of the unit is made by the unit's lane p % step
 #pragma unroll

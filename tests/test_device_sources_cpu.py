@@ -12,3 +12,11 @@ def test_the_error_word_may_be_missing():
               if "atomicOr(" in line and "error_word" in line]
     assert len(writes) > 10
     assert [w for w in writes if "error_word != nullptr" not in w[2]] == []
+
+
+def test_what_a_launch_names_is_not_read_in_front_of_the_kernel_before():
+    """Lengths, starts and positions may have been written by the kernel before, which still runs when these kernels begin: not by loads that the compiler
+    may move in front of the wait for it.  (Every other address depends on one of them.)"""
+    for f in sorted(CSRC.glob("attention*")) + [CSRC / "kv_write.cu", CSRC / "rope.cu"]:
+        for line in f.read_text().splitlines():
+            assert not any(f"__ldg({name}" in line for name in ("r.start", "r.length", "a.positions")), (f.name, line.strip())
