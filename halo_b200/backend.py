@@ -467,7 +467,7 @@ class CudaBackend:
         page = c.n_kv * c.page_tokens * c.head_dim
         out = capi.KvCache(type=capi.KV_E4M3, n_pages=c.n_pages, n_kv=c.n_kv, head_dim=c.head_dim, page_tokens=c.page_tokens, max_pages=c.max_pages,
                            n_seq=c.n_seq, page_stride=c.k.row_stride, scale_stride=c.k_scale.row_stride, table_stride=c.table.row_stride)
-        if c.k.row_stride != c.v.row_stride or c.k_scale.row_stride != c.v_scale.row_stride:
+        if (c.k.row_stride or page) != (c.v.row_stride or page) or (c.k_scale.row_stride or c.n_kv) != (c.v_scale.row_stride or c.n_kv):
             raise HaloError(capi.E_KERNEL, f"{op}: the two pools have one stride")
         for name, row in (("k", page), ("v", page), ("k_scale", c.n_kv), ("v_scale", c.n_kv)):
             ref = getattr(c, name)
