@@ -87,3 +87,85 @@ def test_prompts_among_decoding_sequences_in_a_padded_call(be, kind, dim, page, 
     write(be, c, k, v, rows=c.rows(n_tokens=n))
     ref.kv_write(c.cache, k.double().cpu().numpy(), v.double().cpu().numpy(), c.start, c.length)
     same_cache(c)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("dim,gap", [(64, 16), (128, 48), (256, 16), (256, 80)])
+@pytest.mark.parametrize("rows", [1, 3, 70])
+def test_page_strides_that_are_no_multiple_of_a_row(be, kind, dim, gap, rows):
+    c = Case(62, kind, dim, 32, 2, 4, [rows, rows], [rows + 150, rows])
+    page = c.n_kv * c.page * dim
+    pools = {}
+    for name in ("k", "v"):
+        pools[name] = torch.full((c.n_pages, page + gap), 127, dtype=torch.uint8, device="cuda")
+        pools[name][:, :page] = c.dev[name].view(c.n_pages, page)
+    cache = c.kv(k=pools["k"].data_ptr(), v=pools["v"].data_ptr(), page_stride=page + gap)
+    c.compare(c.run(be, cache=cache))
+    (k, v), (kh, vh) = new_rows(c)
+    write(be, c, k, v, cache=cache)
+    ref.kv_write(c.cache, kh, vh, c.start, c.length)
+    for name in ("k", "v"):
+        c.dev[name] = pools[name][:, :page].reshape(c.dev[name].shape)
+        assert bool((pools[name][:, page:] == 127).all())
+    same_cache(c)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16"])
+@pytest.mark.parametrize("dim,group", [(64, 71), (128, 200), (256, 130)])
+@pytest.mark.parametrize("q_len,window", [([1, 1, 1], 0), ([3, 1, 2], 0), ([5, 40, 1], 60)])
+def test_many_heads_over_one(be, kind, dim, group, q_len, window):
+    """A tile of packed rows has parts of a token's heads, or ends inside the next token's."""
+    c = Case(63, kind, dim, 16, 1, group, q_len, [500, 40, 130])
+    c.compare(c.run(be, window=window), window=window)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("rows", [1, 70])
+def test_a_layers_three_calls_in_one_graph(be, kind, rows):
+    """Rotation in place, write and attention of the fused rows, captured once and replayed as the context grows by them: each reads what the one in front has
+    written, on a device that starts it before that one is done."""
+    n_kv, group, dim, page = 2, 3, 128, 16
+    c = Case(64, kind, dim, page, n_kv, group, [rows, rows], [20 + 6 * rows, 7 + 6 * rows])
+    c.cache["k"][:], c.cache["v"][:], c.cache["k_scale"][:], c.cache["v_scale"][:] = 0, 0, 100, 100
+    c.to_device()
+    f = hb.rope_freqs(64, 1e6)
+    freqs, magnitude = ref.rope_freqs(64, 1e6)
+    n_q = c.n_q
+    fused = torch.zeros((2 * rows, n_q + 2 * n_kv, dim), dtype=c.dtype, device="cuda")
+    q, k, v = fused[:, :n_q], fused[:, n_q:n_q + n_kv], fused[:, n_q + n_kv:]
+    out, pos = torch.zeros((2 * rows, n_q, dim), dtype=c.dtype, device="cuda"), torch.zeros(2 * rows, dtype=torch.int32, device="cuda")
+    turn = capi.Rope(type=c.type, freqs=C.pointer(f), positions=pos.data_ptr(), q=heads(q), k=heads(k), q_out=heads(q), k_out=heads(k), n_tokens=2 * rows, n_q=n_q,
+                     n_kv=n_kv, head_dim=dim)
+    put = capi.KvWrite(type=c.type, cache=c.kv(), rows=c.rows(), k=heads(k), v=heads(v), status=c.status.data_ptr())
+    see = c.call(out, q=heads(q))
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+
+    def calls():
+        check(be.lib.halo_cuda_rope(be.ctx, C.byref(turn), side.cuda_stream))
+        check(be.lib.halo_cuda_kv_write(be.ctx, C.byref(put), side.cuda_stream))
+        check(be.lib.halo_cuda_attention(be.ctx, C.byref(see), side.cuda_stream))
+
+    lengths = [[20 + i * rows, 7 + i * rows] for i in range(1, 7)]
+    c.length_dev.copy_(torch.tensor([0, 0], dtype=torch.int32))  # the call in front of the capture writes nothing
+    torch.cuda.synchronize()
+    calls()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        calls()
+    for i, length in enumerate(lengths):
+        x = torch.from_numpy(c.rng.normal(size=tuple(fused.shape)).astype(np.float32)).to(c.dtype)
+        at = np.concatenate([np.arange(n - rows, n) for n in length]).astype(np.int32)
+        with torch.cuda.stream(side):
+            fused.copy_(x)
+            pos.copy_(torch.from_numpy(at))
+            c.length_dev.copy_(torch.tensor(length, dtype=torch.int32))
+            graph.replay()
+        torch.cuda.synchronize()
+        xd, td = x.double().numpy(), fused.double().cpu().numpy()
+        want = xd.copy()
+        want[:, :n_q + n_kv] = ref.rope(xd[:, :n_q + n_kv], at, freqs, magnitude, False)
+        assert np.all(np.abs(td - want) <= rope_bound(kind, xd, want, 32, magnitude, False) + 1e-300), i
+        ref.kv_write(c.cache, td[:, n_q:n_q + n_kv], td[:, n_q + n_kv:], c.start, length)  # from what the rotation stored
+        same_cache(c)
+        y, weight, top, count = ref.attention(td[:, :n_q], c.cache, c.start, length, dim ** -0.5)
+        assert np.all(np.abs(out.double().cpu().numpy() - y) <= ref.attention_bound(kind, dim, y, weight, top, count)), i
