@@ -5,7 +5,7 @@
 //
 // The scale of a value's page rides in its token's exponent, so that o needs no rescaling between pages and p_t, at most 2^14, is an fp16 number with
 // 11 bits down to 2^-28 of the largest.  e4m3 codes are exact in fp16.  A row of q is multiplied by the power of two that puts its largest magnitude
-// into [2^14, 2^15) and rounded to fp16: exact for fp16 and bf16 operands (but for elements below 2^-29 of the row's largest);
+// into [2^14, 2^15) and rounded to fp16: exact for fp16 and bf16 operands (but for elements below 2^-28 of the row's largest);
 // fp32 operands are taken as two fp16 terms, and so are their p_t.  Accumulators, maxima and sums are fp32.
 //
 // A CTA has 16 packed rows (attention_work.cuh).  Its warps share the keys of a tile, each with a running maximum, sum and accumulators of its own
@@ -13,10 +13,11 @@
 // thread: there two warps share the same keys, each makes half of the scores and all of the weights, and has half of the dims.  A producer warp
 // brings the tiles' codes by TMA, a box for each page, into a ring, and with them the scales of every 16 tokens (a page is at least 16).
 //
-// What bounds it: HBM while the walk lasts (131071 tokens of 8 heads of 128, 268 MB, take 64 us, 4.2 TB/s; of a CTA's 92 thousand clocks the walk has 80,
-// which is 6.2 TB/s, the search for its share 4, the first tile 6).  A byte of the cache costs a warp half a conversion, and a sixteenth of a
-// 16 x 8 x 16 product for 16 rows.  Heads of 256 with fp32 operands, four products for one, are bound by the dependent steps of eight warps an SM (a third of
-// the issue slots used): 2.1 TB/s for single tokens, 12 sequences of 2156 - 4688 with 24 rows each 65 us.
+// What bounds it: HBM while the walk lasts where a sequence is long (131071 tokens of 8 heads of 128 in bf16, 268 MB, take 63 us, 4.2 TB/s; four times the
+// tokens take 193, so that the further ones come at 6.3 TB/s and 20 us are fixed: the launch 8, search, first tile, joins).  Many sequences of all lengths come at
+// 5.0 TB/s (48 of 156 - 7697, pages of 16, 200 MB in 56 us; twice and four times as many 95 and 193): the ends of units.  A byte of the cache costs a warp
+// half a conversion, and a sixteenth of a 16 x 8 x 16 product for 16 rows.  Heads of 256 with fp32 operands, four products for one, are bound by the dependent
+// steps of eight warps an SM (a third of the issue slots used): 12 sequences of 2156 - 4688 with 24 rows each 67 us, further ones at 1.7 TB/s.
 #pragma once
 #include <cuda.h>
 
@@ -819,7 +820,7 @@ int launch_rows_kernel(HaloCudaCtx* ctx, const AttentionCall& c, Work w, cudaStr
     using S = RowsShape<D, TS, TILE, CPS, sizeof(T) == 4 ? 2 : 1>;
     w.rows = S::kRows;
     w.tile = S::kTile;
-    w.pad = 4;
+    w.pad = 4;  // 48 decoding sequences of 156 - 7697 tokens 65.6 us, with 2 or 6 67.6; drafts of 12 sequences 73.9, 74.7 with 2, 73.7 with 6
     w.group = c.group;
     w.group_inverse = static_cast<uint32_t>((0xFFFFFFFFull + c.group) / c.group);
     w.row_tiles = (w.max_rows + S::kRows - 1) / S::kRows;
@@ -858,9 +859,11 @@ int launch_rows_kernel(HaloCudaCtx* ctx, const AttentionCall& c, Work w, cudaStr
 template <int D>
 int launch_kernel(HaloCudaCtx* ctx, const AttentionCall& c, const Work& w, cudaStream_t s);
 
-/// Up to how many packed rows of a sequence the row kernel takes.  12 sequences of 2000 - 4700 tokens, row kernel / tcgen05 kernel, us: heads of 256, 24
-/// rows: fp32 66 / 81, bf16 56 / 58; 36 rows: 89 / 88, 75 / 64.  Heads of 128, 40 rows: fp32 79 / 81, bf16 61 / 93; 64 rows: 100 / 84, 76 / 93.  Heads of
-/// 64, 64 rows: 63 / 67, 55 / 74.
+/// Up to how many packed rows of a sequence the row kernel takes.  12 sequences of 2156 - 4688 tokens, row kernel / tcgen05 kernel, us: heads of 256, 24
+/// rows: fp32 68 / 82, bf16 57 / 52; 48 rows: 93 / 94, 77 / 61.  Heads of 128, 32 rows: fp32 62 / 72; 48 rows: 83 / 75, bf16 64 / 82; 64 rows: bf16 80 / 83; 96
+/// rows: 110 / 86.  Heads of 64, 48 rows: fp32 53 / 57; 64 rows: 65 / 58, bf16 56 / 58; 96 rows: 77 / 60.  One rule between calls that want another: a
+/// single sequence of 1037 tokens is better off here with more rows (heads of 256, 48 rows: bf16 21 / 33, fp32 23 / 44), 48 sequences of 6000 there
+/// with fewer (heads of 256, 24 rows, bf16: 272 / 187; heads of 128, 48 rows, fp32: 462 / 347).
 inline uint32_t few_rows(const AttentionCall& c) { return c.cache.head_dim == 256 ? 32 : c.type == HALO_CUDA_T_F32 ? 48 : 64; }
 
 }  // namespace attn

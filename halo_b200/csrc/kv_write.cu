@@ -9,8 +9,8 @@
 //
 // One block for every (sequence, page it touches, kv head, K or V): the page's scale needs the maximum over all of its new rows.  A thread holds
 // 16 elements of up to four rows in registers between the maximum and the codes, so every row is read once, and stores 16 codes at a time.
-// What bounds it: for prompts HBM (size + 1 bytes an element) and the latency of read, maximum, write in one block (five prompts, 91 MB, 22 us, 4.1 TB/s);
-// the launch and two dependent reads (table, rows) for single tokens.
+// What bounds it: for prompts HBM (size + 1 bytes an element) and the latency of read, maximum, write in one block (five prompts, 91 MB, 27.7 us, 3.3 TB/s; 22 us
+// where the rows are in L2 from the call before); the launch and two dependent reads (table, rows) for single tokens.
 #include <cuda_fp8.h>
 
 #include "attention.h"
@@ -164,7 +164,7 @@ int launch_kv_write(HaloCudaCtx*, const WriteCall& c, cudaStream_t s) {
     return with_type(c.type, [&](auto t) {
         using T = decltype(t);
         // A page's rows at most, or all that a sequence brings: up to four units a thread (five prompts in pages of 512 units: blocks of 512 threads 29.4 us, of
-        // 256 22.8, of 128 22.2), and blocks of 512 threads where 128 would not do.
+        // 256 22.8, of 128 22.2, back to back on the same rows), and blocks of 512 threads where 128 would not do.
         const uint32_t units = std::min(c.cache.page_tokens, c.rows.max_tokens) * (c.cache.head_dim / kUnit);  // <= 2048
         const uint32_t threads = std::min((units + 31u) / 32u * 32u, units > 512u ? 512u : 128u);
         const uint32_t per = (units + threads - 1) / threads;

@@ -4,7 +4,7 @@
 // 2^31 is as exact as that of position 1 (an fp32 product would be off by a tenth of a radian at a million).  Its leading 32 bits go through
 // sincospif, whose argument is then in [-1, 1).
 //
-// What bounds it: HBM, 2 * size bytes an element (8192 tokens of 40 heads of 128 in bf16, 168 MB, 34 us, 4.9 TB/s); for few tokens the launch.  A block takes a few tokens and a share of their heads: it computes the tokens' cosines and
+// What bounds it: HBM, 2 * size bytes an element (8192 tokens of 40 heads of 128 in bf16, 168 MB, 33.4 us, 5.0 TB/s); for few tokens the launch.  A block takes a few tokens and a share of their heads: it computes the tokens' cosines and
 // sines into shared memory while its first loads are under way; a thread has two units in flight, a unit being the 16-byte vectors of both halves of 16 / size
 // pairs (one vector where pairs are adjacent), or a vector to copy.
 #include "rope.h"

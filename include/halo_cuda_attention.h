@@ -112,8 +112,8 @@ typedef struct HaloCudaKvRows {
  * the sequence's earlier tokens: those are then rounded again to the new scale.  Codes are rounded to nearest, ties to even; infinities become
  * +-448, a NaN stays one.  Slots behind the new rows keep their bytes (and no meaning).  Rows at negative positions are skipped.  A page
  * number outside [0, n_pages) sets bit 8 (kStatusBadIndex) of *status (device word, optional) and nothing is written for it.  At most 65535
- * sequences and 32767 kv heads.  Two sequences of one call must not write into the same page: a forked page is copied first
- * (halo_cuda_memcpy_d2d_async of its codes and scale bytes). */
+ * sequences and 32767 kv heads.  Two sequences of one call must not write into the same page, nor one sequence through two columns of
+ * its row: a forked page is copied first (halo_cuda_memcpy_d2d_async of its codes and scale bytes). */
 typedef struct HaloCudaKvWrite {
     uint32_t type, reserved; /* of k and v: HALO_CUDA_T_F32, _F16, _BF16 */
     HaloCudaKvCache cache;
@@ -128,11 +128,11 @@ int halo_cuda_kv_write(HaloCudaCtx* ctx, const HaloCudaKvWrite* args, HaloCudaSt
  * those t > p - window.  A row that sees none gets zeros.  What a row does not see has no influence on it, whatever it holds.  Tokens of a page whose
  * number is outside [0, n_pages) are left out and set bit 8 of *status (device word, optional).  A row whose q holds a NaN or an infinity gets NaN, or
  * zeros where it sees none or all of its scores are minus infinity; no other row is touched by it.
- * Type F32 computes to fp32 accuracy (both factors of the products in two fp16 terms, 22 bits); F16 and BF16 take q exactly and round the weights to
- * 11 bits.  Softmax and sums are fp32; the tensor cores cut a sum off where they add 16 keys to it, so one is taken out and added up, rounded, after at most
- * 64 (F32) or 1024 (F16, BF16) such steps: what is lost of it is below 2^-17 or 2^-13, however long the context.  Weights (times their values' scale)
- * below 2^-20 of the row's largest are rounded to multiples of 2^-30 of it, for all types.  The order of the sums goes with the shape and the lengths of
- * the whole call, and the same call gives the same bits.
+ * Type F32 computes to fp32 accuracy (both factors of the products in two fp16 terms, 22 bits); F16 and BF16 take q exactly (but for elements below
+ * 2^-28 of their row's largest) and round the weights to 11 bits.  Softmax and sums are fp32; the tensor cores cut a sum off where they add 16 keys to it,
+ * so one is taken out and added up, rounded, after at most 64 (F32) or 1024 (F16, BF16) such steps: what is lost of it is below 2^-17 or 2^-13, however
+ * long the context.  Weights (times their values' scale) below 2^-20 of the row's largest are rounded to multiples of 2^-30 of it, for all types.  The
+ * order of the sums goes with the shape and the lengths of the whole call, and the same call gives the same bits.
  * The cache has at least one page, and the table a column.  Uses context scratch, whose size goes with the operands' shapes alone: run a call once
  * before capturing it. */
 typedef struct HaloCudaAttention {
