@@ -157,6 +157,8 @@ int take_attention(const HaloCudaAttention* a, AttentionCall* c) {
     Span q, out;
     if (int rc = take_cache(a->cache, op, &c->cache, &cs)) return rc;
     if (int rc = take_rows(a->rows, op, a->cache.n_seq, &c->rows)) return rc;
+    // A block steps past sequences without rows one by one, and its warps wait 1.3 s for one another: tens of millions would be too many.
+    if (a->cache.n_seq > (1u << 20)) return fail(HALO_CUDA_E_UNSUPPORTED, "%s: %u sequences", op, a->cache.n_seq);
     if (a->n_q == 0 || a->n_q > 32768u || a->n_q % a->cache.n_kv != 0) return fail(HALO_CUDA_E_KERNEL, "%s: %u query heads over %u kv heads", op, a->n_q, a->cache.n_kv);
     if (a->causal > 1) return fail(HALO_CUDA_E_API, "%s: causal is 0 or 1", op);
     if (a->window != 0 && a->causal == 0) return fail(HALO_CUDA_E_UNSUPPORTED, "%s: a window without a causal mask", op);

@@ -133,7 +133,7 @@ int halo_cuda_kv_write(HaloCudaCtx* ctx, const HaloCudaKvWrite* args, HaloCudaSt
  * so one is taken out and added up, rounded, after at most 64 (F32) or 1024 (F16, BF16) such steps: what is lost of it is below 2^-17 or 2^-13, however
  * long the context.  Weights (times their values' scale) below 2^-20 of the row's largest are rounded to multiples of 2^-30 of it, for all types.  The
  * order of the sums goes with the shape and the lengths of the whole call, and the same call gives the same bits.
- * The cache has at least one page, and the table a column.  Uses context scratch, whose size goes with the operands' shapes alone: run a call once
+ * The cache has at least one page, the table a column, and at most 2^20 sequences.  Uses context scratch, whose size goes with the operands' shapes alone: run a call once
  * before capturing it. */
 typedef struct HaloCudaAttention {
     uint32_t type, n_q; /* of q and out; n_q: a multiple of n_kv, at most 32768 */

@@ -1,6 +1,8 @@
 """The attention layer through CudaBackend, as far as it looks at operands on the host."""
 from __future__ import annotations
 
+import ctypes as C
+
 import pytest
 
 from halo_b200 import backend as hb
@@ -39,3 +41,13 @@ def test_pools_of_two_strides_are_refused():
     for kw in (dict(k_stride=4096), dict(k_stride=2048, v_stride=4096), dict(v_scale_stride=3), dict(k_scale_stride=8, v_scale_stride=4)):
         with pytest.raises(hb.HaloError, match="one stride"):
             call(**kw)
+
+
+def test_attention_takes_a_million_sequences():
+    heads = [capi.Heads(BASE + (i << 36), 0, 0) for i in (1, 2)]
+    for n_seq, status, words in ((1 << 20, capi.E_API, "null context"), ((1 << 20) + 1, capi.E_UNSUPPORTED, "1048577 sequences")):
+        cache = capi.KvCache(k=BASE, v=BASE + (1 << 24), k_scale=BASE + (2 << 24), v_scale=BASE + (3 << 24), table=BASE + (4 << 36), type=capi.KV_E4M3, n_pages=2, n_kv=1,
+                             head_dim=64, page_tokens=16, max_pages=1, n_seq=n_seq)
+        a = capi.Attention(type=capi.T_F16, n_q=1, cache=cache, rows=capi.KvRows(BASE + (5 << 36), BASE + (6 << 36), n_seq, 1), q=heads[0], out=heads[1], causal=1, scale=1.0)
+        assert capi.load().halo_cuda_attention(None, C.byref(a), None) == status
+        assert words in capi.last_error()

@@ -169,3 +169,17 @@ def test_a_layers_three_calls_in_one_graph(be, kind, rows):
         same_cache(c)
         y, weight, top, count = ref.attention(td[:, :n_q], c.cache, c.start, length, dim ** -0.5)
         assert np.all(np.abs(out.double().cpu().numpy() - y) <= ref.attention_bound(kind, dim, y, weight, top, count)), i
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("rows", [1, 100])
+def test_a_million_sequences_of_which_few_have_rows(be, kind, rows):
+    """Blocks step past all that have none."""
+    n = 1 << 20
+    q_len, length = [0] * n, [0] * n
+    for i, more in ((5, 300), (6, 0), (n // 2, 40), (n - 1, 700)):
+        q_len[i], length[i] = rows, rows + more
+    q_len[n // 3], length[n // 3] = 2, 20
+    c = Case(65, kind, 64, 16, 1, 1, q_len, length)
+    c.compare(c.run(be))
+    assert be.lib.halo_cuda_stream_sync(be.ctx, stream(), 0) == 0, capi.last_error()
