@@ -95,38 +95,32 @@ __device__ __forceinline__ uint32_t half2_rest(float a, float b, uint32_t first)
 }
 /// Bit 7 of every byte of four that is a NaN code, 0x7F or 0xFF.
 __device__ __forceinline__ uint32_t nan_bits(uint32_t w) { return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u; }
-/// Zeroes the NaN codes of four; true if there were any.
-__device__ __forceinline__ bool drop_nan(uint32_t& w) {
+/// Zeroes the NaN codes of four, or with `keep` of all ones leaves them; true if there were any.
+__device__ __forceinline__ bool drop_nan(uint32_t& w, uint32_t keep = 0) {
     const uint32_t hit = nan_bits(w);
     if (hit == 0) return false;
-    w &= ~((hit >> 7) * 255u);
+    w &= ~((hit >> 7) * 255u) | keep;
     return true;
 }
 
 /// Writes NaN over the results of rows that see a token whose value is NaN there: the walk left those codes out in tiles that some rows do not see
-/// whole, or whose pages are not all there, since a product with weight zero would have spread them.  Only those tiles are looked at (every token of 60000, one
-/// after the other, took 300 to 9000 us).  Called by whole warps that share the segment's codes of dims [first_dim, first_dim + dims), 16 bytes to a thread at a
-/// time; `at(row, d)` is the result's address.  Counts `moved` up, for those who wait for the warps meanwhile.
+/// whole, since a product with weight zero would have spread them to these.  Only those tiles are looked at, a handful at the edges of what a unit's rows see (every
+/// token of 60000, one after the other, took 300 to 9000 us).  Called by whole warps that share the segment's codes of dims [first_dim, first_dim + dims), 16
+/// bytes to a thread at a time; `at(row, d)` is the result's address.
 template <class At>
 __device__ void spread_nan(const AttentionCall& c, const Work& w, const Unit& u, const Segment& g, uint32_t first_row, uint32_t end_row, uint32_t first_dim, uint32_t dims,
-                           uint32_t thread, uint32_t threads, volatile uint32_t* moved, At&& at) {
+                           uint32_t thread, uint32_t threads, At&& at) {
     const uint32_t r0 = u.row0(w), lane = threadIdx.x % 32, chunks = dims / 16;
     const int32_t tile_keys = static_cast<int32_t>(w.tile), page_tokens = static_cast<int32_t>(c.cache.page_tokens);
     const int32_t all_lo = first_key(u.s, w.window, (r0 + u.rows(w) - 1) / c.group), all_hi = end_key(u.s, c.causal, r0 / c.group);
-    auto missing = [&](int32_t t) { return static_cast<uint32_t>(page_of(c.cache, u.seq, t >> c.cache.page_shift)) >= c.cache.n_pages; };
     for (int32_t base = g.lo; base < g.hi; base += 32) {
         const int32_t tile = base + static_cast<int32_t>(lane), t = tile * tile_keys;
-        bool look = false;
-        if (tile < g.hi) {
-            look = t < all_lo || t + tile_keys > all_hi;
-            for (int32_t k = 0; k < tile_keys && !look; k += page_tokens) look = missing(t + k);
-        }
-        if (lane == 0) *moved = *moved + 1;
+        const bool look = tile < g.hi && (t < all_lo || t + tile_keys > all_hi);
         for (uint32_t left = __ballot_sync(0xFFFFFFFFu, look); left != 0; left &= left - 1) {
             const int32_t first = (base + __ffs(left) - 1) * tile_keys;
             for (int32_t t0 = first; t0 < min(first + tile_keys, u.s.length); t0 += 16) {
-                if (missing(t0)) continue;
                 const int32_t page = page_of(c.cache, u.seq, t0 >> c.cache.page_shift);
+                if (static_cast<uint32_t>(page) >= c.cache.n_pages) continue;
                 const uint8_t* v = c.cache.v + page * c.cache.page_stride + (uint64_t{u.head} * c.cache.page_tokens + (t0 & (page_tokens - 1))) * c.cache.head_dim + first_dim;
                 for (uint32_t i = thread; i < dims; i += threads) {  // 16 tokens of `chunks` pieces each
                     const int32_t key = t0 + static_cast<int32_t>(i / chunks);
@@ -284,7 +278,7 @@ __global__ void __launch_bounds__(RowsShape<D, TS, TILE, CPS, sizeof(T) == 4 ? 2
     __shared__ float2 row_ml[TS][16];
     __shared__ float4 told[S::kSplit == 2 ? 2 : 1][TS][S::kSplit][NO][32];  // scores that a pair's warps tell each other, of a tile and the next
     __shared__ float q_unscale[S::kRows];
-    __shared__ uint32_t nan_seen, is_last, moved;
+    __shared__ uint32_t nan_seen, is_last;
     __shared__ Walk walk;
     __shared__ float2 joined_ml[S::kRows];
 
@@ -304,7 +298,6 @@ __global__ void __launch_bounds__(RowsShape<D, TS, TILE, CPS, sizeof(T) == 4 ? 2
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         nan_seen = 0;
-        moved = 0;
     }
     {
         Range range;
@@ -361,7 +354,7 @@ __global__ void __launch_bounds__(RowsShape<D, TS, TILE, CPS, sizeof(T) == 4 ? 2
                 if (page == -2 && c.status != nullptr) atomicOr(c.status, 8u);  // kStatusBadIndex
                 const uint32_t present = __ballot_sync(0xFFFFFFFFu, page >= 0);
                 for (int32_t tile = base; tile < min(base + kLot, g.hi); ++tile) {
-                    if (alive) alive = __all_sync(0xFFFFFFFFu, mbar_wait(empty + 8 * stage, parity ^ 1, &moved));
+                    if (alive) alive = __all_sync(0xFFFFFFFFu, mbar_wait(empty + 8 * stage, parity ^ 1));
                     if (!alive) break;
                     const uint32_t in_tile = (tile - base) * kGroups, here = present >> in_tile & static_cast<uint32_t>((uint64_t{1} << kGroups) - 1);
                     const uint32_t step = page_rows / 16;  // groups of a box
@@ -568,9 +561,12 @@ __global__ void __launch_bounds__(RowsShape<D, TS, TILE, CPS, sizeof(T) == 4 ? 2
                 for (int n = 0; n < NO; ++n) told[tile & 1][ts][ds][n][lane] = make_float4(x[n][0], x[n][1], x[n][2], x[n][3]);
             }
         };
-        // the weights of a tile's scores, and what they add to the sums and rows.  MASKED: some row does not see some token of the tile.
+        // the weights of a tile's scores, and what they add to the sums and rows.  MASKED: some row does not see some token of the tile, because it is at the edge of
+        // what the rows see, or has no page.
         auto weigh = [&](const bool MASKED, int32_t t0, float (&x)[NT][4]) __attribute__((always_inline)) {
             const uint32_t v_at = ring + stage * S::kStage + S::kHalfTile;
+            // a tile that all rows see spreads the NaN codes of those of its pages that are there to all of them, rightly
+            const uint32_t keep = t0 < all_lo || t0 + static_cast<int32_t>(kTile) > all_hi ? 0u : ~0u;
             float top[2] = {-INFINITY, -INFINITY}, inv[NT];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
@@ -655,7 +651,7 @@ __global__ void __launch_bounds__(RowsShape<D, TS, TILE, CPS, sizeof(T) == 4 ? 2
 #pragma unroll
                             for (int b = 0; b < kChunk / 4; ++b) {
                                 if (!held) vw[i][b] = 0;
-                                nan |= drop_nan(vw[i][b]);
+                                nan |= drop_nan(vw[i][b], keep);
                             }
                         }
                     }
@@ -705,7 +701,7 @@ __global__ void __launch_bounds__(RowsShape<D, TS, TILE, CPS, sizeof(T) == 4 ? 2
                 }
                 scores(next, mine);
                 tell(tile + 1, mine);
-                weigh(masked, t0, x);
+                weigh(masked, t0, x);  // a tile that all rows see spreads its NaN codes to all of them, rightly
                 __syncwarp();
                 if (lane == 0) mbar_arrive(empty + 8 * stage);
                 advance();
@@ -781,7 +777,7 @@ __global__ void __launch_bounds__(RowsShape<D, TS, TILE, CPS, sizeof(T) == 4 ? 2
         }
         bar_sync(1, kConsumers);
         if (nan_seen != 0) {
-            spread_nan(c, w, walk.u, walk.g, 0, walk.u.rows(w), 0, D, threadIdx.x, kConsumers, &moved, [&](uint32_t r, uint32_t d) {
+            spread_nan(c, w, walk.u, walk.g, 0, walk.u.rows(w), 0, D, threadIdx.x, kConsumers, [&](uint32_t r, uint32_t d) {
                 if (slot == nullptr) out_at(r)[d] = from_f32<T>(NAN);
                 else slot[r * D + d] = NAN;
             });

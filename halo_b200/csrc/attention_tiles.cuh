@@ -15,7 +15,7 @@
 //   1-3     q -> fp16 in shared memory, of the next segment while the last one's last weights are made (and TMEM's allocation)
 //   4-7     conversion (4-11 where D is 256): each warp makes one part of K or V of every tile in a ring of eight 16 KiB slots (a K slot: 128 keys x
 //           64 dims; a V slot: 8192 / D keys x all dims, the N operand with dims contiguous); keys that no row of the CTA sees, missing pages and,
-//           in tiles that some row does not see whole, NaN codes of values become zeros (spread_nan puts the latter back)
+//           in tiles at the edge of what some row sees, NaN codes of values become zeros (spread_nan puts the latter back)
 //   last 8  softmax, a thread to a row and a tile's keys, or to half of them where NS is 1; also the epilogue, and the joining of shares
 // Work is dealt as in attention_work.cuh, so a causal prompt's long and short rows and a short chunk behind a long context fill the device alike.
 //
@@ -160,7 +160,7 @@ __device__ __forceinline__ void convert_slots(const AttentionCall& c, const Work
     int32_t entry = -1;                 // of the page table, for this warp's next tile; not looked at before that tile's turn
     uint32_t k_byte = 0, v_byte = 0, count = 0;
     uint64_t group_at = 0;              // lane i: where its keys' codes begin in the pool
-    bool plain = false, whole = false;  // every key is there and seen by some row; by all rows
+    bool plain = false, whole = false;  // every key is there and seen by some row; every key that is there is seen by all rows
     const uint8_t* pool = nullptr;
     auto fetch = [&](int32_t of) {
         const int32_t t = of * kTile + static_cast<int32_t>(lane) * 16;
@@ -179,7 +179,7 @@ __device__ __forceinline__ void convert_slots(const AttentionCall& c, const Work
             v_byte = __ldg(c.cache.v_scale + at);
         }
         plain = t0 >= any_lo && t0 + kTile <= any_hi && __all_sync(0xFFFFFFFFu, page >= 0 || lane >= kTile / 16);
-        whole = plain && t0 >= all_lo && t0 + kTile <= all_hi;
+        whole = t0 >= all_lo && t0 + kTile <= all_hi;
         group_at = static_cast<uint32_t>(max(page, 0)) * c.cache.page_stride + ((static_cast<uint32_t>(t0) + lane * 16) & (c.cache.page_tokens - 1)) * D;
         fetch(tile + static_cast<int32_t>(every));
     };
@@ -857,7 +857,7 @@ __global__ void __launch_bounds__(TilesShape<D, sizeof(T) == 4 ? 2 : 1>::kThread
             if (any_row && __any_sync(0xFFFFFFFFu, *static_cast<volatile uint32_t*>(&nan_tiles) > tiles - static_cast<uint32_t>(last_tile - walk.g.lo))) {
                 __syncwarp();
                 const uint32_t top = stream * 128 + quarter * 32, dims = D / S::kHalves;
-                spread_nan(c, w, walk.u, walk.g, top, min(top + 32, walk.rows), half * dims, dims, lane, 32, &moved, [&](uint32_t row, uint32_t d) {
+                spread_nan(c, w, walk.u, walk.g, top, min(top + 32, walk.rows), half * dims, dims, lane, 32, [&](uint32_t row, uint32_t d) {
                     if (walk.g.whole()) out_at(row)[d] = from_f32<T>(NAN);
                     else partial_slot(w, D, blockIdx.x, walk.g.from_start)[row * D + d] = NAN;
                 });

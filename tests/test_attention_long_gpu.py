@@ -28,15 +28,15 @@ def be():
 class Repeated:
     """One sequence of `n` positions, n_kv heads with a query head each, `rows` rows that all see the whole of it."""
 
-    def __init__(self, seed, kind, dim, n_kv, rows, n, table=None):
+    def __init__(self, seed, kind, dim, n_kv, rows, n, table=None, page=PAGE):
         rng = np.random.default_rng(seed)
         self.dtype, self.type = KINDS[kind]
-        self.dim, self.n_kv, self.rows, self.n = dim, n_kv, rows, n
-        shape = (PAGES, n_kv, PAGE, dim)
+        self.dim, self.n_kv, self.rows, self.n, self.page = dim, n_kv, rows, n, page
+        shape = (PAGES, n_kv, page, dim)
         # values of one sign, 0.5 to 1.875: what is lost of a sum does not cancel
         self.k = rng.integers(0x20, 0x40, shape).astype(np.uint8)
         self.v = rng.integers(0x30, 0x40, shape).astype(np.uint8)
-        self.table = (rng.integers(0, PAGES, -(-n // PAGE)) if table is None else np.array(table)).astype(np.int32)
+        self.table = (rng.integers(0, PAGES, -(-n // page)) if table is None else np.array(table)).astype(np.int32)
         self.dev = {name: torch.from_numpy(x).cuda() for name, x in (("k", self.k), ("v", self.v), ("table", self.table))}
         self.scales = torch.full((PAGES, n_kv), 127, dtype=torch.uint8, device="cuda")
         self.q = torch.from_numpy(rng.normal(size=(rows, n_kv, dim)).astype(np.float32)).to(self.dtype).cuda()
@@ -45,7 +45,7 @@ class Repeated:
 
     def call(self, be, out, scale):
         cache = capi.KvCache(k=self.dev["k"].data_ptr(), v=self.dev["v"].data_ptr(), k_scale=self.scales.data_ptr(), v_scale=self.scales.data_ptr(),
-                             table=self.dev["table"].data_ptr(), type=capi.KV_E4M3, n_pages=PAGES, n_kv=self.n_kv, head_dim=self.dim, page_tokens=PAGE,
+                             table=self.dev["table"].data_ptr(), type=capi.KV_E4M3, n_pages=PAGES, n_kv=self.n_kv, head_dim=self.dim, page_tokens=self.page,
                              max_pages=len(self.table), n_seq=1)
         heads = [capi.Heads(t.data_ptr(), 0, 0) for t in (self.q, out)]
         a = capi.Attention(type=self.type, n_q=self.n_kv, cache=cache, rows=capi.KvRows(None, self.length.data_ptr(), self.rows, self.rows), q=heads[0],
@@ -72,9 +72,9 @@ class Repeated:
 
     def want(self, scale=0.0):
         """([row][kv head][dim], largest sum of |q_d k_d| * |scale|), every key of a page counted as often as the table names the page."""
-        times = np.zeros((PAGES, PAGE))
+        times = np.zeros((PAGES, self.page))
         np.add.at(times, self.table[:-1], 1)
-        times[self.table[-1], :(self.n - 1) % PAGE + 1] += 1
+        times[self.table[-1], :(self.n - 1) % self.page + 1] += 1
         k, v, q = ref.VALUES[self.k], ref.VALUES[self.v], self.q.double().cpu().numpy()
         w = np.exp(np.einsum("rhd,phtd->rhpt", q, k, optimize=True) * scale) * times
         return np.einsum("rhpt,phtd->rhd", w, v, optimize=True) / w.sum(axis=(2, 3))[..., None], np.einsum("rhd,phtd->rhpt", np.abs(q), np.abs(k), optimize=True).max() * abs(scale)
@@ -197,3 +197,23 @@ def test_a_row_of_nan_that_sees_nothing_gets_zeros(be, kind, dim, rows):
     out = c.run(be)
     want = c.compare(out, bad=8)
     assert np.all(want[:rows + 1] == 0)
+
+
+@pytest.mark.parametrize("kernel", ["rows", "tiles"])
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_a_nan_among_missing_pages_costs_nothing(be, kernel, kind, dim):
+    """Every tile of a long context is short of pages and has a NaN in one that is there, which all rows see."""
+    n = 60000
+    n_kv, rows = few(kernel, dim)
+    c = Repeated(6, kind, dim, n_kv, rows, n, [0, -1, 1] * (n // 48), page=16)
+    clean, plain = c.run(be, 0.5 / dim), c.time(be, 0.5 / dim)
+    assert np.isfinite(clean).all()
+    c.dev["v"][0, 3, 2, 5] = 255
+    got, slow = c.run(be, 0.5 / dim), c.time(be, 0.5 / dim)
+    nan = np.zeros(got.shape, bool)
+    nan[:, 3, 5] = True
+    assert np.array_equal(np.isnan(got), nan)
+    assert np.array_equal(got[~nan], clean[~nan])
+    print(f"{kernel} {kind} {dim}: {plain:.0f} us, with a NaN {slow:.0f}")
+    assert slow < 1.5 * plain + 100
