@@ -13,11 +13,11 @@
 // thread: there two warps share the same keys, each makes half of the scores and all of the weights, and has half of the dims.  A producer warp
 // brings the tiles' codes by TMA, a box for each page, into a ring, and with them the scales of every 16 tokens (a page is at least 16).
 //
-// What bounds it: HBM while the walk lasts where a sequence is long (131071 tokens of 8 heads of 128 in bf16, 268 MB, take 63 us, 4.2 TB/s; four times the
+// What bounds it: HBM while the walk lasts where a sequence is long (131071 tokens of 8 heads of 128 in bf16, 268 MB, take 64 us, 4.2 TB/s; four times the
 // tokens take 193, so that the further ones come at 6.3 TB/s and 20 us are fixed: the launch 8, search, first tile, joins).  Many sequences of all lengths come at
 // 5.0 TB/s (48 of 156 - 7697, pages of 16, 200 MB in 56 us; twice and four times as many 95 and 193): the ends of units.  A byte of the cache costs a warp
 // half a conversion, and a sixteenth of a 16 x 8 x 16 product for 16 rows.  Heads of 256 with fp32 operands, four products for one, are bound by the dependent
-// steps of eight warps an SM (a third of the issue slots used): 12 sequences of 2156 - 4688 with 24 rows each 67 us, further ones at 1.7 TB/s.
+// steps of eight warps an SM (a third of the issue slots used): 12 sequences of 2156 - 4688 with 24 rows each 68 us, further ones at 1.7 TB/s.
 #pragma once
 #include <cuda.h>
 

@@ -22,7 +22,7 @@
 // What bounds it.  For D = 128 256 rows x 128 keys are 2100 clocks of products, and as many of exponentials (16 a clock).  Prompts of 364 - 1568 tokens (76.6
 // GFLOP, 720 units) take 209 us, 370 TFLOP/s: the two row tiles' chains of scores, maximum, weights and products overlap only in part, and a unit's ends
 // (q, first scores, last rows) cost as much as two or three tiles.  Code size counts as much as instructions: the warps of an SM run five different loops,
-// and unrolled ones waited for instructions more than for anything else.  2048 tokens behind 28000 with D = 256 (1459 GFLOP) take 1616 us, 903 TFLOP/s,
+// and unrolled ones waited for instructions more than for anything else.  2048 tokens behind 28000 with D = 256 (1459 GFLOP) take 1611 us, 906 TFLOP/s,
 // with inputs that change (1480 back to back on the same ones): a little over half of what the tensor cores do; the conversion of the codes, once for 128 rows,
 // holds it up.
 #pragma once

@@ -9,7 +9,7 @@
 //
 // One block for every (sequence, page it touches, kv head, K or V): the page's scale needs the maximum over all of its new rows.  A thread holds
 // 16 elements of up to four rows in registers between the maximum and the codes, so every row is read once, and stores 16 codes at a time.
-// What bounds it: for prompts HBM (size + 1 bytes an element) and the latency of read, maximum, write in one block (five prompts, 91 MB, 27.7 us, 3.3 TB/s; 22 us
+// What bounds it: for prompts HBM (size + 1 bytes an element) and the latency of read, maximum, write in one block (five prompts, 91 MB, 27.5 us, 3.3 TB/s; 22 us
 // where the rows are in L2 from the call before); the launch and two dependent reads (table, rows) for single tokens.
 #include <cuda_fp8.h>
 
